@@ -37,6 +37,7 @@ extern "C" {
 /* 16-bit storage types of x / pools / y. */
 #define PERSONA_DTYPE_F16 0
 #define PERSONA_DTYPE_BF16 1
+#define PERSONA_DTYPE_F32 2 /* probabilities of persona_verify_draft only */
 
 /* Host-side status codes. */
 #define PERSONA_OK 0
@@ -56,6 +57,8 @@ extern "C" {
 #define PERSONA_DEV_ERR_PLAN 8    /* PERSONA_REUSE_PLAN: the workspace holds no plan
                                      for this T and S (nothing was computed), or a
                                      plan entry was out of range (that item skipped) */
+#define PERSONA_DEV_ERR_PAGE 16  /* a position behind the page table, or a page outside the cache */
+#define PERSONA_DEV_ERR_TOKEN 32 /* a drafted token outside the vocabulary (taken as rejected)    */
 
 /* Flags of the BGMV ops. */
 #define PERSONA_REUSE_PLAN 1 /* workspace already holds the plan of these slots */
@@ -327,6 +330,102 @@ int persona_decode_attention(const void* q, const void* k_cache, const void* v_c
 int persona_rope_decode_attention(void* q, void* k, const void* v, void* k_cache, void* v_cache, const int32_t* pos,
                                   const int32_t* len, void* out, int64_t B, int64_t Hq, int64_t Hkv, int64_t L,
                                   float theta, float scale, cudaStream_t stream);
+
+/* ---- paged KV cache ---------------------------------------------------------
+ * No reference counterpart (the reference decodes through Hugging Face's
+ * caches, one length for the whole batch).  A ragged batch of B sequences over
+ * one cache of pages: sequence b's new tokens are rows [indptr[b],
+ * indptr[b + 1]) of the activations and sit at its last positions, the last
+ * one at lengths[b] - 1; position p is in page page_table[b, p / page_size].
+ * indptr [B + 1], lengths [B] and page_table [B, max_pages] are int32 device
+ * arrays, read on the device only, so a captured call follows their contents.
+ * A sequence may have no new tokens.  Rows before indptr[0], behind indptr[B]
+ * or at a negative position belong to no sequence: no call writes them, but
+ * for the zeros that persona_paged_attention gives the last kind.
+ * A position behind the page table or a page outside [0, num_pages) raises
+ * PERSONA_DEV_ERR_PAGE; write and read then leave the row alone, attention
+ * takes zeros in its place.  indptr must not decrease and must end within
+ * `rows`; a sequence that breaks this raises PERSONA_DEV_ERR_SEGMENT in
+ * attention and verification and is left out.
+ *
+ * k and v pages are [num_pages, Hkv, page_size, D], D 64 or 128, any page
+ * size, unit inner stride, the same other strides for both (in elements,
+ * multiples of 16 bytes).  PERSONA_PAGES_16BIT: the activations' own type.
+ * PERSONA_PAGES_E4M3: 8-bit codes and one fp32 scale per page, head and
+ * position (unit position stride): value = code * scale.                    */
+#define PERSONA_PAGES_16BIT 0
+#define PERSONA_PAGES_E4M3 1
+typedef struct persona_paged_cache {
+  void* k;
+  void* v;
+  float* k_scale; /* NULL for 16-bit pages */
+  float* v_scale;
+  int64_t page_stride, head_stride, pos_stride;
+  int64_t scale_page_stride, scale_head_stride;
+  int64_t num_pages, page_size, Hkv, D;
+  const int32_t* page_table;
+  int64_t table_stride, max_pages;
+  const int32_t* indptr;
+  const int32_t* lengths;
+  int64_t B;
+  int kind;
+} persona_paged_cache;
+/* A [rows, heads, D] activation: unit inner stride, 16-byte aligned, the other
+ * strides multiples of 8 elements (a slice of a fused q / k / v buffer).     */
+typedef struct persona_rows {
+  void* p;
+  int64_t row_stride, head_stride;
+} persona_rows;
+/* Rotary embedding (rotate-half, base theta) of every new row's q into q_out
+ * (q itself, or a buffer that does not overlap it) and of its k, and the write
+ * of k and v to the pages; k and v are only read.  Angles from 64-bit products
+ * (exact at far positions), the rotation in fp32, one rounding.  E4M3: scale =
+ * max(max |x| / 448, 2^-40) over a head of D values, codes rounded from the
+ * fp32 value / scale.  Values have to be finite for 8-bit pages: an infinity
+ * or NaN makes that token's head NaN.                                       */
+int persona_paged_rope_cache(const persona_paged_cache* cache, const persona_rows* q, const persona_rows* q_out,
+                             const persona_rows* k, const persona_rows* v, int64_t rows, int64_t Hq, float theta,
+                             int dtype, int32_t* dev_err, cudaStream_t stream);
+/* The way back: k and v of every row's position as 16-bit rows (codes times
+ * scale, one rounding).  With indptr[b + 1] - indptr[b] = lengths[b] a
+ * sequence's whole cache.                                                   */
+int persona_paged_cache_read(const persona_paged_cache* cache, const persona_rows* k, const persona_rows* v,
+                             int64_t rows, int dtype, int32_t* dev_err, cudaStream_t stream);
+/* Causal attention of the new rows over their sequence's pages:
+ * out[r, h] = softmax_j(scale q[r, h] . k[j, h / G]) v[j, h / G], G = Hq / Hkv,
+ * over j <= pos(r) and, with window > 0, j > pos(r) - window; zeros where that
+ * leaves nothing.  The new tokens' k and v are read from the pages, so write
+ * them first.  What lies in the pages behind a sequence's last position is
+ * never used; a NaN or infinity at a position of the sequence itself may reach
+ * every new row of that sequence.
+ * max_new: an upper bound of the new tokens of one sequence, for the choice of
+ * the kernel; a larger number of them is still computed correctly.
+ * workspace: persona_paged_attention_workspace_size(D) bytes for the current
+ * device, 16-byte aligned, any contents; calls that can overlap need one each. */
+size_t persona_paged_attention_workspace_size(int64_t D);
+int persona_paged_attention(const persona_paged_cache* cache, const persona_rows* q, const persona_rows* out,
+                            int64_t rows, int64_t Hq, float scale, int64_t window, int64_t max_new, int dtype,
+                            void* workspace, size_t workspace_bytes, int32_t* dev_err, cudaStream_t stream);
+
+/* ---- verification of drafted tokens -------------------------------------------
+ * Speculative sampling from given random numbers.  Row indptr[b] + i of target
+ * [rows, V] is the target's distribution behind the i-th fed token of sequence
+ * b; every row but a sequence's last one judges a drafted token, d_i =
+ * draft_tokens[row], drawn from row `row` of draft (NULL: a draft that was
+ * certain, q(d_i) = 1).  Drafts are kept while u_accept[row] q_i(d_i) <
+ * p_i(d_i).  The token behind the a kept ones is the first t with
+ * sum_{s <= t} w_s > u_sample[b] sum_s w_s, for w = max(p_a - q_a, 0) where a
+ * draft was rejected (p_a if that has no positive weight), else w = the last
+ * row of p; weights that are not positive, NaN among them, count as none; -1
+ * if there is none at all.  Sums and comparisons in 64 bits.
+ * tokens[row]: d_0 .. d_{a-1}, the drawn token, then -1; accepted[b] = a (0
+ * for an empty sequence).  Probabilities fp16, bf16 or fp32 (prob_type), both
+ * of one type, rows ld_* elements apart; they need not be normalised.       */
+#define PERSONA_VERIFY_MAX_VOCAB 2097152
+int persona_verify_draft(const void* target, int64_t ld_target, const void* draft, int64_t ld_draft, int prob_type,
+                         const int64_t* draft_tokens, const int32_t* indptr, const float* u_accept,
+                         const float* u_sample, int64_t* tokens, int32_t* accepted, int64_t rows, int64_t B, int64_t V,
+                         int32_t* dev_err, cudaStream_t stream);
 
 /* ---- warm-up GEMV ---------------------------------------------------------
  * y[n] = W[n, :] @ x (fp16, fp32 accumulate).  Replaces

@@ -71,6 +71,8 @@ std::string describe_error(int bits) {
   if (bits & PERSONA_DEV_ERR_TIMEOUT) os << " device wait timed out;";
   if (bits & PERSONA_DEV_ERR_SEGMENT) os << " invalid segment table;";
   if (bits & PERSONA_DEV_ERR_PLAN) os << " reused plan does not match the call;";
+  if (bits & PERSONA_DEV_ERR_PAGE) os << " page or position outside the paged cache;";
+  if (bits & PERSONA_DEV_ERR_TOKEN) os << " drafted token outside the vocabulary;";
   return os.str();
 }
 
@@ -741,6 +743,190 @@ void nf4_linear_add_op(const at::Tensor& x, at::TensorList packed, at::TensorLis
 }
 }  // namespace
 
+namespace {
+// ------------------------------------------- paged cache, draft checks ----
+void check_index(const at::Tensor& t, int64_t dim, const at::Tensor& like, const char* op, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == dim && (t.numel() == 0 || t.stride(dim - 1) == 1),
+              op, ": ", name, " must be a CUDA int32 tensor with ", dim, " dimension(s) and unit inner stride");
+  TORCH_CHECK(t.get_device() == like.get_device(), op, ": tensors on different devices");
+}
+
+// A [rows, heads, D] activation of the batch; sizes already checked.
+persona_rows rows_of(const at::Tensor& t, const at::Tensor& like, const char* op, const char* name, bool written) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 3 && t.stride(2) == 1, op, ": ", name,
+              " must be a CUDA [rows, heads, D] tensor with unit inner stride");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), op, ": dtype mismatch");
+  TORCH_CHECK(t.get_device() == like.get_device(), op, ": tensors on different devices");
+  TORCH_CHECK(t.size(0) == like.size(0) && t.size(2) == like.size(2), op, ": ", name, " shape mismatch");
+  TORCH_CHECK(!written || ((t.size(0) <= 1 || t.stride(0) >= t.size(2)) && (t.size(1) <= 1 || t.stride(1) >= t.size(2))),
+              op, ": ", name, " is written and must not overlap itself");
+  return persona_rows{t.data_ptr(), t.size(0) <= 1 ? 0 : t.stride(0), t.size(1) <= 1 ? 0 : t.stride(1)};
+}
+
+persona_paged_cache cache_of(const at::Tensor& k_cache, const at::Tensor& v_cache, const c10::optional<at::Tensor>& k_scale,
+                             const c10::optional<at::Tensor>& v_scale, const at::Tensor& table, const at::Tensor& indptr,
+                             const at::Tensor& lengths, const at::Tensor& like, const char* op) {
+  TORCH_CHECK(k_cache.is_cuda() && v_cache.is_cuda() && k_cache.dim() == 4 && k_cache.stride(3) == 1, op,
+              ": caches must be CUDA [pages, kv heads, page size, D] tensors with unit inner stride");
+  TORCH_CHECK(v_cache.sizes() == k_cache.sizes() && v_cache.strides() == k_cache.strides() &&
+                  v_cache.scalar_type() == k_cache.scalar_type(),
+              op, ": k and v caches must have the same type, shape and strides");
+  TORCH_CHECK(k_cache.get_device() == like.get_device() && v_cache.get_device() == like.get_device(), op,
+              ": tensors on different devices");
+  TORCH_CHECK(k_cache.size(3) == like.size(2), op, ": cache head size mismatch");
+  TORCH_CHECK(like.size(2) == 64 || like.size(2) == 128, op, ": head size must be 64 or 128");
+  const bool e4m3 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(e4m3 || k_cache.scalar_type() == like.scalar_type(), op,
+              ": caches must have the activations' type or be float8_e4m3fn");
+  TORCH_CHECK(k_scale.has_value() == e4m3 && v_scale.has_value() == e4m3, op,
+              ": k_scale and v_scale go with float8_e4m3fn caches, and only with them");
+  persona_paged_cache c = {};
+  c.k = k_cache.data_ptr();
+  c.v = v_cache.data_ptr();
+  c.num_pages = k_cache.size(0);
+  c.Hkv = k_cache.size(1);
+  c.page_size = k_cache.size(2);
+  c.D = k_cache.size(3);
+  // the stride of a dimension of one is never used
+  c.page_stride = c.num_pages <= 1 ? 0 : k_cache.stride(0);
+  c.head_stride = c.Hkv <= 1 ? 0 : k_cache.stride(1);
+  c.pos_stride = c.page_size <= 1 ? c.D : k_cache.stride(2);
+  c.kind = e4m3 ? PERSONA_PAGES_E4M3 : PERSONA_PAGES_16BIT;
+  if (e4m3) {
+    for (const at::Tensor* t : {&*k_scale, &*v_scale}) {
+      TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat && t->dim() == 3 && t->size(0) == c.num_pages &&
+                      t->size(1) == c.Hkv && t->size(2) == c.page_size && (c.page_size <= 1 || t->stride(2) == 1) &&
+                      t->strides() == k_scale->strides() && t->get_device() == like.get_device(),
+                  op, ": scales must be float32 [pages, kv heads, page size] with unit inner stride, strides alike");
+    }
+    c.k_scale = k_scale->data_ptr<float>();
+    c.v_scale = v_scale->data_ptr<float>();
+    c.scale_page_stride = c.num_pages <= 1 ? 0 : k_scale->stride(0);
+    c.scale_head_stride = c.Hkv <= 1 ? 0 : k_scale->stride(1);
+  }
+  check_index(table, 2, like, op, "page_table");
+  check_index(indptr, 1, like, op, "indptr");
+  check_index(lengths, 1, like, op, "lengths");
+  c.B = lengths.size(0);
+  TORCH_CHECK(indptr.size(0) == c.B + 1 && table.size(0) == c.B, op,
+              ": indptr [B + 1], lengths [B] and page_table [B, max pages] do not agree");
+  c.page_table = table.data_ptr<int32_t>();
+  c.max_pages = table.size(1);
+  c.table_stride = c.B <= 1 ? c.max_pages : table.stride(0);
+  c.indptr = indptr.data_ptr<int32_t>();
+  c.lengths = lengths.data_ptr<int32_t>();
+  return c;
+}
+
+void paged_rope_cache_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& q_out,
+                         at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& page_table, const at::Tensor& indptr,
+                         const at::Tensor& lengths, double theta, const c10::optional<at::Tensor>& k_scale,
+                         const c10::optional<at::Tensor>& v_scale) {
+  const char* op = "paged_rope_cache";
+  const persona_rows qr = rows_of(q, q, op, "q", false), kr = rows_of(k, q, op, "k", false),
+                     vr = rows_of(v, q, op, "v", false), qo = rows_of(q_out, q, op, "q_out", true);
+  const int dt = dtype_code(q, op);
+  const persona_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale, page_table, indptr, lengths, q, op);
+  TORCH_CHECK(k.size(1) == c.Hkv && v.size(1) == c.Hkv && q_out.size(1) == q.size(1), op, ": head count mismatch");
+  const at::cuda::OptionalCUDAGuard guard(q.device());
+  const int dev = q.get_device();
+  raise_pending(dev, op);
+  if (q.size(0) == 0) return;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  check_status(persona_paged_rope_cache(&c, &qr, &qo, &kr, &vr, q.size(0), q.size(1), static_cast<float>(theta), dt,
+                                        error_word_device(dev), stream),
+               op);
+  after_launch(dev, op, stream);
+}
+
+void paged_cache_read_op(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& page_table,
+                         const at::Tensor& indptr, const at::Tensor& lengths, at::Tensor& k_out, at::Tensor& v_out,
+                         const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale) {
+  const char* op = "paged_cache_read";
+  const persona_rows kr = rows_of(k_out, k_out, op, "k_out", true), vr = rows_of(v_out, k_out, op, "v_out", true);
+  const int dt = dtype_code(k_out, op);
+  const persona_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale, page_table, indptr, lengths, k_out, op);
+  TORCH_CHECK(k_out.size(1) == c.Hkv && v_out.size(1) == c.Hkv, op, ": head count mismatch");
+  const at::cuda::OptionalCUDAGuard guard(k_out.device());
+  const int dev = k_out.get_device();
+  raise_pending(dev, op);
+  if (k_out.size(0) == 0) return;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  check_status(persona_paged_cache_read(&c, &kr, &vr, k_out.size(0), dt, error_word_device(dev), stream), op);
+  after_launch(dev, op, stream);
+}
+
+void paged_attention_op(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                        const at::Tensor& page_table, const at::Tensor& indptr, const at::Tensor& lengths, at::Tensor& out,
+                        double scale, int64_t window, int64_t max_new, const c10::optional<at::Tensor>& k_scale,
+                        const c10::optional<at::Tensor>& v_scale) {
+  const char* op = "paged_attention";
+  const persona_rows qr = rows_of(q, q, op, "q", false), orow = rows_of(out, q, op, "out", true);
+  const int dt = dtype_code(q, op);
+  const persona_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale, page_table, indptr, lengths, q, op);
+  TORCH_CHECK(out.size(1) == q.size(1) && c.Hkv > 0 && q.size(1) % c.Hkv == 0, op,
+              ": the heads of q and out must be a multiple of the kv heads");
+  TORCH_CHECK(window >= 0, op, ": window must not be negative (0: none)");
+  TORCH_CHECK(max_new >= 1, op, ": max_new must be positive");
+  const at::cuda::OptionalCUDAGuard guard(q.device());
+  const int dev = q.get_device();
+  raise_pending(dev, op);
+  if (q.size(0) == 0 || c.B == 0) return;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  // a buffer of this call's own (from the graph's pool under capture)
+  at::Tensor ws = at::empty({static_cast<int64_t>(persona_paged_attention_workspace_size(c.D))},
+                            q.options().dtype(at::kByte));
+  check_status(persona_paged_attention(&c, &qr, &orow, q.size(0), q.size(1), static_cast<float>(scale), window, max_new,
+                                       dt, ws.data_ptr(), ws.numel(), error_word_device(dev), stream),
+               op);
+  after_launch(dev, op, stream);
+}
+
+void verify_draft_op(const at::Tensor& target, const at::Tensor& draft_tokens, const c10::optional<at::Tensor>& draft,
+                     const at::Tensor& indptr, const at::Tensor& u_accept, const at::Tensor& u_sample,
+                     at::Tensor& tokens, at::Tensor& accepted) {
+  const char* op = "verify_draft";
+  TORCH_CHECK(target.is_cuda() && target.dim() == 2 && (target.size(1) <= 1 || target.stride(1) == 1), op,
+              ": target_probs must be a CUDA [rows, V] matrix with unit inner stride");
+  const int64_t rows = target.size(0), V = target.size(1);
+  const int type = target.scalar_type() == at::kFloat ? PERSONA_DTYPE_F32 : target.scalar_type() == at::kHalf
+                       ? PERSONA_DTYPE_F16 : PERSONA_DTYPE_BF16;
+  TORCH_CHECK(type != PERSONA_DTYPE_BF16 || target.scalar_type() == at::kBFloat16, op,
+              ": probabilities must be float32, float16 or bfloat16");
+  TORCH_CHECK(V >= 1 && V <= PERSONA_VERIFY_MAX_VOCAB, op, ": vocabulary of 1 to ", PERSONA_VERIFY_MAX_VOCAB, " tokens");
+  if (draft.has_value())
+    TORCH_CHECK(draft->is_cuda() && draft->scalar_type() == target.scalar_type() && draft->sizes() == target.sizes() &&
+                    (V <= 1 || draft->stride(1) == 1) && draft->get_device() == target.get_device(),
+                op, ": draft_probs must match target_probs");
+  check_index(indptr, 1, target, op, "indptr");
+  const int64_t B = indptr.size(0) - 1;
+  TORCH_CHECK(B >= 0, op, ": indptr must have B + 1 entries");
+  auto vec = [&](const at::Tensor& t, at::ScalarType ty, int64_t n, const char* name, const char* want) {
+    TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.dim() == 1 && t.scalar_type() == ty && t.size(0) == n &&
+                    t.get_device() == target.get_device(),
+                op, ": ", name, " must be a contiguous CUDA ", want);
+  };
+  vec(draft_tokens, at::kLong, rows, "draft_tokens", "int64 [rows] tensor");
+  vec(u_accept, at::kFloat, rows, "u_accept", "float32 [rows] tensor");
+  vec(u_sample, at::kFloat, B, "u_sample", "float32 [B] tensor");
+  vec(tokens, at::kLong, rows, "tokens", "int64 [rows] tensor");
+  vec(accepted, at::kInt, B, "accepted", "int32 [B] tensor");
+  const at::cuda::OptionalCUDAGuard guard(target.device());
+  const int dev = target.get_device();
+  raise_pending(dev, op);
+  if (B == 0) return;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  check_status(persona_verify_draft(target.data_ptr(), rows <= 1 ? V : target.stride(0),
+                                    draft.has_value() ? draft->data_ptr() : nullptr,
+                                    draft.has_value() && rows > 1 ? draft->stride(0) : V, type,
+                                    draft_tokens.data_ptr<int64_t>(), indptr.data_ptr<int32_t>(),
+                                    u_accept.data_ptr<float>(), u_sample.data_ptr<float>(), tokens.data_ptr<int64_t>(),
+                                    accepted.data_ptr<int32_t>(), rows, B, V, error_word_device(dev), stream),
+               op);
+  after_launch(dev, op, stream);
+}
+}  // namespace
+
 TORCH_LIBRARY(persona, m) {
   // Reference schemas, unchanged (csrc/bindings.cpp:19-23).
   m.def("bgmv_shrink(Tensor x, Tensor a_pool, Tensor slots, Tensor(a!) v) -> ()");
@@ -772,6 +958,16 @@ TORCH_LIBRARY(persona, m) {
   m.def("decode_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor len, Tensor(a!) out, float scale) -> ()");
   m.def("rope_decode_attention(Tensor(a!) q, Tensor(b!) k, Tensor v, Tensor(c!) k_cache, Tensor(d!) v_cache, "
         "Tensor pos, Tensor len, Tensor(e!) out, float theta, float scale) -> ()");
+  // q_out may be q itself: both carry the same alias set.
+  m.def("paged_rope_cache(Tensor(a!) q, Tensor k, Tensor v, Tensor(a!) q_out, Tensor(b!) k_cache, Tensor(c!) v_cache, "
+        "Tensor page_table, Tensor indptr, Tensor lengths, float theta, Tensor(d!)? k_scale=None, "
+        "Tensor(e!)? v_scale=None) -> ()");
+  m.def("paged_cache_read(Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor indptr, Tensor lengths, "
+        "Tensor(a!) k_out, Tensor(b!) v_out, Tensor? k_scale=None, Tensor? v_scale=None) -> ()");
+  m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor indptr, Tensor lengths, "
+        "Tensor(a!) out, float scale, int window, int max_new, Tensor? k_scale=None, Tensor? v_scale=None) -> ()");
+  m.def("verify_draft(Tensor target_probs, Tensor draft_tokens, Tensor? draft_probs, Tensor indptr, Tensor u_accept, "
+        "Tensor u_sample, Tensor(a!) tokens, Tensor(b!) accepted) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(persona, CUDA, m) {
@@ -785,6 +981,10 @@ TORCH_LIBRARY_IMPL(persona, CUDA, m) {
   m.impl("silu_mul", &silu_mul_op);
   m.impl("decode_attention", &decode_attention_op);
   m.impl("rope_decode_attention", &rope_decode_attention_op);
+  m.impl("paged_rope_cache", &paged_rope_cache_op);
+  m.impl("paged_cache_read", &paged_cache_read_op);
+  m.impl("paged_attention", &paged_attention_op);
+  m.impl("verify_draft", &verify_draft_op);
   m.impl("bgmv_shrink", &bgmv_shrink_cuda);
   m.impl("bgmv_expand", &bgmv_expand_cuda);
   m.impl("gemv_fp16", &persona::gemv_fp16_cuda);

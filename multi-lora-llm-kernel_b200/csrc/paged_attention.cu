@@ -1,0 +1,722 @@
+// Causal attention of each sequence's new tokens over its paged KV cache, for
+// few query rows per kv head: single tokens and drafted ones.
+//
+//   out[r, h] = sum_j p_j v[j, h / G],  p = softmax_j(scale q[r, h] . k[j, h / G])
+//
+// over the positions j <= pos(r) (and j > pos(r) - window).  At these sizes
+// the kernel is bound by the pages it has to read once.
+//
+// Work.  A tile is TR = 16 MT query rows (token, head of the group) that
+// share a kv head; a unit is 64 positions of one tile's keys.  The units of
+// all tiles lie in one line (sequence, tile, kv head, position), which is cut
+// into equal ranges, one per CTA, so lengths may differ as they like.  A
+// range that starts or ends inside a tile's units leaves a piece (running
+// maximum, sum and unnormalised output, fp32) that paged_combine_kernel
+// joins, always in the order of the positions.
+//
+// A CTA.  Four warps; warp w takes positions [16 w, 16 w + 16) of every unit
+// through a ring of its own shared memory filled with cp.async, so no warp
+// waits for another inside a piece: scores by mma.sync m16n8k16 (q fragments
+// in registers), one pass with a running maximum per row, and the
+// probabilities, rounded to 16 bits, go from the accumulators' layout
+// straight into the operand's for the second product.  The warps' results
+// are joined in shared memory at the end of a piece.
+//
+// 8-bit pages.  The codes become fp16 in registers, exactly, and the products
+// run in fp16 for either type of q (a bf16 row is first scaled by a power of
+// two into fp16's range).  The k scale multiplies the fp32 score.  The v scale
+// goes into the exponent: the running maximum is taken over x + log2(vs), so
+// that p vs is at most 1 whatever the scales' range, and the sum of p is
+// accumulated as (p vs) / vs.
+//
+// mma.sync, not tcgen05: a tile has 16 or 32 rows, an eighth or a quarter of
+// tcgen05's smallest M, and the tensor work per byte of pages is far below
+// what the warp-level product delivers.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "paged_common.cuh"
+
+namespace persona {
+namespace {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kPos = 16;              // positions of one warp step
+constexpr int kUnit = kPos * kWarps;  // positions of one unit
+constexpr float kNegInf = -INFINITY;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A sequence as the kernels see it.
+struct Seq {
+  int row0, n, len;  // first row, new tokens, cached positions (new ones among them)
+};
+__device__ __forceinline__ Seq load_seq(const PagedAttention& a, int b) {
+  Seq s;
+  const int r0 = a.c.indptr[b], r1 = a.c.indptr[b + 1];
+  const int64_t cap = static_cast<int64_t>(a.c.max_pages) * a.c.page_size;
+  const int len = a.c.lengths[b];
+  const bool bad = r0 < 0 || r1 < r0 || r1 > a.rows;
+  s.row0 = r0;
+  s.n = bad ? 0 : r1 - r0;
+  s.len = len < 0 ? 0 : len > cap ? static_cast<int>(cap) : len;
+  if (bad) raise_error(a.err, PERSONA_DEV_ERR_SEGMENT);
+  if (s.n > 0 && len > cap) raise_error(a.err, PERSONA_DEV_ERR_PAGE);
+  return s;
+}
+// Units of one tile (the same for all tiles of a sequence; a tile that ends
+// before the sequence does leaves its last ones empty) and the first one.
+__device__ __forceinline__ void seq_units(const Seq& s, int window, int TR, int G, int& tiles, int& first, int& per) {
+  tiles = (s.n * G + TR - 1) / TR;
+  const int ctx = s.len - s.n;
+  const int begin = window > 0 ? max(0, ctx + 1 - window) : 0;
+  first = begin / kUnit;
+  per = max(1, (s.len + kUnit - 1) / kUnit - first);
+}
+
+template <int TR, int D> struct Part {  // one piece: TR x D outputs, TR maxima, TR sums
+  static constexpr int kFloats = TR * D + 2 * TR;
+};
+
+// Position p of sequence b: its offset (elements) in the pages of head 0 and
+// of the scales.
+struct Pager {
+  const int32_t* row;  // the sequence's page table
+  int page_size, max_pages, num_pages;
+  int32_t* err;
+  __device__ __forceinline__ int page_of(int p, int& at) const {
+    const int pi = p / page_size;
+    at = p - pi * page_size;
+    const int pg = pi < max_pages ? row[pi] : -1;
+    if (pg < 0 || pg >= num_pages) {
+      raise_error(err, PERSONA_DEV_ERR_PAGE);
+      return -1;
+    }
+    return pg;
+  }
+};
+
+template <typename T, int D, int MT, bool kE4m3, int kStages>
+__global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_constant__ PagedAttention a) {
+  using MT16 = typename std::conditional<kE4m3, __half, T>::type;  // type of the products
+  constexpr int TR = 16 * MT;
+  constexpr int kElt = kE4m3 ? 1 : 2;
+  constexpr int kRowBytes = D * kElt;                  // one position in a ring slot
+  constexpr int kChunks = kRowBytes / 16;
+  constexpr int kHalf = kPos * kRowBytes;              // k (or v) of one warp step
+  constexpr int kSlot = 2 * kHalf + (kE4m3 ? 2 * kPos * 4 : 0);
+  constexpr int kSteps = D / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long s_scan[kWarps + 1];
+  __shared__ int s_b;
+  __shared__ long long s_off;
+  __shared__ float s_m[kWarps][TR], s_l[kWarps][TR];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int cta = blockIdx.x;
+  const int Hkv = a.c.Hkv, G = a.G;
+  pdl_wait();
+  pdl_launch();
+
+  // ---- this CTA's range of units ----
+  long long total = 0;
+  for (int b0 = 0; b0 < a.c.B; b0 += kThreads) {
+    long long u = 0;
+    if (b0 + tid < a.c.B) {
+      int tiles, first, per;
+      seq_units(load_seq(a, b0 + tid), a.window, TR, G, tiles, first, per);
+      u = static_cast<long long>(tiles) * per * Hkv;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    if (lane == 0) s_scan[warp] = u;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) total += s_scan[w];
+    __syncthreads();
+  }
+  if (tid == 0) a.desc[cta] = make_int4(0, 0, 0, 0);
+  // no more CTAs than units, so that every range has one
+  const int ctas = static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
+  if (cta >= ctas) return;
+  const long long u0 = total * cta / ctas, u1 = total * (cta + 1) / ctas;
+  {
+    long long run = 0;
+    for (int b0 = 0; b0 < a.c.B; b0 += kThreads) {
+      long long u = 0;
+      if (b0 + tid < a.c.B) {
+        int tiles, first, per;
+        seq_units(load_seq(a, b0 + tid), a.window, TR, G, tiles, first, per);
+        u = static_cast<long long>(tiles) * per * Hkv;
+      }
+      long long inc = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      if (lane == 31) s_scan[warp] = inc;
+      __syncthreads();
+      long long base = run;
+      for (int w = 0; w < warp; ++w) base += s_scan[w];
+      const long long lo = base + inc - u;
+      if (u0 >= lo && u0 < lo + u) {
+        s_b = b0 + tid;
+        s_off = u0 - lo;
+      }
+      for (int w = 0; w < kWarps; ++w) run += s_scan[w];
+      __syncthreads();
+    }
+  }
+  int b = s_b;
+  long long off = s_off;
+  long long left = u1 - u0;
+  bool first_piece = true;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * kSlot;
+
+  Seq seq = load_seq(a, b);
+  int tiles, kfirst, per;
+  seq_units(seq, a.window, TR, G, tiles, kfirst, per);
+  while (left > 0) {
+    while (off >= static_cast<long long>(tiles) * per * Hkv) {  // the next sequence with units
+      off -= static_cast<long long>(tiles) * per * Hkv;
+      if (++b >= a.c.B) return;  // the arrays changed under the call
+      seq = load_seq(a, b);
+      seq_units(seq, a.window, TR, G, tiles, kfirst, per);
+    }
+    const int item = static_cast<int>(off / per), k0 = static_cast<int>(off - static_cast<long long>(item) * per);
+    const int k1 = static_cast<int>(min(static_cast<long long>(per), k0 + left));
+    const int tile = item / Hkv, h = item - tile * Hkv;
+    const int ctx = seq.len - seq.n;
+    const int m0 = tile * TR, mrows = min(TR, seq.n * G - m0);
+    const int tok0 = m0 / G, tok1 = (m0 + mrows - 1) / G;  // first and last token of the tile
+    const int pend = max(0, min(seq.len, ctx + tok1 + 1));  // keys of the tile end here
+    const int pbegin = a.window > 0 ? max(0, ctx + tok0 + 1 - a.window) : 0;
+    // positions of the steps of this piece that have any key
+    const int p_lo = max((kfirst + k0) * kUnit, pbegin / kUnit * kUnit), p_hi = min((kfirst + k1) * kUnit, pend);
+    const int steps = p_hi > p_lo ? (p_hi - p_lo + kUnit - 1) / kUnit : 0;
+
+    // ---- loads ----
+    const Pager pager{a.c.table + b * a.c.table_stride, a.c.page_size, a.c.max_pages, a.c.num_pages, a.err};
+    const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + static_cast<int64_t>(h) * a.c.head_stride * kElt;
+    const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + static_cast<int64_t>(h) * a.c.head_stride * kElt;
+    const bool whole = a.c.page_size % kPos == 0;  // a step's positions share a page
+    auto load = [&](int s) {
+      const int p0 = p_lo + s * kUnit + warp * kPos;
+      const uint32_t dst = ring + (s % kStages) * kSlot;
+      int64_t base = 0, sbase = 0;
+      bool ok = false;
+      if (whole && p0 < pend) {
+        int at;
+        const int pg = pager.page_of(p0, at);
+        ok = pg >= 0;
+        base = ok ? pg * a.c.page_stride + at * a.c.pos_stride : 0;
+        if (kE4m3) sbase = ok ? pg * a.c.scale_page_stride + at : 0;
+      }
+      constexpr int kRowsPer = 32 / kChunks;
+      const int ch = lane % kChunks;
+#pragma unroll
+      for (int i = 0; i < kPos / kRowsPer; ++i) {
+        const int r = i * kRowsPer + lane / kChunks;
+        int64_t src;
+        bool live;
+        if (whole) {
+          live = ok && p0 + r < pend;
+          src = live ? base + r * a.c.pos_stride : 0;
+        } else {
+          int at, pg = -1;
+          if (p0 + r < pend) pg = pager.page_of(p0 + r, at);
+          live = pg >= 0;
+          src = live ? pg * a.c.page_stride + at * a.c.pos_stride : 0;
+        }
+        // 16-byte chunks are XORed by the row so that the fragment reads
+        // below touch every bank once (8-bit: k reads two rows of four
+        // chunks, v reads even rows of two chunks, per quarter warp)
+        const int ck = kE4m3 ? ch ^ ((r & 1) << 2) : ch ^ (r & 7);
+        const int cv = kE4m3 ? ch ^ (((r >> 1) & 3) << 1) : ch ^ (r & 7);
+        const int mask = kChunks - 1;
+        cp_async16(dst + r * kRowBytes + (ck & mask) * 16, kb + src * kElt + ch * 16, live);
+        cp_async16(dst + kHalf + r * kRowBytes + (cv & mask) * 16, vb + src * kElt + ch * 16, live);
+      }
+      if (kE4m3) {
+        const int r = lane & 15;
+        int64_t src = sbase + r;
+        bool live = ok && p0 + r < pend;
+        if (!whole) {
+          int at, pg = -1;
+          if (p0 + r < pend) pg = pager.page_of(p0 + r, at);
+          live = pg >= 0;
+          src = live ? pg * a.c.scale_page_stride + at : 0;
+        }
+        const float* sp = (lane < 16 ? a.c.k_scale : a.c.v_scale) + static_cast<int64_t>(h) * a.c.scale_head_stride;
+        cp_async4(dst + 2 * kHalf + (lane >> 4) * kPos * 4 + r * 4, sp + (live ? src : 0), live);
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      if (s < steps) load(s);
+      cp_commit();
+    }
+
+    // ---- q fragments ----
+    // 16-bit pages: the operand's own order of d.  8-bit pages: a lane reads
+    // 16 consecutive codes of k, [64 blk + 16 t, ...), so step (blk, s) takes
+    // d = 64 blk + 16 t + 4 s + {0, 1} and {2, 3} where the operand has
+    // k = 2 t + {0, 1} and 2 t + 8 + {0, 1}.
+    uint32_t qf[MT][kSteps][4];
+    float qmul[MT][2];
+    int hi_pos[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int m = mt * 16 + half * 8 + g;
+        const bool live = m < mrows;
+        const int mm = m0 + (live ? m : 0);
+        const int tok = mm / G, hg = mm - tok * G;
+        const T* qp = static_cast<const T*>(a.q.p) + static_cast<int64_t>(seq.row0 + tok) * a.q.row_stride +
+                      static_cast<int64_t>(h * G + hg) * a.q.head_stride;
+        hi_pos[mt][half] = live ? ctx + tok : -1;
+        qmul[mt][half] = a.scale_log2;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          if (!kE4m3) {
+            qf[mt][s][half] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * s + 2 * t) : 0u;
+            qf[mt][s][half + 2] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * s + 8 + 2 * t) : 0u;
+          } else {
+            const int d = 64 * (s / 4) + 16 * t + 4 * (s % 4);
+            const uint2 w = live ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0u, 0u);
+            qf[mt][s][half] = w.x;
+            qf[mt][s][half + 2] = w.y;
+          }
+        }
+        if (kE4m3 && !std::is_same<T, __half>::value) {
+          // bf16 row -> fp16: scaled by the power of two that brings its
+          // largest element into [1, 2); elements 2^-24 below that vanish
+          float mx = 0.f;
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float2 f = Cvt<T>::to2(qf[mt][s][half + 2 * x]);
+              mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          // exponent field of mx, kept where both powers are normal numbers
+          const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23), 2), 252);
+          const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+          qmul[mt][half] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float2 f = Cvt<T>::to2(qf[mt][s][half + 2 * x]);
+              qf[mt][s][half + 2 * x] = Mma<__half>::pack(f.x * down, f.y * down);
+            }
+        }
+      }
+
+    // ---- one pass over the piece's positions ----
+    float acc[MT][D / 8][4];
+    float m_run[MT][2], l_run[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[mt][i][x] = 0.f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        m_run[mt][x] = kNegInf;
+        l_run[mt][x] = 0.f;
+      }
+    }
+    const int full_hi = ctx + tok0;                                          // positions all rows see: <= this
+    const int full_lo = a.window > 0 ? ctx + tok1 - a.window + 1 : 0;       // and >= this
+    for (int s = 0; s < steps; ++s) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      if (s + kStages - 1 < steps) load(s + kStages - 1);
+      cp_commit();
+      const int p0 = p_lo + s * kUnit + warp * kPos;
+      if (p0 >= pend) continue;
+      const uint32_t slot = ring + (s % kStages) * kSlot;
+
+      float sc[MT][2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sc[mt][n][x] = 0.f;
+      if (!kE4m3) {
+        const int r = (lane & 7) + ((lane >> 4) << 3);  // matrices 0, 1: rows 0-7; 2, 3: rows 8-15
+        const uint32_t rowaddr = slot + r * kRowBytes;
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+          const int ch = (2 * ks + ((lane >> 3) & 1)) ^ (r & 7);
+          uint32_t kf[4];
+          ldsm_x4(rowaddr + (ch & (kChunks - 1)) * 16, kf);
+          const uint32_t b0[2] = {kf[0], kf[1]}, b1[2] = {kf[2], kf[3]};
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            Mma<MT16>::k16(sc[mt][0], qf[mt][ks], b0);
+            Mma<MT16>::k16(sc[mt][1], qf[mt][ks], b1);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int r = n * 8 + g;
+#pragma unroll
+          for (int blk = 0; blk < D / 64; ++blk) {
+            const uint4 w = lds128(slot + r * kRowBytes + (((4 * blk + t) ^ ((r & 1) << 2)) & (kChunks - 1)) * 16);
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              uint32_t bf[2];
+              e4m3x4_to_half(u[x], bf[0], bf[1]);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) Mma<MT16>::k16(sc[mt][n], qf[mt][4 * blk + x], bf);
+            }
+          }
+        }
+      }
+
+      // scores in the log2 domain, masked
+      float lv[2][2], rv[2][2];
+      if (kE4m3) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const uint32_t sa = slot + 2 * kHalf + (8 * n + 2 * t) * 4;
+          float ks2[2] = {__uint_as_float(lds32(sa)), __uint_as_float(lds32(sa + 4))};
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float vs = fmaxf(__uint_as_float(lds32(sa + kPos * 4 + 4 * x)), 8.673617379884035e-19f);  // 2^-60
+            lv[n][x] = __log2f(vs);
+            rv[n][x] = __frcp_rn(vs);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              sc[mt][n][x] *= ks2[x];
+              sc[mt][n][2 + x] *= ks2[x];
+            }
+          }
+        }
+      }
+      const bool need_mask = p0 + kPos - 1 > full_hi || p0 < full_lo;
+      bool grow = false;
+      float m_new[MT][2];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float mx = kNegInf;
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              float& v = sc[mt][n][2 * half + x];
+              v = kE4m3 ? fmaf(v, qmul[mt][half], lv[n][x]) : v * a.scale_log2;
+              if (need_mask) {
+                const int p = p0 + 8 * n + 2 * t + x;
+                const bool seen = p <= hi_pos[mt][half] && (a.window == 0 || p > hi_pos[mt][half] - a.window);
+                v = seen ? v : kNegInf;
+              }
+              mx = fmaxf(mx, v);
+            }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          m_new[mt][half] = fmaxf(m_run[mt][half], mx);
+          grow |= m_new[mt][half] > m_run[mt][half];
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          float f[2];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            // a row without a key yet has nothing to rescale
+            f[half] = m_new[mt][half] > m_run[mt][half] ? exp2_approx(m_run[mt][half] - m_new[mt][half]) : 1.f;
+            l_run[mt][half] *= f[half];
+            m_run[mt][half] = m_new[mt][half];
+          }
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            acc[mt][i][0] *= f[0];
+            acc[mt][i][1] *= f[0];
+            acc[mt][i][2] *= f[1];
+            acc[mt][i][3] *= f[1];
+          }
+        }
+      }
+      uint32_t pf[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float mm = m_run[mt][half] == kNegInf ? 0.f : m_run[mt][half];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const float e0 = exp2_approx(sc[mt][n][2 * half] - mm), e1 = exp2_approx(sc[mt][n][2 * half + 1] - mm);
+            l_run[mt][half] += kE4m3 ? fmaf(e0, rv[n][0], e1 * rv[n][1]) : e0 + e1;
+            // 16 bits for the product: half a step, 2^-11 (fp16) or 2^-9
+            // (bf16) of a probability, the precision of v itself
+            pf[mt][half + 2 * n] = Mma<MT16>::pack(e0, e1);
+          }
+        }
+
+      // ---- P V ----
+      const uint32_t vslot = slot + kHalf;
+      if (!kE4m3) {
+        const int r = (lane & 7) + (((lane >> 3) & 1) << 3);  // matrices 0, 2: positions 0-7; 1, 3: 8-15
+        const uint32_t rowaddr = vslot + r * kRowBytes;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const int ch = (2 * i + (lane >> 4)) ^ (r & 7);
+          uint32_t vf[4];
+          ldsm_x4_trans(rowaddr + (ch & (kChunks - 1)) * 16, vf);
+          const uint32_t b0[2] = {vf[0], vf[1]}, b1[2] = {vf[2], vf[3]};
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            Mma<MT16>::k16(acc[mt][2 * i], pf[mt], b0);
+            Mma<MT16>::k16(acc[mt][2 * i + 1], pf[mt], b1);
+          }
+        }
+      } else {
+        // A lane holds D / 8 consecutive dims, [g D / 8, ...), of positions
+        // 2 t, 2 t + 1, 2 t + 8, 2 t + 9: column g of n-tile i is dim g D / 8 + i.
+        constexpr int kW = D / 32;  // words of a lane and position
+        uint32_t w[4][kW];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int r = 2 * t + (x & 1) + 8 * (x >> 1);
+          if (D == 128) {
+            const uint4 v = lds128(vslot + r * kRowBytes + ((g ^ (((r >> 1) & 3) << 1)) & (kChunks - 1)) * 16);
+            w[x][0] = v.x;
+            w[x][1] = v.y;
+            w[x][kW - 2] = v.z;
+            w[x][kW - 1] = v.w;
+          } else {
+            const uint32_t ad = vslot + r * kRowBytes + (((g >> 1) ^ (((r >> 1) & 3) << 1)) & (kChunks - 1)) * 16 + (g & 1) * 8;
+            w[x][0] = lds32(ad);
+            w[x][1] = lds32(ad + 4);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kW; ++j) {
+          uint32_t bfr[4][2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            // bytes (p, p + 1) side by side, then two conversions of pairs
+            const uint32_t ab = __byte_perm(w[2 * x][j], w[2 * x + 1][j], 0x5140);
+            const uint32_t cd = __byte_perm(w[2 * x][j], w[2 * x + 1][j], 0x7362);
+            e4m3x4_to_half(ab, bfr[0][x], bfr[1][x]);
+            e4m3x4_to_half(cd, bfr[2][x], bfr[3][x]);
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) Mma<MT16>::k16(acc[mt][4 * j + x], pf[mt], bfr[x]);
+        }
+      }
+      __syncwarp();
+    }
+    cp_wait<0>();
+    __syncthreads();  // every warp is done with the ring, which now takes the warps' results
+
+    // ---- join the warps ----
+    float* accs = reinterpret_cast<float*>(smem);  // [kWarps][TR][D]
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int m = mt * 16 + half * 8 + g;
+        float l = l_run[mt][half];
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (t == 0) {
+          s_m[warp][m] = m_run[mt][half];
+          s_l[warp][m] = l;
+        }
+        float* dst = accs + (warp * TR + m) * D;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const float x0 = acc[mt][i][2 * half], x1 = acc[mt][i][2 * half + 1];
+          if (!kE4m3) {
+            *reinterpret_cast<float2*>(dst + 8 * i + 2 * t) = make_float2(x0, x1);
+          } else {
+            dst[2 * t * (D / 8) + i] = x0;
+            dst[(2 * t + 1) * (D / 8) + i] = x1;
+          }
+        }
+      }
+    __syncthreads();
+    const bool complete = k0 == 0 && k1 == per;
+    float* part = a.part + static_cast<int64_t>(2 * cta + (first_piece ? 0 : 1)) * Part<TR, D>::kFloats;
+    for (int i = tid; i < mrows * (D / 8); i += kThreads) {
+      const int m = i / (D / 8), d = (i % (D / 8)) * 8;
+      float mx = kNegInf;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_m[w][m]);
+      float l = 0.f, o[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) o[x] = 0.f;
+      if (mx != kNegInf) {
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = exp2_approx(s_m[w][m] - mx);
+          l = fmaf(f, s_l[w][m], l);
+          const float* src = accs + (w * TR + m) * D + d;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) o[x] = fmaf(f, src[x], o[x]);
+        }
+      }
+      if (complete) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const int mm = m0 + m, tok = mm / G;
+        T* dst = static_cast<T*>(a.out.p) + static_cast<int64_t>(seq.row0 + tok) * a.out.row_stride +
+                 static_cast<int64_t>(h * G + mm - tok * G) * a.out.head_stride + d;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(Mma<T>::pack(o[0] * inv, o[1] * inv), Mma<T>::pack(o[2] * inv, o[3] * inv),
+                                                    Mma<T>::pack(o[4] * inv, o[5] * inv), Mma<T>::pack(o[6] * inv, o[7] * inv));
+      } else {
+        float4* dst = reinterpret_cast<float4*>(part + m * D + d);
+        dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+        dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+        if (d == 0) {
+          part[TR * D + m] = mx;
+          part[TR * D + TR + m] = l;
+        }
+      }
+    }
+    if (tid == 0 && k0 == 0 && k1 < per) {
+      // the first piece of a tile that goes on in later CTAs: the last of
+      // them is the one whose range holds the tile's last unit
+      const long long end = u1 - left - k0 + per - 1;
+      long long c = end * ctas / total;
+      while (total * (c + 1) / ctas <= end) ++c;
+      while (total * c / ctas > end) --c;
+      a.desc[cta] = make_int4(b, item, static_cast<int>(c), first_piece ? 1 : 2);
+    }
+    __syncthreads();  // the ring is free again
+    off += k1 - k0;
+    left -= k1 - k0;
+    first_piece = false;
+  }
+}
+
+// Joins the pieces of one cut tile: CTA c looks after the tile whose first
+// piece CTA c of the attention left.  A warp per row, pieces in order.
+template <typename T, int D, int TR>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PagedAttention a) {
+  pdl_wait();
+  pdl_launch();
+  const int4 d = a.desc[blockIdx.x];
+  if (d.w == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = d.x, tile = d.y / a.c.Hkv, h = d.y % a.c.Hkv, first = blockIdx.x, pieces = d.z - first + 1;
+  const Seq seq = load_seq(a, b);
+  const int m0 = tile * TR, mrows = min(TR, seq.n * a.G - m0);
+  constexpr int kF = Part<TR, D>::kFloats, kV = D / 32;
+  const float* p0 = a.part + static_cast<int64_t>(2 * first + d.w - 1) * kF;
+  // piece i > 0 is the first piece of CTA first + i
+  auto piece = [&](int i) { return i == 0 ? p0 : a.part + static_cast<int64_t>(2 * (first + i)) * kF; };
+  for (int m = warp; m < mrows; m += 8) {
+    float mx = kNegInf;
+    for (int i = lane; i < pieces; i += 32) mx = fmaxf(mx, piece(i)[TR * D + m]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    float l = 0.f, o[kV];
+#pragma unroll
+    for (int x = 0; x < kV; ++x) o[x] = 0.f;
+    if (mx != kNegInf) {
+#pragma unroll 4
+      for (int i = 0; i < pieces; ++i) {
+        const float* p = piece(i);
+        const float f = exp2_approx(p[TR * D + m] - mx);
+        l = fmaf(f, p[TR * D + TR + m], l);
+#pragma unroll
+        for (int x = 0; x < kV; ++x) o[x] = fmaf(f, p[m * D + lane * kV + x], o[x]);
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int mm = m0 + m, tok = mm / a.G;
+    T* dst = static_cast<T*>(a.out.p) + static_cast<int64_t>(seq.row0 + tok) * a.out.row_stride +
+             static_cast<int64_t>(h * a.G + mm - tok * a.G) * a.out.head_stride + lane * kV;
+#pragma unroll
+    for (int x = 0; x < kV; x += 2)
+      *reinterpret_cast<uint32_t*>(dst + x) = Mma<T>::pack(o[x] * inv, o[x + 1] * inv);
+  }
+}
+
+constexpr int kCtasPerSm = 2;
+
+int sm_count() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return n;
+}
+
+template <typename T, int D, int MT, bool kE4m3>
+cudaError_t attention_launch(const PagedAttention& a, cudaStream_t st) {
+  // ring slots: 3 x 8 KB (16-bit) or 6 x 4.1 KB (8-bit) per warp at D = 128,
+  // 96 KB per CTA, two CTAs per SM
+  constexpr int kStages = (kE4m3 ? 6 : 3) * (128 / D);
+  constexpr int kSlot = 2 * kPos * D * (kE4m3 ? 1 : 2) + (kE4m3 ? 2 * kPos * 4 : 0);
+  constexpr int kRing = kWarps * kStages * kSlot, kJoin = kWarps * 16 * MT * D * 4;
+  constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  auto k = paged_attention_kernel<T, D, MT, kE4m3, kStages>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  const int ctas = kCtasPerSm * sm_count();
+  e = launch_paged(k, dim3(ctas), dim3(kThreads), kSmem, 1, st, a);
+  if (e != cudaSuccess) return e;
+  return launch_paged(paged_combine_kernel<T, D, 16 * MT>, dim3(ctas), dim3(256), 0, 1, st, a);
+}
+template <typename T, int D, int MT>
+cudaError_t attention_pages(const PagedAttention& a, cudaStream_t st) {
+  return a.c.k_scale != nullptr ? attention_launch<T, D, MT, true>(a, st) : attention_launch<T, D, MT, false>(a, st);
+}
+template <typename T, int D>
+cudaError_t attention_rows(const PagedAttention& a, int max_new, cudaStream_t st) {
+  return static_cast<int64_t>(max_new) * a.G <= 16 ? attention_pages<T, D, 1>(a, st) : attention_pages<T, D, 2>(a, st);
+}
+template <typename T>
+cudaError_t attention_dim(const PagedAttention& a, int max_new, cudaStream_t st) {
+  return a.c.D == 128 ? attention_rows<T, 128>(a, max_new, st) : attention_rows<T, 64>(a, max_new, st);
+}
+
+}  // namespace
+
+size_t paged_attention_ws_bytes(int D) {
+  const size_t ctas = static_cast<size_t>(kCtasPerSm) * sm_count();
+  return ctas * sizeof(int4) + ctas * 2 * (32 * static_cast<size_t>(D) + 64) * sizeof(float);
+}
+
+cudaError_t launch_paged_attention(PagedAttention a, int dtype, int max_new, void* workspace, cudaStream_t st) {
+  const size_t ctas = static_cast<size_t>(kCtasPerSm) * sm_count();
+  a.desc = static_cast<int4*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + ctas * sizeof(int4));
+  return dtype == PERSONA_DTYPE_BF16 ? attention_dim<__nv_bfloat16>(a, max_new, st) : attention_dim<__half>(a, max_new, st);
+}
+
+}  // namespace persona

@@ -1,0 +1,147 @@
+// extern "C" entry points of the paged KV cache operators and of the draft
+// verification: argument checks, then one enqueue.  Nothing here synchronises
+// with the device or allocates device memory.
+#include <cmath>
+
+#include "paged_args.h"
+#include "persona_bgmv.h"
+
+namespace persona {
+namespace {
+
+constexpr int64_t kI32Max = 2147483647;
+constexpr int64_t kMaxHeads = 1024;
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+int status(cudaError_t e) { return e == cudaSuccess ? PERSONA_OK : PERSONA_ERR_CUDA; }
+
+int check_cache(const persona_paged_cache* c, int dtype, PagedCache& out) {
+  if (c == nullptr) return PERSONA_ERR_INVALID_ARG;
+  if (dtype != PERSONA_DTYPE_F16 && dtype != PERSONA_DTYPE_BF16) return PERSONA_ERR_DTYPE;
+  const bool e4m3 = c->kind == PERSONA_PAGES_E4M3;
+  if (!e4m3 && c->kind != PERSONA_PAGES_16BIT) return PERSONA_ERR_DTYPE;
+  if (c->k == nullptr || c->v == nullptr || c->page_table == nullptr || c->indptr == nullptr || c->lengths == nullptr)
+    return PERSONA_ERR_INVALID_ARG;
+  if (e4m3 != (c->k_scale != nullptr) || e4m3 != (c->v_scale != nullptr)) return PERSONA_ERR_INVALID_ARG;
+  if ((c->D != 64 && c->D != 128) || c->Hkv <= 0 || c->Hkv > kMaxHeads || c->num_pages <= 0 || c->num_pages > kI32Max ||
+      c->page_size <= 0 || c->page_size > kI32Max || c->max_pages < 0 || c->max_pages > kI32Max || c->B < 0 ||
+      c->B > kI32Max / 2 || c->table_stride < c->max_pages)
+    return PERSONA_ERR_SHAPE;
+  const int64_t unit = e4m3 ? 16 : 8;  // elements of 16 bytes
+  if (c->page_stride < 0 || c->head_stride < 0 || c->pos_stride < c->D) return PERSONA_ERR_SHAPE;
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->page_stride % unit || c->head_stride % unit || c->pos_stride % unit)
+    return PERSONA_ERR_ALIGNMENT;
+  if (e4m3 && (c->scale_page_stride < 0 || c->scale_head_stride < 0)) return PERSONA_ERR_SHAPE;
+  if (!aligned(c->k_scale, 4) || !aligned(c->v_scale, 4) || !aligned(c->page_table, 4) || !aligned(c->indptr, 4) ||
+      !aligned(c->lengths, 4))
+    return PERSONA_ERR_ALIGNMENT;
+  out = PagedCache{c->k, c->v, c->k_scale, c->v_scale, c->page_stride, c->head_stride, c->pos_stride,
+                   c->scale_page_stride, c->scale_head_stride, c->page_table, c->table_stride, c->indptr, c->lengths,
+                   static_cast<int>(c->num_pages), static_cast<int>(c->page_size), static_cast<int>(c->max_pages),
+                   static_cast<int>(c->Hkv), static_cast<int>(c->D), static_cast<int>(c->B)};
+  return PERSONA_OK;
+}
+
+int check_rows(const persona_rows* r, PagedRows& out) {
+  if (r == nullptr || r->p == nullptr) return PERSONA_ERR_INVALID_ARG;
+  if (r->row_stride < 0 || r->head_stride < 0) return PERSONA_ERR_SHAPE;
+  if (!aligned(r->p, 16) || r->row_stride % 8 || r->head_stride % 8) return PERSONA_ERR_ALIGNMENT;
+  out = PagedRows{r->p, r->row_stride, r->head_stride};
+  return PERSONA_OK;
+}
+
+}  // namespace
+}  // namespace persona
+
+using namespace persona;
+
+#define PERSONA_TRY(x)                      \
+  do {                                      \
+    const int st_ = (x);                    \
+    if (st_ != PERSONA_OK) return st_;      \
+  } while (0)
+
+extern "C" {
+
+int persona_paged_rope_cache(const persona_paged_cache* cache, const persona_rows* q, const persona_rows* q_out,
+                             const persona_rows* k, const persona_rows* v, int64_t rows, int64_t Hq, float theta,
+                             int dtype, int32_t* dev_err, cudaStream_t stream) {
+  PagedWrite a;
+  PERSONA_TRY(check_cache(cache, dtype, a.c));
+  if (rows < 0 || rows > kI32Max || Hq <= 0 || Hq > kMaxHeads || !(theta > 1.f) || !std::isfinite(theta))
+    return PERSONA_ERR_SHAPE;
+  if (rows == 0 || cache->B == 0) return PERSONA_OK;
+  PERSONA_TRY(check_rows(q, a.q));
+  PERSONA_TRY(check_rows(q_out, a.q_out));
+  PERSONA_TRY(check_rows(k, a.k));
+  PERSONA_TRY(check_rows(v, a.v));
+  a.rows = static_cast<int>(rows);
+  a.Hq = static_cast<int>(Hq);
+  const int D = a.c.D;
+  const double two_pi = 6.283185307179586476925;
+  for (int j = 0; j < 64; ++j)
+    a.turns[j] = j < D / 2 ? std::pow(static_cast<double>(theta), -2.0 * j / D) / two_pi : 0.0;
+  return status(launch_paged_write(a, dtype, dev_err, stream));
+}
+
+int persona_paged_cache_read(const persona_paged_cache* cache, const persona_rows* k, const persona_rows* v,
+                             int64_t rows, int dtype, int32_t* dev_err, cudaStream_t stream) {
+  PagedRead a;
+  PERSONA_TRY(check_cache(cache, dtype, a.c));
+  if (rows < 0 || rows > kI32Max) return PERSONA_ERR_SHAPE;
+  if (rows == 0 || cache->B == 0) return PERSONA_OK;
+  PERSONA_TRY(check_rows(k, a.k));
+  PERSONA_TRY(check_rows(v, a.v));
+  a.rows = static_cast<int>(rows);
+  return status(launch_paged_read(a, dtype, dev_err, stream));
+}
+
+size_t persona_paged_attention_workspace_size(int64_t D) {
+  return D == 64 || D == 128 ? paged_attention_ws_bytes(static_cast<int>(D)) : 0;
+}
+
+int persona_paged_attention(const persona_paged_cache* cache, const persona_rows* q, const persona_rows* out,
+                            int64_t rows, int64_t Hq, float scale, int64_t window, int64_t max_new, int dtype,
+                            void* workspace, size_t workspace_bytes, int32_t* dev_err, cudaStream_t stream) {
+  PagedAttention a;
+  PERSONA_TRY(check_cache(cache, dtype, a.c));
+  if (rows < 0 || Hq <= 0 || Hq > kMaxHeads || Hq % cache->Hkv || rows > kI32Max / Hq || window < 0 || max_new < 1 ||
+      !std::isfinite(scale))
+    return PERSONA_ERR_SHAPE;
+  // positions of a sequence are 32-bit numbers
+  if (cache->max_pages > kI32Max / cache->page_size - 64 / cache->page_size - 1) return PERSONA_ERR_SHAPE;
+  if (rows == 0 || cache->B == 0) return PERSONA_OK;
+  PERSONA_TRY(check_rows(q, a.q));
+  PERSONA_TRY(check_rows(out, a.out));
+  if (workspace == nullptr || workspace_bytes < paged_attention_ws_bytes(a.c.D)) return PERSONA_ERR_WORKSPACE;
+  if (!aligned(workspace, 16)) return PERSONA_ERR_ALIGNMENT;
+  a.rows = static_cast<int>(rows);
+  a.G = static_cast<int>(Hq / cache->Hkv);
+  a.window = window > kI32Max ? 0 : static_cast<int>(window);  // wider than any position
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.err = dev_err;
+  return status(launch_paged_attention(a, dtype, static_cast<int>(max_new > rows ? rows : max_new), workspace, stream));
+}
+
+int persona_verify_draft(const void* target, int64_t ld_target, const void* draft, int64_t ld_draft, int prob_type,
+                         const int64_t* draft_tokens, const int32_t* indptr, const float* u_accept,
+                         const float* u_sample, int64_t* tokens, int32_t* accepted, int64_t rows, int64_t B, int64_t V,
+                         int32_t* dev_err, cudaStream_t stream) {
+  if (prob_type < PERSONA_DTYPE_F16 || prob_type > PERSONA_DTYPE_F32) return PERSONA_ERR_DTYPE;
+  if (rows < 0 || rows > kI32Max || B < 0 || B > kI32Max / 8 || V <= 0 || V > PERSONA_VERIFY_MAX_VOCAB || ld_target < V ||
+      (draft != nullptr && ld_draft < V))
+    return PERSONA_ERR_SHAPE;
+  if (B == 0) return PERSONA_OK;
+  if (indptr == nullptr || u_sample == nullptr || accepted == nullptr) return PERSONA_ERR_INVALID_ARG;
+  if (rows > 0 && (target == nullptr || draft_tokens == nullptr || u_accept == nullptr || tokens == nullptr))
+    return PERSONA_ERR_INVALID_ARG;
+  const uintptr_t e = prob_type == PERSONA_DTYPE_F32 ? 4 : 2;
+  if (!aligned(target, e) || !aligned(draft, e) || !aligned(draft_tokens, 8) || !aligned(tokens, 8) || !aligned(indptr, 4) ||
+      !aligned(u_accept, 4) || !aligned(u_sample, 4) || !aligned(accepted, 4))
+    return PERSONA_ERR_ALIGNMENT;
+  const VerifyDraft a{target, draft, ld_target, ld_draft, draft_tokens, indptr, u_accept, u_sample, tokens, accepted,
+                      static_cast<int>(rows), static_cast<int>(B), static_cast<int>(V), dev_err};
+  return status(launch_verify_draft(a, prob_type, stream));
+}
+
+}  // extern "C"

@@ -21,6 +21,10 @@ New in this build:
 * ``bgmv_plan`` -- groups a batch's rows by adapter slot once on the device;
   pass the result as ``plan=`` to every shrink/expand/fused call that uses
   the same slots (a decode step's 7 projections x 32 layers share one).
+* ``paged_rope_cache`` / ``paged_cache_read`` / ``paged_attention`` -- a
+  ragged batch of new tokens (single ones, drafted ones, prompt chunks) over a
+  paged KV cache with 16-bit or e4m3 pages; ``verify_draft`` -- acceptance of
+  drafted tokens.
 * ``check_errors`` -- out-of-range slots are detected on the device (no
   per-row host sync); the next op on that device, or this function, raises.
 """
@@ -180,6 +184,10 @@ def check_errors(device: Optional[torch.device] = None, synchronize: bool = True
             what.append("invalid segment table")
         if bits & 8:
             what.append("reused plan does not match the call")
+        if bits & 16:
+            what.append("page or position outside the paged cache")
+        if bits & 32:
+            what.append("drafted token outside the vocabulary")
         raise RuntimeError(f"persona: device error 0x{bits:x}: {', '.join(what)}")
 
 
@@ -230,3 +238,76 @@ def bgmv_lora_delta_multi(xs, a_pools, b_pools, slots: torch.Tensor, deltas):
     _require_cuda("bgmv_lora_delta_multi", slots, *xs, *a_pools, *b_pools, *deltas)
     torch.ops.persona.bgmv_lora_delta_multi(list(xs), list(a_pools), list(b_pools), slots, list(deltas))
     return deltas
+
+
+# ---- paged KV cache and drafted tokens ---------------------------------------
+def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     page_table: torch.Tensor, indptr: torch.Tensor, lengths: torch.Tensor, theta: float,
+                     q_out: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
+                     v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary embedding of a ragged batch of new tokens and the write of their
+    k and v to a paged cache; returns the rotated q (``q_out``, by default
+    ``q`` itself; k and v are left as they are).
+
+    ``q`` [rows, Hq, D], ``k`` / ``v`` [rows, Hkv, D] (fp16 or bf16, D 64 or
+    128, views with unit inner stride).  Rows ``indptr[b]`` to ``indptr[b+1]``
+    are sequence b's new tokens, at its last positions: the last one is at
+    ``lengths[b] - 1``.  Caches [pages, Hkv, page size, D]; position p of
+    sequence b is in page ``page_table[b, p // page_size]``.  Caches of
+    ``float8_e4m3fn`` take fp32 scales [pages, Hkv, page size]: one per token
+    and head, ``max|x| / 448``.  Rows of no sequence are left alone."""
+    q_out = q if q_out is None else q_out
+    _require_cuda("paged_rope_cache", q, k, v, k_cache, v_cache, page_table, indptr, lengths, q_out)
+    torch.ops.persona.paged_rope_cache(q, k, v, q_out, k_cache, v_cache, page_table, indptr, lengths, theta, k_scale,
+                                       v_scale)
+    return q_out
+
+
+def paged_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, indptr: torch.Tensor,
+                     lengths: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor,
+                     k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
+    """k and v of the last ``indptr[b+1] - indptr[b]`` positions of each
+    sequence, out of the pages into ``k_out`` / ``v_out`` [rows, Hkv, D]
+    (e4m3 pages: code times scale)."""
+    _require_cuda("paged_cache_read", k_cache, v_cache, page_table, indptr, lengths, k_out, v_out)
+    torch.ops.persona.paged_cache_read(k_cache, v_cache, page_table, indptr, lengths, k_out, v_out, k_scale, v_scale)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    indptr: torch.Tensor, lengths: torch.Tensor, out: torch.Tensor, scale: float, window: int = 0,
+                    max_new: Optional[int] = None, k_scale: Optional[torch.Tensor] = None,
+                    v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of each sequence's new tokens over its pages, theirs
+    included (write them first); with ``window`` over the last ``window``
+    positions only.  Layouts as in ``paged_rope_cache``; ``out`` like ``q``.
+    A row that sees no position gives zeros.
+
+    ``max_new``: an upper bound of the new tokens of one sequence, which
+    chooses the kernel (default: what ``rows`` allows if every sequence has
+    a token); it never changes what is computed."""
+    _require_cuda("paged_attention", q, k_cache, v_cache, page_table, indptr, lengths, out)
+    if max_new is None:
+        max_new = max(1, q.shape[0] - lengths.shape[0] + 1)
+    torch.ops.persona.paged_attention(q, k_cache, v_cache, page_table, indptr, lengths, out, scale, window, max_new,
+                                      k_scale, v_scale)
+    return out
+
+
+def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_probs: Optional[torch.Tensor],
+                 indptr: torch.Tensor, u_accept: torch.Tensor, u_sample: torch.Tensor, tokens: torch.Tensor,
+                 accepted: torch.Tensor):
+    """Speculative sampling from given uniform numbers; returns ``tokens`` and
+    ``accepted``.
+
+    Row ``indptr[b] + i`` of ``target_probs`` [rows, V] is the target's
+    distribution behind the i-th token fed for sequence b; all rows but the
+    sequence's last judge the drafted token ``draft_tokens[row]``, drawn from
+    ``draft_probs[row]`` (None: a draft without probabilities, certain of its
+    token).  Drafts are kept while ``u_accept[row] * q < p``.  Then one token
+    is drawn with ``u_sample[b]``: from ``max(p - q, 0)`` where a draft was
+    rejected, else from the last row.  ``tokens`` [rows] int64: the kept
+    drafts, the drawn token, then -1; ``accepted`` [B] int32: how many."""
+    _require_cuda("verify_draft", target_probs, draft_tokens, indptr, u_accept, u_sample, tokens, accepted)
+    torch.ops.persona.verify_draft(target_probs, draft_tokens, draft_probs, indptr, u_accept, u_sample, tokens,
+                                   accepted)
+    return tokens, accepted
