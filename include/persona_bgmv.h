@@ -394,7 +394,7 @@ int persona_paged_cache_read(const persona_paged_cache* cache, const persona_row
 /* Causal attention of the new rows over their sequence's pages:
  * out[r, h] = softmax_j(scale q[r, h] . k[j, h / G]) v[j, h / G], G = Hq / Hkv,
  * over j <= pos(r) and, with window > 0, j > pos(r) - window; zeros where that
- * leaves nothing.  The new tokens' k and v are read from the pages, so write
+ * leaves nothing; scale > 0.  The new tokens' k and v are read from the pages, so write
  * them first.  What lies in the pages behind a sequence's last position is
  * never used; a NaN or infinity at a position of the sequence itself may reach
  * every new row of that sequence.

@@ -62,6 +62,9 @@ cudaError_t launch_paged_read(const PagedRead& a, int dtype, int32_t* err, cudaS
 // Bytes of part and desc for any call with this head size on the current device.
 size_t paged_attention_ws_bytes(int D);
 cudaError_t launch_paged_attention(PagedAttention a, int dtype, int max_new, void* workspace, cudaStream_t st);
+// The same for many rows per kv head (paged_chunk.cu).
+size_t paged_chunk_ws_bytes(int D);
+cudaError_t launch_paged_chunk(PagedAttention a, int dtype, void* workspace, cudaStream_t st);
 
 struct VerifyDraft {
   const void* target;  // [rows, V], row stride ld_target

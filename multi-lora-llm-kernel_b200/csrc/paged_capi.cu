@@ -11,6 +11,7 @@ namespace {
 
 constexpr int64_t kI32Max = 2147483647;
 constexpr int64_t kMaxHeads = 1024;
+constexpr int64_t kFewRows = 64;
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 int status(cudaError_t e) { return e == cudaSuccess ? PERSONA_OK : PERSONA_ERR_CUDA; }
@@ -97,7 +98,9 @@ int persona_paged_cache_read(const persona_paged_cache* cache, const persona_row
 }
 
 size_t persona_paged_attention_workspace_size(int64_t D) {
-  return D == 64 || D == 128 ? paged_attention_ws_bytes(static_cast<int>(D)) : 0;
+  if (D != 64 && D != 128) return 0;
+  const size_t few = paged_attention_ws_bytes(static_cast<int>(D)), many = paged_chunk_ws_bytes(static_cast<int>(D));
+  return few > many ? few : many;
 }
 
 int persona_paged_attention(const persona_paged_cache* cache, const persona_rows* q, const persona_rows* out,
@@ -106,21 +109,23 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
   PagedAttention a;
   PERSONA_TRY(check_cache(cache, dtype, a.c));
   if (rows < 0 || Hq <= 0 || Hq > kMaxHeads || Hq % cache->Hkv || rows > kI32Max / Hq || window < 0 || max_new < 1 ||
-      !std::isfinite(scale))
+      !(scale > 0.f) || !std::isfinite(scale))
     return PERSONA_ERR_SHAPE;
   // positions of a sequence are 32-bit numbers
   if (cache->max_pages > kI32Max / cache->page_size - 64 / cache->page_size - 1) return PERSONA_ERR_SHAPE;
   if (rows == 0 || cache->B == 0) return PERSONA_OK;
   PERSONA_TRY(check_rows(q, a.q));
   PERSONA_TRY(check_rows(out, a.out));
-  if (workspace == nullptr || workspace_bytes < paged_attention_ws_bytes(a.c.D)) return PERSONA_ERR_WORKSPACE;
+  if (workspace == nullptr || workspace_bytes < persona_paged_attention_workspace_size(a.c.D)) return PERSONA_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return PERSONA_ERR_ALIGNMENT;
   a.rows = static_cast<int>(rows);
   a.G = static_cast<int>(Hq / cache->Hkv);
   a.window = window > kI32Max ? 0 : static_cast<int>(window);  // wider than any position
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = dev_err;
-  return status(launch_paged_attention(a, dtype, static_cast<int>(max_new > rows ? rows : max_new), workspace, stream));
+  const int most = static_cast<int>(max_new > rows ? rows : max_new);
+  if (static_cast<int64_t>(most) * a.G > kFewRows) return status(launch_paged_chunk(a, dtype, workspace, stream));
+  return status(launch_paged_attention(a, dtype, most, workspace, stream));
 }
 
 int persona_verify_draft(const void* target, int64_t ld_target, const void* draft, int64_t ld_draft, int prob_type,

@@ -1,0 +1,705 @@
+// Causal attention of each sequence's new tokens over its paged KV cache, for
+// many query rows per kv head (prompt chunks): the same result as
+// paged_attention.cu, on the tensor cores' tcgen05 path.
+//
+// A tile is up to 256 query rows (token, head of the group) of one sequence
+// and kv head, in two halves A and B of 128 rows; a unit is one block of 128
+// positions of a tile.  The units of all tiles lie in one line (sequence,
+// tile, kv head, block), cut into equal ranges, one per CTA and SM; tiles end
+// at their last row's position, so a range of units is a range of work.  Cut
+// tiles leave pieces that paged_combine_kernel joins in order.
+//
+// Per block and half: S = Q K^T (operands in shared memory, 128 x 128 fp32
+// accumulator in tensor memory), softmax with one thread per row, P written
+// back over S as 16 bits, O += P V (P from tensor memory, V from shared
+// memory).  While one half is in its softmax the tensor cores work on the
+// other.  512 columns of tensor memory: S/P and O of both halves.
+//
+// Warps: 0-3 and 4-7 softmax of halves A and B (thread = row), 8-11 load
+// (pages to swizzled shared memory), 12 issues the MMAs.  Rows are loaded by
+// cp.async from per-position offsets, so pages may end anywhere in a block.
+//
+// The running maximum is only moved, and O only rescaled, once a row's new
+// maximum exceeds it by 2^8: until then the weights may grow to 256, which
+// fp16, bf16 and the fp32 sums hold as exactly as weights up to 1.
+//
+// What bounds it: 4 x 128 x 128 x D multiply-adds per half and block on the
+// tensor cores against 128 x 128 exponentials, which at 16 per cycle and SM
+// take as long.
+//
+// 8-bit pages: codes become fp16 in shared memory, exactly; the k scale
+// multiplies the fp32 score and log2 of the v scale joins its exponent (see
+// paged_attention.cu).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "paged_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace persona {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kBlock = 128;  // positions of a unit
+constexpr int kTile = 256;   // rows of a tile
+constexpr int kLoaders = 128;
+// Registers per thread after the split: two softmax warpgroups, loaders, MMA.
+// 2 x 192 + 72 + 40 = 496 <= 4 x 128, what the block is launched with.
+constexpr int kRegsSoftmax = 192, kRegsLoad = 72, kRegsMma = 40, kRegsLaunch = 128;
+static_assert(2 * kRegsSoftmax + kRegsLoad + kRegsMma <= 4 * kRegsLaunch, "register split");
+constexpr float kGrow = 8.f;  // log2 of the growth that moves the running maximum
+
+template <int D> struct Cfg {
+  static constexpr int kStages = 256 / D;              // k and v slots
+  static constexpr int kHalfBytes = 128 * 128;         // 128 rows of 64 16-bit elements
+  static constexpr int kSlot = kHalfBytes * (D / 64);  // 128 x D, 64-element columns side by side
+  static constexpr int kScales = kStages + 1;          // slots of scales: the softmax may be one block behind the k slots
+  static constexpr int kSmem = 1024 + kSlot * (2 + 2 * kStages);
+};
+
+struct Shared {
+  uint64_t q_full, q_empty;
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t s_full[2], p_ready[2], pv_done[2], drained;
+  uint32_t tmem;
+  int abort;
+  int b, tile;
+  long long off, sum[16], total;
+  long long at[2][kBlock];   // page offset (elements) of each position of a block, -1: none
+  alignas(16) float ks[5][kBlock];  // read four at a time
+  alignas(16) float lv[5][kBlock];
+  alignas(16) float rv[5][kBlock];
+  float qmul[2][kTile];      // by piece: the next one's rows are loaded while this one's are read
+};
+
+struct TileGeo {
+  int m0, mrows, first, per, pend;
+};
+__device__ __forceinline__ TileGeo tile_geo(const Seq& s, int window, int G, int t) {
+  TileGeo g;
+  g.m0 = t * kTile;
+  g.mrows = min(kTile, s.n * G - g.m0);
+  const int ctx = s.len - s.n, tok0 = g.m0 / G, tok1 = (g.m0 + g.mrows - 1) / G;
+  g.pend = max(0, min(s.len, ctx + tok1 + 1));
+  g.first = (window > 0 ? max(0, ctx + tok0 + 1 - window) : 0) / kBlock;
+  g.per = max(1, (g.pend + kBlock - 1) / kBlock - g.first);
+  return g;
+}
+__device__ __forceinline__ int seq_tiles(const Seq& s, int G) { return (s.n * G + kTile - 1) / kTile; }
+
+// The pieces of a CTA's range of units, walked alike by every role.
+struct Walk {
+  const PagedAttention& a;
+  int b, t, h, k;
+  long long left;
+  Seq seq;
+  TileGeo g;
+  int k0, k1;
+  bool first;
+  __device__ __forceinline__ Walk(const PagedAttention& a_, int b_, int t_, long long off, long long left_)
+      : a(a_), b(b_), t(t_), left(left_), first(true) {
+    seq = load_seq(a, b);
+    g = tile_geo(seq, a.window, a.G, t);
+    h = static_cast<int>(off / g.per);
+    k1 = static_cast<int>(off - static_cast<long long>(h) * g.per);
+    k0 = k1;
+  }
+  // to the next piece: tile (t, h) of sequence b, blocks [k0, k1)
+  __device__ __forceinline__ bool next() {
+    if (left <= 0) return false;
+    if (k0 != k1) first = false;
+    if (k1 == g.per) {
+      k1 = 0;
+      if (++h == a.c.Hkv) {
+        h = 0;
+        ++t;
+        while (t >= seq_tiles(seq, a.G)) {
+          if (++b >= a.c.B) return false;
+          seq = load_seq(a, b);
+          t = 0;
+        }
+        g = tile_geo(seq, a.window, a.G, t);
+      }
+    }
+    k0 = k1;
+    k1 = static_cast<int>(min(static_cast<long long>(g.per), k0 + left));
+    left -= k1 - k0;
+    return true;
+  }
+  __device__ __forceinline__ int blocks() const { return g.pend > 0 ? k1 - k0 : 0; }
+  __device__ __forceinline__ bool has_b() const { return g.mrows > 128; }
+};
+
+template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <typename T, int D, bool kE4m3>
+__global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_constant__ PagedAttention a) {
+  using C = Cfg<D>;
+  using PT = typename std::conditional<kE4m3, __half, T>::type;  // type of the products
+  constexpr bool kScaleQ = kE4m3 && !std::is_same<T, __half>::value;
+  constexpr int kSt = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Shared sh;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t s_q = base, s_k = base + 2 * C::kSlot, s_v = s_k + kSt * C::kSlot;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x, G = a.G;
+  // Wait before anything else, the allocation of tensor memory included: a
+  // kernel before this one may still hold some.
+  pdl_wait();
+  if (warp == 12) {
+    tc::tmem_alloc(&sh.tmem, 512);
+    tc::tmem_relinquish();
+  }
+  if (tid == 0) {
+    mbar_init(&sh.q_full, kLoaders);
+    mbar_init(&sh.q_empty, 1);
+    for (int i = 0; i < kSt; ++i) {
+      mbar_init(&sh.k_full[i], kLoaders);
+      mbar_init(&sh.v_full[i], kLoaders);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_ready[i], 128);
+      mbar_init(&sh.pv_done[i], 1);
+    }
+    mbar_init(&sh.drained, 1);
+    sh.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    a.desc[cta] = make_int4(0, 0, 0, 0);
+  }
+
+  // ---- this CTA's range of units ----
+  auto seq_sum = [&](int b) -> long long {
+    if (b >= a.c.B) return 0;
+    const Seq s = load_seq(a, b);
+    long long u = 0;
+    const int tiles = seq_tiles(s, G);
+    for (int t = 0; t < tiles; ++t) u += tile_geo(s, a.window, G, t).per;
+    return u * a.c.Hkv;
+  };
+  long long total = 0, mine = 0;
+  for (int b0 = 0; b0 < a.c.B; b0 += kThreads) {
+    const long long u = seq_sum(b0 + tid);
+    if (b0 == 0) mine = u;
+    long long w = u;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    if (lane == 0) sh.sum[warp] = w;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) total += sh.sum[i];
+    __syncthreads();
+  }
+  const int ctas = static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
+  const bool works = cta < ctas;
+  const long long u0 = works ? total * cta / ctas : 0, u1 = works ? total * (cta + 1) / ctas : 0;
+  if (works) {
+    long long run = 0;
+    for (int b0 = 0; b0 < a.c.B && run <= u0; b0 += kThreads) {
+      const long long u = b0 == 0 ? mine : seq_sum(b0 + tid);
+      long long inc = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      if (lane == 31) sh.sum[warp] = inc;
+      __syncthreads();
+      long long lo = run;
+      for (int i = 0; i < warp; ++i) lo += sh.sum[i];
+      lo += inc - u;
+      if (u0 >= lo && u0 < lo + u) {
+        long long off = u0 - lo;
+        const Seq s = load_seq(a, b0 + tid);
+        const int tiles = seq_tiles(s, G);
+        int t = 0;
+        for (; t < tiles - 1; ++t) {
+          const long long c = static_cast<long long>(tile_geo(s, a.window, G, t).per) * a.c.Hkv;
+          if (off < c) break;
+          off -= c;
+        }
+        sh.b = b0 + tid;
+        sh.tile = t;
+        sh.off = off;
+      }
+      for (int i = 0; i < 16; ++i) run += sh.sum[i];
+      __syncthreads();
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  pdl_launch();  // after the allocation: a dependent that takes tensor memory must find ours taken
+  const uint32_t tmem = sh.tmem;
+  int* const abort = &sh.abort;
+  int32_t* const err = a.err;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax --
+    regs_inc<kRegsSoftmax>();
+    const int half = warp >> 2;
+    const int r = half * 128 + (warp & 3) * 32 + lane;  // row of the tile
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + half * 128, t_o = tmem + lanes + 256 + half * D;
+    int n_s = 0, n_pv = 0, n_sc = 0, n_q = 0;  // blocks so far: of this half, and of all (the scales' slots); pieces
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int n) {  // the same answer in the whole warp, as the tensor memory loads need
+      ok = __all_sync(0xffffffffu, mbar_wait_abortable(bar, n & 1, err, abort));
+      tc::fence_after_sync();
+      return ok;
+    };
+    if (works) {
+      Walk w(a, sh.b, sh.tile, sh.off, u1 - u0);
+      while (ok && w.next()) {
+        const int nb = w.blocks();
+        const bool act = half == 0 || w.has_b();
+        const int ctx = w.seq.len - w.seq.n;
+        const bool live = r < w.g.mrows;
+        const int mm = w.g.m0 + (live ? r : 0), tok = mm / G, hg = mm - tok * G;
+        const int hi = live ? ctx + tok : -1;                        // last position this row sees
+        const int lo = a.window > 0 ? max(0, hi - a.window + 1) : 0;  // and the first
+        // positions that every row of the tile sees
+        const int all_hi = ctx + w.g.m0 / G;
+        const int all_lo = a.window > 0 ? ctx + (w.g.m0 + w.g.mrows - 1) / G - a.window + 1 : 0;
+        float m = kNegInf, l = 0.f, qm = a.scale_log2;
+        for (int j = 0; act && j < nb; ++j) {
+          if (!wait(&sh.s_full[half], n_s)) break;
+          ++n_s;
+          if (kScaleQ && j == 0) qm = sh.qmul[n_q & 1][r];
+          float s[kBlock];
+          uint32_t* su = reinterpret_cast<uint32_t*>(s);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tc::ld32(t_s + 32 * c, su + 32 * c);
+          tc::wait_ld();
+          const int p0 = (w.g.first + w.k0 + j) * kBlock;
+          const int sc = (n_sc + j) % C::kScales;
+          if (kE4m3) {
+            const float4* ks = reinterpret_cast<const float4*>(sh.ks[sc]);
+            const float4* lv = reinterpret_cast<const float4*>(sh.lv[sc]);
+#pragma unroll
+            for (int c = 0; c < kBlock / 4; ++c) {
+              const float4 k4 = ks[c], l4 = lv[c];
+              s[4 * c] = fmaf(s[4 * c] * k4.x, qm, l4.x);
+              s[4 * c + 1] = fmaf(s[4 * c + 1] * k4.y, qm, l4.y);
+              s[4 * c + 2] = fmaf(s[4 * c + 2] * k4.z, qm, l4.z);
+              s[4 * c + 3] = fmaf(s[4 * c + 3] * k4.w, qm, l4.w);
+            }
+          }
+          if (p0 + kBlock - 1 > all_hi || p0 < all_lo || !live) {
+            const int c1 = hi - p0, c0 = lo - p0;
+#pragma unroll
+            for (int c = 0; c < kBlock; ++c) s[c] = c <= c1 && c >= c0 ? s[c] : kNegInf;
+          }
+          float mx = kNegInf;
+#pragma unroll
+          for (int c = 0; c < kBlock; c += 2) mx = fmaxf(mx, fmaxf(s[c], s[c + 1]));
+          const float mul = kE4m3 ? 1.f : a.scale_log2;
+          mx *= mul;
+          if (j == 0) {
+            m = mx;
+          } else {
+            const bool grow = mx > m + kGrow;
+            if (__any_sync(0xffffffffu, grow)) {
+              // the products before this block have to be in O first
+              if (!wait(&sh.pv_done[half], n_pv + j - 1)) break;
+              const float f = grow ? exp2_approx(m - mx) : 1.f;
+              m = grow ? mx : m;
+              l *= f;
+#pragma unroll
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tc::ld32(t_o + 32 * c, o);
+                tc::wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tc::st32(t_o + 32 * c, o);
+              }
+            }
+          }
+          const float neg = m == kNegInf ? 0.f : -m;
+          float sum0 = 0.f, sum1 = 0.f;
+          const float4* rv = reinterpret_cast<const float4*>(sh.rv[sc]);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const int c = 64 * q + 2 * i;
+              const float e0 = exp2_approx(kE4m3 ? s[c] + neg : fmaf(s[c], a.scale_log2, neg));
+              const float e1 = exp2_approx(kE4m3 ? s[c + 1] + neg : fmaf(s[c + 1], a.scale_log2, neg));
+              const float e2 = exp2_approx(kE4m3 ? s[c + 2] + neg : fmaf(s[c + 2], a.scale_log2, neg));
+              const float e3 = exp2_approx(kE4m3 ? s[c + 3] + neg : fmaf(s[c + 3], a.scale_log2, neg));
+              if (kE4m3) {
+                const float4 r4 = rv[c / 4];
+                sum0 = fmaf(e0, r4.x, sum0);
+                sum1 = fmaf(e1, r4.y, sum1);
+                sum0 = fmaf(e2, r4.z, sum0);
+                sum1 = fmaf(e3, r4.w, sum1);
+              } else {
+                sum0 += e0 + e1;
+                sum1 += e2 + e3;
+              }
+              pk[i] = Mma<PT>::pack(e0, e1);
+              pk[i + 1] = Mma<PT>::pack(e2, e3);
+            }
+            tc::st32(t_s + 32 * q, pk);
+          }
+          l += sum0 + sum1;
+          tc::wait_st();
+          tc::fence_before_sync();
+          mbar_arrive(&sh.p_ready[half]);
+        }
+        if (!ok) break;
+        n_sc += nb;
+        if (nb > 0) ++n_q;
+        if (!act) continue;
+        // ---- this piece's rows ----
+        if (nb > 0) {
+          if (!wait(&sh.pv_done[half], n_pv + nb - 1)) break;
+          n_pv += nb;
+        }
+        const bool complete = w.k0 == 0 && w.k1 == w.g.per;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        float* part = a.part + static_cast<int64_t>(2 * cta + (w.first ? 0 : 1)) * Part<kTile, D>::kFloats;
+        T* dst = static_cast<T*>(a.out.p) + static_cast<int64_t>(w.seq.row0 + tok) * a.out.row_stride +
+                 static_cast<int64_t>(w.h * G + hg) * a.out.head_stride;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          if (nb > 0) {
+            tc::ld32(t_o + 32 * c, reinterpret_cast<uint32_t*>(o));
+            tc::wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          }
+          if (live && complete) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              *reinterpret_cast<uint4*>(dst + 32 * c + i) =
+                  make_uint4(Mma<T>::pack(o[i] * inv, o[i + 1] * inv), Mma<T>::pack(o[i + 2] * inv, o[i + 3] * inv),
+                             Mma<T>::pack(o[i + 4] * inv, o[i + 5] * inv), Mma<T>::pack(o[i + 6] * inv, o[i + 7] * inv));
+          } else if (live) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(part + r * D + 32 * c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+          __syncwarp();
+        }
+        if (live && !complete) {
+          part[kTile * D + r] = m;
+          part[kTile * D + kTile + r] = l;
+        }
+        // O is read: the first product of the next piece waits for this
+        // half's next p_ready, which comes after
+        tc::fence_before_sync();
+        if (r == 0 && w.k0 == 0 && w.k1 < w.g.per) {
+          const long long end = u1 - w.left - w.k1 + w.g.per - 1;  // the tile's last unit
+          long long c = end * ctas / total;
+          while (total * (c + 1) / ctas <= end) ++c;
+          while (total * c / ctas > end) --c;
+          a.desc[cta] = make_int4(w.b, w.t * a.c.Hkv + w.h, static_cast<int>(c), w.first ? 1 : 2);
+        }
+      }
+    }
+  } else if (warp < 12) {
+    // -------------------------------------------------------------- loads --
+    regs_dec<kRegsLoad>();
+    const int t = tid - 256;
+    int n_k = 0, n_q = 0;  // blocks and pieces so far
+    bool ok = true;
+    uint64_t* pending = nullptr;  // loads under way whose arrival is due
+    auto flush = [&]() {
+      if (pending != nullptr) {
+        cp_wait<0>();
+        tc::fence_proxy_async();
+        mbar_arrive(pending);
+        pending = nullptr;
+      }
+    };
+    auto issued = [&](uint64_t* bar) {
+      cp_commit();
+      if (pending != nullptr) {
+        cp_wait<1>();
+        tc::fence_proxy_async();
+        mbar_arrive(pending);
+      }
+      pending = bar;
+    };
+    auto acquire = [&](uint64_t* bar, uint32_t parity) {
+      if (mbar_try_wait(bar, parity)) return true;
+      flush();  // nobody waits for what this thread holds back
+      return mbar_wait_abortable(bar, parity, err, abort);
+    };
+    if (works) {
+      Walk w(a, sh.b, sh.tile, sh.off, u1 - u0);
+      // A wait that gave up (ok) ends the loads but not the walk: the barrier
+      // of the four warps needs them all.
+      while (w.next()) {
+        const int nb = w.blocks();
+        if (nb == 0) continue;
+        // ---- q rows ----
+        if (n_q > 0) ok = ok && acquire(&sh.q_empty, (n_q - 1) & 1);
+        if (ok) {
+          constexpr int kCh = D / 8, kPer = kLoaders / kCh;
+          const int c = t % kCh, rows = w.has_b() ? 256 : 128;
+          const T* qb = static_cast<const T*>(a.q.p) + static_cast<int64_t>(w.seq.row0) * a.q.row_stride +
+                        static_cast<int64_t>(w.h * G) * a.q.head_stride + c * 8;
+          for (int i = t / kCh; i < rows; i += kPer) {
+            const bool live = i < w.g.mrows;
+            const int mm = w.g.m0 + (live ? i : 0), tok = mm / G, hg = mm - tok * G;
+            const T* src = qb + static_cast<int64_t>(tok) * a.q.row_stride + static_cast<int64_t>(hg) * a.q.head_stride;
+            const int r = i & 127;
+            const uint32_t dst = s_q + (i >> 7) * C::kSlot + (c >> 3) * C::kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+            if (!kScaleQ) {
+              cp_async16(dst, src, live);
+            } else {
+              // bf16 row -> fp16, scaled by the power of two that brings its
+              // largest element into [1, 2)
+              const uint4 v = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+              const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+              float f[8], mx = 0.f;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float2 p = Cvt<T>::to2(u[x]);
+                f[2 * x] = p.x;
+                f[2 * x + 1] = p.y;
+                mx = fmaxf(mx, fmaxf(fabsf(p.x), fabsf(p.y)));
+              }
+#pragma unroll
+              for (int o = kCh / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+              const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23), 2), 252);
+              const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+              if (c == 0) sh.qmul[n_q & 1][i] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e) << 23);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(Mma<__half>::pack(f[0] * down, f[1] * down)),
+                           "r"(Mma<__half>::pack(f[2] * down, f[3] * down)), "r"(Mma<__half>::pack(f[4] * down, f[5] * down)),
+                           "r"(Mma<__half>::pack(f[6] * down, f[7] * down))
+                           : "memory");
+            }
+          }
+        }
+        if (ok) issued(&sh.q_full);
+        ++n_q;
+        // ---- blocks ----
+        const int32_t* row = a.c.table + w.b * a.c.table_stride;
+        const int first = w.g.first + w.k0;
+        // Thread t looks up position t of a block, one block ahead: the page
+        // is read here and used when the block is due.
+        int pg = -1, at = 0;
+        bool seen = false;
+        auto fetch = [&](int j) {
+          const int p = (first + j) * kBlock + t, pi = p / a.c.page_size;
+          at = p - pi * a.c.page_size;
+          seen = p < w.g.pend;
+          pg = -1;
+          if (seen && pi < a.c.max_pages) pg = row[pi];
+        };
+        fetch(0);
+        constexpr int kElt = kE4m3 ? 1 : 2, kCh = D * kElt / 16, kPer = kLoaders / kCh;  // 16-byte chunks of a position
+        const int c = t % kCh, r0 = t / kCh;
+        const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + static_cast<int64_t>(w.h) * a.c.head_stride * kElt + c * 16;
+        const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + static_cast<int64_t>(w.h) * a.c.head_stride * kElt + c * 16;
+        for (int j = 0; j < nb; ++j) {
+          float k_sc = 0.f, v_sc = 0.f;
+          const bool there = pg >= 0 && pg < a.c.num_pages;
+          if (seen && !there) raise_error(err, PERSONA_DEV_ERR_PAGE);
+          if (kE4m3 && there) {
+            const int64_t so = pg * a.c.scale_page_stride + at + static_cast<int64_t>(w.h) * a.c.scale_head_stride;
+            k_sc = a.c.k_scale[so];
+            v_sc = a.c.v_scale[so];
+          }
+          long long* const places = sh.at[n_k & 1];
+          places[t] = there ? pg * a.c.page_stride + at * a.c.pos_stride : -1;
+          named_sync(1, kLoaders);
+          if (j + 1 < nb) fetch(j + 1);
+          const int st = n_k % kSt;
+          const uint32_t parity = (n_k / kSt - 1) & 1;
+          for (int kv = 0; kv < 2; ++kv) {
+            uint64_t* empty = kv == 0 ? &sh.k_empty[st] : &sh.v_empty[st];
+            if (n_k >= kSt) ok = ok && acquire(empty, parity);
+            if (!ok) continue;
+            const uint8_t* src = kv == 0 ? kb : vb;
+            const uint32_t slot = (kv == 0 ? s_k : s_v) + st * C::kSlot;
+            if (!kE4m3) {
+#pragma unroll
+              for (int i = 0; i < kBlock / kPer; ++i) {
+                const int r = r0 + i * kPer;
+                const long long o = places[r];
+                cp_async16(slot + (c >> 3) * C::kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (o < 0 ? 0 : o) * kElt,
+                           o >= 0);
+              }
+              issued(kv == 0 ? &sh.k_full[st] : &sh.v_full[st]);
+            } else {
+              if (kv == 0) {
+                const int sc = n_k % C::kScales;
+                const float vs = fmaxf(v_sc, 8.673617379884035e-19f);  // 2^-60
+                sh.ks[sc][t] = k_sc;
+                sh.lv[sc][t] = __log2f(vs);
+                sh.rv[sc][t] = __frcp_rn(vs);
+              }
+              uint4 x[kBlock / kPer];
+#pragma unroll
+              for (int i = 0; i < kBlock / kPer; ++i) {
+                const long long o = places[r0 + i * kPer];
+                x[i] = o >= 0 ? *reinterpret_cast<const uint4*>(src + o) : make_uint4(0u, 0u, 0u, 0u);
+              }
+#pragma unroll
+              for (int i = 0; i < kBlock / kPer; ++i) {
+                const int r = r0 + i * kPer;
+                const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  const int cc = 2 * c + y;
+                  uint32_t hh[4];
+                  e4m3x4_to_half(u[2 * y], hh[0], hh[1]);
+                  e4m3x4_to_half(u[2 * y + 1], hh[2], hh[3]);
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                   slot + (cc >> 3) * C::kHalfBytes + r * 128 + (((cc & 7) ^ (r & 7)) << 4)),
+                               "r"(hh[0]), "r"(hh[1]), "r"(hh[2]), "r"(hh[3])
+                               : "memory");
+                }
+              }
+              flush();
+              tc::fence_proxy_async();
+              mbar_arrive(kv == 0 ? &sh.k_full[st] : &sh.v_full[st]);
+            }
+          }
+          ++n_k;
+        }
+      }
+      flush();
+    }
+  } else {
+    // ---------------------------------------------------------------- MMA --
+    regs_dec<kRegsMma>();
+    if (warp == 12 && works) {
+      const bool one = lane == 0;
+      constexpr uint32_t kFmt = std::is_same<PT, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t kIdescS = tc::idesc_f16(kFmt, 128, kBlock);
+      constexpr uint32_t kIdescO = tc::idesc_f16(kFmt, 128, D) | tc::kIdescBMnMajor;
+      int n_k = 0, n_q = 0, n_p[2] = {0, 0};
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int n) {
+        if (ok && !mbar_wait_abortable(bar, n & 1, err, abort)) ok = false;
+        if (ok) tc::fence_after_sync();
+        return ok;
+      };
+      auto mma_s = [&](int half, int st) {  // S = Q K^T
+        if (one) {
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t in = (ks >> 2) * C::kHalfBytes + (ks & 3) * 32;
+            tc::mma_f16(tmem + half * 128, tc::smem_desc(s_q + half * C::kSlot + in, 1024, tc::kLayoutSw128),
+                        tc::smem_desc(s_k + st * C::kSlot + in, 1024, tc::kLayoutSw128), kIdescS, ks > 0 ? 1u : 0u);
+          }
+          tc::commit(&sh.s_full[half]);
+        }
+      };
+      auto mma_o = [&](int half, int st, bool first) {  // O += P V
+        if (one) {
+#pragma unroll
+          for (int ks = 0; ks < kBlock / 16; ++ks)
+            tc::mma_f16_ts(tmem + 256 + half * D, tmem + half * 128 + ks * 8,
+                           tc::smem_desc_mn128(s_v + st * C::kSlot + ks * 2048, C::kHalfBytes, 1024), kIdescO,
+                           first && ks == 0 ? 0u : 1u);
+          tc::commit(&sh.pv_done[half]);
+        }
+      };
+      Walk w(a, sh.b, sh.tile, sh.off, u1 - u0);
+      while (ok && w.next()) {
+        const int nb = w.blocks();
+        if (nb == 0) continue;
+        const bool two = w.has_b();
+        if (!wait(&sh.q_full, n_q)) break;
+        if (!wait(&sh.k_full[n_k % kSt], n_k / kSt)) break;
+        mma_s(0, n_k % kSt);
+        if (two) mma_s(1, n_k % kSt);
+        if (one) {
+          tc::commit(&sh.k_empty[n_k % kSt]);
+          if (nb == 1) tc::commit(&sh.q_empty);
+        }
+        for (int j = 0; j < nb; ++j) {
+          const int st = n_k % kSt, nst = (n_k + 1) % kSt;
+          const bool more = j + 1 < nb;
+          if (!wait(&sh.v_full[st], n_k / kSt)) break;
+          if (!wait(&sh.p_ready[0], n_p[0])) break;
+          ++n_p[0];
+          mma_o(0, st, j == 0);
+          // S of the next block may be written over P: the tensor cores take
+          // the products in the order of their issue
+          if (more) {
+            if (!wait(&sh.k_full[nst], (n_k + 1) / kSt)) break;
+            mma_s(0, nst);
+          }
+          if (two) {
+            if (!wait(&sh.p_ready[1], n_p[1])) break;
+            ++n_p[1];
+            mma_o(1, st, j == 0);
+          }
+          if (one) tc::commit(&sh.v_empty[st]);
+          if (more) {
+            if (two) mma_s(1, nst);
+            if (one) {
+              tc::commit(&sh.k_empty[nst]);
+              if (j + 2 == nb) tc::commit(&sh.q_empty);
+            }
+          }
+          ++n_k;
+        }
+        ++n_q;
+      }
+      if (!ok && one) {  // gave up: nothing of ours may be under way when the memory goes
+        tc::commit(&sh.drained);
+        mbar_wait(&sh.drained, 0, err);
+      }
+    }
+    __syncwarp();
+  }
+  // ---- end: every product has been waited for by its softmax rows ----
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 12) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int D, bool kE4m3>
+cudaError_t chunk_launch(const PagedAttention& a, cudaStream_t st) {
+  auto k = paged_chunk_kernel<T, D, kE4m3>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  // the register split above draws on kRegsLaunch registers a thread
+  cudaFuncAttributes attr;
+  e = cudaFuncGetAttributes(&attr, k);
+  if (e != cudaSuccess) return e;
+  if (attr.numRegs != kRegsLaunch) return cudaErrorInvalidConfiguration;
+  const int ctas = sm_count();
+  e = launch_paged(k, dim3(ctas), dim3(kThreads), Cfg<D>::kSmem, 1, st, a);
+  if (e != cudaSuccess) return e;
+  return launch_paged(paged_combine_kernel<T, D, kTile>, dim3(ctas, 8), dim3(256), 0, 1, st, a);
+}
+template <typename T>
+cudaError_t chunk_for(const PagedAttention& a, cudaStream_t st) {
+  const bool e = a.c.k_scale != nullptr;
+  if (a.c.D == 128) return e ? chunk_launch<T, 128, true>(a, st) : chunk_launch<T, 128, false>(a, st);
+  return e ? chunk_launch<T, 64, true>(a, st) : chunk_launch<T, 64, false>(a, st);
+}
+
+}  // namespace
+
+size_t paged_chunk_ws_bytes(int D) {
+  const size_t ctas = sm_count();
+  return ctas * sizeof(int4) + ctas * 2 * (kTile * static_cast<size_t>(D) + 2 * kTile) * sizeof(float);
+}
+
+cudaError_t launch_paged_chunk(PagedAttention a, int dtype, void* workspace, cudaStream_t st) {
+  a.desc = static_cast<int4*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sm_count() * sizeof(int4));
+  return dtype == PERSONA_DTYPE_BF16 ? chunk_for<__nv_bfloat16>(a, st) : chunk_for<__half>(a, st);
+}
+
+}  // namespace persona

@@ -280,7 +280,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Causal attention of each sequence's new tokens over its pages, theirs
     included (write them first); with ``window`` over the last ``window``
     positions only.  Layouts as in ``paged_rope_cache``; ``out`` like ``q``.
-    A row that sees no position gives zeros.
+    A row that sees no position gives zeros; ``scale`` is positive.
 
     ``max_new``: an upper bound of the new tokens of one sequence, which
     chooses the kernel (default: what ``rows`` allows if every sequence has

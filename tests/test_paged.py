@@ -72,6 +72,7 @@ def test_attention_statuses(lib):
         assert _attend(lib, _cache(**change)) == want, change
     assert _attend(lib, Hq=33) == SHAPE and _attend(lib, Hq=0) == SHAPE and _attend(lib, rows=-1) == SHAPE
     assert _attend(lib, window=-1) == SHAPE and _attend(lib, max_new=0) == SHAPE
+    assert _attend(lib, scale=0.0) == SHAPE and _attend(lib, scale=-0.1) == SHAPE
     assert _attend(lib, scale=float("nan")) == SHAPE and _attend(lib, scale=float("inf")) == SHAPE
     assert _attend(lib, rows=1 << 30) == SHAPE and _attend(lib, dtype=2) == DTYPE
     assert _attend(lib, q=Rows(FAKE + 2, 4096, 128)) == ALIGN and _attend(lib, q=Rows(FAKE, 4095, 128)) == ALIGN
