@@ -44,8 +44,8 @@ constexpr int kBlock = 128;  // positions of a unit
 constexpr int kTile = 256;   // rows of a tile
 constexpr int kLoaders = 128;
 // Registers per thread after the split: two softmax warpgroups, loaders, MMA.
-// 2 x 192 + 72 + 40 = 496 <= 4 x 128, what the block is launched with.
-constexpr int kRegsSoftmax = 192, kRegsLoad = 72, kRegsMma = 40, kRegsLaunch = 128;
+// 2 x 184 + 72 + 72 = 512 <= 4 x 128, what the block is launched with.
+constexpr int kRegsSoftmax = 184, kRegsLoad = 72, kRegsMma = 72, kRegsLaunch = 128;
 static_assert(2 * kRegsSoftmax + kRegsLoad + kRegsMma <= 4 * kRegsLaunch, "register split");
 constexpr float kGrow = 8.f;  // log2 of the growth that moves the running maximum
 
@@ -298,36 +298,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           for (int c = 0; c < kBlock; c += 2) mx = fmaxf(mx, fmaxf(s[c], s[c + 1]));
           const float mul = kE4m3 ? 1.f : a.scale_log2;
           mx *= mul;
-          if (j == 0) {
-            m = mx;
-          } else {
-            const bool grow = mx > m + kGrow;
-            if (__any_sync(0xffffffffu, grow)) {
-              // the products before this block have to be in O first
-              if (!wait(&sh.pv_done[half], n_pv + j - 1)) break;
-              const float f = grow ? exp2_approx(m - mx) : 1.f;
-              m = grow ? mx : m;
-              l *= f;
-#pragma unroll
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                tc::ld32(t_o + 32 * c, o);
-                tc::wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tc::st32(t_o + 32 * c, o);
-              }
-            }
-          }
+          const bool grow = j > 0 && mx > m + kGrow;
+          const float shrink = grow ? exp2_approx(m - mx) : 1.f;
+          if (j == 0 || grow) m = mx;
           const float neg = m == kNegInf ? 0.f : -m;
           float sum0 = 0.f, sum1 = 0.f;
           const float4* rv = reinterpret_cast<const float4*>(sh.rv[sc]);
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint32_t pk[32];
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const int c = 64 * q + 2 * i;
+            for (int i = 0; i < 16; i += 2) {
+              const int c = 32 * q + 2 * i;
               const float e0 = exp2_approx(kE4m3 ? s[c] + neg : fmaf(s[c], a.scale_log2, neg));
               const float e1 = exp2_approx(kE4m3 ? s[c + 1] + neg : fmaf(s[c + 1], a.scale_log2, neg));
               const float e2 = exp2_approx(kE4m3 ? s[c + 2] + neg : fmaf(s[c + 2], a.scale_log2, neg));
@@ -345,9 +327,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
               pk[i] = Mma<PT>::pack(e0, e1);
               pk[i + 1] = Mma<PT>::pack(e2, e3);
             }
-            tc::st32(t_s + 32 * q, pk);
+            tc::st16(t_s + 16 * q, pk);
           }
-          l += sum0 + sum1;
+          l = fmaf(l, shrink, sum0 + sum1);
+          if (__any_sync(0xffffffffu, grow)) {
+            // the products before this block have to be in O first
+            if (!wait(&sh.pv_done[half], n_pv + j - 1)) break;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tc::ld32(t_o + 32 * c, o);
+              tc::wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+              tc::st32(t_o + 32 * c, o);
+            }
+          }
           tc::wait_st();
           tc::fence_before_sync();
           mbar_arrive(&sh.p_ready[half]);
@@ -587,24 +582,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         if (ok) tc::fence_after_sync();
         return ok;
       };
+      // Descriptors differ in the start address alone (bits 0-13, units of 16
+      // bytes, below 2^14 for any shared address): the rest is added once.
+      const uint32_t dq = static_cast<uint32_t>(tc::smem_desc(s_q, 1024, tc::kLayoutSw128));
+      const uint32_t dk = static_cast<uint32_t>(tc::smem_desc(s_k, 1024, tc::kLayoutSw128));
+      const uint32_t dv = static_cast<uint32_t>(tc::smem_desc_mn128(s_v, C::kHalfBytes, 1024));
+      const uint32_t hk = static_cast<uint32_t>(tc::smem_desc(s_k, 1024, tc::kLayoutSw128) >> 32);
+      const uint32_t hv = static_cast<uint32_t>(tc::smem_desc_mn128(s_v, C::kHalfBytes, 1024) >> 32);
       auto mma_s = [&](int half, int st) {  // S = Q K^T
         if (one) {
+          const uint32_t q = dq + half * (C::kSlot >> 4), k = dk + st * (C::kSlot >> 4);
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
-            const uint32_t in = (ks >> 2) * C::kHalfBytes + (ks & 3) * 32;
-            tc::mma_f16(tmem + half * 128, tc::smem_desc(s_q + half * C::kSlot + in, 1024, tc::kLayoutSw128),
-                        tc::smem_desc(s_k + st * C::kSlot + in, 1024, tc::kLayoutSw128), kIdescS, ks > 0 ? 1u : 0u);
+            constexpr int kHalf16 = C::kHalfBytes >> 4;
+            const int in = (ks >> 2) * kHalf16 + (ks & 3) * 2;
+            tc::mma_f16_lo(tmem + half * 128, q + in, hk, k + in, hk, kIdescS, ks > 0 ? 1u : 0u);
           }
           tc::commit(&sh.s_full[half]);
         }
       };
       auto mma_o = [&](int half, int st, bool first) {  // O += P V
         if (one) {
+          const uint32_t v = dv + st * (C::kSlot >> 4);
 #pragma unroll
           for (int ks = 0; ks < kBlock / 16; ++ks)
-            tc::mma_f16_ts(tmem + 256 + half * D, tmem + half * 128 + ks * 8,
-                           tc::smem_desc_mn128(s_v + st * C::kSlot + ks * 2048, C::kHalfBytes, 1024), kIdescO,
-                           first && ks == 0 ? 0u : 1u);
+            tc::mma_f16_ts_lo(tmem + 256 + half * D, tmem + half * 128 + ks * 8, v + ks * (2048 >> 4), hv, kIdescO,
+                              first && ks == 0 ? 0u : 1u);
           tc::commit(&sh.pv_done[half]);
         }
       };
