@@ -47,6 +47,7 @@ constexpr int kLoaders = 128;
 // 2 x 184 + 72 + 72 = 512 <= 4 x 128, what the block is launched with.
 constexpr int kRegsSoftmax = 184, kRegsLoad = 72, kRegsMma = 72, kRegsLaunch = 128;
 static_assert(2 * kRegsSoftmax + kRegsLoad + kRegsMma <= 4 * kRegsLaunch, "register split");
+constexpr int kPoly = 0;  // of 8 pairs of exponentials, this many take the polynomial (0 to 4)
 constexpr float kGrow = 8.f;  // log2 of the growth that moves the running maximum
 
 template <int D> struct Cfg {
@@ -60,12 +61,12 @@ template <int D> struct Cfg {
 struct Shared {
   uint64_t q_full, q_empty;
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t s_full[2], p_ready[2], pv_done[2], drained;
+  uint64_t s_full[2], p_ready[2], p_rest[2], pv_done[2], drained;
   uint32_t tmem;
   int abort;
   int b, tile;
   long long off, sum[16], total;
-  long long at[2][kBlock];   // page offset (elements) of each position of a block, -1: none
+  long long at[2][kBlock];   // page offset (bytes) of each position of a block, -1: none
   alignas(16) float ks[5][kBlock];  // read four at a time
   alignas(16) float lv[5][kBlock];
   alignas(16) float rv[5][kBlock];
@@ -130,6 +131,55 @@ struct Walk {
   __device__ __forceinline__ bool has_b() const { return g.mrows > 128; }
 };
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x of two values without the special-function unit, whose 16 exponentials
+// per cycle and SM are as scarce here as the tensor cores: x = n + f with
+// |f| <= 1/2 by the addition of 1.5 2^23, a polynomial for 2^f (degree 5,
+// fitted to the smallest relative error by weighted least squares, 7.5e-8)
+// and n added to the exponent.  Below -126 the result stays near 2^-126.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const float2 t = add2(x, both(12582912.f));
+  const float2 f = add2(x, fma2(t, both(-1.f), both(12582912.f)));
+  float2 p = fma2(f, both(0.0013276443f), both(0.0096755373f));
+  p = fma2(p, f, both(0.0555071332f));
+  p = fma2(p, f, both(0.2402211980f));
+  p = fma2(p, f, both(0.6931469671f));
+  p = fma2(p, f, both(1.0000000716f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
@@ -164,6 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_ready[i], 128);
+      mbar_init(&sh.p_rest[i], 128);
       mbar_init(&sh.pv_done[i], 1);
     }
     mbar_init(&sh.drained, 1);
@@ -270,9 +321,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           ++n_s;
           if (kScaleQ && j == 0) qm = sh.qmul[n_q & 1][r];
           float s[kBlock];
-          uint32_t* su = reinterpret_cast<uint32_t*>(s);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tc::ld32(t_s + 32 * c, su + 32 * c);
+          for (int c = 0; c < 4; ++c) tc::ld32(t_s + 32 * c, reinterpret_cast<uint32_t*>(s) + 32 * c);
           tc::wait_ld();
           const int p0 = (w.g.first + w.k0 + j) * kBlock;
           const int sc = (n_sc + j) % C::kScales;
@@ -280,12 +330,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             const float4* ks = reinterpret_cast<const float4*>(sh.ks[sc]);
             const float4* lv = reinterpret_cast<const float4*>(sh.lv[sc]);
 #pragma unroll
-            for (int c = 0; c < kBlock / 4; ++c) {
-              const float4 k4 = ks[c], l4 = lv[c];
-              s[4 * c] = fmaf(s[4 * c] * k4.x, qm, l4.x);
-              s[4 * c + 1] = fmaf(s[4 * c + 1] * k4.y, qm, l4.y);
-              s[4 * c + 2] = fmaf(s[4 * c + 2] * k4.z, qm, l4.z);
-              s[4 * c + 3] = fmaf(s[4 * c + 3] * k4.w, qm, l4.w);
+            for (int c = 0; c < kBlock; c += 4) {
+              const float4 k4 = ks[c / 4], l4 = lv[c / 4];
+              const float2 x = fma2(mul2(make_float2(s[c], s[c + 1]), make_float2(k4.x, k4.y)), both(qm), make_float2(l4.x, l4.y));
+              const float2 y = fma2(mul2(make_float2(s[c + 2], s[c + 3]), make_float2(k4.z, k4.w)), both(qm), make_float2(l4.z, l4.w));
+              s[c] = x.x;
+              s[c + 1] = x.y;
+              s[c + 2] = y.x;
+              s[c + 3] = y.y;
             }
           }
           if (p0 + kBlock - 1 > all_hi || p0 < all_lo || !live) {
@@ -293,59 +345,70 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 #pragma unroll
             for (int c = 0; c < kBlock; ++c) s[c] = c <= c1 && c >= c0 ? s[c] : kNegInf;
           }
-          float mx = kNegInf;
+          float mxs[8];
 #pragma unroll
-          for (int c = 0; c < kBlock; c += 2) mx = fmaxf(mx, fmaxf(s[c], s[c + 1]));
+          for (int c = 0; c < 8; ++c) mxs[c] = fmaxf(s[c], s[c + 8]);
+#pragma unroll
+          for (int c = 16; c < kBlock; c += 16)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) mxs[x] = max3(mxs[x], s[c + x], s[c + 8 + x]);
           const float mul = kE4m3 ? 1.f : a.scale_log2;
-          mx *= mul;
+          const float mx = mul * fmaxf(max3(max3(mxs[0], mxs[1], mxs[2]), mxs[3], mxs[4]), max3(mxs[5], mxs[6], mxs[7]));
           const bool grow = j > 0 && mx > m + kGrow;
           const float shrink = grow ? exp2_approx(m - mx) : 1.f;
           if (j == 0 || grow) m = mx;
-          const float neg = m == kNegInf ? 0.f : -m;
-          float sum0 = 0.f, sum1 = 0.f;
+          const float2 neg = both(m == kNegInf ? 0.f : -m);
+          float2 sum[2] = {both(0.f), both(0.f)};
           const float4* rv = reinterpret_cast<const float4*>(sh.rv[sc]);
+          // The weights go back over S, 32 positions at a time, and the tensor
+          // cores start on the first half of them.
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t pk[16];
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
               const int c = 32 * q + 2 * i;
-              const float e0 = exp2_approx(kE4m3 ? s[c] + neg : fmaf(s[c], a.scale_log2, neg));
-              const float e1 = exp2_approx(kE4m3 ? s[c + 1] + neg : fmaf(s[c + 1], a.scale_log2, neg));
-              const float e2 = exp2_approx(kE4m3 ? s[c + 2] + neg : fmaf(s[c + 2], a.scale_log2, neg));
-              const float e3 = exp2_approx(kE4m3 ? s[c + 3] + neg : fmaf(s[c + 3], a.scale_log2, neg));
+              float2 x = make_float2(s[c], s[c + 1]), y = make_float2(s[c + 2], s[c + 3]);
+              x = kE4m3 ? add2(x, neg) : fma2(x, both(a.scale_log2), neg);
+              y = kE4m3 ? add2(y, neg) : fma2(y, both(a.scale_log2), neg);
+              x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+              y = i / 2 % 4 < kPoly ? exp2_poly(y) : make_float2(exp2_approx(y.x), exp2_approx(y.y));
               if (kE4m3) {
                 const float4 r4 = rv[c / 4];
-                sum0 = fmaf(e0, r4.x, sum0);
-                sum1 = fmaf(e1, r4.y, sum1);
-                sum0 = fmaf(e2, r4.z, sum0);
-                sum1 = fmaf(e3, r4.w, sum1);
+                sum[0] = fma2(x, make_float2(r4.x, r4.y), sum[0]);
+                sum[1] = fma2(y, make_float2(r4.z, r4.w), sum[1]);
               } else {
-                sum0 += e0 + e1;
-                sum1 += e2 + e3;
+                sum[0] = add2(sum[0], x);
+                sum[1] = add2(sum[1], y);
               }
-              pk[i] = Mma<PT>::pack(e0, e1);
-              pk[i + 1] = Mma<PT>::pack(e2, e3);
+              pk[i] = Mma<PT>::pack(x.x, x.y);
+              pk[i + 1] = Mma<PT>::pack(y.x, y.y);
             }
             tc::st16(t_s + 16 * q, pk);
-          }
-          l = fmaf(l, shrink, sum0 + sum1);
-          if (__any_sync(0xffffffffu, grow)) {
-            // the products before this block have to be in O first
-            if (!wait(&sh.pv_done[half], n_pv + j - 1)) break;
+            if (q == 1) {
+              if (__any_sync(0xffffffffu, grow)) {
+                // the products before this block have to be in O first
+                if (!wait(&sh.pv_done[half], n_pv + j - 1)) break;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tc::ld32(t_o + 32 * c, o);
-              tc::wait_ld();
+                for (int c = 0; c < D / 32; ++c) {
+                  uint32_t o[32];
+                  tc::ld32(t_o + 32 * c, o);
+                  tc::wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-              tc::st32(t_o + 32 * c, o);
+                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+                  tc::st32(t_o + 32 * c, o);
+                }
+              }
+              tc::wait_st();
+              tc::fence_before_sync();
+              mbar_arrive(&sh.p_ready[half]);
             }
           }
+          if (!ok) break;
+          l = fmaf(l, shrink, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
           tc::wait_st();
           tc::fence_before_sync();
-          mbar_arrive(&sh.p_ready[half]);
+          mbar_arrive(&sh.p_rest[half]);
         }
         if (!ok) break;
         n_sc += nb;
@@ -357,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           n_pv += nb;
         }
         const bool complete = w.k0 == 0 && w.k1 == w.g.per;
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = l > 0.f && m != kNegInf ? 1.f / l : 0.f;
         float* part = a.part + static_cast<int64_t>(2 * cta + (w.first ? 0 : 1)) * Part<kTile, D>::kFloats;
         T* dst = static_cast<T*>(a.out.p) + static_cast<int64_t>(w.seq.row0 + tok) * a.out.row_stride +
                  static_cast<int64_t>(w.h * G + hg) * a.out.head_stride;
@@ -507,9 +570,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             v_sc = a.c.v_scale[so];
           }
           long long* const places = sh.at[n_k & 1];
-          places[t] = there ? pg * a.c.page_stride + at * a.c.pos_stride : -1;
+          places[t] = there ? (pg * a.c.page_stride + at * a.c.pos_stride) * kElt : -1;
           named_sync(1, kLoaders);
           if (j + 1 < nb) fetch(j + 1);
+          long long place[kBlock / kPer];  // bytes, of this thread's rows
+#pragma unroll
+          for (int i = 0; i < kBlock / kPer; ++i) place[i] = places[r0 + i * kPer];
           const int st = n_k % kSt;
           const uint32_t parity = (n_k / kSt - 1) & 1;
           for (int kv = 0; kv < 2; ++kv) {
@@ -522,9 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 #pragma unroll
               for (int i = 0; i < kBlock / kPer; ++i) {
                 const int r = r0 + i * kPer;
-                const long long o = places[r];
-                cp_async16(slot + (c >> 3) * C::kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (o < 0 ? 0 : o) * kElt,
-                           o >= 0);
+                cp_async16(slot + (c >> 3) * C::kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                           src + (place[i] < 0 ? 0 : place[i]), place[i] >= 0);
               }
               issued(kv == 0 ? &sh.k_full[st] : &sh.v_full[st]);
             } else {
@@ -538,8 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
               uint4 x[kBlock / kPer];
 #pragma unroll
               for (int i = 0; i < kBlock / kPer; ++i) {
-                const long long o = places[r0 + i * kPer];
-                x[i] = o >= 0 ? *reinterpret_cast<const uint4*>(src + o) : make_uint4(0u, 0u, 0u, 0u);
+                x[i] = place[i] >= 0 ? *reinterpret_cast<const uint4*>(src + place[i]) : make_uint4(0u, 0u, 0u, 0u);
               }
 #pragma unroll
               for (int i = 0; i < kBlock / kPer; ++i) {
@@ -571,7 +635,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     // ---------------------------------------------------------------- MMA --
     regs_dec<kRegsMma>();
     if (warp == 12 && works) {
-      const bool one = lane == 0;
+      const bool one = tc::elect_one();
+      const uint32_t tm = tc::uniform(tmem);
       constexpr uint32_t kFmt = std::is_same<PT, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t kIdescS = tc::idesc_f16(kFmt, 128, kBlock);
       constexpr uint32_t kIdescO = tc::idesc_f16(kFmt, 128, D) | tc::kIdescBMnMajor;
@@ -584,30 +649,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       };
       // Descriptors differ in the start address alone (bits 0-13, units of 16
       // bytes, below 2^14 for any shared address): the rest is added once.
-      const uint32_t dq = static_cast<uint32_t>(tc::smem_desc(s_q, 1024, tc::kLayoutSw128));
-      const uint32_t dk = static_cast<uint32_t>(tc::smem_desc(s_k, 1024, tc::kLayoutSw128));
-      const uint32_t dv = static_cast<uint32_t>(tc::smem_desc_mn128(s_v, C::kHalfBytes, 1024));
+      const uint32_t dq = tc::uniform(static_cast<uint32_t>(tc::smem_desc(s_q, 1024, tc::kLayoutSw128)));
+      const uint32_t dk = tc::uniform(static_cast<uint32_t>(tc::smem_desc(s_k, 1024, tc::kLayoutSw128)));
+      const uint32_t dv = tc::uniform(static_cast<uint32_t>(tc::smem_desc_mn128(s_v, C::kHalfBytes, 1024)));
       const uint32_t hk = static_cast<uint32_t>(tc::smem_desc(s_k, 1024, tc::kLayoutSw128) >> 32);
       const uint32_t hv = static_cast<uint32_t>(tc::smem_desc_mn128(s_v, C::kHalfBytes, 1024) >> 32);
-      auto mma_s = [&](int half, int st) {  // S = Q K^T
+      auto mma_s = [&](int half, uint32_t st) {  // S = Q K^T
         if (one) {
           const uint32_t q = dq + half * (C::kSlot >> 4), k = dk + st * (C::kSlot >> 4);
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             constexpr int kHalf16 = C::kHalfBytes >> 4;
             const int in = (ks >> 2) * kHalf16 + (ks & 3) * 2;
-            tc::mma_f16_lo(tmem + half * 128, q + in, hk, k + in, hk, kIdescS, ks > 0 ? 1u : 0u);
+            tc::mma_f16_lo(tm + half * 128, q, k, hk, in, kIdescS, ks > 0 ? 1u : 0u);
           }
           tc::commit(&sh.s_full[half]);
         }
       };
-      auto mma_o = [&](int half, int st, bool first) {  // O += P V
+      auto mma_o = [&](int half, uint32_t st, bool first) {  // O += P V, as the halves of P come
+        if (!wait(&sh.p_ready[half], n_p[half])) return;
+        const uint32_t v = dv + st * (C::kSlot >> 4);
         if (one) {
-          const uint32_t v = dv + st * (C::kSlot >> 4);
 #pragma unroll
-          for (int ks = 0; ks < kBlock / 16; ++ks)
-            tc::mma_f16_ts_lo(tmem + 256 + half * D, tmem + half * 128 + ks * 8, v + ks * (2048 >> 4), hv, kIdescO,
+          for (int ks = 0; ks < 4; ++ks)
+            tc::mma_f16_ts_lo(tm + 256 + half * D, tm + half * 128, ks * 8, v, hv, ks * (2048 >> 4), kIdescO,
                               first && ks == 0 ? 0u : 1u);
+        }
+        if (!wait(&sh.p_rest[half], n_p[half]++)) return;
+        if (one) {
+#pragma unroll
+          for (int ks = 4; ks < 8; ++ks)
+            tc::mma_f16_ts_lo(tm + 256 + half * D, tm + half * 128, ks * 8, v, hv, ks * (2048 >> 4), kIdescO, 1u);
           tc::commit(&sh.pv_done[half]);
         }
       };
@@ -618,19 +690,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         const bool two = w.has_b();
         if (!wait(&sh.q_full, n_q)) break;
         if (!wait(&sh.k_full[n_k % kSt], n_k / kSt)) break;
-        mma_s(0, n_k % kSt);
-        if (two) mma_s(1, n_k % kSt);
+        const uint32_t st0 = tc::uniform(n_k % kSt);
+        mma_s(0, st0);
+        if (two) mma_s(1, st0);
         if (one) {
           tc::commit(&sh.k_empty[n_k % kSt]);
           if (nb == 1) tc::commit(&sh.q_empty);
         }
         for (int j = 0; j < nb; ++j) {
-          const int st = n_k % kSt, nst = (n_k + 1) % kSt;
+          const uint32_t st = tc::uniform(n_k % kSt), nst = tc::uniform((n_k + 1) % kSt);
           const bool more = j + 1 < nb;
           if (!wait(&sh.v_full[st], n_k / kSt)) break;
-          if (!wait(&sh.p_ready[0], n_p[0])) break;
-          ++n_p[0];
           mma_o(0, st, j == 0);
+          if (!ok) break;
           // S of the next block may be written over P: the tensor cores take
           // the products in the order of their issue
           if (more) {
@@ -638,9 +710,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             mma_s(0, nst);
           }
           if (two) {
-            if (!wait(&sh.p_ready[1], n_p[1])) break;
-            ++n_p[1];
             mma_o(1, st, j == 0);
+            if (!ok) break;
           }
           if (one) tc::commit(&sh.v_empty[st]);
           if (more) {

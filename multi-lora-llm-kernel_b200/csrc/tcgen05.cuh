@@ -29,6 +29,16 @@ __device__ __forceinline__ void fence_after_sync() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// The same value of the whole warp, known to be one: instructions of the
+// tensor cores take their operands from uniform registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // ---- descriptors ----------------------------------------------------------
 // Swizzle codes of the shared-memory matrix descriptor (bits 61..63).
 constexpr uint32_t kLayoutSw128 = 2, kLayoutSw64 = 4, kLayoutSw32 = 6;
@@ -77,22 +87,26 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
 }
 
 // The same with descriptors given as halves: tiles of a ring differ in the low
-// half alone, so that a loop's descriptors take one register each.
-__device__ __forceinline__ void mma_f16_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+// half alone, and `off` (16-byte units) is added where the instruction is
+// issued, so that an unrolled loop keeps no descriptor per step alive.
+__device__ __forceinline__ void mma_f16_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t off,
                                           uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %6, 0;\n\tadd.u32 x, %1, %4;\n\t"
+      "add.u32 y, %2, %4;\n\tmov.b64 a, {x, %3};\n\tmov.b64 b, {y, %3};\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(off), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// D[tmem] (+)= A[tmem] * B[smem]; A: 16-bit pairs, lane = row, 8 columns per 16 of K.
-__device__ __forceinline__ void mma_f16_ts_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
-                                             uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] * B[smem]; A: 16-bit pairs, lane = row, 8 columns per 16
+// of K, `a_off` columns behind a_tmem.
+__device__ __forceinline__ void mma_f16_ts_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t a_off, uint32_t b_lo, uint32_t b_hi,
+                                             uint32_t b_off, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %7, 0;\n\tadd.u32 x, %1, %2;\n\t"
+      "add.u32 y, %3, %5;\n\tmov.b64 b, {y, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %6, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(a_off), "r"(b_lo), "r"(b_hi), "r"(b_off), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
