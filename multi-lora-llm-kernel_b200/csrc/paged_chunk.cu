@@ -47,6 +47,7 @@ constexpr int kLoaders = 128;
 // 2 x 184 + 72 + 72 = 512 <= 4 x 128, what the block is launched with.
 constexpr int kRegsSoftmax = 184, kRegsLoad = 72, kRegsMma = 72, kRegsLaunch = 128;
 static_assert(2 * kRegsSoftmax + kRegsLoad + kRegsMma <= 4 * kRegsLaunch, "register split");
+constexpr int kFirstPart = 3;  // quarters of P that the first products take
 constexpr int kPoly = 0;  // of 8 pairs of exponentials, this many take the polynomial (0 to 4)
 constexpr float kGrow = 8.f;  // log2 of the growth that moves the running maximum
 
@@ -361,18 +362,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           float2 sum[2] = {both(0.f), both(0.f)};
           const float4* rv = reinterpret_cast<const float4*>(sh.rv[sc]);
           // The weights go back over S, 32 positions at a time, and the tensor
-          // cores start on the first half of them.
+          // cores start on the first three quarters of them.
+          auto weights = [&](auto from, auto to) {
+            constexpr int kFrom = decltype(from)::value, kTo = decltype(to)::value;
+            uint32_t pk[(kTo - kFrom) / 2];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const int c = 32 * q + 2 * i;
+            for (int c = kFrom; c < kTo; c += 4) {
               float2 x = make_float2(s[c], s[c + 1]), y = make_float2(s[c + 2], s[c + 3]);
               x = kE4m3 ? add2(x, neg) : fma2(x, both(a.scale_log2), neg);
               y = kE4m3 ? add2(y, neg) : fma2(y, both(a.scale_log2), neg);
               x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-              y = i / 2 % 4 < kPoly ? exp2_poly(y) : make_float2(exp2_approx(y.x), exp2_approx(y.y));
+              y = c / 4 % 4 < kPoly ? exp2_poly(y) : make_float2(exp2_approx(y.x), exp2_approx(y.y));
               if (kE4m3) {
                 const float4 r4 = rv[c / 4];
                 sum[0] = fma2(x, make_float2(r4.x, r4.y), sum[0]);
@@ -381,30 +381,30 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                 sum[0] = add2(sum[0], x);
                 sum[1] = add2(sum[1], y);
               }
-              pk[i] = Mma<PT>::pack(x.x, x.y);
-              pk[i + 1] = Mma<PT>::pack(y.x, y.y);
+              pk[(c - kFrom) / 2] = Mma<PT>::pack(x.x, x.y);
+              pk[(c - kFrom) / 2 + 1] = Mma<PT>::pack(y.x, y.y);
             }
-            tc::st16(t_s + 16 * q, pk);
-            if (q == 1) {
-              if (__any_sync(0xffffffffu, grow)) {
-                // the products before this block have to be in O first
-                if (!wait(&sh.pv_done[half], n_pv + j - 1)) break;
-#pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                  uint32_t o[32];
-                  tc::ld32(t_o + 32 * c, o);
-                  tc::wait_ld();
 #pragma unroll
-                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-                  tc::st32(t_o + 32 * c, o);
-                }
-              }
-              tc::wait_st();
-              tc::fence_before_sync();
-              mbar_arrive(&sh.p_ready[half]);
+            for (int c = 0; c < (kTo - kFrom) / 32; ++c) tc::st16(t_s + kFrom / 2 + 16 * c, pk + 16 * c);
+          };
+          weights(std::integral_constant<int, 0>(), std::integral_constant<int, 32 * kFirstPart>());
+          if (__any_sync(0xffffffffu, grow)) {
+            // the products before this block have to be in O first
+            if (!wait(&sh.pv_done[half], n_pv + j - 1)) break;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tc::ld32(t_o + 32 * c, o);
+              tc::wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+              tc::st32(t_o + 32 * c, o);
             }
           }
-          if (!ok) break;
+          tc::wait_st();
+          tc::fence_before_sync();
+          mbar_arrive(&sh.p_ready[half]);
+          weights(std::integral_constant<int, 32 * kFirstPart>(), std::integral_constant<int, kBlock>());
           l = fmaf(l, shrink, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
           tc::wait_st();
           tc::fence_before_sync();
@@ -671,14 +671,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         const uint32_t v = dv + st * (C::kSlot >> 4);
         if (one) {
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
+          for (int ks = 0; ks < 2 * kFirstPart; ++ks)
             tc::mma_f16_ts_lo(tm + 256 + half * D, tm + half * 128, ks * 8, v, hv, ks * (2048 >> 4), kIdescO,
                               first && ks == 0 ? 0u : 1u);
         }
         if (!wait(&sh.p_rest[half], n_p[half]++)) return;
         if (one) {
 #pragma unroll
-          for (int ks = 4; ks < 8; ++ks)
+          for (int ks = 2 * kFirstPart; ks < 8; ++ks)
             tc::mma_f16_ts_lo(tm + 256 + half * D, tm + half * 128, ks * 8, v, hv, ks * (2048 >> 4), kIdescO, 1u);
           tc::commit(&sh.pv_done[half]);
         }
@@ -701,14 +701,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           const uint32_t st = tc::uniform(n_k % kSt), nst = tc::uniform((n_k + 1) % kSt);
           const bool more = j + 1 < nb;
           if (!wait(&sh.v_full[st], n_k / kSt)) break;
+          if (more && !wait(&sh.k_full[nst], (n_k + 1) / kSt)) break;
           mma_o(0, st, j == 0);
           if (!ok) break;
           // S of the next block may be written over P: the tensor cores take
           // the products in the order of their issue
-          if (more) {
-            if (!wait(&sh.k_full[nst], (n_k + 1) / kSt)) break;
-            mma_s(0, nst);
-          }
+          if (more) mma_s(0, nst);
           if (two) {
             mma_o(1, st, j == 0);
             if (!ok) break;
