@@ -25,6 +25,7 @@ struct PagedCache {
   const int32_t* indptr;
   const int32_t* lengths;
   int num_pages, page_size, max_pages, Hkv, D, B;
+  int page_shift;  // log2(page_size), -1 if it is no power of two
 };
 
 // One [rows, heads, D] activation: unit inner stride, others in elements.
@@ -53,7 +54,7 @@ struct PagedAttention {
   int window;          // 0: none
   float scale_log2;    // softmax scale times log2(e)
   float* part;         // partial results, see paged_attention.cu
-  int4* desc;
+  int4* desc;          // two per CTA
   int32_t* err;
 };
 

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
     for (int w = 0; w < kWarps; ++w) total += s_scan[w];
     __syncthreads();
   }
-  if (tid == 0) a.desc[cta] = make_int4(0, 0, 0, 0);
+  if (tid == 0) a.desc[2 * cta] = make_int4(0, 0, 0, 0);
   // no more CTAs than units, so that every range has one
   const int ctas = static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
   if (cta >= ctas) return;
@@ -159,7 +159,15 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
     const int steps = p_hi > p_lo ? (p_hi - p_lo + kUnit - 1) / kUnit : 0;
 
     // ---- loads ----
-    const Pager pager{a.c.table + b * a.c.table_stride, a.c.page_size, a.c.max_pages, a.c.num_pages, a.err};
+    const int32_t* const pages = a.c.table + b * a.c.table_stride;
+    auto page_of = [&](int p, int& at) {
+      const int pi = page_index(a.c, p);
+      at = p - pi * a.c.page_size;
+      const int pg = pi < a.c.max_pages ? pages[pi] : -1;
+      if (pg >= 0 && pg < a.c.num_pages) return pg;
+      raise_error(a.err, PERSONA_DEV_ERR_PAGE);
+      return -1;
+    };
     const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + static_cast<int64_t>(h) * a.c.head_stride * kElt;
     const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + static_cast<int64_t>(h) * a.c.head_stride * kElt;
     const bool whole = a.c.page_size % kPos == 0;  // a step's positions share a page
@@ -170,7 +178,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
       bool ok = false;
       if (whole && p0 < pend) {
         int at;
-        const int pg = pager.page_of(p0, at);
+        const int pg = page_of(p0, at);
         ok = pg >= 0;
         base = ok ? pg * a.c.page_stride + at * a.c.pos_stride : 0;
         if (kE4m3) sbase = ok ? pg * a.c.scale_page_stride + at : 0;
@@ -187,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           src = live ? base + r * a.c.pos_stride : 0;
         } else {
           int at, pg = -1;
-          if (p0 + r < pend) pg = pager.page_of(p0 + r, at);
+          if (p0 + r < pend) pg = page_of(p0 + r, at);
           live = pg >= 0;
           src = live ? pg * a.c.page_stride + at * a.c.pos_stride : 0;
         }
@@ -206,7 +214,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         bool live = ok && p0 + r < pend;
         if (!whole) {
           int at, pg = -1;
-          if (p0 + r < pend) pg = pager.page_of(p0 + r, at);
+          if (p0 + r < pend) pg = page_of(p0 + r, at);
           live = pg >= 0;
           src = live ? pg * a.c.scale_page_stride + at : 0;
         }
@@ -355,9 +363,9 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           float ks2[2] = {__uint_as_float(lds32(sa)), __uint_as_float(lds32(sa + 4))};
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const float vs = fmaxf(__uint_as_float(lds32(sa + kPos * 4 + 4 * x)), 8.673617379884035e-19f);  // 2^-60
-            lv[n][x] = __log2f(vs);
-            rv[n][x] = __frcp_rn(vs);
+            const float vs = fmaxf(__uint_as_float(lds32(sa + kPos * 4 + 4 * x)), kLeastScale);
+            lv[n][x] = log2_approx(vs);
+            rv[n][x] = rcp_approx(vs);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               sc[mt][n][x] *= ks2[x];
@@ -389,8 +397,10 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
             }
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          m_new[mt][half] = fmaxf(m_run[mt][half], mx);
-          grow |= m_new[mt][half] > m_run[mt][half];
+          // the maximum moves at the first key and when outgrown by 2^8
+          const bool up = mx > (m_run[mt][half] == kNegInf ? kNegInf : m_run[mt][half] + kGrow);
+          m_new[mt][half] = up ? mx : m_run[mt][half];
+          grow |= up;
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -398,8 +408,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           float f[2];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            // a row without a key yet has nothing to rescale
-            f[half] = m_new[mt][half] > m_run[mt][half] ? exp2_approx(m_run[mt][half] - m_new[mt][half]) : 1.f;
+            f[half] = m_new[mt][half] != m_run[mt][half] ? exp2_approx(m_run[mt][half] - m_new[mt][half]) : 1.f;
             l_run[mt][half] *= f[half];
             m_run[mt][half] = m_new[mt][half];
           }
@@ -558,7 +567,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
       long long c = end * ctas / total;
       while (total * (c + 1) / ctas <= end) ++c;
       while (total * c / ctas > end) --c;
-      a.desc[cta] = make_int4(b, item, static_cast<int>(c), first_piece ? 1 : 2);
+      note_cut(a, cta, first_piece, static_cast<int>(c), m0, mrows, seq.row0, h);
     }
     __syncthreads();  // the ring is free again
     off += k1 - k0;
@@ -583,7 +592,7 @@ cudaError_t attention_launch(const PagedAttention& a, cudaStream_t st) {
   const int ctas = kCtasPerSm * sm_count();
   e = launch_paged(k, dim3(ctas), dim3(kThreads), kSmem, 1, st, a);
   if (e != cudaSuccess) return e;
-  return launch_paged(paged_combine_kernel<T, D, 16 * MT>, dim3(ctas), dim3(256), 0, 1, st, a);
+  return launch_paged(paged_combine_kernel<T, D, 16 * MT>, dim3(ctas, 2 * MT), dim3(256), 0, 1, st, a);
 }
 template <typename T, int D, int MT>
 cudaError_t attention_pages(const PagedAttention& a, cudaStream_t st) {
@@ -602,13 +611,13 @@ cudaError_t attention_dim(const PagedAttention& a, int max_new, cudaStream_t st)
 
 size_t paged_attention_ws_bytes(int D) {
   const size_t ctas = static_cast<size_t>(kCtasPerSm) * sm_count();
-  return ctas * sizeof(int4) + ctas * 2 * (32 * static_cast<size_t>(D) + 64) * sizeof(float);
+  return ctas * 2 * sizeof(int4) + ctas * 2 * (32 * static_cast<size_t>(D) + 64) * sizeof(float);
 }
 
 cudaError_t launch_paged_attention(PagedAttention a, int dtype, int max_new, void* workspace, cudaStream_t st) {
   const size_t ctas = static_cast<size_t>(kCtasPerSm) * sm_count();
   a.desc = static_cast<int4*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + ctas * sizeof(int4));
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + ctas * 2 * sizeof(int4));
   return dtype == PERSONA_DTYPE_BF16 ? attention_dim<__nv_bfloat16>(a, max_new, st) : attention_dim<__half>(a, max_new, st);
 }
 

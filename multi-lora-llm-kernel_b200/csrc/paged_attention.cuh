@@ -25,6 +25,23 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// log2 of how far a row's maximum may outgrow the one its weights are taken
+// against before they are rescaled: weights up to 2^8 round as well as those
+// up to 1 do, and a rescaling of all outputs becomes rare.
+constexpr float kGrow = 8.f;
+// Smallest v scale the kernels compute with (its logarithm and reciprocal).
+constexpr float kLeastScale = 8.673617379884035e-19f;  // 2^-60
+
 // A sequence as the kernels see it.
 struct Seq {
   int row0, n, len;  // first row, new tokens, cached positions (new ones among them)
@@ -46,63 +63,77 @@ template <int TR, int D> struct Part {  // one piece: TR x D outputs, TR maxima,
   static constexpr int kFloats = TR * D + 2 * TR;
 };
 
-// Position p of sequence b: its offset (elements) in the pages of head 0 and
-// of the scales.
-struct Pager {
-  const int32_t* row;  // the sequence's page table
-  int page_size, max_pages, num_pages;
-  int32_t* err;
-  __device__ __forceinline__ int page_of(int p, int& at) const {
-    const int pi = p / page_size;
-    at = p - pi * page_size;
-    const int pg = pi < max_pages ? row[pi] : -1;
-    if (pg < 0 || pg >= num_pages) {
-      raise_error(err, PERSONA_DEV_ERR_PAGE);
-      return -1;
-    }
-    return pg;
-  }
-};
+// A CTA notes the tile whose first piece it leaves unfinished, for the kernel
+// below: {part slot of that piece, last CTA with a piece, first row of the
+// tile, rows} and {first row of the sequence, kv head, -, -}; no rows: none.
+__device__ __forceinline__ void note_cut(const PagedAttention& a, int cta, bool first_piece, int last_cta, int m0, int mrows,
+                                         int row0, int h) {
+  a.desc[2 * cta] = make_int4(2 * cta + (first_piece ? 0 : 1), last_cta, m0, mrows);
+  a.desc[2 * cta + 1] = make_int4(row0, h, 0, 0);
+}
 
 // Joins the pieces of one cut tile: CTA c looks after the tile whose first
-// piece CTA c of the attention left.  A warp per row, pieces in order;
-// gridDim.y CTAs share the rows.
+// piece CTA c of the attention left.  A warp per row; gridDim.y CTAs share the
+// rows.  The weights of up to 32 pieces sit in the lanes, so that the pieces'
+// rows are read without waiting for one another, and are added in order.
 template <typename T, int D, int TR>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PagedAttention a) {
   pdl_wait();
   pdl_launch();
-  const int4 d = a.desc[blockIdx.x];
+  const int4 d = a.desc[2 * blockIdx.x];
   if (d.w == 0) return;
+  const int4 e = a.desc[2 * blockIdx.x + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = d.x, tile = d.y / a.c.Hkv, h = d.y % a.c.Hkv, first = blockIdx.x, pieces = d.z - first + 1;
-  const Seq seq = load_seq(a, b);
-  const int m0 = tile * TR, mrows = min(TR, seq.n * a.G - m0);
+  const int first = blockIdx.x, pieces = d.y - first + 1, m0 = d.z, mrows = d.w;
   constexpr int kF = Part<TR, D>::kFloats, kV = D / 32;
-  const float* p0 = a.part + static_cast<int64_t>(2 * first + d.w - 1) * kF;
   // piece i > 0 is the first piece of CTA first + i
-  auto piece = [&](int i) { return i == 0 ? p0 : a.part + static_cast<int64_t>(2 * (first + i)) * kF; };
+  auto piece = [&](int i) { return a.part + static_cast<int64_t>(i == 0 ? d.x : 2 * (first + i)) * kF; };
   for (int m = blockIdx.y * 8 + warp; m < mrows; m += 8 * gridDim.y) {
-    float mx = kNegInf;
-    for (int i = lane; i < pieces; i += 32) mx = fmaxf(mx, piece(i)[TR * D + m]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    float l = 0.f, o[kV];
+    float mx = kNegInf, l = 0.f, o[kV];
 #pragma unroll
     for (int x = 0; x < kV; ++x) o[x] = 0.f;
-    if (mx != kNegInf) {
-#pragma unroll 4
-      for (int i = 0; i < pieces; ++i) {
-        const float* p = piece(i);
-        const float f = exp2_approx(p[TR * D + m] - mx);
-        l = fmaf(f, p[TR * D + TR + m], l);
+    for (int i0 = 0; i0 < pieces; i0 += 32) {
+      const int n = min(32, pieces - i0);
+      float pm = kNegInf, pl = 0.f;
+      if (lane < n) {
+        const float* p = piece(i0 + lane) + TR * D + m;
+        pm = p[0];
+        pl = p[TR];
+      }
+      float top = pm;
 #pragma unroll
-        for (int x = 0; x < kV; ++x) o[x] = fmaf(f, p[m * D + lane * kV + x], o[x]);
+      for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+      top = fmaxf(top, mx);
+      if (top == kNegInf) continue;  // nothing seen so far
+      const float f = exp2_approx(pm - top), old = exp2_approx(mx - top);
+      mx = top;
+      pl *= f;
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) pl += __shfl_xor_sync(0xffffffffu, pl, s);
+      l = fmaf(l, old, pl);
+#pragma unroll
+      for (int x = 0; x < kV; ++x) o[x] *= old;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float* p = piece(i0 + i) + m * D + lane * kV;
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+        if constexpr (kV == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p);
+          o[0] = fmaf(fi, v.x, o[0]);
+          o[1] = fmaf(fi, v.y, o[1]);
+          o[2] = fmaf(fi, v.z, o[2]);
+          o[3] = fmaf(fi, v.w, o[3]);
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(p);
+          o[0] = fmaf(fi, v.x, o[0]);
+          o[1] = fmaf(fi, v.y, o[1]);
+        }
       }
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const int mm = m0 + m, tok = mm / a.G;
-    T* dst = static_cast<T*>(a.out.p) + static_cast<int64_t>(seq.row0 + tok) * a.out.row_stride +
-             static_cast<int64_t>(h * a.G + mm - tok * a.G) * a.out.head_stride + lane * kV;
+    T* dst = static_cast<T*>(a.out.p) + static_cast<int64_t>(e.x + tok) * a.out.row_stride +
+             static_cast<int64_t>(e.y * a.G + mm - tok * a.G) * a.out.head_stride + lane * kV;
 #pragma unroll
     for (int x = 0; x < kV; x += 2)
       *reinterpret_cast<uint32_t*>(dst + x) = Mma<T>::pack(o[x] * inv, o[x + 1] * inv);

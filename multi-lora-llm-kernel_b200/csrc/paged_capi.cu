@@ -39,7 +39,9 @@ int check_cache(const persona_paged_cache* c, int dtype, PagedCache& out) {
   out = PagedCache{c->k, c->v, c->k_scale, c->v_scale, c->page_stride, c->head_stride, c->pos_stride,
                    c->scale_page_stride, c->scale_head_stride, c->page_table, c->table_stride, c->indptr, c->lengths,
                    static_cast<int>(c->num_pages), static_cast<int>(c->page_size), static_cast<int>(c->max_pages),
-                   static_cast<int>(c->Hkv), static_cast<int>(c->D), static_cast<int>(c->B)};
+                   static_cast<int>(c->Hkv), static_cast<int>(c->D), static_cast<int>(c->B), -1};
+  if ((c->page_size & (c->page_size - 1)) == 0)
+    for (out.page_shift = 0; (int64_t{1} << out.page_shift) < c->page_size;) ++out.page_shift;
   return PERSONA_OK;
 }
 

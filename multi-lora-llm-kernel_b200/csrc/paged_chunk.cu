@@ -49,7 +49,6 @@ constexpr int kRegsSoftmax = 184, kRegsLoad = 72, kRegsMma = 72, kRegsLaunch = 1
 static_assert(2 * kRegsSoftmax + kRegsLoad + kRegsMma <= 4 * kRegsLaunch, "register split");
 constexpr int kFirstPart = 3;  // quarters of P that the first products take
 constexpr int kPoly = 0;  // of 8 pairs of exponentials, this many take the polynomial (0 to 4)
-constexpr float kGrow = 8.f;  // log2 of the growth that moves the running maximum
 
 template <int D> struct Cfg {
   static constexpr int kStages = 256 / D;              // k and v slots
@@ -221,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     mbar_init(&sh.drained, 1);
     sh.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    a.desc[cta] = make_int4(0, 0, 0, 0);
+    a.desc[2 * cta] = make_int4(0, 0, 0, 0);
   }
 
   // ---- this CTA's range of units ----
@@ -459,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           long long c = end * ctas / total;
           while (total * (c + 1) / ctas <= end) ++c;
           while (total * c / ctas > end) --c;
-          a.desc[cta] = make_int4(w.b, w.t * a.c.Hkv + w.h, static_cast<int>(c), w.first ? 1 : 2);
+          note_cut(a, cta, w.first, static_cast<int>(c), w.g.m0, w.g.mrows, w.seq.row0, w.h);
         }
       }
     }
@@ -549,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         int pg = -1, at = 0;
         bool seen = false;
         auto fetch = [&](int j) {
-          const int p = (first + j) * kBlock + t, pi = p / a.c.page_size;
+          const int p = (first + j) * kBlock + t, pi = page_index(a.c, p);
           at = p - pi * a.c.page_size;
           seen = p < w.g.pend;
           pg = -1;
@@ -595,10 +594,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             } else {
               if (kv == 0) {
                 const int sc = n_k % C::kScales;
-                const float vs = fmaxf(v_sc, 8.673617379884035e-19f);  // 2^-60
+                const float vs = fmaxf(v_sc, kLeastScale);
                 sh.ks[sc][t] = k_sc;
-                sh.lv[sc][t] = __log2f(vs);
-                sh.rv[sc][t] = __frcp_rn(vs);
+                sh.lv[sc][t] = log2_approx(vs);
+                sh.rv[sc][t] = rcp_approx(vs);
               }
               uint4 x[kBlock / kPer];
 #pragma unroll
@@ -752,7 +751,7 @@ cudaError_t chunk_launch(const PagedAttention& a, cudaStream_t st) {
   const int ctas = sm_count();
   e = launch_paged(k, dim3(ctas), dim3(kThreads), Cfg<D>::kSmem, 1, st, a);
   if (e != cudaSuccess) return e;
-  return launch_paged(paged_combine_kernel<T, D, kTile>, dim3(ctas, 8), dim3(256), 0, 1, st, a);
+  return launch_paged(paged_combine_kernel<T, D, kTile>, dim3(ctas, kTile / 8), dim3(256), 0, 1, st, a);
 }
 template <typename T>
 cudaError_t chunk_for(const PagedAttention& a, cudaStream_t st) {
@@ -765,12 +764,12 @@ cudaError_t chunk_for(const PagedAttention& a, cudaStream_t st) {
 
 size_t paged_chunk_ws_bytes(int D) {
   const size_t ctas = sm_count();
-  return ctas * sizeof(int4) + ctas * 2 * (kTile * static_cast<size_t>(D) + 2 * kTile) * sizeof(float);
+  return ctas * 2 * sizeof(int4) + ctas * 2 * (kTile * static_cast<size_t>(D) + 2 * kTile) * sizeof(float);
 }
 
 cudaError_t launch_paged_chunk(PagedAttention a, int dtype, void* workspace, cudaStream_t st) {
   a.desc = static_cast<int4*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sm_count() * sizeof(int4));
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sm_count() * 2 * sizeof(int4));
   return dtype == PERSONA_DTYPE_BF16 ? chunk_for<__nv_bfloat16>(a, st) : chunk_for<__half>(a, st);
 }
 

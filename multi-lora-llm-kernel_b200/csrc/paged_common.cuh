@@ -9,6 +9,11 @@ namespace persona {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;"); }
 
+// Page of a position.
+__device__ __forceinline__ int page_index(const PagedCache& c, int p) {
+  return c.page_shift >= 0 ? p >> c.page_shift : p / c.page_size;
+}
+
 // The sequence that row r belongs to: the largest b in [0, B) with
 // indptr[b] <= r, or -1.  Warp-wide: 32 probes per step, so one step up to
 // 32 sequences and two up to 1024.  Whatever indptr holds, b stays in range.
@@ -38,7 +43,7 @@ __device__ __forceinline__ bool locate_row(const PagedCache& c, int r, int32_t* 
   if (r >= end) return false;
   const int64_t p = static_cast<int64_t>(c.lengths[b]) - (static_cast<int64_t>(end) - r);
   if (p < 0) return false;
-  const int64_t pi = p / c.page_size;
+  const int64_t pi = p < 2147483647 ? page_index(c, static_cast<int>(p)) : p / c.page_size;
   const int pg = pi < c.max_pages ? c.table[b * c.table_stride + pi] : -1;
   if (pg < 0 || pg >= c.num_pages) {
     if ((threadIdx.x & 31) == 0) raise_error(err, PERSONA_DEV_ERR_PAGE);
