@@ -7,7 +7,7 @@
 // positions of a tile.  The units of all tiles lie in one line (sequence,
 // tile, kv head, block), cut into equal ranges, one per CTA and SM; tiles end
 // at their last row's position, so a range of units is a range of work.  Cut
-// tiles leave pieces that paged_combine_kernel joins in order.
+// tiles leave pieces that a second kernel joins in order.
 //
 // Per block and half: S = Q K^T (operands in shared memory, 128 x 128 fp32
 // accumulator in tensor memory), softmax with one thread per row, P written
@@ -44,10 +44,9 @@ constexpr int kBlock = 128;  // positions of a unit
 constexpr int kTile = 256;   // rows of a tile
 constexpr int kLoaders = 128;
 // Registers per thread after the split: two softmax warpgroups, loaders, MMA.
-// 2 x 184 + 72 + 72 = 512 <= 4 x 128, what the block is launched with.
-constexpr int kRegsSoftmax = 184, kRegsLoad = 72, kRegsMma = 72, kRegsLaunch = 128;
+// 2 x 184 + 96 + 48 = 512 <= 4 x 128, what the block is launched with.
+constexpr int kRegsSoftmax = 184, kRegsLoad = 96, kRegsMma = 48, kRegsLaunch = 128;
 static_assert(2 * kRegsSoftmax + kRegsLoad + kRegsMma <= 4 * kRegsLaunch, "register split");
-constexpr int kFirstPart = 3;  // quarters of P that the first products take
 constexpr int kPoly = 0;  // of 8 pairs of exponentials, this many take the polynomial (0 to 4)
 
 template <int D> struct Cfg {
@@ -70,6 +69,8 @@ struct Shared {
   alignas(16) float ks[5][kBlock];  // read four at a time
   alignas(16) float lv[5][kBlock];
   alignas(16) float rv[5][kBlock];
+  long long q_at[2][kTile];  // offset (elements) of each row of a tile, -1: none; by piece
+  alignas(16) uint8_t stage[8][2048];  // finished rows on their way out, by softmax warp
   float qmul[2][kTile];      // by piece: the next one's rows are loaded while this one's are read
 };
 
@@ -189,6 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   using PT = typename std::conditional<kE4m3, __half, T>::type;  // type of the products
   constexpr bool kScaleQ = kE4m3 && !std::is_same<T, __half>::value;
   constexpr int kSt = C::kStages;
+  constexpr int kFirstPart = kE4m3 ? 2 : 3;  // quarters of P that the first products take (8-bit: registers)
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -331,6 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             const float4* lv = reinterpret_cast<const float4*>(sh.lv[sc]);
 #pragma unroll
             for (int c = 0; c < kBlock; c += 4) {
+              if (c % 16 == 0) asm volatile("" ::: "memory");  // keeps the loads near their use, in few registers
               const float4 k4 = ks[c / 4], l4 = lv[c / 4];
               const float2 x = fma2(mul2(make_float2(s[c], s[c + 1]), make_float2(k4.x, k4.y)), both(qm), make_float2(l4.x, l4.y));
               const float2 y = fma2(mul2(make_float2(s[c + 2], s[c + 3]), make_float2(k4.z, k4.w)), both(qm), make_float2(l4.z, l4.w));
@@ -340,10 +343,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
               s[c + 3] = y.y;
             }
           }
-          if (p0 + kBlock - 1 > all_hi || p0 < all_lo || !live) {
-            const int c1 = hi - p0, c0 = lo - p0;
+          if (p0 + kBlock - 1 > all_hi || p0 < all_lo) {
 #pragma unroll
-            for (int c = 0; c < kBlock; ++c) s[c] = c <= c1 && c >= c0 ? s[c] : kNegInf;
+            for (int x = 0; x < kBlock / 32; ++x) {
+              // bits of the positions that this row sees
+              const int n1 = min(max(hi - p0 + 1 - 32 * x, 0), 32), n0 = min(max(lo - p0 - 32 * x, 0), 32);
+              const uint32_t keep = static_cast<uint32_t>((1ull << n1) - 1) & ~static_cast<uint32_t>((1ull << n0) - 1);
+#pragma unroll
+              for (int c = 0; c < 32; ++c) s[32 * x + c] = (keep & (1u << c)) != 0 ? s[32 * x + c] : kNegInf;
+            }
           }
           float mxs[8];
 #pragma unroll
@@ -361,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           float2 sum[2] = {both(0.f), both(0.f)};
           const float4* rv = reinterpret_cast<const float4*>(sh.rv[sc]);
           // The weights go back over S, 32 positions at a time, and the tensor
-          // cores start on the first three quarters of them.
+          // cores start on the first of them.
           auto weights = [&](auto from, auto to) {
             constexpr int kFrom = decltype(from)::value, kTo = decltype(to)::value;
             uint32_t pk[(kTo - kFrom) / 2];
@@ -373,6 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
               x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
               y = c / 4 % 4 < kPoly ? exp2_poly(y) : make_float2(exp2_approx(y.x), exp2_approx(y.y));
               if (kE4m3) {
+                if (c % 16 == 0) asm volatile("" ::: "memory");
                 const float4 r4 = rv[c / 4];
                 sum[0] = fma2(x, make_float2(r4.x, r4.y), sum[0]);
                 sum[1] = fma2(y, make_float2(r4.z, r4.w), sum[1]);
@@ -421,9 +430,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         const bool complete = w.k0 == 0 && w.k1 == w.g.per;
         const float inv = l > 0.f && m != kNegInf ? 1.f / l : 0.f;
         float* part = a.part + static_cast<int64_t>(2 * cta + (w.first ? 0 : 1)) * Part<kTile, D>::kFloats;
-        T* dst = static_cast<T*>(a.out.p) + static_cast<int64_t>(w.seq.row0 + tok) * a.out.row_stride +
-                 static_cast<int64_t>(w.h * G + hg) * a.out.head_stride;
+        // Finished rows go through 2 KB of shared memory per warp, 32 columns at
+        // a time, so that four lanes write 64 bytes of a row side by side;
+        // pieces are kept column by column, a lane per row.
+        const long long mine = live ? static_cast<int64_t>(w.seq.row0 + tok) * a.out.row_stride +
+                                          static_cast<int64_t>(w.h * G + hg) * a.out.head_stride
+                                    : -1;
+        long long to[4];
+        if (complete) {
 #pragma unroll
+          for (int i = 0; i < 4; ++i) to[i] = __shfl_sync(0xffffffffu, mine, 8 * i + (lane >> 2));
+        }
+        const uint32_t stage = smem_u32(sh.stage[warp]);
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
           if (nb > 0) {
@@ -433,20 +452,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.f;
           }
-          if (live && complete) {
+          if (complete) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              *reinterpret_cast<uint4*>(dst + 32 * c + i) =
-                  make_uint4(Mma<T>::pack(o[i] * inv, o[i + 1] * inv), Mma<T>::pack(o[i + 2] * inv, o[i + 3] * inv),
-                             Mma<T>::pack(o[i + 4] * inv, o[i + 5] * inv), Mma<T>::pack(o[i + 6] * inv, o[i + 7] * inv));
-          } else if (live) {
+            for (int i = 0; i < 4; ++i)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)),
+                           "r"(Mma<T>::pack(o[8 * i] * inv, o[8 * i + 1] * inv)), "r"(Mma<T>::pack(o[8 * i + 2] * inv, o[8 * i + 3] * inv)),
+                           "r"(Mma<T>::pack(o[8 * i + 4] * inv, o[8 * i + 5] * inv)), "r"(Mma<T>::pack(o[8 * i + 6] * inv, o[8 * i + 7] * inv))
+                           : "memory");
+            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(part + r * D + 32 * c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            for (int i = 0; i < 4; ++i) {
+              const int row = 8 * i + (lane >> 2);
+              const uint4 v = lds128(stage + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
+              if (to[i] >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(a.out.p) + to[i] + 32 * c + 8 * (lane & 3)) = v;
+            }
+            __syncwarp();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) part[(32 * c + i) * kTile + r] = o[i];
           }
-          __syncwarp();
         }
-        if (live && !complete) {
+        if (!complete) {
           part[kTile * D + r] = m;
           part[kTile * D + kTile + r] = l;
         }
@@ -466,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     // -------------------------------------------------------------- loads --
     regs_dec<kRegsLoad>();
     const int t = tid - 256;
-    int n_k = 0, n_q = 0;  // blocks and pieces so far
+    int n_k = 0, n_q = 0, n_at = 0;  // blocks, pieces and published blocks so far
     bool ok = true;
     uint64_t* pending = nullptr;  // loads under way whose arrival is due
     auto flush = [&]() {
@@ -501,40 +527,60 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         // ---- q rows ----
         if (n_q > 0) ok = ok && acquire(&sh.q_empty, (n_q - 1) & 1);
         if (ok) {
-          constexpr int kCh = D / 8, kPer = kLoaders / kCh;
+          // thread t works out where rows t and 128 + t are
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int i = t + 128 * x, mm = w.g.m0 + i, tok = mm / G;
+            sh.q_at[n_q & 1][i] = i < w.g.mrows ? static_cast<int64_t>(tok) * a.q.row_stride +
+                                                      static_cast<int64_t>(mm - tok * G) * a.q.head_stride
+                                                : -1;
+          }
+        }
+        named_sync(1, kLoaders);
+        if (ok) {
+          constexpr int kCh = D / 8, kPer = kLoaders / kCh, kAhead = 8;
           const int c = t % kCh, rows = w.has_b() ? 256 : 128;
           const T* qb = static_cast<const T*>(a.q.p) + static_cast<int64_t>(w.seq.row0) * a.q.row_stride +
                         static_cast<int64_t>(w.h * G) * a.q.head_stride + c * 8;
-          for (int i = t / kCh; i < rows; i += kPer) {
-            const bool live = i < w.g.mrows;
-            const int mm = w.g.m0 + (live ? i : 0), tok = mm / G, hg = mm - tok * G;
-            const T* src = qb + static_cast<int64_t>(tok) * a.q.row_stride + static_cast<int64_t>(hg) * a.q.head_stride;
-            const int r = i & 127;
-            const uint32_t dst = s_q + (i >> 7) * C::kSlot + (c >> 3) * C::kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-            if (!kScaleQ) {
-              cp_async16(dst, src, live);
+          for (int i0 = t / kCh; i0 < rows; i0 += kPer * kAhead) {
+            long long from[kAhead];
+#pragma unroll
+            for (int x = 0; x < kAhead; ++x) from[x] = sh.q_at[n_q & 1][i0 + x * kPer];
+            auto place = [&](int i) {
+              return s_q + (i >> 7) * C::kSlot + (c >> 3) * C::kHalfBytes + (i & 127) * 128 + (((c & 7) ^ (i & 7)) << 4);
+            };
+            if constexpr (!kScaleQ) {
+#pragma unroll
+              for (int x = 0; x < kAhead; ++x) cp_async16(place(i0 + x * kPer), qb + (from[x] < 0 ? 0 : from[x]), from[x] >= 0);
             } else {
               // bf16 row -> fp16, scaled by the power of two that brings its
               // largest element into [1, 2)
-              const uint4 v = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
-              const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-              float f[8], mx = 0.f;
+              uint4 v[kAhead];
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const float2 p = Cvt<T>::to2(u[x]);
-                f[2 * x] = p.x;
-                f[2 * x + 1] = p.y;
-                mx = fmaxf(mx, fmaxf(fabsf(p.x), fabsf(p.y)));
+              for (int x = 0; x < kAhead; ++x)
+                v[x] = from[x] >= 0 ? __ldg(reinterpret_cast<const uint4*>(qb + from[x])) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+              for (int x = 0; x < kAhead; ++x) {
+                const int i = i0 + x * kPer;
+                const uint32_t u[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+                float f[8], mx = 0.f;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const float2 p = Cvt<T>::to2(u[y]);
+                  f[2 * y] = p.x;
+                  f[2 * y + 1] = p.y;
+                  mx = fmaxf(mx, fmaxf(fabsf(p.x), fabsf(p.y)));
+                }
+#pragma unroll
+                for (int o = kCh / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23), 2), 252);
+                const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+                if (c == 0) sh.qmul[n_q & 1][i] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e) << 23);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(i)), "r"(Mma<__half>::pack(f[0] * down, f[1] * down)),
+                             "r"(Mma<__half>::pack(f[2] * down, f[3] * down)), "r"(Mma<__half>::pack(f[4] * down, f[5] * down)),
+                             "r"(Mma<__half>::pack(f[6] * down, f[7] * down))
+                             : "memory");
               }
-#pragma unroll
-              for (int o = kCh / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-              const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23), 2), 252);
-              const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-              if (c == 0) sh.qmul[n_q & 1][i] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e) << 23);
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(Mma<__half>::pack(f[0] * down, f[1] * down)),
-                           "r"(Mma<__half>::pack(f[2] * down, f[3] * down)), "r"(Mma<__half>::pack(f[4] * down, f[5] * down)),
-                           "r"(Mma<__half>::pack(f[6] * down, f[7] * down))
-                           : "memory");
             }
           }
         }
@@ -559,31 +605,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         const int c = t % kCh, r0 = t / kCh;
         const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + static_cast<int64_t>(w.h) * a.c.head_stride * kElt + c * 16;
         const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + static_cast<int64_t>(w.h) * a.c.head_stride * kElt + c * 16;
-        for (int j = 0; j < nb; ++j) {
-          float k_sc = 0.f, v_sc = 0.f;
+        float k_sc = 0.f, v_sc = 0.f;
+        long long place[kBlock / kPer];  // bytes, of this thread's rows
+        auto publish = [&](int j) {      // of block j, and its scales
           const bool there = pg >= 0 && pg < a.c.num_pages;
           if (seen && !there) raise_error(err, PERSONA_DEV_ERR_PAGE);
-          if (kE4m3 && there) {
-            const int64_t so = pg * a.c.scale_page_stride + at + static_cast<int64_t>(w.h) * a.c.scale_head_stride;
-            k_sc = a.c.k_scale[so];
-            v_sc = a.c.v_scale[so];
+          if (kE4m3) {
+            k_sc = v_sc = 0.f;
+            if (there) {
+              const int64_t so = pg * a.c.scale_page_stride + at + static_cast<int64_t>(w.h) * a.c.scale_head_stride;
+              k_sc = a.c.k_scale[so];
+              v_sc = a.c.v_scale[so];
+            }
           }
-          long long* const places = sh.at[n_k & 1];
+          long long* const places = sh.at[n_at & 1];
+          ++n_at;
           places[t] = there ? (pg * a.c.page_stride + at * a.c.pos_stride) * kElt : -1;
           named_sync(1, kLoaders);
           if (j + 1 < nb) fetch(j + 1);
-          long long place[kBlock / kPer];  // bytes, of this thread's rows
 #pragma unroll
           for (int i = 0; i < kBlock / kPer; ++i) place[i] = places[r0 + i * kPer];
-          const int st = n_k % kSt;
-          const uint32_t parity = (n_k / kSt - 1) & 1;
-          for (int kv = 0; kv < 2; ++kv) {
-            uint64_t* empty = kv == 0 ? &sh.k_empty[st] : &sh.v_empty[st];
-            if (n_k >= kSt) ok = ok && acquire(empty, parity);
-            if (!ok) continue;
-            const uint8_t* src = kv == 0 ? kb : vb;
-            const uint32_t slot = (kv == 0 ? s_k : s_v) + st * C::kSlot;
-            if (!kE4m3) {
+        };
+        publish(0);
+        if constexpr (!kE4m3) {
+          for (int j = 0; j < nb; ++j) {
+            const int st = n_k % kSt;
+            const uint32_t parity = (n_k / kSt - 1) & 1;
+            for (int kv = 0; kv < 2; ++kv) {
+              if (n_k >= kSt) ok = ok && acquire(kv == 0 ? &sh.k_empty[st] : &sh.v_empty[st], parity);
+              if (!ok) continue;
+              const uint8_t* src = kv == 0 ? kb : vb;
+              const uint32_t slot = (kv == 0 ? s_k : s_v) + st * C::kSlot;
 #pragma unroll
               for (int i = 0; i < kBlock / kPer; ++i) {
                 const int r = r0 + i * kPer;
@@ -591,41 +643,63 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                            src + (place[i] < 0 ? 0 : place[i]), place[i] >= 0);
               }
               issued(kv == 0 ? &sh.k_full[st] : &sh.v_full[st]);
-            } else {
-              if (kv == 0) {
-                const int sc = n_k % C::kScales;
-                const float vs = fmaxf(v_sc, kLeastScale);
-                sh.ks[sc][t] = k_sc;
-                sh.lv[sc][t] = log2_approx(vs);
-                sh.rv[sc][t] = rcp_approx(vs);
-              }
-              uint4 x[kBlock / kPer];
+            }
+            ++n_k;
+            if (j + 1 < nb) publish(j + 1);
+          }
+        } else {
+          // Codes go through registers: while one tile's are converted and
+          // stored, the next tile's (k, v, the next block's k, ...) are loaded
+          // into the registers that this frees.
+          uint4 x[kBlock / kPer];
+          auto load = [&](int i, const uint8_t* src) {
+            x[i] = place[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(src + place[i])) : make_uint4(0u, 0u, 0u, 0u);
+          };
+          auto convert = [&](uint32_t slot, const uint8_t* next) {
 #pragma unroll
-              for (int i = 0; i < kBlock / kPer; ++i) {
-                x[i] = place[i] >= 0 ? *reinterpret_cast<const uint4*>(src + place[i]) : make_uint4(0u, 0u, 0u, 0u);
-              }
+            for (int i = 0; i < kBlock / kPer; ++i) {
+              const int r = r0 + i * kPer;
+              const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+              if (next != nullptr) load(i, next);
 #pragma unroll
-              for (int i = 0; i < kBlock / kPer; ++i) {
-                const int r = r0 + i * kPer;
-                const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                  const int cc = 2 * c + y;
-                  uint32_t hh[4];
-                  e4m3x4_to_half(u[2 * y], hh[0], hh[1]);
-                  e4m3x4_to_half(u[2 * y + 1], hh[2], hh[3]);
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                   slot + (cc >> 3) * C::kHalfBytes + r * 128 + (((cc & 7) ^ (r & 7)) << 4)),
-                               "r"(hh[0]), "r"(hh[1]), "r"(hh[2]), "r"(hh[3])
-                               : "memory");
-                }
+              for (int y = 0; y < 2; ++y) {
+                const int cc = 2 * c + y;
+                uint32_t hh[4];
+                e4m3x4_to_half(u[2 * y], hh[0], hh[1]);
+                e4m3x4_to_half(u[2 * y + 1], hh[2], hh[3]);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                 slot + (cc >> 3) * C::kHalfBytes + r * 128 + (((cc & 7) ^ (r & 7)) << 4)),
+                             "r"(hh[0]), "r"(hh[1]), "r"(hh[2]), "r"(hh[3])
+                             : "memory");
               }
+            }
+          };
+#pragma unroll
+          for (int i = 0; i < kBlock / kPer; ++i) load(i, kb);
+          for (int j = 0; j < nb; ++j) {
+            const int st = n_k % kSt;
+            const uint32_t parity = (n_k / kSt - 1) & 1;
+            if (n_k >= kSt) ok = ok && acquire(&sh.k_empty[st], parity);
+            if (ok) {
+              const int sc = n_k % C::kScales;
+              const float vs = fmaxf(v_sc, kLeastScale);
+              sh.ks[sc][t] = k_sc;
+              sh.lv[sc][t] = log2_approx(vs);
+              sh.rv[sc][t] = rcp_approx(vs);
+              convert(s_k + st * C::kSlot, vb);
               flush();
               tc::fence_proxy_async();
-              mbar_arrive(kv == 0 ? &sh.k_full[st] : &sh.v_full[st]);
+              mbar_arrive(&sh.k_full[st]);
             }
+            if (j + 1 < nb) publish(j + 1);
+            if (n_k >= kSt) ok = ok && acquire(&sh.v_empty[st], parity);
+            if (ok) {
+              convert(s_v + st * C::kSlot, j + 1 < nb ? kb : nullptr);
+              tc::fence_proxy_async();
+              mbar_arrive(&sh.v_full[st]);
+            }
+            ++n_k;
           }
-          ++n_k;
         }
       }
       flush();
@@ -738,6 +812,46 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   }
 }
 
+// Joins the pieces of one cut tile, which lie column by column: CTA (c, y)
+// looks after rows [32 y, 32 y + 32) of the tile whose first piece CTA c left;
+// a lane is a row, a warp an eighth of the columns.  Pieces in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_chunk_join_kernel(const __grid_constant__ PagedAttention a) {
+  pdl_wait();
+  pdl_launch();
+  const int4 d = a.desc[2 * blockIdx.x];
+  const int r = blockIdx.y * 32 + (threadIdx.x & 31);
+  if (static_cast<int>(blockIdx.y) * 32 >= d.w) return;
+  const int4 e = a.desc[2 * blockIdx.x + 1];
+  constexpr int kF = Part<kTile, D>::kFloats, kV = D / 8;
+  const int first = blockIdx.x, pieces = d.y - first + 1, c0 = (threadIdx.x >> 5) * kV;
+  auto piece = [&](int i) { return a.part + static_cast<int64_t>(i == 0 ? d.x : 2 * (first + i)) * kF; };
+  float mx = kNegInf, l = 0.f, o[kV];
+#pragma unroll
+  for (int x = 0; x < kV; ++x) o[x] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < pieces; ++i) mx = fmaxf(mx, piece(i)[kTile * D + r]);
+  const float neg = mx == kNegInf ? 0.f : -mx;  // a row that saw nothing: weights of 0
+#pragma unroll 2
+  for (int i = 0; i < pieces; ++i) {
+    const float* p = piece(i);
+    const float f = exp2_approx(p[kTile * D + r] + neg);
+    l = fmaf(f, p[kTile * D + kTile + r], l);
+#pragma unroll
+    for (int x = 0; x < kV; ++x) o[x] = fmaf(f, p[(c0 + x) * kTile + r], o[x]);
+  }
+  if (r >= d.w) return;
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int mm = d.z + r, tok = mm / a.G;
+  T* dst = static_cast<T*>(a.out.p) + static_cast<int64_t>(e.x + tok) * a.out.row_stride +
+           static_cast<int64_t>(e.y * a.G + mm - tok * a.G) * a.out.head_stride + c0;
+#pragma unroll
+  for (int x = 0; x < kV; x += 8)
+    *reinterpret_cast<uint4*>(dst + x) =
+        make_uint4(Mma<T>::pack(o[x] * inv, o[x + 1] * inv), Mma<T>::pack(o[x + 2] * inv, o[x + 3] * inv),
+                   Mma<T>::pack(o[x + 4] * inv, o[x + 5] * inv), Mma<T>::pack(o[x + 6] * inv, o[x + 7] * inv));
+}
+
 template <typename T, int D, bool kE4m3>
 cudaError_t chunk_launch(const PagedAttention& a, cudaStream_t st) {
   auto k = paged_chunk_kernel<T, D, kE4m3>;
@@ -751,7 +865,7 @@ cudaError_t chunk_launch(const PagedAttention& a, cudaStream_t st) {
   const int ctas = sm_count();
   e = launch_paged(k, dim3(ctas), dim3(kThreads), Cfg<D>::kSmem, 1, st, a);
   if (e != cudaSuccess) return e;
-  return launch_paged(paged_combine_kernel<T, D, kTile>, dim3(ctas, kTile / 8), dim3(256), 0, 1, st, a);
+  return launch_paged(paged_chunk_join_kernel<T, D>, dim3(ctas, kTile / 32), dim3(256), 0, 1, st, a);
 }
 template <typename T>
 cudaError_t chunk_for(const PagedAttention& a, cudaStream_t st) {
