@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         float* part = a.part + static_cast<int64_t>(2 * cta + (w.first ? 0 : 1)) * Part<kTile, D>::kFloats;
         // Finished rows go through 2 KB of shared memory per warp, 32 columns at
         // a time, so that four lanes write 64 bytes of a row side by side;
-        // pieces are kept column by column, a lane per row.
+        // pieces are kept four columns by four, a lane per row.
         const long long mine = live ? static_cast<int64_t>(w.seq.row0 + tok) * a.out.row_stride +
                                           static_cast<int64_t>(w.h * G + hg) * a.out.head_stride
                                     : -1;
@@ -469,7 +469,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             __syncwarp();
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) part[(32 * c + i) * kTile + r] = o[i];
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(part + (8 * c + i / 4) * (4 * kTile) + 4 * r) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         }
         if (!complete) {
@@ -812,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   }
 }
 
-// Joins the pieces of one cut tile, which lie column by column: CTA (c, y)
+// Joins the pieces of one cut tile, which lie four columns by four: CTA (c, y)
 // looks after rows [32 y, 32 y + 32) of the tile whose first piece CTA c left;
 // a lane is a row, a warp an eighth of the columns.  Pieces in order.
 template <typename T, int D>
@@ -838,7 +839,13 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const __grid_cons
     const float f = exp2_approx(p[kTile * D + r] + neg);
     l = fmaf(f, p[kTile * D + kTile + r], l);
 #pragma unroll
-    for (int x = 0; x < kV; ++x) o[x] = fmaf(f, p[(c0 + x) * kTile + r], o[x]);
+    for (int x = 0; x < kV; x += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + (c0 + x) * kTile + 4 * r);
+      o[x] = fmaf(f, v.x, o[x]);
+      o[x + 1] = fmaf(f, v.y, o[x + 1]);
+      o[x + 2] = fmaf(f, v.z, o[x + 2]);
+      o[x + 3] = fmaf(f, v.w, o[x + 3]);
+    }
   }
   if (r >= d.w) return;
   const float inv = l > 0.f ? 1.f / l : 0.f;
