@@ -1039,6 +1039,13 @@ void sgmv_fused_tp_op(const at::Tensor& x, const at::Tensor& a_pool, const at::T
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  // The paged-cache ops for persona.ops, past the dispatcher: half of a small
+  // call's time on the host is spent there.  The same functions are registered
+  // as torch.ops.persona.*.
+  m.def("paged_rope_cache", &paged_rope_cache_op);
+  m.def("paged_cache_read", &paged_cache_read_op);
+  m.def("paged_attention", &paged_attention_op);
+  m.def("verify_draft", &verify_draft_op);
   m.def("sgmv_fused_tp", &sgmv_fused_tp_op,
         "Tensor-parallel segmented fused LoRA: columns [n0, n1) of y, every finished tile also stored into the "
         "peers' y (pointers from ipc_import).");

@@ -43,6 +43,9 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kPos = 16;              // positions of one warp step
 constexpr int kUnit = kPos * kWarps;  // positions of one unit
+// What starting and ending a tile costs, in units: so many stand before its
+// first one in the line.  None where every unit has a CTA of its own.
+constexpr int kPieceUnits = 3;
 
 __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -70,9 +73,9 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   constexpr int kSlot = 2 * kHalf + (kE4m3 ? 2 * kPos * 4 : 0);
   constexpr int kSteps = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long s_scan[kWarps + 1];
+  __shared__ long long s_scan[kWarps], s_items[kWarps], s_begin;
   __shared__ int s_b;
-  __shared__ long long s_off;
+  __shared__ long long s_off, s_end;
   __shared__ float s_m[kWarps][TR], s_l[kWarps][TR];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -82,35 +85,58 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   pdl_launch();
 
   // ---- this CTA's range of units ----
-  long long total = 0;
+  auto count = [&](int b, int& per) -> int {  // tiles times heads, units of each
+    if (b >= a.c.B) return 0;
+    int tiles, first;
+    seq_units(load_seq(a, b), a.window, TR, G, tiles, first, per);
+    return tiles * Hkv;
+  };
+  long long total = 0, items = 0;
+  int my_items = 0, my_per = 0;
   for (int b0 = 0; b0 < a.c.B; b0 += kThreads) {
-    long long u = 0;
-    if (b0 + tid < a.c.B) {
-      int tiles, first, per;
-      seq_units(load_seq(a, b0 + tid), a.window, TR, G, tiles, first, per);
-      u = static_cast<long long>(tiles) * per * Hkv;
+    int per = 0;
+    const int n = count(b0 + tid, per);
+    if (b0 == 0) {
+      my_items = n;
+      my_per = per;
     }
+    long long u = static_cast<long long>(n) * per, v = n;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-    if (lane == 0) s_scan[warp] = u;
+    for (int o = 16; o > 0; o >>= 1) {
+      u += __shfl_xor_sync(0xffffffffu, u, o);
+      v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    if (lane == 0) {
+      s_scan[warp] = u;
+      s_items[warp] = v;
+    }
     __syncthreads();
-    for (int w = 0; w < kWarps; ++w) total += s_scan[w];
+    for (int w = 0; w < kWarps; ++w) {
+      total += s_scan[w];
+      items += s_items[w];
+    }
     __syncthreads();
   }
+  const int lead = total <= gridDim.x ? 0 : kPieceUnits;
+  total += lead * items;
   if (tid == 0) a.desc[2 * cta] = make_int4(0, 0, 0, 0);
-  // no more CTAs than units, so that every range has one
+  // no more CTAs than units, so that every range (before the move below) has one
   const int ctas = static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
   if (cta >= ctas) return;
-  const long long u0 = total * cta / ctas, u1 = total * (cta + 1) / ctas;
+  // a cut inside what a tile costs to start is moved before it
+  const long long raw0 = total * cta / ctas, raw1 = total * (cta + 1) / ctas;
+  auto start_of = [&](long long off, int per) {
+    const int k = static_cast<int>(off % per);
+    return k < lead ? off - k : off;
+  };
+  if (tid == 0) s_end = raw1;
   {
     long long run = 0;
-    for (int b0 = 0; b0 < a.c.B; b0 += kThreads) {
-      long long u = 0;
-      if (b0 + tid < a.c.B) {
-        int tiles, first, per;
-        seq_units(load_seq(a, b0 + tid), a.window, TR, G, tiles, first, per);
-        u = static_cast<long long>(tiles) * per * Hkv;
-      }
+    for (int b0 = 0; b0 < a.c.B && run <= raw1; b0 += kThreads) {
+      int per = my_per;
+      const int n = b0 == 0 ? my_items : count(b0 + tid, per);
+      per += lead;
+      const long long u = static_cast<long long>(n) * per;
       long long inc = u;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -119,17 +145,20 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
       }
       if (lane == 31) s_scan[warp] = inc;
       __syncthreads();
-      long long base = run;
-      for (int w = 0; w < warp; ++w) base += s_scan[w];
-      const long long lo = base + inc - u;
-      if (u0 >= lo && u0 < lo + u) {
+      long long lo = run + inc - u;
+      for (int w = 0; w < warp; ++w) lo += s_scan[w];
+      if (raw0 >= lo && raw0 < lo + u) {
         s_b = b0 + tid;
-        s_off = u0 - lo;
+        s_off = start_of(raw0 - lo, per);
+        s_begin = lo + s_off;
       }
+      if (raw1 >= lo && raw1 < lo + u) s_end = lo + start_of(raw1 - lo, per);
       for (int w = 0; w < kWarps; ++w) run += s_scan[w];
       __syncthreads();
     }
   }
+  const long long u0 = s_begin, u1 = s_end;
+  if (u0 >= u1) return;
   int b = s_b;
   long long off = s_off;
   long long left = u1 - u0;
@@ -139,12 +168,14 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   Seq seq = load_seq(a, b);
   int tiles, kfirst, per;
   seq_units(seq, a.window, TR, G, tiles, kfirst, per);
+  per += lead;
   while (left > 0) {
     while (off >= static_cast<long long>(tiles) * per * Hkv) {  // the next sequence with units
       off -= static_cast<long long>(tiles) * per * Hkv;
       if (++b >= a.c.B) return;  // the arrays changed under the call
       seq = load_seq(a, b);
       seq_units(seq, a.window, TR, G, tiles, kfirst, per);
+      per += lead;
     }
     const int item = static_cast<int>(off / per), k0 = static_cast<int>(off - static_cast<long long>(item) * per);
     const int k1 = static_cast<int>(min(static_cast<long long>(per), k0 + left));
@@ -155,7 +186,8 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
     const int pend = max(0, min(seq.len, ctx + tok1 + 1));  // keys of the tile end here
     const int pbegin = a.window > 0 ? max(0, ctx + tok0 + 1 - a.window) : 0;
     // positions of the steps of this piece that have any key
-    const int p_lo = max((kfirst + k0) * kUnit, pbegin / kUnit * kUnit), p_hi = min((kfirst + k1) * kUnit, pend);
+    const int p_lo = max((kfirst + max(k0 - lead, 0)) * kUnit, pbegin / kUnit * kUnit);
+    const int p_hi = min((kfirst + max(k1 - lead, 0)) * kUnit, pend);
     const int steps = p_hi > p_lo ? (p_hi - p_lo + kUnit - 1) / kUnit : 0;
 
     // ---- loads ----
@@ -587,7 +619,8 @@ cudaError_t attention_launch(const PagedAttention& a, cudaStream_t st) {
   constexpr int kRing = kWarps * kStages * kSlot, kJoin = kWarps * 16 * MT * D * 4;
   constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
   auto k = paged_attention_kernel<T, D, MT, kE4m3, kStages>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static std::atomic<bool> done[64];
+  cudaError_t e = prepare_kernel(done, k, kSmem, 0);
   if (e != cudaSuccess) return e;
   const int ctas = kCtasPerSm * sm_count();
   e = launch_paged(k, dim3(ctas), dim3(kThreads), kSmem, 1, st, a);

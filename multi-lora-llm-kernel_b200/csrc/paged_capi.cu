@@ -81,9 +81,10 @@ int persona_paged_rope_cache(const persona_paged_cache* cache, const persona_row
   a.rows = static_cast<int>(rows);
   a.Hq = static_cast<int>(Hq);
   const int D = a.c.D;
-  const double two_pi = 6.283185307179586476925;
-  for (int j = 0; j < 64; ++j)
-    a.turns[j] = j < D / 2 ? std::pow(static_cast<double>(theta), -2.0 * j / D) / two_pi : 0.0;
+  // theta^(-2j / D) / (2 pi) by multiplication: 63 roundings of 2^-53
+  const double ratio = std::pow(static_cast<double>(theta), -2.0 / D);
+  double f = 1.0 / 6.283185307179586476925;
+  for (int j = 0; j < 64; ++j, f *= ratio) a.turns[j] = j < D / 2 ? f : 0.0;
   return status(launch_paged_write(a, dtype, dev_err, stream));
 }
 

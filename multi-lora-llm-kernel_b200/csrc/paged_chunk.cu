@@ -862,13 +862,10 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const __grid_cons
 template <typename T, int D, bool kE4m3>
 cudaError_t chunk_launch(const PagedAttention& a, cudaStream_t st) {
   auto k = paged_chunk_kernel<T, D, kE4m3>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
-  if (e != cudaSuccess) return e;
+  static std::atomic<bool> done[64];
   // the register split above draws on kRegsLaunch registers a thread
-  cudaFuncAttributes attr;
-  e = cudaFuncGetAttributes(&attr, k);
+  cudaError_t e = prepare_kernel(done, k, Cfg<D>::kSmem, kRegsLaunch);
   if (e != cudaSuccess) return e;
-  if (attr.numRegs != kRegsLaunch) return cudaErrorInvalidConfiguration;
   const int ctas = sm_count();
   e = launch_paged(k, dim3(ctas), dim3(kThreads), Cfg<D>::kSmem, 1, st, a);
   if (e != cudaSuccess) return e;

@@ -241,6 +241,15 @@ def bgmv_lora_delta_multi(xs, a_pools, b_pools, slots: torch.Tensor, deltas):
 
 
 # ---- paged KV cache and drafted tokens ---------------------------------------
+# These calls are short enough for the host's time to count: they go straight
+# to the extension's functions (the same as torch.ops.persona.*), which check
+# every tensor themselves.
+def _paged(op: str, first: torch.Tensor):
+    if not first.is_cuda:
+        _require_cuda(op, first)
+    return _load()
+
+
 def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                      page_table: torch.Tensor, indptr: torch.Tensor, lengths: torch.Tensor, theta: float,
                      q_out: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
@@ -257,9 +266,8 @@ def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache:
     ``float8_e4m3fn`` take fp32 scales [pages, Hkv, page size]: one per token
     and head, ``max|x| / 448``.  Rows of no sequence are left alone."""
     q_out = q if q_out is None else q_out
-    _require_cuda("paged_rope_cache", q, k, v, k_cache, v_cache, page_table, indptr, lengths, q_out)
-    torch.ops.persona.paged_rope_cache(q, k, v, q_out, k_cache, v_cache, page_table, indptr, lengths, theta, k_scale,
-                                       v_scale)
+    _paged("paged_rope_cache", q).paged_rope_cache(q, k, v, q_out, k_cache, v_cache, page_table, indptr, lengths, theta,
+                                                   k_scale, v_scale)
     return q_out
 
 
@@ -269,8 +277,8 @@ def paged_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: t
     """k and v of the last ``indptr[b+1] - indptr[b]`` positions of each
     sequence, out of the pages into ``k_out`` / ``v_out`` [rows, Hkv, D]
     (e4m3 pages: code times scale)."""
-    _require_cuda("paged_cache_read", k_cache, v_cache, page_table, indptr, lengths, k_out, v_out)
-    torch.ops.persona.paged_cache_read(k_cache, v_cache, page_table, indptr, lengths, k_out, v_out, k_scale, v_scale)
+    _paged("paged_cache_read", k_cache).paged_cache_read(k_cache, v_cache, page_table, indptr, lengths, k_out, v_out,
+                                                         k_scale, v_scale)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -285,11 +293,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``max_new``: an upper bound of the new tokens of one sequence, which
     chooses the kernel (default: what ``rows`` allows if every sequence has
     a token); it never changes what is computed."""
-    _require_cuda("paged_attention", q, k_cache, v_cache, page_table, indptr, lengths, out)
+    ext = _paged("paged_attention", q)
     if max_new is None:
         max_new = max(1, q.shape[0] - lengths.shape[0] + 1)
-    torch.ops.persona.paged_attention(q, k_cache, v_cache, page_table, indptr, lengths, out, scale, window, max_new,
-                                      k_scale, v_scale)
+    ext.paged_attention(q, k_cache, v_cache, page_table, indptr, lengths, out, scale, window, max_new, k_scale, v_scale)
     return out
 
 
@@ -307,7 +314,6 @@ def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_p
     is drawn with ``u_sample[b]``: from ``max(p - q, 0)`` where a draft was
     rejected, else from the last row.  ``tokens`` [rows] int64: the kept
     drafts, the drawn token, then -1; ``accepted`` [B] int32: how many."""
-    _require_cuda("verify_draft", target_probs, draft_tokens, indptr, u_accept, u_sample, tokens, accepted)
-    torch.ops.persona.verify_draft(target_probs, draft_tokens, draft_probs, indptr, u_accept, u_sample, tokens,
-                                   accepted)
+    _paged("verify_draft", target_probs).verify_draft(target_probs, draft_tokens, draft_probs, indptr, u_accept,
+                                                      u_sample, tokens, accepted)
     return tokens, accepted
