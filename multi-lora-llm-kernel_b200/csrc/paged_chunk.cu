@@ -64,7 +64,7 @@ struct Shared {
   uint32_t tmem;
   int abort;
   int b, tile;
-  long long off, sum[16], total;
+  long long off, begin, end, sum[16], items[16];
   long long at[2][kBlock];   // page offset (bytes) of each position of a block, -1: none
   alignas(16) float ks[5][kBlock];  // read four at a time
   alignas(16) float lv[5][kBlock];
@@ -74,17 +74,21 @@ struct Shared {
   float qmul[2][kTile];      // by piece: the next one's rows are loaded while this one's are read
 };
 
+// What starting and ending a tile costs, in units: so many stand before its
+// first one in the line.  None where every unit has a CTA of its own.
+constexpr int kPieceUnits = 2;
+
 struct TileGeo {
-  int m0, mrows, first, per, pend;
+  int m0, mrows, first, per, pend;  // per: with the `lead` units above
 };
-__device__ __forceinline__ TileGeo tile_geo(const Seq& s, int window, int G, int t) {
+__device__ __forceinline__ TileGeo tile_geo(const Seq& s, int window, int G, int t, int lead) {
   TileGeo g;
   g.m0 = t * kTile;
   g.mrows = min(kTile, s.n * G - g.m0);
   const int ctx = s.len - s.n, tok0 = g.m0 / G, tok1 = (g.m0 + g.mrows - 1) / G;
   g.pend = max(0, min(s.len, ctx + tok1 + 1));
   g.first = (window > 0 ? max(0, ctx + tok0 + 1 - window) : 0) / kBlock;
-  g.per = max(1, (g.pend + kBlock - 1) / kBlock - g.first);
+  g.per = max(1, (g.pend + kBlock - 1) / kBlock - g.first) + lead;
   return g;
 }
 __device__ __forceinline__ int seq_tiles(const Seq& s, int G) { return (s.n * G + kTile - 1) / kTile; }
@@ -92,16 +96,17 @@ __device__ __forceinline__ int seq_tiles(const Seq& s, int G) { return (s.n * G 
 // The pieces of a CTA's range of units, walked alike by every role.
 struct Walk {
   const PagedAttention& a;
-  int b, t, h, k;
+  int lead;
+  int b, t, h;
   long long left;
   Seq seq;
   TileGeo g;
   int k0, k1;
   bool first;
-  __device__ __forceinline__ Walk(const PagedAttention& a_, int b_, int t_, long long off, long long left_)
-      : a(a_), b(b_), t(t_), left(left_), first(true) {
+  __device__ __forceinline__ Walk(const PagedAttention& a_, int lead_, int b_, int t_, long long off, long long left_)
+      : a(a_), lead(lead_), b(b_), t(t_), left(left_), first(true) {
     seq = load_seq(a, b);
-    g = tile_geo(seq, a.window, a.G, t);
+    g = tile_geo(seq, a.window, a.G, t, lead);
     h = static_cast<int>(off / g.per);
     k1 = static_cast<int>(off - static_cast<long long>(h) * g.per);
     k0 = k1;
@@ -120,7 +125,7 @@ struct Walk {
           seq = load_seq(a, b);
           t = 0;
         }
-        g = tile_geo(seq, a.window, a.G, t);
+        g = tile_geo(seq, a.window, a.G, t, lead);
       }
     }
     k0 = k1;
@@ -128,7 +133,8 @@ struct Walk {
     left -= k1 - k0;
     return true;
   }
-  __device__ __forceinline__ int blocks() const { return g.pend > 0 ? k1 - k0 : 0; }
+  __device__ __forceinline__ int block0() const { return g.first + max(k0 - lead, 0); }
+  __device__ __forceinline__ int blocks() const { return g.pend > 0 ? max(k1 - lead, 0) - max(k0 - lead, 0) : 0; }
   __device__ __forceinline__ bool has_b() const { return g.mrows > 128; }
 };
 
@@ -226,33 +232,54 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   }
 
   // ---- this CTA's range of units ----
-  auto seq_sum = [&](int b) -> long long {
+  auto seq_sum = [&](int b, int& items) -> long long {  // units without the lead, and tiles times heads
+    items = 0;
     if (b >= a.c.B) return 0;
     const Seq s = load_seq(a, b);
     long long u = 0;
     const int tiles = seq_tiles(s, G);
-    for (int t = 0; t < tiles; ++t) u += tile_geo(s, a.window, G, t).per;
+    for (int t = 0; t < tiles; ++t) u += tile_geo(s, a.window, G, t, 0).per;
+    items = tiles * a.c.Hkv;
     return u * a.c.Hkv;
   };
-  long long total = 0, mine = 0;
+  long long total = 0, all_items = 0, mine = 0;
+  int my_items = 0;
   for (int b0 = 0; b0 < a.c.B; b0 += kThreads) {
-    const long long u = seq_sum(b0 + tid);
-    if (b0 == 0) mine = u;
-    long long w = u;
+    int n;
+    const long long u = seq_sum(b0 + tid, n);
+    if (b0 == 0) {
+      mine = u;
+      my_items = n;
+    }
+    long long w = u, v = n;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    if (lane == 0) sh.sum[warp] = w;
+    for (int o = 16; o > 0; o >>= 1) {
+      w += __shfl_xor_sync(0xffffffffu, w, o);
+      v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    if (lane == 0) {
+      sh.sum[warp] = w;
+      sh.items[warp] = v;
+    }
     __syncthreads();
-    for (int i = 0; i < 16; ++i) total += sh.sum[i];
+    for (int i = 0; i < 16; ++i) {
+      total += sh.sum[i];
+      all_items += sh.items[i];
+    }
     __syncthreads();
   }
+  const int lead = total <= gridDim.x ? 0 : kPieceUnits;
+  total += lead * all_items;
+  // no more CTAs than units, so that every range (before the move below) has one
   const int ctas = static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
-  const bool works = cta < ctas;
-  const long long u0 = works ? total * cta / ctas : 0, u1 = works ? total * (cta + 1) / ctas : 0;
-  if (works) {
+  if (tid == 0) sh.begin = sh.end = cta < ctas ? total * (cta + 1) / ctas : 0;
+  if (cta < ctas) {
+    const long long raw0 = total * cta / ctas, raw1 = total * (cta + 1) / ctas;
     long long run = 0;
-    for (int b0 = 0; b0 < a.c.B && run <= u0; b0 += kThreads) {
-      const long long u = b0 == 0 ? mine : seq_sum(b0 + tid);
+    for (int b0 = 0; b0 < a.c.B && run <= raw1; b0 += kThreads) {
+      int n = my_items;
+      long long u = b0 == 0 ? mine : seq_sum(b0 + tid, n);
+      u += static_cast<long long>(n) * lead;
       long long inc = u;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -261,27 +288,40 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       }
       if (lane == 31) sh.sum[warp] = inc;
       __syncthreads();
-      long long lo = run;
+      long long lo = run + inc - u;
       for (int i = 0; i < warp; ++i) lo += sh.sum[i];
-      lo += inc - u;
-      if (u0 >= lo && u0 < lo + u) {
-        long long off = u0 - lo;
+#pragma unroll 1
+      for (int side = 0; side < 2; ++side) {  // both ends: tile, and offset in its units
+        const long long raw = side == 0 ? raw0 : raw1;
+        if (raw < lo || raw >= lo + u) continue;
+        long long off = raw - lo;
         const Seq s = load_seq(a, b0 + tid);
         const int tiles = seq_tiles(s, G);
-        int t = 0;
-        for (; t < tiles - 1; ++t) {
-          const long long c = static_cast<long long>(tile_geo(s, a.window, G, t).per) * a.c.Hkv;
-          if (off < c) break;
+        int t = 0, per = 1;
+        for (; t < tiles; ++t) {
+          per = tile_geo(s, a.window, G, t, lead).per;
+          const long long c = static_cast<long long>(per) * a.c.Hkv;
+          if (off < c || t == tiles - 1) break;
           off -= c;
         }
-        sh.b = b0 + tid;
-        sh.tile = t;
-        sh.off = off;
+        // a cut inside what a tile costs to start is moved before it
+        const int k = static_cast<int>(off % per), back = k < lead ? k : 0;
+        if (side == 0) {
+          sh.b = b0 + tid;
+          sh.tile = t;
+          sh.off = off - back;
+          sh.begin = raw - back;
+        } else {
+          sh.end = raw - back;
+        }
       }
       for (int i = 0; i < 16; ++i) run += sh.sum[i];
       __syncthreads();
     }
   }
+  __syncthreads();
+  const long long u0 = sh.begin, u1 = sh.end;
+  const bool works = u0 < u1;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -305,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       return ok;
     };
     if (works) {
-      Walk w(a, sh.b, sh.tile, sh.off, u1 - u0);
+      Walk w(a, lead, sh.b, sh.tile, sh.off, u1 - u0);
       while (ok && w.next()) {
         const int nb = w.blocks();
         const bool act = half == 0 || w.has_b();
@@ -326,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 #pragma unroll
           for (int c = 0; c < 4; ++c) tc::ld32(t_s + 32 * c, reinterpret_cast<uint32_t*>(s) + 32 * c);
           tc::wait_ld();
-          const int p0 = (w.g.first + w.k0 + j) * kBlock;
+          const int p0 = (w.block0() + j) * kBlock;
           const int sc = (n_sc + j) % C::kScales;
           if (kE4m3) {
             const float4* ks = reinterpret_cast<const float4*>(sh.ks[sc]);
@@ -519,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       return mbar_wait_abortable(bar, parity, err, abort);
     };
     if (works) {
-      Walk w(a, sh.b, sh.tile, sh.off, u1 - u0);
+      Walk w(a, lead, sh.b, sh.tile, sh.off, u1 - u0);
       // A wait that gave up (ok) ends the loads but not the walk: the barrier
       // of the four warps needs them all.
       while (w.next()) {
@@ -589,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         ++n_q;
         // ---- blocks ----
         const int32_t* row = a.c.table + w.b * a.c.table_stride;
-        const int first = w.g.first + w.k0;
+        const int first = w.block0();
         // Thread t looks up position t of a block, one block ahead: the page
         // is read here and used when the block is due.
         int pg = -1, at = 0;
@@ -757,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           tc::commit(&sh.pv_done[half]);
         }
       };
-      Walk w(a, sh.b, sh.tile, sh.off, u1 - u0);
+      Walk w(a, lead, sh.b, sh.tile, sh.off, u1 - u0);
       while (ok && w.next()) {
         const int nb = w.blocks();
         if (nb == 0) continue;
