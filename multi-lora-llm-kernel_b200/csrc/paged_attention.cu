@@ -203,55 +203,71 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
     const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + static_cast<int64_t>(h) * a.c.head_stride * kElt;
     const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + static_cast<int64_t>(h) * a.c.head_stride * kElt;
     const bool whole = a.c.page_size % kPos == 0;  // a step's positions share a page
+    constexpr int kRowsPer = 32 / kChunks;
+    const int ch = lane % kChunks, lr = lane / kChunks;  // this lane's chunk, and its row among kRowsPer
+    const uint8_t* const kl = kb + lr * a.c.pos_stride * kElt + ch * 16;
+    const uint8_t* const vl = vb + lr * a.c.pos_stride * kElt + ch * 16;
+    const int64_t row_step = kRowsPer * a.c.pos_stride * kElt;
+    const float* const sl = kE4m3 ? (lane < 16 ? a.c.k_scale : a.c.v_scale) + static_cast<int64_t>(h) * a.c.scale_head_stride : nullptr;
+    // 16-byte chunks are XORed by the row so that the fragment reads below touch
+    // every bank once (8-bit: k reads two rows of four chunks, v reads even rows
+    // of two chunks, per quarter warp).  A lane's row is lr plus a multiple of
+    // kRowsPer, whose bits do not meet.
+    constexpr int kMask = kChunks - 1;
+    const int ck0 = kE4m3 ? ch ^ ((lr & 1) << 2) : ch ^ (lr & 7), cv0 = kE4m3 ? ch ^ (((lr >> 1) & 3) << 1) : ck0;
+    // Where a step's positions share a page, the pages of 32 steps are read at
+    // once, one a lane.
+    int pages32 = -1;
     auto load = [&](int s) {
       const int p0 = p_lo + s * kUnit + warp * kPos;
       const uint32_t dst = ring + (s % kStages) * kSlot;
-      int64_t base = 0, sbase = 0;
-      bool ok = false;
-      if (whole && p0 < pend) {
-        int at;
-        const int pg = page_of(p0, at);
-        ok = pg >= 0;
-        base = ok ? pg * a.c.page_stride + at * a.c.pos_stride : 0;
-        if (kE4m3) sbase = ok ? pg * a.c.scale_page_stride + at : 0;
-      }
-      constexpr int kRowsPer = 32 / kChunks;
-      const int ch = lane % kChunks;
+      if (whole) {
+        if ((s & 31) == 0) {
+          const int p = p0 + lane * kUnit, pi = page_index(a.c, p);
+          pages32 = p < pend && pi < a.c.max_pages ? pages[pi] : -1;
+        }
+        const int pg = __shfl_sync(0xffffffffu, pages32, s & 31);
+        int rem = pend - p0;  // positions of this step
+        if (rem > 0 && (pg < 0 || pg >= a.c.num_pages)) {
+          raise_error(a.err, PERSONA_DEV_ERR_PAGE);
+          rem = 0;
+        }
+        const int at = p0 - page_index(a.c, p0) * a.c.page_size;
+        const int64_t base = rem > 0 ? (pg * a.c.page_stride + at * a.c.pos_stride) * kElt : 0;
+        const uint8_t *kp = kl + base, *vp = vl + base;
 #pragma unroll
-      for (int i = 0; i < kPos / kRowsPer; ++i) {
-        const int r = i * kRowsPer + lane / kChunks;
-        int64_t src;
-        bool live;
-        if (whole) {
-          live = ok && p0 + r < pend;
-          src = live ? base + r * a.c.pos_stride : 0;
-        } else {
-          int at, pg = -1;
-          if (p0 + r < pend) pg = page_of(p0 + r, at);
-          live = pg >= 0;
-          src = live ? pg * a.c.page_stride + at * a.c.pos_stride : 0;
+        for (int i = 0; i < kPos / kRowsPer; ++i, kp += row_step, vp += row_step) {
+          constexpr int kStep = kRowsPer;
+          const int ck = kE4m3 ? ck0 : ck0 ^ ((i * kStep) & 7), cv = kE4m3 ? cv0 ^ (((i * kStep / 2) & 3) << 1) : ck;
+          const bool live = lr + i * kStep < rem;
+          const uint32_t to = dst + (lr + i * kStep) * kRowBytes;
+          cp_async16(to + (ck & kMask) * 16, live ? kp : kl, live);
+          cp_async16(to + kHalf + (cv & kMask) * 16, live ? vp : vl, live);
         }
-        // 16-byte chunks are XORed by the row so that the fragment reads
-        // below touch every bank once (8-bit: k reads two rows of four
-        // chunks, v reads even rows of two chunks, per quarter warp)
-        const int ck = kE4m3 ? ch ^ ((r & 1) << 2) : ch ^ (r & 7);
-        const int cv = kE4m3 ? ch ^ (((r >> 1) & 3) << 1) : ch ^ (r & 7);
-        const int mask = kChunks - 1;
-        cp_async16(dst + r * kRowBytes + (ck & mask) * 16, kb + src * kElt + ch * 16, live);
-        cp_async16(dst + kHalf + r * kRowBytes + (cv & mask) * 16, vb + src * kElt + ch * 16, live);
-      }
-      if (kE4m3) {
-        const int r = lane & 15;
-        int64_t src = sbase + r;
-        bool live = ok && p0 + r < pend;
-        if (!whole) {
-          int at, pg = -1;
-          if (p0 + r < pend) pg = page_of(p0 + r, at);
-          live = pg >= 0;
-          src = live ? pg * a.c.scale_page_stride + at : 0;
+        if (kE4m3) {
+          const int r = lane & 15;
+          const bool live = r < rem;
+          cp_async4(dst + 2 * kHalf + lane * 4, live ? sl + (pg * a.c.scale_page_stride + at + r) : sl, live);
         }
-        const float* sp = (lane < 16 ? a.c.k_scale : a.c.v_scale) + static_cast<int64_t>(h) * a.c.scale_head_stride;
-        cp_async4(dst + 2 * kHalf + (lane >> 4) * kPos * 4 + r * 4, sp + (live ? src : 0), live);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPos / kRowsPer; ++i) {
+          const int r = lr + i * kRowsPer;
+          const int ck = kE4m3 ? ck0 : ck0 ^ ((i * kRowsPer) & 7), cv = kE4m3 ? cv0 ^ (((i * kRowsPer / 2) & 3) << 1) : ck;
+          int at = 0;
+          const int pg = p0 + r < pend ? page_of(p0 + r, at) : -1;
+          const bool live = pg >= 0;
+          const int64_t src = live ? (pg * a.c.page_stride + at * a.c.pos_stride) * kElt : 0;
+          const uint32_t to = dst + r * kRowBytes;
+          cp_async16(to + (ck & kMask) * 16, kb + src + ch * 16, live);
+          cp_async16(to + kHalf + (cv & kMask) * 16, vb + src + ch * 16, live);
+        }
+        if (kE4m3) {
+          const int p = p0 + (lane & 15);
+          int at = 0;
+          const int pg = p < pend ? page_of(p, at) : -1;
+          cp_async4(dst + 2 * kHalf + lane * 4, pg >= 0 ? sl + (pg * a.c.scale_page_stride + at) : sl, pg >= 0);
+        }
       }
     };
 #pragma unroll
@@ -530,6 +546,14 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
 
     // ---- join the warps ----
     float* accs = reinterpret_cast<float*>(smem);  // [kWarps][TR][D]
+    // Where dim d of row m is: 8-dim chunks XORed by the row, or (8-bit pages,
+    // whose lanes hold D / 8 dims in a row) those dims turned by row and lane.
+    auto join_at = [&](int m, int d) {
+      if (!kE4m3) return d ^ ((m & 7) << 3);
+      constexpr int kW = D / 8;
+      const int blk = d / kW;
+      return blk * kW + ((d + 2 * (m & 7) + (blk >> 2)) & (kW - 1));
+    };
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -542,15 +566,17 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           s_m[warp][m] = m_run[mt][half];
           s_l[warp][m] = l;
         }
+        if (mt * 16 + half * 8 >= mrows) continue;  // no such rows
         float* dst = accs + (warp * TR + m) * D;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           const float x0 = acc[mt][i][2 * half], x1 = acc[mt][i][2 * half + 1];
           if (!kE4m3) {
-            *reinterpret_cast<float2*>(dst + 8 * i + 2 * t) = make_float2(x0, x1);
-          } else {
-            dst[2 * t * (D / 8) + i] = x0;
-            dst[(2 * t + 1) * (D / 8) + i] = x1;
+            *reinterpret_cast<float2*>(dst + join_at(m, 8 * i + 2 * t)) = make_float2(x0, x1);
+          } else {  // the odd lanes the other way round: 32 lanes, 32 banks
+            const int a0 = join_at(m, 2 * t * (D / 8) + i), a1 = join_at(m, (2 * t + 1) * (D / 8) + i);
+            dst[(t & 1) == 0 ? a0 : a1] = (t & 1) == 0 ? x0 : x1;
+            dst[(t & 1) == 0 ? a1 : a0] = (t & 1) == 0 ? x1 : x0;
           }
         }
       }
@@ -570,9 +596,9 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         for (int w = 0; w < kWarps; ++w) {
           const float f = exp2_approx(s_m[w][m] - mx);
           l = fmaf(f, s_l[w][m], l);
-          const float* src = accs + (w * TR + m) * D + d;
+          const float* src = accs + (w * TR + m) * D;
 #pragma unroll
-          for (int x = 0; x < 8; ++x) o[x] = fmaf(f, src[x], o[x]);
+          for (int x = 0; x < 8; ++x) o[x] = fmaf(f, src[kE4m3 ? join_at(m, d + x) : join_at(m, d) + x], o[x]);
         }
       }
       if (complete) {
@@ -623,9 +649,9 @@ cudaError_t attention_launch(const PagedAttention& a, cudaStream_t st) {
   cudaError_t e = prepare_kernel(done, k, kSmem, 0);
   if (e != cudaSuccess) return e;
   const int ctas = kCtasPerSm * sm_count();
-  e = launch_paged(k, dim3(ctas), dim3(kThreads), kSmem, 1, st, a);
+  e = launch_paged(k, dim3(ctas), dim3(kThreads), kSmem, 1, false, st, a);
   if (e != cudaSuccess) return e;
-  return launch_paged(paged_combine_kernel<T, D, 16 * MT>, dim3(ctas, 2 * MT), dim3(256), 0, 1, st, a);
+  return launch_paged(paged_combine_kernel<T, D, 16 * MT>, dim3(ctas, 2 * MT), dim3(256), 0, 1, true, st, a);
 }
 template <typename T, int D, int MT>
 cudaError_t attention_pages(const PagedAttention& a, cudaStream_t st) {

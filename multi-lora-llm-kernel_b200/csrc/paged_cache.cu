@@ -173,14 +173,14 @@ cudaError_t write_for(const PagedWrite& a, int32_t* err, cudaStream_t st) {
   const bool e = a.c.k_scale != nullptr;
   auto k = a.c.D == 128 ? (e ? paged_write_kernel<T, 128, true> : paged_write_kernel<T, 128, false>)
                         : (e ? paged_write_kernel<T, 64, true> : paged_write_kernel<T, 64, false>);
-  return launch_paged(k, dim3(a.rows), dim3(kWriteThreads), 0, 1, st, a, err);
+  return launch_paged(k, dim3(a.rows), dim3(kWriteThreads), 0, 1, true, st, a, err);
 }
 template <typename T>
 cudaError_t read_for(const PagedRead& a, int32_t* err, cudaStream_t st) {
   const bool e = a.c.k_scale != nullptr;
   auto k = a.c.D == 128 ? (e ? paged_read_kernel<T, 128, true> : paged_read_kernel<T, 128, false>)
                         : (e ? paged_read_kernel<T, 64, true> : paged_read_kernel<T, 64, false>);
-  return launch_paged(k, dim3((a.rows + 3) / 4), dim3(128), 0, 1, st, a, err);
+  return launch_paged(k, dim3((a.rows + 3) / 4), dim3(128), 0, 1, true, st, a, err);
 }
 
 }  // namespace

@@ -907,9 +907,9 @@ cudaError_t chunk_launch(const PagedAttention& a, cudaStream_t st) {
   cudaError_t e = prepare_kernel(done, k, Cfg<D>::kSmem, kRegsLaunch);
   if (e != cudaSuccess) return e;
   const int ctas = sm_count();
-  e = launch_paged(k, dim3(ctas), dim3(kThreads), Cfg<D>::kSmem, 1, st, a);
+  e = launch_paged(k, dim3(ctas), dim3(kThreads), Cfg<D>::kSmem, 1, false, st, a);
   if (e != cudaSuccess) return e;
-  return launch_paged(paged_chunk_join_kernel<T, D>, dim3(ctas, kTile / 32), dim3(256), 0, 1, st, a);
+  return launch_paged(paged_chunk_join_kernel<T, D>, dim3(ctas, kTile / 32), dim3(256), 0, 1, true, st, a);
 }
 template <typename T>
 cudaError_t chunk_for(const PagedAttention& a, cudaStream_t st) {

@@ -317,7 +317,7 @@ cudaError_t launch_verify_draft(const VerifyDraft& a, int type, cudaStream_t st)
   while (split > 1 && static_cast<int64_t>(a.B) * split > 4 * 148 &&
          a.V <= static_cast<int64_t>(kMaxTiles - 2) * kTile * (split / 2))
     split /= 2;
-  return launch_paged(k, dim3(a.B * split), dim3(kThreads), 0, split, st, a);
+  return launch_paged(k, dim3(a.B * split), dim3(kThreads), 0, split, true, st, a);
 }
 
 }  // namespace persona
