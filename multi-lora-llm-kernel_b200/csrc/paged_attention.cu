@@ -62,6 +62,13 @@ __device__ __forceinline__ void seq_units(const Seq& s, int window, int TR, int 
   per = max(1, (s.len + kUnit - 1) / kUnit - first);
 }
 
+// Shared memory of the ring, which also holds the warps' results at a piece's end.
+template <int D, int MT, bool kE4m3, int kStages> struct RingBytes {
+  static constexpr int kSlot = 2 * kPos * D * (kE4m3 ? 1 : 2) + (kE4m3 ? 2 * kPos * 4 : 0);
+  static constexpr int kRing = kWarps * kStages * kSlot, kJoin = kWarps * 16 * MT * D * 4;
+  static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
+};
+
 template <typename T, int D, int MT, bool kE4m3, int kStages>
 __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   using MT16 = typename std::conditional<kE4m3, __half, T>::type;  // type of the products
@@ -72,6 +79,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   constexpr int kHalf = kPos * kRowBytes;              // k (or v) of one warp step
   constexpr int kSlot = 2 * kHalf + (kE4m3 ? 2 * kPos * 4 : 0);
   constexpr int kSteps = D / 16;
+  constexpr int kQAt = RingBytes<D, MT, kE4m3, kStages>::kBytes;  // q fragments behind the ring (MT = 2)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_scan[kWarps], s_items[kWarps], s_begin;
   __shared__ int s_b;
@@ -335,6 +343,33 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         }
       }
 
+    // With two row tiles the fragments would take 64 registers beside 128 of
+    // outputs: they go to shared memory, one 16-byte read a lane, row tile and step.
+    const uint32_t s_qf = smem_u32(smem) + kQAt + lane * 16;
+    if constexpr (MT == 2) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks)
+          if (ks / (kSteps / kWarps) == warp)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s_qf + (mt * kSteps + ks) * 512), "r"(qf[mt][ks][0]),
+                         "r"(qf[mt][ks][1]), "r"(qf[mt][ks][2]), "r"(qf[mt][ks][3])
+                         : "memory");
+      __syncthreads();
+    }
+    auto q_of = [&](int mt, int ks, uint32_t (&f)[4]) {
+      if constexpr (MT == 2) {
+        const uint4 v = lds128(s_qf + (mt * kSteps + ks) * 512);
+        f[0] = v.x;
+        f[1] = v.y;
+        f[2] = v.z;
+        f[3] = v.w;
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) f[x] = qf[mt][ks][x];
+      }
+    };
+
     // ---- one pass over the piece's positions ----
     float acc[MT][D / 8][4];
     float m_run[MT][2], l_run[MT][2];
@@ -379,24 +414,36 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           const uint32_t b0[2] = {kf[0], kf[1]}, b1[2] = {kf[2], kf[3]};
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            Mma<MT16>::k16(sc[mt][0], qf[mt][ks], b0);
-            Mma<MT16>::k16(sc[mt][1], qf[mt][ks], b1);
+            uint32_t f[4];
+            q_of(mt, ks, f);
+            Mma<MT16>::k16(sc[mt][0], f, b0);
+            Mma<MT16>::k16(sc[mt][1], f, b1);
           }
         }
       } else {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int r = n * 8 + g;
+        for (int blk = 0; blk < D / 64; ++blk) {
+          uint32_t u[2][4];
 #pragma unroll
-          for (int blk = 0; blk < D / 64; ++blk) {
+          for (int n = 0; n < 2; ++n) {
+            const int r = n * 8 + g;
             const uint4 w = lds128(slot + r * kRowBytes + (((4 * blk + t) ^ ((r & 1) << 2)) & (kChunks - 1)) * 16);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            u[n][0] = w.x;
+            u[n][1] = w.y;
+            u[n][2] = w.z;
+            u[n][3] = w.w;
+          }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint32_t bf[2];
-              e4m3x4_to_half(u[x], bf[0], bf[1]);
+          for (int x = 0; x < 4; ++x) {
+            uint32_t b0[2], b1[2];
+            e4m3x4_to_half(u[0][x], b0[0], b0[1]);
+            e4m3x4_to_half(u[1][x], b1[0], b1[1]);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) Mma<MT16>::k16(sc[mt][n], qf[mt][4 * blk + x], bf);
+            for (int mt = 0; mt < MT; ++mt) {
+              uint32_t f[4];
+              q_of(mt, 4 * blk + x, f);
+              Mma<MT16>::k16(sc[mt][0], f, b0);
+              Mma<MT16>::k16(sc[mt][1], f, b1);
             }
           }
         }
@@ -638,12 +685,11 @@ constexpr int kCtasPerSm = 2;
 
 template <typename T, int D, int MT, bool kE4m3>
 cudaError_t attention_launch(const PagedAttention& a, cudaStream_t st) {
-  // ring slots: 3 x 8 KB (16-bit) or 6 x 4.1 KB (8-bit) per warp at D = 128,
-  // 96 KB per CTA, two CTAs per SM
-  constexpr int kStages = (kE4m3 ? 6 : 3) * (128 / D);
-  constexpr int kSlot = 2 * kPos * D * (kE4m3 ? 1 : 2) + (kE4m3 ? 2 * kPos * 4 : 0);
-  constexpr int kRing = kWarps * kStages * kSlot, kJoin = kWarps * 16 * MT * D * 4;
-  constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  // Ring slots of 8 KB (16-bit) or 4.1 KB (8-bit) per warp at D = 128, two CTAs
+  // per SM: 3 and 6 (96 KB a CTA); with two row tiles over 8-bit pages 4 (77.7
+  // against 81.3 us for 32 x 5 rows).
+  constexpr int kStages = (kE4m3 ? (MT == 2 ? 4 : 6) : 3) * (128 / D);
+  constexpr int kSmem = RingBytes<D, MT, kE4m3, kStages>::kBytes + (MT == 2 ? MT * (D / 16) * 512 : 0);
   auto k = paged_attention_kernel<T, D, MT, kE4m3, kStages>;
   static std::atomic<bool> done[64];
   cudaError_t e = prepare_kernel(done, k, kSmem, 0);
