@@ -125,8 +125,10 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const __grid
   }
 }
 
-// One warp per row: the position's k and v of every head, 8 elements a lane
-// and step.  Codes times scale are rounded once, to the rows' 16-bit type.
+// One warp per row: the position's k and v of every head, 16 bytes of the cache
+// a lane and step.  Codes times scale are rounded once, to the rows' 16-bit
+// type.  (Two to eight rows a warp, to share the search for the sequence, took
+// as long at 36213 rows and 1.3 to 2.7 times as long at 1999.)
 template <typename T, int D, bool kE4m3>
 __global__ void __launch_bounds__(128) paged_read_kernel(const __grid_constant__ PagedRead a, int32_t* err) {
   pdl_wait();
@@ -136,34 +138,39 @@ __global__ void __launch_bounds__(128) paged_read_kernel(const __grid_constant__
   int pos, at;
   int64_t page;
   if (!locate_row(a.c, r, err, pos, page, at)) return;
-  const int64_t slot = page * a.c.page_stride + at * a.c.pos_stride;
-  const int64_t sslot = page * a.c.scale_page_stride + at;
-  constexpr int kChunks = D / 8;
+  const int64_t from = page * a.c.page_stride + at * a.c.pos_stride;
+  const int64_t sfrom = page * a.c.scale_page_stride + at;
+  constexpr int kEach = kE4m3 ? 16 : 8;  // elements of 16 bytes in the cache
+  constexpr int kChunks = D / kEach;
   const int n = 2 * a.c.Hkv * kChunks;
 #pragma unroll 4
   for (int x = lane; x < n; x += 32) {
-    const int hh = x / kChunks, d = (x % kChunks) * 8;
+    const int hh = x / kChunks, d = (x % kChunks) * kEach;
     const bool is_v = hh >= a.c.Hkv;
-    const int kh = is_v ? hh - a.c.Hkv : hh;
+    const int64_t kh = is_v ? hh - a.c.Hkv : hh;
     const PagedRows& dst = is_v ? a.v : a.k;
-    T* o = static_cast<T*>(dst.p) + static_cast<int64_t>(r) * dst.row_stride + static_cast<int64_t>(kh) * dst.head_stride + d;
-    const int64_t src = slot + static_cast<int64_t>(kh) * a.c.head_stride + d;
+    T* o = static_cast<T*>(dst.p) + static_cast<int64_t>(r) * dst.row_stride + kh * dst.head_stride + d;
+    const char* src = static_cast<const char*>(is_v ? a.c.v : a.c.k) + (from + kh * a.c.head_stride + d) * (kE4m3 ? 1 : 2);
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(src));
     if (!kE4m3) {
-      *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(static_cast<const T*>(is_v ? a.c.v : a.c.k) + src);
+      *reinterpret_cast<uint4*>(o) = w;
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(is_v ? a.c.v : a.c.k) + src);
-      const float sc = (is_v ? a.c.v_scale : a.c.k_scale)[sslot + static_cast<int64_t>(kh) * a.c.scale_head_stride];
-      uint32_t h[4];
-      e4m3x4_to_half(w.x, h[0], h[1]);
-      e4m3x4_to_half(w.y, h[2], h[3]);
-      float f[8];
+      const float sc = __ldg((is_v ? a.c.v_scale : a.c.k_scale) + sfrom + kh * a.c.scale_head_stride);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 p = Cvt<__half>::to2(h[j]);
-        f[2 * j] = p.x * sc;
-        f[2 * j + 1] = p.y * sc;
+      for (int y = 0; y < 2; ++y) {
+        uint32_t h[4];
+        e4m3x4_to_half(u[2 * y], h[0], h[1]);
+        e4m3x4_to_half(u[2 * y + 1], h[2], h[3]);
+        float f[8];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const float2 p = Cvt<__half>::to2(h[z]);
+          f[2 * z] = p.x * sc;
+          f[2 * z + 1] = p.y * sc;
+        }
+        *reinterpret_cast<uint4*>(o + 8 * y) = pack8<T>(f);
       }
-      *reinterpret_cast<uint4*>(o) = pack8<T>(f);
     }
   }
 }

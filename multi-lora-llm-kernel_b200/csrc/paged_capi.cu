@@ -11,7 +11,12 @@ namespace {
 
 constexpr int64_t kI32Max = 2147483647;
 constexpr int64_t kMaxHeads = 1024;
-constexpr int64_t kFewRows = 64;
+// Most query rows per kv head (new tokens times heads of a group) for the
+// warp-level kernel, which reads the pages once per 32 rows.  Measured with 32
+// sequences of up to 6000 tokens: over 16-bit pages 36 rows take it 118 us and
+// the tcgen05 kernel 77 (20 rows: 66 and 77); over 8-bit pages, whose codes the
+// tcgen05 kernel has to convert for each of its tiles, 64 rows take 129 and 149.
+constexpr int64_t kFewRows16 = 32, kFewRows8 = 64;
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 int status(cudaError_t e) { return e == cudaSuccess ? PERSONA_OK : PERSONA_ERR_CUDA; }
@@ -127,7 +132,8 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = dev_err;
   const int most = static_cast<int>(max_new > rows ? rows : max_new);
-  if (static_cast<int64_t>(most) * a.G > kFewRows) return status(launch_paged_chunk(a, dtype, workspace, stream));
+  if (static_cast<int64_t>(most) * a.G > (a.c.k_scale != nullptr ? kFewRows8 : kFewRows16))
+    return status(launch_paged_chunk(a, dtype, workspace, stream));
   return status(launch_paged_attention(a, dtype, most, workspace, stream));
 }
 
