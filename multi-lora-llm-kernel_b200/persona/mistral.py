@@ -15,6 +15,8 @@ package's kernels:
   up, one each for o and down);
 * LoRA: ``ops.bgmv_fused_multi`` on a plan computed once per batch at decode;
   ``ops.sgmv_fused`` over the request segments at prefill;
+* ragged chunks over a paged cache (``extend``): ``ops.paged_rope_cache`` and
+  ``ops.paged_attention``, LoRA over the sequences as segments;
 * the rest: ``ops.add_rmsnorm`` (residual add fused into the
   next norm), ``rope_cache`` (rotary embedding + KV-cache write) at prefill,
   ``rope_decode_attention`` (the same and the attention, one launch) at
@@ -29,7 +31,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
-from typing import List, Optional
+from typing import List, Optional, Sequence
 
 import torch
 import torch.nn.functional as F
@@ -86,6 +88,52 @@ class DecodeState:
     v_cache: List[torch.Tensor]
     bufs: dict = field(default_factory=dict)
     graph: Optional[torch.cuda.CUDAGraph] = None
+
+
+@dataclass
+class PagedState:
+    """A batch over a paged KV cache: sequences of any lengths, which grow by
+    chunks (prompt chunks, single tokens, drafted tokens)."""
+
+    slots: torch.Tensor           # [B] int32 adapter slot per sequence
+    page_size: int
+    page_table: torch.Tensor      # [B, max_pages] int32
+    k_cache: List[torch.Tensor]   # per layer [pages, Hkv, page_size, 128], fp16 or e4m3
+    v_cache: List[torch.Tensor]
+    k_scale: List[Optional[torch.Tensor]]  # per layer [pages, Hkv, page_size], e4m3 only
+    v_scale: List[Optional[torch.Tensor]]
+    lengths: List[int]            # cached tokens per sequence
+    pages: List[List[int]]        # pages held by each sequence
+    free: List[int]
+
+    def set_length(self, b: int, length: int) -> None:
+        """Sequence b keeps its first ``length`` tokens (rejected drafts, or 0
+        to start over); pages behind them are free again."""
+        if not 0 <= length <= self.lengths[b]:
+            raise ValueError("a sequence can only be cut back")
+        keep = -(-length // self.page_size)
+        self.free.extend(self.pages[b][keep:])
+        del self.pages[b][keep:]
+        self.lengths[b] = length
+
+    def _grow(self, new: Sequence[int]) -> None:
+        """Pages for ``new`` more tokens per sequence; lengths are moved on."""
+        want = [-(-(n + add) // self.page_size) for n, add in zip(self.lengths, new)]
+        if any(w > self.page_table.shape[1] for w in want):
+            raise ValueError("a sequence outgrows its page table")
+        if sum(w - len(p) for w, p in zip(want, self.pages)) > len(self.free):
+            raise ValueError("the paged cache has no free pages left")
+        table = None
+        for b, w in enumerate(want):
+            while len(self.pages[b]) < w:
+                self.pages[b].append(self.free.pop())
+                table = True
+            self.lengths[b] += new[b]
+        if table:
+            host = torch.zeros(self.page_table.shape, dtype=torch.int32)
+            for b, p in enumerate(self.pages):
+                host[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
+            self.page_table.copy_(host)
 
 
 class MistralLoRAModel:
@@ -204,6 +252,84 @@ class MistralLoRAModel:
         st.pos.fill_(T)
         st.length.fill_(T + 1)
         return logits
+
+    # ---- ragged chunks over a paged cache --------------------------------------
+    def new_paged_state(self, slots: torch.Tensor, num_pages: int, page_size: int = 16, max_seq: int = 4096,
+                        kv_dtype: torch.dtype = torch.float16) -> PagedState:
+        """Empty sequences, one per adapter slot of ``slots``, over ``num_pages``
+        pages per layer; ``kv_dtype`` fp16, or float8_e4m3fn with one scale per
+        token and head."""
+        cfg, d = self.cfg, self.device
+        e4m3 = kv_dtype == torch.float8_e4m3fn
+        if not e4m3 and kv_dtype != torch.float16:
+            raise ValueError("paged caches are float16 or float8_e4m3fn")
+        B = int(slots.numel())
+        shape = (num_pages, cfg.n_kv_heads, page_size, 128)
+
+        def per_layer(*size, dtype):
+            return [torch.zeros(*size, dtype=dtype, device=d) for _ in range(cfg.num_layers)]
+
+        none = [None] * cfg.num_layers
+        return PagedState(slots=slots.to(d, torch.int32).contiguous(), page_size=page_size,
+                          page_table=torch.zeros(B, -(-max_seq // page_size), dtype=torch.int32, device=d),
+                          k_cache=per_layer(*shape, dtype=kv_dtype), v_cache=per_layer(*shape, dtype=kv_dtype),
+                          k_scale=per_layer(*shape[:3], dtype=torch.float32) if e4m3 else none,
+                          v_scale=per_layer(*shape[:3], dtype=torch.float32) if e4m3 else none,
+                          lengths=[0] * B, pages=[[] for _ in range(B)], free=list(range(num_pages)))
+
+    @torch.inference_mode()
+    def extend(self, st: PagedState, chunks: Sequence[Sequence[int]]) -> tuple:
+        """Feed every sequence its chunk of token ids (any length, also none).
+        Returns the logits behind every fed token, [rows, V], and ``indptr``
+        [B + 1] int32: sequence b's rows are indptr[b] .. indptr[b + 1] (what
+        ``sampling.verify_drafts`` takes for chunks of a last token and drafts)."""
+        cfg, d = self.cfg, self.device
+        new = [len(c) for c in chunks]
+        if len(new) != len(st.lengths):
+            raise ValueError("one chunk per sequence")
+        st._grow(new)
+        R = sum(new)
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        indptr = torch.tensor(starts, dtype=torch.int32, device=d)
+        lengths = torch.tensor(st.lengths, dtype=torch.int32, device=d)
+        tokens = torch.tensor([t for c in chunks for t in c], dtype=torch.int64, device=d)
+        if R == 0:
+            return torch.empty(0, cfg.vocab, dtype=torch.float16, device=d), indptr
+        h = self.embed.index_select(0, tokens)
+        xn = torch.empty_like(h)
+        attn = torch.empty(R, cfg.n_heads, 128, dtype=torch.float16, device=d)
+        scale, most = 1.0 / math.sqrt(128), max(new)
+
+        def lora_apply(x, lora, names, ys):
+            for name, y in zip(names, ys):
+                ops.sgmv_fused(x, *lora[name], indptr, st.slots, y)
+
+        delta = None
+        for li, lw in enumerate(self.layers):
+            lora = self._lora[li]
+            kv = (st.k_cache[li], st.v_cache[li], st.page_table, indptr, lengths)
+            scales = dict(k_scale=st.k_scale[li], v_scale=st.v_scale[li])
+            ops.add_rmsnorm(h, delta, lw.in_norm, xn, cfg.rms_eps)
+            q, k, v = nf4.linear(xn, [lw.q, lw.k, lw.v])
+            lora_apply(xn, lora, ("q_proj", "k_proj", "v_proj"), (q, k, v))
+            q3, k3, v3 = (t.view(R, -1, 128) for t in (q, k, v))
+            ops.paged_rope_cache(q3, k3, v3, *kv, cfg.rope_theta, **scales)
+            ops.paged_attention(q3, *kv, attn, scale, max_new=most, **scales)
+            flat = attn.view(R, cfg.q_dim)
+            o = nf4.linear(flat, [lw.o])[0]
+            lora_apply(flat, lora, ("o_proj",), (o,))
+            ops.add_rmsnorm(h, o, lw.post_norm, xn, cfg.rms_eps)
+            g_, u_ = nf4.linear(xn, [lw.gate, lw.up])
+            lora_apply(xn, lora, ("gate_proj", "up_proj"), (g_, u_))
+            act = torch.empty_like(g_)
+            ops.silu_mul(g_, u_, act)
+            dn = nf4.linear(act, [lw.down])[0]
+            lora_apply(act, lora, ("down_proj",), (dn,))
+            delta = dn
+        ops.add_rmsnorm(h, delta, self.final_norm, xn, cfg.rms_eps)
+        return torch.matmul(xn, self.lm_head.t()), indptr
 
     # ---- decode --------------------------------------------------------------
     def _decode_body(self, st: DecodeState) -> None:

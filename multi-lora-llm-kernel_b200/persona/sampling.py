@@ -59,3 +59,35 @@ def sample_next_token(logits: torch.Tensor, params: SamplingParams,
     u = torch.rand(z.shape, device=z.device, generator=generator)
     gumbel = -torch.log(-torch.log(u.clamp_(min=torch.finfo(torch.float32).tiny)))
     return (z + gumbel).argmax(dim=-1)
+
+
+def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, draft_probs: Optional[torch.Tensor],
+                  indptr: torch.Tensor, params: SamplingParams, generator: Optional[torch.Generator] = None):
+    """Which drafted tokens of each sequence to keep, and the token behind them.
+
+    ``target_logits`` [rows, V] are the model's behind every token of the fed
+    chunks (a sequence's last token, then its drafts; rows ``indptr[b]`` to
+    ``indptr[b+1]``), ``draft_tokens`` [rows] the token that the draft put
+    behind each row's (ignored at a sequence's last row), ``draft_probs``
+    [rows, V] fp32 its distributions under the same ``params``, or None for
+    drafts without probabilities.  Returns ``(tokens [rows], accepted [B])``
+    as ``ops.verify_draft``.  Temperature 0 keeps a draft while it is the
+    most probable token."""
+    from persona import ops
+
+    rows, dev = target_logits.shape[0], target_logits.device
+    B = indptr.numel() - 1
+    if params.temperature <= 0:
+        best = target_logits.argmax(dim=-1, keepdim=True)
+        p = torch.zeros(target_logits.shape, dtype=torch.float32, device=dev).scatter_(1, best, 1.0)
+        draft_probs = None
+    else:
+        z = target_logits.float() / params.temperature
+        if params.top_p < 1.0:
+            z = _nucleus_mask(z, params.top_p)
+        p = torch.softmax(z, dim=-1)
+    u_accept = torch.rand(rows, device=dev, generator=generator)
+    u_sample = torch.rand(B, device=dev, generator=generator)
+    tokens = torch.empty(rows, dtype=torch.int64, device=dev)
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    return ops.verify_draft(p, draft_tokens, draft_probs, indptr, u_accept, u_sample, tokens, accepted)
