@@ -35,9 +35,12 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cooperative_groups.h>
+
 #include "paged_attention.cuh"
 
 namespace persona {
+namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
@@ -65,11 +68,12 @@ __device__ __forceinline__ void seq_units(const Seq& s, int window, int TR, int 
 // Shared memory of the ring, which also holds the warps' results at a piece's end.
 template <int D, int MT, bool kE4m3, int kStages> struct RingBytes {
   static constexpr int kSlot = 2 * kPos * D * (kE4m3 ? 1 : 2) + (kE4m3 ? 2 * kPos * 4 : 0);
-  static constexpr int kRing = kWarps * kStages * kSlot, kJoin = kWarps * 16 * MT * D * 4;
+  static constexpr int kRing = kWarps * kStages * kSlot, kWarpOut = kWarps * 16 * MT * D * 4;
+  static constexpr int kJoin = kWarpOut + 16 * MT * D * 4;  // the warps' results, and a cluster's share of them
   static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
 };
 
-template <typename T, int D, int MT, bool kE4m3, int kStages>
+template <typename T, int D, int MT, bool kE4m3, int kStages, bool kCluster>
 __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   using MT16 = typename std::conditional<kE4m3, __half, T>::type;  // type of the products
   constexpr int TR = 16 * MT;
@@ -85,6 +89,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   __shared__ int s_b;
   __shared__ long long s_off, s_end;
   __shared__ float s_m[kWarps][TR], s_l[kWarps][TR];
+  __shared__ float s_cm[kCluster ? TR : 1], s_cl[kCluster ? TR : 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x;
@@ -93,83 +98,92 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   pdl_launch();
 
   // ---- this CTA's range of units ----
-  auto count = [&](int b, int& per) -> int {  // tiles times heads, units of each
-    if (b >= a.c.B) return 0;
-    int tiles, first;
-    seq_units(load_seq(a, b), a.window, TR, G, tiles, first, per);
-    return tiles * Hkv;
-  };
-  long long total = 0, items = 0;
-  int my_items = 0, my_per = 0;
-  for (int b0 = 0; b0 < a.c.B; b0 += kThreads) {
-    int per = 0;
-    const int n = count(b0 + tid, per);
-    if (b0 == 0) {
-      my_items = n;
-      my_per = per;
-    }
-    long long u = static_cast<long long>(n) * per, v = n;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      u += __shfl_xor_sync(0xffffffffu, u, o);
-      v += __shfl_xor_sync(0xffffffffu, v, o);
-    }
-    if (lane == 0) {
-      s_scan[warp] = u;
-      s_items[warp] = v;
-    }
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w) {
-      total += s_scan[w];
-      items += s_items[w];
-    }
-    __syncthreads();
-  }
-  const int lead = total <= gridDim.x ? 0 : kPieceUnits;
-  total += lead * items;
-  if (tid == 0) a.desc[2 * cta] = make_int4(0, 0, 0, 0);
-  // no more CTAs than units, so that every range (before the move below) has one
-  const int ctas = static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
-  if (cta >= ctas) return;
-  // a cut inside what a tile costs to start is moved before it
-  const long long raw0 = total * cta / ctas, raw1 = total * (cta + 1) / ctas;
-  auto start_of = [&](long long off, int per) {
-    const int k = static_cast<int>(off % per);
-    return k < lead ? off - k : off;
-  };
-  if (tid == 0) s_end = raw1;
-  {
-    long long run = 0;
-    for (int b0 = 0; b0 < a.c.B && run <= raw1; b0 += kThreads) {
-      int per = my_per;
-      const int n = b0 == 0 ? my_items : count(b0 + tid, per);
-      per += lead;
-      const long long u = static_cast<long long>(n) * per;
-      long long inc = u;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
+  // A cluster takes one tile after another and cuts each into equal parts;
+  // otherwise the CTA has a range of the line of all units.
+  const int split = kCluster ? a.split : 1, rank = kCluster ? cta % split : 0;
+  const int index = cta / split;  // cluster: sequence, first tile, kv head
+  int b = kCluster ? index / (Hkv * a.tile_step) : 0, next_tile = kCluster ? index / Hkv % a.tile_step : 0;
+  int lead = 0, ctas = 0;
+  long long total = 0, u1 = 0, off = 0, left = 0;
+  if constexpr (!kCluster) {
+    auto count = [&](int b, int& per) -> int {  // tiles times heads, units of each
+      if (b >= a.c.B) return 0;
+      int tiles, first;
+      seq_units(load_seq(a, b), a.window, TR, G, tiles, first, per);
+      return tiles * Hkv;
+    };
+    long long items = 0;
+    int my_items = 0, my_per = 0;
+    for (int b0 = 0; b0 < a.c.B; b0 += kThreads) {
+      int per = 0;
+      const int n = count(b0 + tid, per);
+      if (b0 == 0) {
+        my_items = n;
+        my_per = per;
       }
-      if (lane == 31) s_scan[warp] = inc;
+      long long u = static_cast<long long>(n) * per, v = n;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        u += __shfl_xor_sync(0xffffffffu, u, o);
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+      }
+      if (lane == 0) {
+        s_scan[warp] = u;
+        s_items[warp] = v;
+      }
       __syncthreads();
-      long long lo = run + inc - u;
-      for (int w = 0; w < warp; ++w) lo += s_scan[w];
-      if (raw0 >= lo && raw0 < lo + u) {
-        s_b = b0 + tid;
-        s_off = start_of(raw0 - lo, per);
-        s_begin = lo + s_off;
+      for (int w = 0; w < kWarps; ++w) {
+        total += s_scan[w];
+        items += s_items[w];
       }
-      if (raw1 >= lo && raw1 < lo + u) s_end = lo + start_of(raw1 - lo, per);
-      for (int w = 0; w < kWarps; ++w) run += s_scan[w];
       __syncthreads();
     }
+    lead = total <= gridDim.x ? 0 : kPieceUnits;
+    total += lead * items;
+    if (tid == 0) a.desc[2 * cta] = make_int4(0, 0, 0, 0);
+    // no more CTAs than units, so that every range (before the move below) has one
+    ctas = static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
+    if (cta >= ctas) return;
+    // a cut inside what a tile costs to start is moved before it
+    const long long raw0 = total * cta / ctas, raw1 = total * (cta + 1) / ctas;
+    auto start_of = [&](long long off, int per) {
+      const int k = static_cast<int>(off % per);
+      return k < lead ? off - k : off;
+    };
+    if (tid == 0) s_end = raw1;
+    {
+      long long run = 0;
+      for (int b0 = 0; b0 < a.c.B && run <= raw1; b0 += kThreads) {
+        int per = my_per;
+        const int n = b0 == 0 ? my_items : count(b0 + tid, per);
+        per += lead;
+        const long long u = static_cast<long long>(n) * per;
+        long long inc = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += up;
+        }
+        if (lane == 31) s_scan[warp] = inc;
+        __syncthreads();
+        long long lo = run + inc - u;
+        for (int w = 0; w < warp; ++w) lo += s_scan[w];
+        if (raw0 >= lo && raw0 < lo + u) {
+          s_b = b0 + tid;
+          s_off = start_of(raw0 - lo, per);
+          s_begin = lo + s_off;
+        }
+        if (raw1 >= lo && raw1 < lo + u) s_end = lo + start_of(raw1 - lo, per);
+        for (int w = 0; w < kWarps; ++w) run += s_scan[w];
+        __syncthreads();
+      }
+    }
+    u1 = s_end;
+    if (s_begin >= u1) return;
+    b = s_b;
+    off = s_off;
+    left = u1 - s_begin;
   }
-  const long long u0 = s_begin, u1 = s_end;
-  if (u0 >= u1) return;
-  int b = s_b;
-  long long off = s_off;
-  long long left = u1 - u0;
   bool first_piece = true;
   const uint32_t ring = smem_u32(smem) + warp * kStages * kSlot;
 
@@ -177,16 +191,27 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   int tiles, kfirst, per;
   seq_units(seq, a.window, TR, G, tiles, kfirst, per);
   per += lead;
-  while (left > 0) {
-    while (off >= static_cast<long long>(tiles) * per * Hkv) {  // the next sequence with units
-      off -= static_cast<long long>(tiles) * per * Hkv;
-      if (++b >= a.c.B) return;  // the arrays changed under the call
-      seq = load_seq(a, b);
-      seq_units(seq, a.window, TR, G, tiles, kfirst, per);
-      per += lead;
+  while (true) {
+    int item, k0, k1;
+    if constexpr (kCluster) {
+      if (next_tile >= tiles) break;
+      item = next_tile * Hkv + index % Hkv;
+      next_tile += a.tile_step;
+      k0 = per * rank / split;
+      k1 = per * (rank + 1) / split;
+    } else {
+      if (left <= 0) break;
+      while (off >= static_cast<long long>(tiles) * per * Hkv) {  // the next sequence with units
+        off -= static_cast<long long>(tiles) * per * Hkv;
+        if (++b >= a.c.B) return;  // the arrays changed under the call
+        seq = load_seq(a, b);
+        seq_units(seq, a.window, TR, G, tiles, kfirst, per);
+        per += lead;
+      }
+      item = static_cast<int>(off / per);
+      k0 = static_cast<int>(off - static_cast<long long>(item) * per);
+      k1 = static_cast<int>(min(static_cast<long long>(per), k0 + left));
     }
-    const int item = static_cast<int>(off / per), k0 = static_cast<int>(off - static_cast<long long>(item) * per);
-    const int k1 = static_cast<int>(min(static_cast<long long>(per), k0 + left));
     const int tile = item / Hkv, h = item - tile * Hkv;
     const int ctx = seq.len - seq.n;
     const int m0 = tile * TR, mrows = min(TR, seq.n * G - m0);
@@ -526,8 +551,8 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           for (int n = 0; n < 2; ++n) {
             const float e0 = exp2_approx(sc[mt][n][2 * half] - mm), e1 = exp2_approx(sc[mt][n][2 * half + 1] - mm);
             l_run[mt][half] += kE4m3 ? fmaf(e0, rv[n][0], e1 * rv[n][1]) : e0 + e1;
-            // 16 bits for the product: half a step, 2^-11 (fp16) or 2^-9
-            // (bf16) of a probability, the precision of v itself
+            // 16 bits for the product: half a step, 2^-11 (fp16) or 2^-8
+            // (bf16) of a weight, the precision of v itself
             pf[mt][half + 2 * n] = Mma<MT16>::pack(e0, e1);
           }
         }
@@ -628,7 +653,8 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         }
       }
     __syncthreads();
-    const bool complete = k0 == 0 && k1 == per;
+    const bool complete = !kCluster && k0 == 0 && k1 == per;
+    float* const mine = reinterpret_cast<float*>(smem + RingBytes<D, MT, kE4m3, kStages>::kWarpOut);  // [TR][D], cluster
     float* part = a.part + static_cast<int64_t>(2 * cta + (first_piece ? 0 : 1)) * Part<TR, D>::kFloats;
     for (int i = tid; i < mrows * (D / 8); i += kThreads) {
       const int m = i / (D / 8), d = (i % (D / 8)) * 8;
@@ -656,14 +682,53 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         *reinterpret_cast<uint4*>(dst) = make_uint4(Mma<T>::pack(o[0] * inv, o[1] * inv), Mma<T>::pack(o[2] * inv, o[3] * inv),
                                                     Mma<T>::pack(o[4] * inv, o[5] * inv), Mma<T>::pack(o[6] * inv, o[7] * inv));
       } else {
-        float4* dst = reinterpret_cast<float4*>(part + m * D + d);
+        float4* dst = reinterpret_cast<float4*>((kCluster ? mine : part) + m * D + d);
         dst[0] = make_float4(o[0], o[1], o[2], o[3]);
         dst[1] = make_float4(o[4], o[5], o[6], o[7]);
-        if (d == 0) {
+        if (kCluster && d == 0) {
+          s_cm[m] = mx;
+          s_cl[m] = l;
+        } else if (d == 0) {
           part[TR * D + m] = mx;
           part[TR * D + TR + m] = l;
         }
       }
+    }
+    if constexpr (kCluster) {
+      // every CTA of the cluster has its part of the tile: each writes a slice
+      // of the rows, joined over the parts in order
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      for (int i = rank * kThreads + tid; i < mrows * (D / 8); i += kThreads * split) {
+        const int m = i / (D / 8), d = (i % (D / 8)) * 8;
+        float mx = kNegInf;
+        for (int c = 0; c < split; ++c) mx = fmaxf(mx, *cluster.map_shared_rank(&s_cm[m], c));
+        float l = 0.f, o[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) o[x] = 0.f;
+        for (int c = 0; mx != kNegInf && c < split; ++c) {
+          const float f = exp2_approx(*cluster.map_shared_rank(&s_cm[m], c) - mx);
+          l = fmaf(f, *cluster.map_shared_rank(&s_cl[m], c), l);
+          const float4* src = reinterpret_cast<const float4*>(cluster.map_shared_rank(mine + m * D + d, c));
+          const float4 v0 = src[0], v1 = src[1];
+          o[0] = fmaf(f, v0.x, o[0]);
+          o[1] = fmaf(f, v0.y, o[1]);
+          o[2] = fmaf(f, v0.z, o[2]);
+          o[3] = fmaf(f, v0.w, o[3]);
+          o[4] = fmaf(f, v1.x, o[4]);
+          o[5] = fmaf(f, v1.y, o[5]);
+          o[6] = fmaf(f, v1.z, o[6]);
+          o[7] = fmaf(f, v1.w, o[7]);
+        }
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const int mm = m0 + m, tok = mm / G;
+        T* dst = static_cast<T*>(a.out.p) + static_cast<int64_t>(seq.row0 + tok) * a.out.row_stride +
+                 static_cast<int64_t>(h * G + mm - tok * G) * a.out.head_stride + d;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(Mma<T>::pack(o[0] * inv, o[1] * inv), Mma<T>::pack(o[2] * inv, o[3] * inv),
+                                                    Mma<T>::pack(o[4] * inv, o[5] * inv), Mma<T>::pack(o[6] * inv, o[7] * inv));
+      }
+      cluster.sync();  // the parts have been read: they may go
+      continue;
     }
     if (tid == 0 && k0 == 0 && k1 < per) {
       // the first piece of a tile that goes on in later CTAs: the last of
@@ -684,28 +749,51 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
 constexpr int kCtasPerSm = 2;
 
 template <typename T, int D, int MT, bool kE4m3>
-cudaError_t attention_launch(const PagedAttention& a, cudaStream_t st) {
+cudaError_t attention_launch(const PagedAttention& a, int max_new, cudaStream_t st) {
   // Ring slots of 8 KB (16-bit) or 4.1 KB (8-bit) per warp at D = 128, two CTAs
   // per SM: 3 and 6 (96 KB a CTA); with two row tiles over 8-bit pages 4 (77.7
   // against 81.3 us for 32 x 5 rows).
   constexpr int kStages = (kE4m3 ? (MT == 2 ? 4 : 6) : 3) * (128 / D);
   constexpr int kSmem = RingBytes<D, MT, kE4m3, kStages>::kBytes + (MT == 2 ? MT * (D / 16) * 512 : 0);
-  auto k = paged_attention_kernel<T, D, MT, kE4m3, kStages>;
+  const int sms = sm_count();
+  // Where the page table cannot hold long sequences: a cluster per tile, in one
+  // launch, as many CTAs as keep every cluster resident.  8 sequences of up to
+  // 255 positions take 7.1 us so, and 10.2 by ranges of the line and the join
+  // that goes with them; one of 4000 12.3 and 17.8.  A CTA takes at most 8 units:
+  // longer sequences are balanced better by the line.
+  const int64_t units = (static_cast<int64_t>(a.c.max_pages) * a.c.page_size + kUnit - 1) / kUnit;
+  const int64_t most = (static_cast<int64_t>(max_new) * a.G + 16 * MT - 1) / (16 * MT);  // tiles of a sequence
+  const int64_t items = most * a.c.Hkv * a.c.B;
+  int split = 8;
+  while (split > 1 && (items * split > kCtasPerSm * sms || split / 2 >= units)) split /= 2;
+  if (items * split <= kCtasPerSm * sms && units <= 8 * split) {
+    PagedAttention c = a;
+    c.split = split;
+    c.tile_step = static_cast<int>(most);
+    auto k = paged_attention_kernel<T, D, MT, kE4m3, kStages, true>;
+    static std::atomic<bool> done[64];
+    const cudaError_t e = prepare_kernel(done, k, kSmem, 0);
+    if (e != cudaSuccess) return e;
+    return launch_paged(k, dim3(static_cast<unsigned>(items * split)), dim3(kThreads), kSmem, split, false, st, c);
+  }
+  auto k = paged_attention_kernel<T, D, MT, kE4m3, kStages, false>;
   static std::atomic<bool> done[64];
   cudaError_t e = prepare_kernel(done, k, kSmem, 0);
   if (e != cudaSuccess) return e;
-  const int ctas = kCtasPerSm * sm_count();
+  const int ctas = kCtasPerSm * sms;
   e = launch_paged(k, dim3(ctas), dim3(kThreads), kSmem, 1, false, st, a);
   if (e != cudaSuccess) return e;
   return launch_paged(paged_combine_kernel<T, D, 16 * MT>, dim3(ctas, 2 * MT), dim3(256), 0, 1, true, st, a);
 }
 template <typename T, int D, int MT>
-cudaError_t attention_pages(const PagedAttention& a, cudaStream_t st) {
-  return a.c.k_scale != nullptr ? attention_launch<T, D, MT, true>(a, st) : attention_launch<T, D, MT, false>(a, st);
+cudaError_t attention_pages(const PagedAttention& a, int max_new, cudaStream_t st) {
+  return a.c.k_scale != nullptr ? attention_launch<T, D, MT, true>(a, max_new, st)
+                                : attention_launch<T, D, MT, false>(a, max_new, st);
 }
 template <typename T, int D>
 cudaError_t attention_rows(const PagedAttention& a, int max_new, cudaStream_t st) {
-  return static_cast<int64_t>(max_new) * a.G <= 16 ? attention_pages<T, D, 1>(a, st) : attention_pages<T, D, 2>(a, st);
+  return static_cast<int64_t>(max_new) * a.G <= 16 ? attention_pages<T, D, 1>(a, max_new, st)
+                                                  : attention_pages<T, D, 2>(a, max_new, st);
 }
 template <typename T>
 cudaError_t attention_dim(const PagedAttention& a, int max_new, cudaStream_t st) {

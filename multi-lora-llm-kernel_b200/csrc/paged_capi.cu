@@ -131,6 +131,7 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
   a.window = window > kI32Max ? 0 : static_cast<int>(window);  // wider than any position
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = dev_err;
+  a.split = a.tile_step = 1;
   const int most = static_cast<int>(max_new > rows ? rows : max_new);
   if (static_cast<int64_t>(most) * a.G > (a.c.k_scale != nullptr ? kFewRows8 : kFewRows16))
     return status(launch_paged_chunk(a, dtype, workspace, stream));

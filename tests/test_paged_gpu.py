@@ -386,6 +386,23 @@ def test_a_speculative_step(e4m3):
         _check(got, want, want.abs() * (2.0 ** -4 if e4m3 else 0) + (want.abs().amax(-1, keepdim=True) / 448 * 2.0 ** -9 if e4m3 else 0))
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_short_and_wide_page_tables(e4m3):
+    """The same sequences behind a page table of their own width and a wide one
+    (another division of the work), and more new tokens than the hint says."""
+    outs = []
+    for width in (None, 4, 40, 600):
+        bt = R.Batch([3, 1, 9, 0], [37, 2, 44, 5], 16, 2, 128, H, e4m3, seed=8, width=width)
+        bt.fill()
+        q = bt.randn(bt.rows, 8, 128)
+        outs += [_attend(bt, q, max_new=n) for n in (1, 3, 9)]
+        bt.lengths.zero_()  # nothing cached: all rows lie before the start
+        out = torch.full_like(q, 7.0)
+        ops.paged_attention(q, *bt.args(), out, 0.1, **bt.scales())
+        assert torch.all(out == 0)
+    ops.check_errors(torch.device("cuda", 0))
+
+
 def test_long_step_of_many_rows_of_the_chunk_shape():
     """A prompt chunk over a long cache, beside decoding sequences."""
     bt = R.Batch([600, 1, 1, 129], [3000, 2500, 0, 1], 64, 2, 128, H, False)
