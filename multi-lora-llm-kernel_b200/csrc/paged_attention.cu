@@ -759,14 +759,15 @@ cudaError_t attention_launch(const PagedAttention& a, int max_new, cudaStream_t 
   // Where the page table cannot hold long sequences: a cluster per tile, in one
   // launch, as many CTAs as keep every cluster resident.  8 sequences of up to
   // 255 positions take 7.1 us so, and 10.2 by ranges of the line and the join
-  // that goes with them; one of 4000 12.3 and 17.8.  A CTA takes at most 8 units:
-  // longer sequences are balanced better by the line.
+  // that goes with them; 4 of up to 8000 15.8 and 19.0.  A CTA takes at most 16
+  // units so: from 32 on longer sequences are balanced better by the line (one
+  // of 16000: 32.3 and 27.5).
   const int64_t units = (static_cast<int64_t>(a.c.max_pages) * a.c.page_size + kUnit - 1) / kUnit;
   const int64_t most = (static_cast<int64_t>(max_new) * a.G + 16 * MT - 1) / (16 * MT);  // tiles of a sequence
   const int64_t items = most * a.c.Hkv * a.c.B;
   int split = 8;
   while (split > 1 && (items * split > kCtasPerSm * sms || split / 2 >= units)) split /= 2;
-  if (items * split <= kCtasPerSm * sms && units <= 8 * split) {
+  if (items * split <= kCtasPerSm * sms && units <= 16 * split) {
     PagedAttention c = a;
     c.split = split;
     c.tile_step = static_cast<int>(most);
