@@ -344,7 +344,8 @@ int persona_rope_decode_attention(void* q, void* k, const void* v, void* k_cache
  * for the zeros that persona_paged_attention gives the last kind.
  * A position behind the page table or a page outside [0, num_pages) raises
  * PERSONA_DEV_ERR_PAGE; write and read then leave the row alone, attention
- * takes zeros in its place.  indptr must not decrease and must end within
+ * takes zeros in its place.  A page table holds at most 2^30 positions a
+ * sequence for attention.  indptr must not decrease and must end within
  * `rows`; a sequence that breaks this raises PERSONA_DEV_ERR_SEGMENT in
  * attention and verification and is left out.
  *

@@ -828,6 +828,8 @@ void paged_rope_cache_op(const at::Tensor& q, const at::Tensor& k, const at::Ten
   const int dt = dtype_code(q, op);
   const persona_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale, page_table, indptr, lengths, q, op);
   TORCH_CHECK(k.size(1) == c.Hkv && v.size(1) == c.Hkv && q_out.size(1) == q.size(1), op, ": head count mismatch");
+  TORCH_CHECK((c.num_pages <= 1 || c.page_stride >= c.D) && (c.Hkv <= 1 || c.head_stride >= c.D), op,
+              ": caches are written and must not overlap themselves");
   const at::cuda::OptionalCUDAGuard guard(q.device());
   const int dev = q.get_device();
   raise_pending(dev, op);

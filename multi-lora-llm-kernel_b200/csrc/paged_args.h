@@ -54,7 +54,7 @@ struct PagedAttention {
   int window;          // 0: none
   float scale_log2;    // softmax scale times log2(e)
   int split, tile_step;  // a cluster per tile: its CTAs, and the first tiles taken per sequence and head
-  float* part;         // partial results, see paged_attention.cu
+  float* part;         // partial results, see paged_attention.cuh
   int4* desc;          // two per CTA
   int32_t* err;
 };

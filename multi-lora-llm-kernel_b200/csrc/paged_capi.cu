@@ -11,6 +11,7 @@ namespace {
 
 constexpr int64_t kI32Max = 2147483647;
 constexpr int64_t kMaxHeads = 1024;
+constexpr int64_t kMaxPositions = int64_t{1} << 30;
 // Most query rows per kv head (new tokens times heads of a group) for the
 // warp-level kernel, which reads the pages once per 32 rows.  Measured with 32
 // sequences of up to 6000 tokens: over 16-bit pages 36 rows take it 118 us and
@@ -119,8 +120,9 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
   if (rows < 0 || Hq <= 0 || Hq > kMaxHeads || Hq % cache->Hkv || rows > kI32Max / Hq || window < 0 || max_new < 1 ||
       !(scale > 0.f) || !std::isfinite(scale))
     return PERSONA_ERR_SHAPE;
-  // positions of a sequence are 32-bit numbers
-  if (cache->max_pages > kI32Max / cache->page_size - 64 / cache->page_size - 1) return PERSONA_ERR_SHAPE;
+  // positions of a sequence, and what the kernels add to and take from them
+  // (blocks ahead, a window), are 32-bit numbers
+  if (cache->max_pages > kMaxPositions / cache->page_size) return PERSONA_ERR_SHAPE;
   if (rows == 0 || cache->B == 0) return PERSONA_OK;
   PERSONA_TRY(check_rows(q, a.q));
   PERSONA_TRY(check_rows(out, a.out));
@@ -128,7 +130,7 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
   if (!aligned(workspace, 16)) return PERSONA_ERR_ALIGNMENT;
   a.rows = static_cast<int>(rows);
   a.G = static_cast<int>(Hq / cache->Hkv);
-  a.window = window > kI32Max ? 0 : static_cast<int>(window);  // wider than any position
+  a.window = window >= kMaxPositions ? 0 : static_cast<int>(window);  // wider than any sequence
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = dev_err;
   a.split = a.tile_step = 1;

@@ -80,7 +80,7 @@ constexpr float kMinScale = 9.094947017729282e-13f;
 // `early`.  A kernel that takes most of an SM's shared memory is not launched
 // early: the SM keeps the division of its memory for as long as the kernel
 // before is resident, and a grid that is meant to be resident as a whole gets
-// fewer blocks per SM (three blocks of 68 KB became two: 77 us instead of 50).
+// fewer blocks per SM (three blocks of 68 KB became two: 77 us instead of 55).
 template <typename... KArgs, typename... Args>
 cudaError_t launch_paged(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, int cluster_x, bool early,
                          cudaStream_t st, Args... args) {
