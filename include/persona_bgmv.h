@@ -396,8 +396,9 @@ int persona_paged_cache_read(const persona_paged_cache* cache, const persona_row
  * out[r, h] = softmax_j(scale q[r, h] . k[j, h / G]) v[j, h / G], G = Hq / Hkv,
  * over j <= pos(r) and, with window > 0, j > pos(r) - window; zeros where that
  * leaves nothing; scale > 0.  The new tokens' k and v are read from the pages, so write
- * them first.  What lies in the pages behind a sequence's last position is
- * never used; a NaN or infinity at a position of the sequence itself may reach
+ * them first.  What lies in the pages behind a sequence's last position, or
+ * before the window of its first new token, is never used, and the page table's
+ * entries for the latter are not either; a NaN or infinity at a position of the sequence itself may reach
  * every new row of that sequence.
  * max_new: an upper bound of the new tokens of one sequence, for the choice of
  * the kernel; a larger number of them is still computed correctly.

@@ -271,11 +271,16 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           pages32 = p < pend && pi < a.c.max_pages ? pages[pi] : -1;
         }
         const int pg = __shfl_sync(0xffffffffu, pages32, s & 31);
-        int rem = pend - p0;  // positions of this step
+        // positions of this step: those from `skip` on, `rem` of them (what lies
+        // before the window may be in a page that was given back)
+        const int skip = max(pbegin - p0, 0);
+        int rem = min(pend - p0, kPos) - skip;
         if (rem > 0 && (pg < 0 || pg >= a.c.num_pages)) {
           raise_error(a.err, PERSONA_DEV_ERR_PAGE);
           rem = 0;
         }
+        rem = max(rem, 0);
+        const int lrs = lr - skip;
         const int at = p0 - page_index(a.c, p0) * a.c.page_size;
         const int64_t base = rem > 0 ? (pg * a.c.page_stride + at * a.c.pos_stride) * kElt : 0;
         const uint8_t *kp = kl + base, *vp = vl + base;
@@ -283,14 +288,14 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         for (int i = 0; i < kPos / kRowsPer; ++i, kp += row_step, vp += row_step) {
           constexpr int kStep = kRowsPer;
           const int ck = kE4m3 ? ck0 : ck0 ^ ((i * kStep) & 7), cv = kE4m3 ? cv0 ^ (((i * kStep / 2) & 3) << 1) : ck;
-          const bool live = lr + i * kStep < rem;
+          const bool live = static_cast<uint32_t>(lrs + i * kStep) < static_cast<uint32_t>(rem);
           const uint32_t to = dst + (lr + i * kStep) * kRowBytes;
           cp_async16(to + (ck & kMask) * 16, live ? kp : kl, live);
           cp_async16(to + kHalf + (cv & kMask) * 16, live ? vp : vl, live);
         }
         if (kE4m3) {
           const int r = lane & 15;
-          const bool live = r < rem;
+          const bool live = static_cast<uint32_t>(r - skip) < static_cast<uint32_t>(rem);
           cp_async4(dst + 2 * kHalf + lane * 4, live ? sl + (pg * a.c.scale_page_stride + at + r) : sl, live);
         }
       } else {
@@ -299,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           const int r = lr + i * kRowsPer;
           const int ck = kE4m3 ? ck0 : ck0 ^ ((i * kRowsPer) & 7), cv = kE4m3 ? cv0 ^ (((i * kRowsPer / 2) & 3) << 1) : ck;
           int at = 0;
-          const int pg = p0 + r < pend ? page_of(p0 + r, at) : -1;
+          const int pg = p0 + r >= pbegin && p0 + r < pend ? page_of(p0 + r, at) : -1;
           const bool live = pg >= 0;
           const int64_t src = live ? (pg * a.c.page_stride + at * a.c.pos_stride) * kElt : 0;
           const uint32_t to = dst + r * kRowBytes;
@@ -309,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         if (kE4m3) {
           const int p = p0 + (lane & 15);
           int at = 0;
-          const int pg = p < pend ? page_of(p, at) : -1;
+          const int pg = p >= pbegin && p < pend ? page_of(p, at) : -1;
           cp_async4(dst + 2 * kHalf + lane * 4, pg >= 0 ? sl + (pg * a.c.scale_page_stride + at) : sl, pg >= 0);
         }
       }

@@ -83,7 +83,7 @@ struct Shared {
 constexpr int kPieceUnits = 2;
 
 struct TileGeo {
-  int m0, mrows, first, per, pend;  // per: with the `lead` units above
+  int m0, mrows, first, per, pbegin, pend;  // per: with the `lead` units above
 };
 __device__ __forceinline__ TileGeo tile_geo(const Seq& s, int window, int G, int t, int lead) {
   TileGeo g;
@@ -91,7 +91,8 @@ __device__ __forceinline__ TileGeo tile_geo(const Seq& s, int window, int G, int
   g.mrows = min(kTile, s.n * G - g.m0);
   const int ctx = s.len - s.n, tok0 = g.m0 / G, tok1 = (g.m0 + g.mrows - 1) / G;
   g.pend = max(0, min(s.len, ctx + tok1 + 1));
-  g.first = (window > 0 ? max(0, ctx + tok0 + 1 - window) : 0) / kBlock;
+  g.pbegin = window > 0 ? max(0, ctx + tok0 + 1 - window) : 0;
+  g.first = g.pbegin / kBlock;
   g.per = max(1, (g.pend + kBlock - 1) / kBlock - g.first) + lead;
   return g;
 }
@@ -623,7 +624,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         auto fetch = [&](int j) {
           const int p = (first + j) * kBlock + t, pi = page_index(a.c, p);
           at = p - pi * a.c.page_size;
-          seen = p < w.g.pend;
+          // (what lies before the window may be in a page that was given back)
+          seen = p >= w.g.pbegin && p < w.g.pend;
           pg = -1;
           if (seen && pi < a.c.max_pages) pg = row[pi];
         };

@@ -287,7 +287,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of each sequence's new tokens over its pages, theirs
     included (write them first); with ``window`` over the last ``window``
-    positions only.  Layouts as in ``paged_rope_cache``; ``out`` like ``q``.
+    positions only (pages that no new token's window reaches may be given
+    back: their table entries and contents are not used).  Layouts as in ``paged_rope_cache``; ``out`` like ``q``.
     A row that sees no position gives zeros; ``scale`` is positive.
 
     ``max_new``: an upper bound of the new tokens of one sequence, which

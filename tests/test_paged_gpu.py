@@ -408,3 +408,70 @@ def test_long_step_of_many_rows_of_the_chunk_shape():
     bt = R.Batch([600, 1, 1, 129], [3000, 2500, 0, 1], 64, 2, 128, H, False)
     bt.fill()
     _attend(bt, bt.randn(bt.rows, 8, 128), max_new=600)
+
+
+@pytest.mark.parametrize("page", [16, 7, 1])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("n", [1, 5, 150])
+def test_pages_before_the_window_may_be_given_back(n, e4m3, page):
+    """Table entries of the pages that the first new token's window does not
+    reach point nowhere, and what is left of the last such page is NaN.  What
+    is computed then is what it was with the pages still there."""
+    window, ctx = 45, [400, 83, 20]
+    bt = R.Batch([n] * 3, ctx, page, 2, 128, H, e4m3, seed=n)
+    bt.fill()
+    q = bt.randn(bt.rows, 8, 128)
+    want, tol = R.attention(bt, q, 0.1, window)
+    for b, c in enumerate(ctx):
+        first = max(0, c + 1 - window)
+        if first:
+            pg, at = bt.where(b, 0, first)
+            for x in (bt.k_cache, bt.v_cache):
+                if e4m3:
+                    x.view(torch.uint8)[pg, :, at] = 0x7F  # NaN
+                else:
+                    x[pg, :, at] = float("nan")
+            if e4m3:
+                bt.k_scale[pg, :, at] = bt.v_scale[pg, :, at] = float("nan")
+            bt.table[b, :first // page] = -1
+    out = torch.zeros_like(q)
+    ops.paged_attention(q, *bt.args(), out, 0.1, window=window, max_new=n, **bt.scales())
+    ops.check_errors(q.device)
+    _check(out, want, tol)
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_many_sequences(n):
+    """More sequences than threads of a CTA, in both kernels."""
+    B = 700
+    bt = R.Batch([n if b % 3 else 0 for b in range(B)], [b * 7 % 90 for b in range(B)], 16, 1, 64, H, seed=2, pad=2)
+    bt.fill()
+    _attend(bt, bt.randn(bt.rows, 4, 64), max_new=n)
+
+
+def test_captured_chunks_on_two_streams():
+    """Prompt chunks captured on their own streams, both graphs under way at once."""
+    made = []
+    for seed in range(2):
+        bt = R.Batch([300, 40], [200 + 50 * seed, 0], 16, 2, 128, H, seed=seed)
+        bt.fill()
+        q = bt.randn(bt.rows, 8, 128)
+        out, s = torch.zeros_like(q), torch.cuda.Stream()
+        ops.paged_attention(q, *bt.args(), out, 0.1, max_new=300)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.paged_attention(q, *bt.args(), out, 0.1, max_new=300)
+        made.append((bt, q, out, s, g))
+    for _ in range(4):
+        for bt, q, out, s, g in made:
+            out.zero_()
+        torch.cuda.synchronize()
+        for *_, s, g in made:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for bt, q, out, *_ in made:
+            want, tol = R.attention(bt, q, 0.1)
+            _check(out, want, tol)
+    ops.check_errors(torch.device("cuda", 0))
