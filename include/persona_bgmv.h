@@ -389,7 +389,7 @@ int persona_paged_rope_cache(const persona_paged_cache* cache, const persona_row
                              int dtype, int32_t* dev_err, cudaStream_t stream);
 /* The way back: k and v of every row's position as 16-bit rows (codes times
  * scale, one rounding).  With indptr[b + 1] - indptr[b] = lengths[b] a
- * sequence's whole cache.                                                   */
+ * sequence's whole cache.  k and v do not overlap.                          */
 int persona_paged_cache_read(const persona_paged_cache* cache, const persona_rows* k, const persona_rows* v,
                              int64_t rows, int dtype, int32_t* dev_err, cudaStream_t stream);
 /* Causal attention of the new rows over their sequence's pages:
@@ -399,7 +399,7 @@ int persona_paged_cache_read(const persona_paged_cache* cache, const persona_row
  * them first.  What lies in the pages behind a sequence's last position, or
  * before the window of its first new token, is never used, and the page table's
  * entries for the latter are not either; a NaN or infinity at a position of the sequence itself may reach
- * every new row of that sequence.
+ * every new row of that sequence.  out does not overlap q.
  * max_new: an upper bound of the new tokens of one sequence, for the choice of
  * the kernel; a larger number of them is still computed correctly.
  * workspace: persona_paged_attention_workspace_size(D) bytes for the current
@@ -422,7 +422,8 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
  * if there is none at all.  Sums and comparisons in 64 bits.
  * tokens[row]: d_0 .. d_{a-1}, the drawn token, then -1; accepted[b] = a (0
  * for an empty sequence).  Probabilities fp16, bf16 or fp32 (prob_type), both
- * of one type, rows ld_* elements apart; they need not be normalised.       */
+ * of one type, rows ld_* elements apart; they need not be normalised.  tokens
+ * does not overlap draft_tokens.                                            */
 #define PERSONA_VERIFY_MAX_VOCAB 2097152
 int persona_verify_draft(const void* target, int64_t ld_target, const void* draft, int64_t ld_draft, int prob_type,
                          const int64_t* draft_tokens, const int32_t* indptr, const float* u_accept,

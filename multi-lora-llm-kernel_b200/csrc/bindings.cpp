@@ -763,6 +763,28 @@ persona_rows rows_of(const at::Tensor& t, const at::Tensor& like, const char* op
   return persona_rows{t.data_ptr(), t.size(0) <= 1 ? 0 : t.stride(0), t.size(1) <= 1 ? 0 : t.stride(1)};
 }
 
+// Whether two [rows, heads, D] activations of the same number of rows share an
+// element.  Exact for slices of one fused buffer (the same row stride, rows that
+// do not reach into one another); elsewhere, whether their extents meet.
+bool rows_meet(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const int64_t e = a.element_size(), rows = a.size(0);
+  const auto width = [](const at::Tensor& t) { return (t.size(1) <= 1 ? 0 : (t.size(1) - 1) * t.stride(1)) + t.size(2); };
+  const auto step = [&](const at::Tensor& t) { return rows <= 1 ? 0 : t.stride(0); };
+  const int64_t wa = width(a), wb = width(b);
+  const int64_t pa = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.data_ptr())),
+                pb = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data_ptr()));
+  if (pa + ((rows - 1) * step(a) + wa) * e <= pb || pb + ((rows - 1) * step(b) + wb) * e <= pa) return false;
+  const int64_t s = step(a) * e;
+  if (step(a) != step(b) || step(a) < wa || step(b) < wb) return true;
+  const int64_t d = ((pb - pa) % s + s) % s;  // where b starts in a row of a
+  return d < wa * e || s - d < wb * e;
+}
+
+bool same_rows(const at::Tensor& a, const at::Tensor& b) {
+  return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
+}
+
 persona_paged_cache cache_of(const at::Tensor& k_cache, const at::Tensor& v_cache, const c10::optional<at::Tensor>& k_scale,
                              const c10::optional<at::Tensor>& v_scale, const at::Tensor& table, const at::Tensor& indptr,
                              const at::Tensor& lengths, const at::Tensor& like, const char* op) {
@@ -830,6 +852,8 @@ void paged_rope_cache_op(const at::Tensor& q, const at::Tensor& k, const at::Ten
   TORCH_CHECK(k.size(1) == c.Hkv && v.size(1) == c.Hkv && q_out.size(1) == q.size(1), op, ": head count mismatch");
   TORCH_CHECK((c.num_pages <= 1 || c.page_stride >= c.D) && (c.Hkv <= 1 || c.head_stride >= c.D), op,
               ": caches are written and must not overlap themselves");
+  TORCH_CHECK(same_rows(q, q_out) || !rows_meet(q, q_out), op, ": q_out must be q or not overlap it");
+  TORCH_CHECK(!rows_meet(k, q_out) && !rows_meet(v, q_out), op, ": q_out must not overlap k or v");
   const at::cuda::OptionalCUDAGuard guard(q.device());
   const int dev = q.get_device();
   raise_pending(dev, op);
@@ -849,6 +873,7 @@ void paged_cache_read_op(const at::Tensor& k_cache, const at::Tensor& v_cache, c
   const int dt = dtype_code(k_out, op);
   const persona_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale, page_table, indptr, lengths, k_out, op);
   TORCH_CHECK(k_out.size(1) == c.Hkv && v_out.size(1) == c.Hkv, op, ": head count mismatch");
+  TORCH_CHECK(!rows_meet(k_out, v_out), op, ": k_out and v_out must not overlap");
   const at::cuda::OptionalCUDAGuard guard(k_out.device());
   const int dev = k_out.get_device();
   raise_pending(dev, op);
@@ -868,6 +893,8 @@ void paged_attention_op(const at::Tensor& q, const at::Tensor& k_cache, const at
   const persona_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale, page_table, indptr, lengths, q, op);
   TORCH_CHECK(out.size(1) == q.size(1) && c.Hkv > 0 && q.size(1) % c.Hkv == 0, op,
               ": the heads of q and out must be a multiple of the kv heads");
+  // a row's q is read again by the CTAs that share its positions
+  TORCH_CHECK(!rows_meet(q, out), op, ": out must not overlap q");
   TORCH_CHECK(window >= 0, op, ": window must not be negative (0: none)");
   TORCH_CHECK(max_new >= 1, op, ": max_new must be positive");
   const at::cuda::OptionalCUDAGuard guard(q.device());
@@ -913,6 +940,9 @@ void verify_draft_op(const at::Tensor& target, const at::Tensor& draft_tokens, c
   vec(u_sample, at::kFloat, B, "u_sample", "float32 [B] tensor");
   vec(tokens, at::kLong, rows, "tokens", "int64 [rows] tensor");
   vec(accepted, at::kInt, B, "accepted", "int32 [B] tensor");
+  TORCH_CHECK(rows == 0 || tokens.data_ptr<int64_t>() + rows <= draft_tokens.data_ptr<int64_t>() ||
+                  draft_tokens.data_ptr<int64_t>() + rows <= tokens.data_ptr<int64_t>(),
+              op, ": tokens must not overlap draft_tokens");
   const at::cuda::OptionalCUDAGuard guard(target.device());
   const int dev = target.get_device();
   raise_pending(dev, op);

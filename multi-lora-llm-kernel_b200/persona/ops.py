@@ -286,7 +286,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     max_new: Optional[int] = None, k_scale: Optional[torch.Tensor] = None,
                     v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of each sequence's new tokens over its pages, theirs
-    included (write them first); with ``window`` over the last ``window``
+    included (write them first; ``out`` must not overlap ``q``); with ``window`` over the last ``window``
     positions only (pages that no new token's window reaches may be given
     back: their table entries and contents are not used).  Layouts as in ``paged_rope_cache``; ``out`` like ``q``.
     A row that sees no position gives zeros; ``scale`` is positive.
@@ -314,7 +314,8 @@ def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_p
     token).  Drafts are kept while ``u_accept[row] * q < p``.  Then one token
     is drawn with ``u_sample[b]``: from ``max(p - q, 0)`` where a draft was
     rejected, else from the last row.  ``tokens`` [rows] int64: the kept
-    drafts, the drawn token, then -1; ``accepted`` [B] int32: how many."""
+    drafts, the drawn token, then -1 (a buffer apart from ``draft_tokens``);
+    ``accepted`` [B] int32: how many."""
     _paged("verify_draft", target_probs).verify_draft(target_probs, draft_tokens, draft_probs, indptr, u_accept,
                                                       u_sample, tokens, accepted)
     return tokens, accepted

@@ -163,3 +163,12 @@ def test_plain_verification_by_hand():
     assert R.verify(p, d, q, ip, torch.tensor([0.9, 0.1, 0.0]), torch.tensor([0.15])) == ([0, 0, 1], [2])
     # a certain draft: kept while u < p; not drawn again
     assert R.verify(p, d, None, ip, torch.tensor([0.6, 0.0, 0.0]), torch.tensor([0.0])) == ([1, -1, -1], [0])
+
+
+def test_page_tables_hold_at_most_2_30_positions(lib):
+    """One page more is refused; the limit itself goes on to the next check
+    (a workspace that is missing)."""
+    for page in (1, 16, 64, 4096):
+        most = (1 << 30) // page
+        at = lambda n: _cache(page_size=page, max_pages=n, table_stride=n)  # noqa: E731
+        assert _attend(lib, at(most + 1)) == 2 and _attend(lib, at(most), ws=None) == 6

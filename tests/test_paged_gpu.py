@@ -475,3 +475,30 @@ def test_captured_chunks_on_two_streams():
             want, tol = R.attention(bt, q, 0.1)
             _check(out, want, tol)
     ops.check_errors(torch.device("cuda", 0))
+
+
+def test_outputs_that_overlap_inputs_are_refused():
+    bt = R.Batch([4, 3], [60, 9], 16, 2, 128, H, pad=1)
+    bt.fill()
+    fused = bt.randn(bt.rows, 24, 128)
+    q, k, v = fused[:, :8], fused[:, 8:10], fused[:, 10:12]
+    for out in (q, fused[:, 1:9], fused[:, 7:15]):
+        with pytest.raises(RuntimeError, match="out must not overlap q"):
+            ops.paged_attention(q, *bt.args(), out, 0.1)
+    # q and out as slices of one buffer that share nothing
+    want, tol = R.attention(bt, q, 0.1)
+    out = fused[:, 16:24]
+    ops.paged_attention(q, *bt.args(), out, 0.1)
+    _check(out[:7], want[:7], tol[:7])
+    with pytest.raises(RuntimeError, match="q_out must be q"):
+        ops.paged_rope_cache(q, k, v, *bt.args(), THETA, q_out=fused[:, 1:9])
+    with pytest.raises(RuntimeError, match="must not overlap k or v"):
+        ops.paged_rope_cache(q, k, v, *bt.args(), THETA, q_out=fused[:, 9:17])
+    with pytest.raises(RuntimeError, match="k_out and v_out"):
+        ops.paged_cache_read(*bt.args(), fused[:, 8:10], fused[:, 9:11])
+    ops.paged_cache_read(*bt.args(), k, v)
+    want = bt.get("v", 1, 9, 12)
+    _check(v[4:7], want, 0 * want)
+    flat = bt.k_cache[0].expand_as(bt.k_cache)
+    with pytest.raises(RuntimeError, match="overlap themselves"):
+        ops.paged_rope_cache(q, k, v, flat, flat, *bt.args()[2:], THETA)

@@ -133,3 +133,15 @@ def test_captured():
         g.replay()
         want, want_a = R.verify(p, d, q, indptr, ua, us)
         assert tokens.tolist() == want and acc.tolist() == want_a
+
+
+def test_tokens_over_the_drafts_are_refused():
+    p, d, q, indptr, ua, us = _case([3, 2], 50, torch.float32, 8)
+    acc = torch.zeros(2, dtype=torch.int32, device=DEV)
+    both = torch.cat([d, d])
+    for tokens in (both[:5], both[1:6]):
+        with pytest.raises(RuntimeError, match="must not overlap draft_tokens"):
+            ops.verify_draft(p, both[:5], q, indptr, ua, us, tokens, acc)
+    tokens, _ = ops.verify_draft(p, both[:5], q, indptr, ua, us, both[5:], acc)
+    want, want_a = R.verify(p, d, q, indptr, ua, us)
+    assert tokens.tolist() == want and acc.tolist() == want_a
