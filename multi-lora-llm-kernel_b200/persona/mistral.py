@@ -287,6 +287,10 @@ class MistralLoRAModel:
         new = [len(c) for c in chunks]
         if len(new) != len(st.lengths):
             raise ValueError("one chunk per sequence")
+        flat_ids = [t for c in chunks for t in c]
+        # (the -1 behind a verified sequence's drawn token is not one to feed)
+        if flat_ids and not 0 <= min(flat_ids) <= max(flat_ids) < cfg.vocab:
+            raise ValueError("token id outside the vocabulary")
         st._grow(new)
         R = sum(new)
         starts = [0]
@@ -294,7 +298,7 @@ class MistralLoRAModel:
             starts.append(starts[-1] + n)
         indptr = torch.tensor(starts, dtype=torch.int32, device=d)
         lengths = torch.tensor(st.lengths, dtype=torch.int32, device=d)
-        tokens = torch.tensor([t for c in chunks for t in c], dtype=torch.int64, device=d)
+        tokens = torch.tensor(flat_ids, dtype=torch.int64, device=d)
         if R == 0:
             return torch.empty(0, cfg.vocab, dtype=torch.float16, device=d), indptr
         h = self.embed.index_select(0, tokens)

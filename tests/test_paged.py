@@ -172,3 +172,22 @@ def test_page_tables_hold_at_most_2_30_positions(lib):
         most = (1 << 30) // page
         at = lambda n: _cache(page_size=page, max_pages=n, table_stride=n)  # noqa: E731
         assert _attend(lib, at(most + 1)) == 2 and _attend(lib, at(most), ws=None) == 6
+
+
+def test_extend_refuses_token_ids_outside_the_vocabulary():
+    """Before the state moves on (no model or GPU is reached)."""
+    from types import SimpleNamespace
+
+    from persona.mistral import MistralLoRAModel, PagedState
+
+    none = [None]
+    st = PagedState(slots=torch.zeros(2, dtype=torch.int32), page_size=4, page_table=torch.zeros(2, 2, dtype=torch.int32),
+                    k_cache=none, v_cache=none, k_scale=none, v_scale=none, lengths=[0, 0], pages=[[], []],
+                    free=list(range(4)))
+    model = SimpleNamespace(cfg=SimpleNamespace(vocab=50), device=torch.device("cpu"))
+    for bad in (-1, 50, 1 << 40):
+        with pytest.raises(ValueError, match="outside the vocabulary"):
+            MistralLoRAModel.extend(model, st, [[1, 49], [0, bad]])
+    with pytest.raises(ValueError, match="one chunk"):
+        MistralLoRAModel.extend(model, st, [[1]])
+    assert st.lengths == [0, 0] and st.pages == [[], []] and len(st.free) == 4
