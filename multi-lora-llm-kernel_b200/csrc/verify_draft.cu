@@ -7,11 +7,13 @@
 // What it must read is one row of each distribution per sequence, so it is
 // bound by its chain of dependent steps (rows, tokens, their probabilities, the
 // row, the sums, the tile): 8 sequences of 4 drafts over 32000 tokens take 5.6
-// us, 256 of up to 7 over 50257 (fp16) 20 us, 0.39 of the measured HBM
-// rate.
+// us, 256 of up to 7 over 50257 17 us in fp16 (0.46 of the measured HBM
+// rate) and 21 us in bf16, whose sums take more conversions to 64 bits.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "paged_common.cuh"
 
@@ -103,7 +105,7 @@ __device__ __forceinline__ double warp_scan(double v) {
   return v;
 }
 
-// Sums over the warp of kN values (2 or 4) at once: every exchange halves how
+// Sums over the warp of kN values (a power of two) at once: every exchange halves how
 // many a lane still carries.  Value i ends in the lanes whose top bits are i.
 template <int kN> __device__ __forceinline__ double warp_sums(double (&s)[kN]) {
   const int lane = threadIdx.x & 31;
@@ -197,8 +199,26 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const __grid_
     for (int i = 0; i < 8; ++i) w[i] = x + i == skip ? 0.0 : weight(p[i], f[i]);
     return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
   };
-  // tiles of a warp's step, all of whose loads are under way at once
-  constexpr int kStep = sizeof(T) == 4 ? 2 : 4;
+  // The sum alone.  fp16: differences of two numbers are multiples of 2^-24, and
+  // fp32 holds those below 1 exactly, so a sum of such weights that comes out
+  // below 1 had no larger part and no rounding: one conversion to 64 bits for
+  // eight tokens instead of sixteen, which the SM makes 16 of per cycle.
+  auto weight_sum = [&](const Raw<T>& rp, const Raw<T>& rq, int x) {
+    if constexpr (std::is_same<T, __half>::value) {
+      float p[8], f[8];
+      rp.values(p);
+      rq.values(f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = p[i] > f[i] ? p[i] - f[i] : 0.f;
+      const float s = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      if (s < 1.f && static_cast<unsigned>(skip - x) >= 8u) return static_cast<double>(s);
+    }
+    double w[8];
+    return weights(rp, rq, x, w);
+  };
+  // tiles of a warp's step, all of whose loads are under way at once (256
+  // sequences: four of fp16 take 18.9 us, two 17.1; of bf16 23.5 and 21.0)
+  constexpr int kStep = 2;
   double total = 0.0, before = 0.0;
   int last = -1;  // the last CTA with weight
   int mode = rejected ? 1 : 0;
@@ -222,10 +242,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const __grid_
       }
       double s[kStep];
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        double w[8];
-        s[i] = weights(rp[i], rq[i], x0 + (t + i) * kTile + lane * 8, w);
-      }
+      for (int i = 0; i < kStep; ++i) s[i] = weight_sum(rp[i], rq[i], x0 + (t + i) * kTile + lane * 8);
       const double v = warp_sums<kStep>(s);
       const int i = lane / (32 / kStep);
       if (lane % (32 / kStep) == 0 && t + i < end) s_tile[t + i] = v;

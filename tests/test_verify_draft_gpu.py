@@ -145,3 +145,22 @@ def test_tokens_over_the_drafts_are_refused():
     tokens, _ = ops.verify_draft(p, both[:5], q, indptr, ua, us, both[5:], acc)
     want, want_a = R.verify(p, d, q, indptr, ua, us)
     assert tokens.tolist() == want and acc.tolist() == want_a
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -20, 2.0 ** -3, 0.3, 1.0, 40.0, 60000.0])
+@pytest.mark.parametrize("drafts", ["none", "certain", "given"])
+def test_fp16_weights_of_any_size(scale, drafts):
+    """Unnormalised fp16 weights, from subnormals to its largest values, whose
+    sums of eight lie below, around and above 1.  Both sides sum them exactly
+    (multiples of 2^-24 below 2^29), so the tokens are the same."""
+    V, n = 5003, 4
+    g = torch.Generator(device=DEV).manual_seed(31)
+    p, q = ((torch.rand(n * 12, V, device=DEV, generator=g) * scale).half() for _ in range(2))
+    p[:, ::97] = 2.0 ** -24
+    p[5, 4000:4008] = 1.0
+    d = torch.randint(0, V, (n * 12,), device=DEV, generator=g)
+    new = [1] * 48 if drafts == "none" else [n] * 12
+    indptr = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+    ua = torch.full((n * 12,), 0.9, device=DEV)
+    us = torch.rand(len(new), device=DEV, generator=g)
+    _same(p, d, q if drafts == "given" else None, indptr, ua, us)
