@@ -224,8 +224,13 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const __grid_
   int mode = rejected ? 1 : 0;
   while (true) {
     q = mode == 1 ? a.draft : nullptr;
-    // a draft that was certain of its token: it is the only one with q > 0
-    skip = mode == 1 && a.draft == nullptr ? static_cast<int>(a.draft_tokens[row]) : -1;
+    // a draft that was certain of its token: it is the only one with q > 0 (one
+    // outside the vocabulary is no token of the row, whatever its low 32 bits)
+    skip = -1;
+    if (mode == 1 && a.draft == nullptr) {
+      const int64_t d = a.draft_tokens[row];
+      if (d >= 0 && d < a.V) skip = static_cast<int>(d);
+    }
     double sum = 0.0;
     const int end = tiles * (warp + 1) / kWarps;
     for (int t = tiles * warp / kWarps; t < end; t += kStep) {

@@ -1,0 +1,29 @@
+"""verify_draft where its 32-bit indices, its random numbers and its division of
+a sequence among CTAs reach their ends, against the definition on the host."""
+
+import pytest
+import torch
+
+import paged_ref as R
+from persona import ops
+from test_verify_draft_gpu import DEV, _case, _run, _same
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("token", [(1 << 32) + 5, -(1 << 32) + 5, (1 << 31) + 5, -1, 50])
+def test_a_drafted_token_outside_the_vocabulary_takes_no_weight_from_another(token):
+    """Such a token is rejected and was nobody's: every token of the row keeps
+    its weight, also the one that the low 32 bits name (5, which has nearly all
+    of it in the first sequence)."""
+    p, d, _, indptr, ua, us = _case([2, 3], 50, torch.float32, 11)
+    p[0] = 0.001
+    p[0, 5] = 1
+    us[0] = 0.5
+    d[0] = d[2] = token
+    tokens, acc = _run(p, d, None, indptr, ua * 0, us)
+    with pytest.raises(RuntimeError, match="outside the vocabulary"):
+        ops.check_errors(torch.device(DEV, 0))
+    want, want_a = R.verify(p, d, None, indptr, ua * 0, us)
+    assert acc.tolist() == want_a == [0, 0] and tokens.tolist() == want
+    assert int(tokens[0]) == 5
