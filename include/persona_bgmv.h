@@ -419,7 +419,10 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
  * sum_{s <= t} w_s > u_sample[b] sum_s w_s, for w = max(p_a - q_a, 0) where a
  * draft was rejected (p_a if that has no positive weight), else w = the last
  * row of p; weights that are not positive, NaN among them, count as none; -1
- * if there is none at all.  Sums and comparisons in 64 bits.
+ * if there is none at all.  u_sample lies in [0, 1): a smaller number or NaN is
+ * taken as 0 (the first token with weight), and where no sum exceeds a larger
+ * one's share, the last token with weight is drawn.  Sums and comparisons in
+ * 64 bits.
  * tokens[row]: d_0 .. d_{a-1}, the drawn token, then -1; accepted[b] = a (0
  * for an empty sequence).  Probabilities fp16, bf16 or fp32 (prob_type), both
  * of one type, rows ld_* elements apart; they need not be normalised.  tokens

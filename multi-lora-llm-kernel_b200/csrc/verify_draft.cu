@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const __grid_
     // The number falls into the first tile whose running sum exceeds it; where
     // rounding (or a number of 1) leaves none, the last tile with weight has it.
     // (before + s_sum is the next CTA's `before` to the bit, so one CTA goes on.)
-    const double target = static_cast<double>(us) * total;
+    // A number below 0, or a NaN, counts as 0: no CTA's sums lie below 0.
+    const double target = fmax(static_cast<double>(us) * total, 0.0);
     const bool chosen = total > target ? before + s_sum[mode] > target && !(before > target) : rank == last;
     if (chosen) {
       int at = -1;  // the tile, and the sum before it

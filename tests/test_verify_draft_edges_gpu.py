@@ -27,3 +27,18 @@ def test_a_drafted_token_outside_the_vocabulary_takes_no_weight_from_another(tok
     want, want_a = R.verify(p, d, None, indptr, ua * 0, us)
     assert acc.tolist() == want_a == [0, 0] and tokens.tolist() == want
     assert int(tokens[0]) == 5
+
+
+@pytest.mark.parametrize("split", [1, 60])  # eight CTAs a sequence, and several sequences a wave
+@pytest.mark.parametrize("number", [-1e-30, -0.25, float("-inf"), float("nan"), -0.0])
+def test_a_number_below_zero_draws_as_zero_does(number, split):
+    """The first token with weight, in every sequence; nothing is left unwritten."""
+    p, d, q, indptr, ua, us = _case([2, 1, 3] * split, 3001, torch.float32, 12)
+    p[:, :7] = 0  # tokens without weight before the first one with some
+    q[:, :7] = 0
+    reject = torch.full_like(ua, 1e9)
+    for draft in (q, None):
+        want, want_a = R.verify(p, d, draft, indptr, reject, us * 0)
+        tokens, acc = _run(p, d, draft, indptr, reject, torch.full_like(us, number))
+        ops.check_errors(torch.device(DEV, 0))
+        assert acc.tolist() == want_a and tokens.tolist() == want
