@@ -141,20 +141,10 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
   }
 }
 
-// SMs of the current device, and a kernel's attributes set once per device.
-inline int sm_count() {
-  static std::atomic<int> known[64];
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  n = known[dev].load(std::memory_order_relaxed);
-  if (n > 0) return n;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  known[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
-// Allows `smem` bytes of dynamic shared memory and, where regs > 0, checks that
-// the kernel is launched with that many registers a thread.  `done`: one flag
-// per device, static at the caller.
+// A kernel's attributes, set once per device: allows `smem` bytes of dynamic
+// shared memory and, where regs > 0, checks that the kernel is launched with
+// that many registers a thread.  `done`: one flag per device, static at the
+// caller.
 template <typename K> cudaError_t prepare_kernel(std::atomic<bool> (&done)[64], K kernel, int smem, int regs) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);

@@ -1,6 +1,8 @@
 // Device helpers shared by the paged KV cache kernels.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 #include "paged_args.h"
 
@@ -75,6 +77,18 @@ constexpr float kE4m3Max = 448.f;
 // Smallest scale written: 2^-40 keeps 1 / scale and scale * 448 far inside
 // fp32 and lies below what the smallest fp16 value needs (2^-24 / 448).
 constexpr float kMinScale = 9.094947017729282e-13f;
+
+// SMs of the current device.
+inline int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  n = known[dev].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
 
 // Launches `kern`, as a programmatic dependent of the kernel before it if
 // `early`.  A kernel that takes most of an SM's shared memory is not launched

@@ -338,7 +338,7 @@ cudaError_t launch_verify_draft(const VerifyDraft& a, int type, cudaStream_t st)
   // As many CTAs per sequence as keep the batch within about four per SM (one
   // wave), and no fewer than the tile table allows.
   int split = kMaxSplit;
-  while (split > 1 && static_cast<int64_t>(a.B) * split > 4 * 148 &&
+  while (split > 1 && static_cast<int64_t>(a.B) * split > 4 * sm_count() &&
          a.V <= static_cast<int64_t>(kMaxTiles - 2) * kTile * (split / 2))
     split /= 2;
   return launch_paged(k, dim3(a.B * split), dim3(kThreads), 0, split, true, st, a);

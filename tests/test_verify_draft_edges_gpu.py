@@ -42,3 +42,35 @@ def test_a_number_below_zero_draws_as_zero_does(number, split):
         tokens, acc = _run(p, d, draft, indptr, reject, torch.full_like(us, number))
         ops.check_errors(torch.device(DEV, 0))
         assert acc.tolist() == want_a and tokens.tolist() == want
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("B", [74, 75, 100, 149, 200, 297, 400])
+def test_every_number_of_ctas_a_sequence(B, dtype):
+    """Eight CTAs to one, by the number of sequences, over several tiles a warp."""
+    p, d, q, indptr, ua, us = _case([1 + b % 3 for b in range(B)], 5003, dtype, B, pad=1)
+    _same(p, d, q, indptr, ua, us)
+    _same(p, d, None, indptr, ua * 0.05, us)
+
+
+@pytest.mark.parametrize("B,V", [(2, 2097152), (75, 1062912), (75, 1062913), (149, 531456), (149, 531457),
+                                 (297, 265728), (297, 265729)])
+def test_largest_vocabularies_of_each_division(B, V):
+    """The most tokens that fewer CTAs a sequence may share, and one more; rows
+    start off a 16-byte boundary, so that the tiles are as many as they can be.
+    fp16 weights are multiples of 2^-24: sums of them are exact on both sides."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    wide = torch.zeros(B, V + 9, dtype=torch.float16, device=DEV)
+    p = wide[:, 1:V + 1]
+    p.copy_(torch.rand(B, V, device=DEV, generator=g))
+    indptr = torch.arange(B + 1, dtype=torch.int32, device=DEV)
+    d, ua = torch.zeros(B, dtype=torch.int64, device=DEV), torch.zeros(B, device=DEV)
+    us = torch.rand(B, device=DEV, generator=g)
+    us[0], us[-1] = 0.0, 1.0  # the ends: the first and the last token with weight
+    tokens, acc = _run(p, d, None, indptr, ua, us)
+    ops.check_errors(torch.device(DEV, 0))
+    assert not acc.any()
+    for b in range(B):
+        cum = p[b].double().cumsum(0)
+        want = int(torch.searchsorted(cum, us[b].double() * cum[-1], right=True))
+        assert int(tokens[b]) == (want if want < V else int(p[b].nonzero()[-1])), b
