@@ -49,6 +49,7 @@ extern "C" {
 #define PERSONA_ERR_WORKSPACE 6   /* workspace missing or too small          */
 #define PERSONA_ERR_CUDA 7        /* CUDA runtime / launch failure           */
 #define PERSONA_ERR_NOALLOC_ROWS 8 /* T above PERSONA_NOALLOC_MAX_ROWS          */
+#define PERSONA_ERR_OVERLAP 9      /* a written buffer overlaps itself or another one */
 
 /* Device error-word bits (ORed into *dev_err by the kernels). */
 #define PERSONA_DEV_ERR_SLOT 1    /* a slot < -1 or >= S: that row was left alone */
@@ -348,6 +349,13 @@ int persona_rope_decode_attention(void* q, void* k, const void* v, void* k_cache
  * sequence for attention.  indptr must not decrease and must end within
  * `rows`; a sequence that breaks this raises PERSONA_DEV_ERR_SEGMENT in
  * attention and verification and is left out.
+ * What a call writes (and attention's workspace) may overlap neither itself
+ * nor anything else that the call is given, but for q_out, which may be q;
+ * PERSONA_ERR_OVERLAP otherwise.  Slices of one buffer that share no element
+ * are fine among the activations, among the pages and among the scales; an
+ * activation's address range must not meet that of the pages, the scales or
+ * the int32 arrays.  A write's pages and scales are not compared with each
+ * other, so that both may lie in one pool.
  *
  * k and v pages are [num_pages, Hkv, page_size, D], D 64 or 128, any page
  * size, unit inner stride, the same other strides for both (in elements,
@@ -426,7 +434,7 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
  * tokens[row]: d_0 .. d_{a-1}, the drawn token, then -1; accepted[b] = a (0
  * for an empty sequence).  Probabilities fp16, bf16 or fp32 (prob_type), both
  * of one type, rows ld_* elements apart; they need not be normalised.  tokens
- * does not overlap draft_tokens.                                            */
+ * and accepted overlap neither each other nor an input (PERSONA_ERR_OVERLAP). */
 #define PERSONA_VERIFY_MAX_VOCAB 2097152
 int persona_verify_draft(const void* target, int64_t ld_target, const void* draft, int64_t ld_draft, int prob_type,
                          const int64_t* draft_tokens, const int32_t* indptr, const float* u_accept,

@@ -217,6 +217,7 @@ const char* persona_status_string(int status) {
     case PERSONA_ERR_WORKSPACE: return "workspace missing, misaligned or too small";
     case PERSONA_ERR_CUDA: return "CUDA runtime or launch failure";
     case PERSONA_ERR_NOALLOC_ROWS: return "T above PERSONA_NOALLOC_MAX_ROWS, the fixed plan scratch of persona_bgmv_fused_noalloc";
+    case PERSONA_ERR_OVERLAP: return "a buffer that is written overlaps itself or another argument";
     default: return "unknown status";
   }
 }

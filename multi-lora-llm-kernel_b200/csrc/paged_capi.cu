@@ -3,6 +3,7 @@
 // with the device or allocates device memory.
 #include <cmath>
 
+#include "overlap.h"
 #include "paged_args.h"
 #include "persona_bgmv.h"
 
@@ -59,6 +60,38 @@ int check_rows(const persona_rows* r, PagedRows& out) {
   return PERSONA_OK;
 }
 
+// ---- what a call writes ----
+using overlap::View;
+
+View rows_view(const PagedRows& r, int64_t rows, int64_t heads, int64_t D) {
+  return View{r.p, D * 2, {rows, heads, 1}, {r.row_stride * 2, r.head_stride * 2, 0}};
+}
+View pages_view(const PagedCache& c, const void* p) {
+  const int64_t e = c.k_scale != nullptr ? 1 : 2;
+  return View{p, c.D * e, {c.num_pages, c.Hkv, c.page_size}, {c.page_stride * e, c.head_stride * e, c.pos_stride * e}};
+}
+View scales_view(const PagedCache& c, const void* p) {
+  return View{p, int64_t{4} * c.page_size, {c.num_pages, c.Hkv, 1}, {c.scale_page_stride * 4, c.scale_head_stride * 4, 0}};
+}
+template <typename T> View array_view(const T* p, int64_t n, int64_t stride = 1) {
+  return View{p, static_cast<int64_t>(sizeof(T)), {n, 1, 1}, {stride * static_cast<int64_t>(sizeof(T)), 0, 0}};
+}
+// Whether the address range of `v` meets that of the page table, indptr or lengths.
+bool meets_index(const View& v, const PagedCache& c) {
+  const View table{c.table, int64_t{4} * c.max_pages, {c.B, 1, 1}, {c.table_stride * 4, 0, 0}};
+  return overlap::ranges_meet(v, table) || overlap::ranges_meet(v, array_view(c.indptr, int64_t{c.B} + 1)) ||
+         overlap::ranges_meet(v, array_view(c.lengths, c.B));
+}
+bool meets_pages(const View& v, const PagedCache& c) {
+  if (overlap::ranges_meet(v, pages_view(c, c.k)) || overlap::ranges_meet(v, pages_view(c, c.v))) return true;
+  return c.k_scale != nullptr &&
+         (overlap::ranges_meet(v, scales_view(c, c.k_scale)) || overlap::ranges_meet(v, scales_view(c, c.v_scale)));
+}
+// Rows that a call writes: none twice, and nothing that it reads of the cache.
+bool rows_apart(const View& v, const PagedCache& c) {
+  return overlap::nested(v) && !meets_pages(v, c) && !meets_index(v, c);
+}
+
 }  // namespace
 }  // namespace persona
 
@@ -87,6 +120,21 @@ int persona_paged_rope_cache(const persona_paged_cache* cache, const persona_row
   a.rows = static_cast<int>(rows);
   a.Hq = static_cast<int>(Hq);
   const int D = a.c.D;
+  // (the scales may lie inside the pool of the pages, so those two are not compared)
+  const View pk = pages_view(a.c, a.c.k), pv = pages_view(a.c, a.c.v);
+  if (!overlap::nested(pk) || overlap::share(pk, pv) || meets_index(pk, a.c) || meets_index(pv, a.c))
+    return PERSONA_ERR_OVERLAP;
+  if (a.c.k_scale != nullptr) {
+    const View sk = scales_view(a.c, a.c.k_scale), sv = scales_view(a.c, a.c.v_scale);
+    if (!overlap::nested(sk) || overlap::share(sk, sv) || meets_index(sk, a.c) || meets_index(sv, a.c))
+      return PERSONA_ERR_OVERLAP;
+  }
+  const View vq = rows_view(a.q, rows, Hq, D), vo = rows_view(a.q_out, rows, Hq, D), vk = rows_view(a.k, rows, a.c.Hkv, D),
+             vv = rows_view(a.v, rows, a.c.Hkv, D);
+  const bool in_place = a.q.p == a.q_out.p && a.q.row_stride == a.q_out.row_stride && a.q.head_stride == a.q_out.head_stride;
+  if (!rows_apart(vo, a.c) || (!in_place && overlap::share(vq, vo)) || overlap::share(vk, vo) || overlap::share(vv, vo) ||
+      meets_pages(vq, a.c) || meets_pages(vk, a.c) || meets_pages(vv, a.c))
+    return PERSONA_ERR_OVERLAP;
   // theta^(-2j / D) / (2 pi) by multiplication: 63 roundings of 2^-53
   const double ratio = std::pow(static_cast<double>(theta), -2.0 / D);
   double f = 1.0 / 6.283185307179586476925;
@@ -102,6 +150,8 @@ int persona_paged_cache_read(const persona_paged_cache* cache, const persona_row
   if (rows == 0 || cache->B == 0) return PERSONA_OK;
   PERSONA_TRY(check_rows(k, a.k));
   PERSONA_TRY(check_rows(v, a.v));
+  const View vk = rows_view(a.k, rows, a.c.Hkv, a.c.D), vv = rows_view(a.v, rows, a.c.Hkv, a.c.D);
+  if (!rows_apart(vk, a.c) || !rows_apart(vv, a.c) || overlap::share(vk, vv)) return PERSONA_ERR_OVERLAP;
   a.rows = static_cast<int>(rows);
   return status(launch_paged_read(a, dtype, dev_err, stream));
 }
@@ -128,6 +178,12 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
   PERSONA_TRY(check_rows(out, a.out));
   if (workspace == nullptr || workspace_bytes < persona_paged_attention_workspace_size(a.c.D)) return PERSONA_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return PERSONA_ERR_ALIGNMENT;
+  // a row's q is read again by the CTAs that share its positions
+  const View vq = rows_view(a.q, rows, Hq, a.c.D), vo = rows_view(a.out, rows, Hq, a.c.D);
+  const View ws = array_view(static_cast<const char*>(workspace), static_cast<int64_t>(persona_paged_attention_workspace_size(a.c.D)));
+  if (!rows_apart(vo, a.c) || overlap::share(vq, vo) || overlap::ranges_meet(ws, vo) || overlap::ranges_meet(ws, vq) ||
+      meets_pages(ws, a.c) || meets_index(ws, a.c))
+    return PERSONA_ERR_OVERLAP;
   a.rows = static_cast<int>(rows);
   a.G = static_cast<int>(Hq / cache->Hkv);
   a.window = window >= kMaxPositions ? 0 : static_cast<int>(window);  // wider than any sequence
@@ -156,6 +212,14 @@ int persona_verify_draft(const void* target, int64_t ld_target, const void* draf
   if (!aligned(target, e) || !aligned(draft, e) || !aligned(draft_tokens, 8) || !aligned(tokens, 8) || !aligned(indptr, 4) ||
       !aligned(u_accept, 4) || !aligned(u_sample, 4) || !aligned(accepted, 4))
     return PERSONA_ERR_ALIGNMENT;
+  // the CTAs of a cluster, and those of other sequences, read the inputs at any time
+  const View out = array_view(tokens, rows), kept = array_view(accepted, B);
+  const View in[] = {View{target, V * static_cast<int64_t>(e), {rows, 1, 1}, {ld_target * static_cast<int64_t>(e), 0, 0}},
+                     View{draft, draft != nullptr ? V * static_cast<int64_t>(e) : 0, {rows, 1, 1}, {ld_draft * static_cast<int64_t>(e), 0, 0}},
+                     array_view(draft_tokens, rows), array_view(indptr, B + 1), array_view(u_accept, rows), array_view(u_sample, B)};
+  if (overlap::ranges_meet(out, kept)) return PERSONA_ERR_OVERLAP;
+  for (const View& v : in)
+    if (overlap::ranges_meet(out, v) || overlap::ranges_meet(kept, v)) return PERSONA_ERR_OVERLAP;
   const VerifyDraft a{target, draft, ld_target, ld_draft, draft_tokens, indptr, u_accept, u_sample, tokens, accepted,
                       static_cast<int>(rows), static_cast<int>(B), static_cast<int>(V), dev_err};
   return status(launch_verify_draft(a, prob_type, stream));
