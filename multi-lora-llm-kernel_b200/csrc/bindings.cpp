@@ -23,6 +23,7 @@
 #include <mutex>
 #include <sstream>
 
+#include "overlap.h"
 #include "persona_bgmv.h"
 
 namespace {
@@ -763,22 +764,14 @@ persona_rows rows_of(const at::Tensor& t, const at::Tensor& like, const char* op
   return persona_rows{t.data_ptr(), t.size(0) <= 1 ? 0 : t.stride(0), t.size(1) <= 1 ? 0 : t.stride(1)};
 }
 
-// Whether two [rows, heads, D] activations of the same number of rows share an
-// element.  Exact for slices of one fused buffer (the same row stride, rows that
-// do not reach into one another); elsewhere, whether their extents meet.
+// Whether two [rows, heads, D] activations share an element: exact where they
+// step alike, as slices of one buffer do, elsewhere whether their ranges meet.
 bool rows_meet(const at::Tensor& a, const at::Tensor& b) {
-  if (a.numel() == 0 || b.numel() == 0) return false;
-  const int64_t e = a.element_size(), rows = a.size(0);
-  const auto width = [](const at::Tensor& t) { return (t.size(1) <= 1 ? 0 : (t.size(1) - 1) * t.stride(1)) + t.size(2); };
-  const auto step = [&](const at::Tensor& t) { return rows <= 1 ? 0 : t.stride(0); };
-  const int64_t wa = width(a), wb = width(b);
-  const int64_t pa = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.data_ptr())),
-                pb = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data_ptr()));
-  if (pa + ((rows - 1) * step(a) + wa) * e <= pb || pb + ((rows - 1) * step(b) + wb) * e <= pa) return false;
-  const int64_t s = step(a) * e;
-  if (step(a) != step(b) || step(a) < wa || step(b) < wb) return true;
-  const int64_t d = ((pb - pa) % s + s) % s;  // where b starts in a row of a
-  return d < wa * e || s - d < wb * e;
+  const auto view = [](const at::Tensor& t) {
+    const int64_t e = t.element_size();
+    return persona::overlap::View{t.data_ptr(), t.size(2) * e, {t.size(0), t.size(1), 1}, {t.stride(0) * e, t.stride(1) * e, 0}};
+  };
+  return persona::overlap::share(view(a), view(b));
 }
 
 bool same_rows(const at::Tensor& a, const at::Tensor& b) {

@@ -110,3 +110,25 @@ def test_pools_of_every_order():
         bt.fill()
         _write_and_read(bt, q, k, v)
         _attend(bt, q)
+
+
+def test_a_fused_buffer_of_a_head_at_a_time():
+    """q, k and v of every head side by side ([rows, heads, 3, D]): slices that
+    share nothing, whatever their ranges."""
+    bt = R.Batch([4, 3], [60, 9], 16, 8, 128, H, pad=1)
+    bt.fill()
+    qkv = bt.randn(bt.rows, 8, 4, 128)
+    q, k, v, out = qkv.unbind(2)
+    before = qkv.clone()
+    _write_and_read(bt, q, k, v)
+    assert torch.equal(qkv[:, :, 1:], before[:, :, 1:])
+    rotated = q.clone()
+    want, tol = R.attention(bt, rotated, 0.1)
+    ops.paged_attention(q, *bt.args(), out, 0.1)
+    ops.check_errors(q.device)
+    _check(out[:7], want[:7], tol[:7])
+    assert torch.equal(q, rotated) and torch.equal(qkv[:, :, 1:3], before[:, :, 1:3])
+    ops.paged_cache_read(*bt.args(), k, v)
+    assert torch.equal(q, rotated)
+    for other in (qkv.view(bt.rows, 32, 128)[:, 1:9], qkv.view(bt.rows, 32, 128)[:, :32:4]):
+        _refused(ops.paged_attention, q, *bt.args(), other, 0.1)
