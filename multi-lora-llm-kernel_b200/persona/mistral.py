@@ -116,6 +116,13 @@ class PagedState:
         del self.pages[b][keep:]
         self.lengths[b] = length
 
+    def _back_to(self, lengths: Sequence[int], held: Sequence[int]) -> None:
+        """The state of before a ``_grow``: lengths, and pages held by each sequence."""
+        for b in reversed(range(len(held))):  # (in the order that takes them out alike again)
+            self.free.extend(reversed(self.pages[b][held[b]:]))
+            del self.pages[b][held[b]:]
+        self.lengths[:] = lengths
+
     def _grow(self, new: Sequence[int]) -> None:
         """Pages for ``new`` more tokens per sequence; lengths are moved on."""
         want = [-(-(n + add) // self.page_size) for n, add in zip(self.lengths, new)]
@@ -282,16 +289,25 @@ class MistralLoRAModel:
         """Feed every sequence its chunk of token ids (any length, also none).
         Returns the logits behind every fed token, [rows, V], and ``indptr``
         [B + 1] int32: sequence b's rows are indptr[b] .. indptr[b + 1] (what
-        ``sampling.verify_drafts`` takes for chunks of a last token and drafts)."""
-        cfg, d = self.cfg, self.device
+        ``sampling.verify_drafts`` takes for chunks of a last token and drafts).
+        A call that raises leaves the sequences as they were."""
         new = [len(c) for c in chunks]
         if len(new) != len(st.lengths):
             raise ValueError("one chunk per sequence")
         flat_ids = [t for c in chunks for t in c]
         # (the -1 behind a verified sequence's drawn token is not one to feed)
-        if flat_ids and not 0 <= min(flat_ids) <= max(flat_ids) < cfg.vocab:
+        if flat_ids and not 0 <= min(flat_ids) <= max(flat_ids) < self.cfg.vocab:
             raise ValueError("token id outside the vocabulary")
-        st._grow(new)
+        lengths, held = list(st.lengths), [len(p) for p in st.pages]
+        try:
+            st._grow(new)
+            return self._extend_rows(st, new, flat_ids)
+        except BaseException:
+            st._back_to(lengths, held)
+            raise
+
+    def _extend_rows(self, st: PagedState, new: List[int], flat_ids: List[int]) -> tuple:
+        cfg, d = self.cfg, self.device
         R = sum(new)
         starts = [0]
         for n in new:
