@@ -28,7 +28,9 @@ int check_cache(const persona_paged_cache* c, int dtype, PagedCache& out) {
   if (dtype != PERSONA_DTYPE_F16 && dtype != PERSONA_DTYPE_BF16) return PERSONA_ERR_DTYPE;
   const bool e4m3 = c->kind == PERSONA_PAGES_E4M3;
   if (!e4m3 && c->kind != PERSONA_PAGES_16BIT) return PERSONA_ERR_DTYPE;
-  if (c->k == nullptr || c->v == nullptr || c->page_table == nullptr || c->indptr == nullptr || c->lengths == nullptr)
+  // (arrays without an element may be null: no sequences, or a table without columns)
+  if (c->k == nullptr || c->v == nullptr || (c->B != 0 && (c->indptr == nullptr || c->lengths == nullptr)) ||
+      (c->B != 0 && c->max_pages != 0 && c->page_table == nullptr))
     return PERSONA_ERR_INVALID_ARG;
   if (e4m3 != (c->k_scale != nullptr) || e4m3 != (c->v_scale != nullptr)) return PERSONA_ERR_INVALID_ARG;
   if ((c->D != 64 && c->D != 128) || c->Hkv <= 0 || c->Hkv > kMaxHeads || c->num_pages <= 0 || c->num_pages > kI32Max ||
