@@ -13,6 +13,7 @@ namespace {
 constexpr int64_t kI32Max = 2147483647;
 constexpr int64_t kMaxHeads = 1024;
 constexpr int64_t kMaxPositions = int64_t{1} << 30;
+constexpr float kLog2E = 1.4426950408889634f;
 // Most query rows per kv head (new tokens times heads of a group) for the
 // warp-level kernel, which reads the pages once per 32 rows.  Measured with 32
 // sequences of up to 6000 tokens: over 16-bit pages 36 rows take it 118 us and
@@ -170,7 +171,7 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
   PagedAttention a;
   PERSONA_TRY(check_cache(cache, dtype, a.c));
   if (rows < 0 || Hq <= 0 || Hq > kMaxHeads || Hq % cache->Hkv || rows > kI32Max / Hq || window < 0 || max_new < 1 ||
-      !(scale > 0.f) || !std::isfinite(scale))
+      !(scale > 0.f) || !std::isfinite(scale * kLog2E))
     return PERSONA_ERR_SHAPE;
   // positions of a sequence, and what the kernels add to and take from them
   // (blocks ahead, a window), are 32-bit numbers
@@ -189,7 +190,7 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
   a.rows = static_cast<int>(rows);
   a.G = static_cast<int>(Hq / cache->Hkv);
   a.window = window >= kMaxPositions ? 0 : static_cast<int>(window);  // wider than any sequence
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2E;
   a.err = dev_err;
   a.split = a.tile_step = 1;
   const int most = static_cast<int>(max_new > rows ? rows : max_new);
