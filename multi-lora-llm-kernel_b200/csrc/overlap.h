@@ -11,28 +11,22 @@ namespace overlap {
 
 using wide = __int128;
 
-// A strided view: up to three dimensions over a run of `inner` bytes.
+// A strided view: up to three dimensions over a run of `inner` bytes, and the
+// addresses from its first byte to behind its last one (0, 0: no element).
 struct View {
-  const void* p;
-  int64_t inner;
-  int64_t size[3], stride[3];
+  uint64_t lo, hi;
+  int64_t inner, size[3], stride[3];
+  View(const void* p, int64_t run, const int64_t (&n)[3], const int64_t (&step)[3])
+      : lo(reinterpret_cast<uintptr_t>(p)), inner(run), size{n[0], n[1], n[2]}, stride{step[0], step[1], step[2]} {
+    wide end = static_cast<wide>(lo) + inner;
+    for (int i = 0; i < 3; ++i) end += static_cast<wide>(size[i] - 1) * stride[i];
+    hi = end > static_cast<wide>(UINT64_MAX) ? UINT64_MAX : static_cast<uint64_t>(end);
+    if (inner <= 0 || size[0] <= 0 || size[1] <= 0 || size[2] <= 0) lo = hi = 0;
+  }
 };
 
-inline wide at(const void* p) { return static_cast<wide>(reinterpret_cast<uintptr_t>(p)); }
-
-inline bool empty(const View& v) { return v.inner <= 0 || v.size[0] <= 0 || v.size[1] <= 0 || v.size[2] <= 0; }
-
-// Bytes from the first element to the last one's end.
-inline wide extent(const View& v) {
-  wide e = v.inner;
-  for (int i = 0; i < 3; ++i) e += static_cast<wide>(v.size[i] - 1) * v.stride[i];
-  return e;
-}
-
 // Whether the address ranges meet (also where the elements do not).
-inline bool ranges_meet(const View& a, const View& b) {
-  return !empty(a) && !empty(b) && at(a.p) < at(b.p) + extent(b) && at(b.p) < at(a.p) + extent(a);
-}
+inline bool ranges_meet(const View& a, const View& b) { return a.lo < b.hi && b.lo < a.hi; }
 
 // The dimensions along which a or b takes a step, largest stride first, with
 // each one's size.  False where both take steps of different length in one.
@@ -91,7 +85,7 @@ inline bool share(const View& a, const View& b) {
       if (k < dims.a[i] && -k < dims.b[i] && self(self, d - k * dims.stride[i], i + 1)) return true;
     return false;
   };
-  return reach(reach, at(b.p) - at(a.p), 0);
+  return reach(reach, static_cast<wide>(b.lo) - static_cast<wide>(a.lo), 0);
 }
 
 }  // namespace overlap

@@ -69,31 +69,44 @@ using overlap::View;
 View rows_view(const PagedRows& r, int64_t rows, int64_t heads, int64_t D) {
   return View{r.p, D * 2, {rows, heads, 1}, {r.row_stride * 2, r.head_stride * 2, 0}};
 }
-View pages_view(const PagedCache& c, const void* p) {
-  const int64_t e = c.k_scale != nullptr ? 1 : 2;
-  return View{p, c.D * e, {c.num_pages, c.Hkv, c.page_size}, {c.page_stride * e, c.head_stride * e, c.pos_stride * e}};
+template <typename T> View array_view(const T* p, int64_t n) {
+  return View{p, static_cast<int64_t>(sizeof(T)) * n, {1, 1, 1}, {0, 0, 0}};
 }
-View scales_view(const PagedCache& c, const void* p) {
-  return View{p, int64_t{4} * c.page_size, {c.num_pages, c.Hkv, 1}, {c.scale_page_stride * 4, c.scale_head_stride * 4, 0}};
-}
-template <typename T> View array_view(const T* p, int64_t n, int64_t stride = 1) {
-  return View{p, static_cast<int64_t>(sizeof(T)), {n, 1, 1}, {stride * static_cast<int64_t>(sizeof(T)), 0, 0}};
-}
-// Whether the address range of `v` meets that of the page table, indptr or lengths.
-bool meets_index(const View& v, const PagedCache& c) {
-  const View table{c.table, int64_t{4} * c.max_pages, {c.B, 1, 1}, {c.table_stride * 4, 0, 0}};
-  return overlap::ranges_meet(v, table) || overlap::ranges_meet(v, array_view(c.indptr, int64_t{c.B} + 1)) ||
-         overlap::ranges_meet(v, array_view(c.lengths, c.B));
-}
-bool meets_pages(const View& v, const PagedCache& c) {
-  if (overlap::ranges_meet(v, pages_view(c, c.k)) || overlap::ranges_meet(v, pages_view(c, c.v))) return true;
-  return c.k_scale != nullptr &&
-         (overlap::ranges_meet(v, scales_view(c, c.k_scale)) || overlap::ranges_meet(v, scales_view(c, c.v_scale)));
-}
-// Rows that a call writes: none twice, and nothing that it reads of the cache.
-bool rows_apart(const View& v, const PagedCache& c) {
-  return overlap::nested(v) && !meets_pages(v, c) && !meets_index(v, c);
-}
+// The memory of a cache and of the int32 arrays that go with it.
+struct CacheViews {
+  const PagedCache& c;
+  const int64_t e;
+  const View k, v, k_scale, v_scale, table, indptr, lengths;
+  explicit CacheViews(const PagedCache& a)
+      : c(a), e(a.k_scale != nullptr ? 1 : 2), k(pages(a.k)), v(pages(a.v)), k_scale(scales(a.k_scale)),
+        v_scale(scales(a.v_scale)), table(a.table, int64_t{4} * a.max_pages, {a.B, 1, 1}, {a.table_stride * 4, 0, 0}),
+        indptr(array_view(a.indptr, int64_t{a.B} + 1)), lengths(array_view(a.lengths, a.B)) {}
+  View pages(const void* p) const {
+    return View{p, c.D * e, {c.num_pages, c.Hkv, c.page_size}, {c.page_stride * e, c.head_stride * e, c.pos_stride * e}};
+  }
+  View scales(const void* p) const {
+    return View{p, p != nullptr ? int64_t{4} * c.page_size : 0, {c.num_pages, c.Hkv, 1},
+                {c.scale_page_stride * 4, c.scale_head_stride * 4, 0}};
+  }
+  // Whether the address range of x meets that of the page table, indptr or lengths,
+  bool meet_index(const View& x) const {
+    return overlap::ranges_meet(x, table) || overlap::ranges_meet(x, indptr) || overlap::ranges_meet(x, lengths);
+  }
+  // or that of the pages or scales.
+  bool meet_pages(const View& x) const {
+    return overlap::ranges_meet(x, k) || overlap::ranges_meet(x, v) || overlap::ranges_meet(x, k_scale) ||
+           overlap::ranges_meet(x, v_scale);
+  }
+  // Rows that a call writes: none twice, and nothing that it reads of the cache.
+  bool apart(const View& x) const { return overlap::nested(x) && !meet_pages(x) && !meet_index(x); }
+  // Pages and scales that a call writes.  (The scales may lie inside the pool
+  // of the pages, so those two are not compared.)
+  bool writable() const {
+    if (!overlap::nested(k) || overlap::share(k, v) || meet_index(k) || meet_index(v)) return false;
+    return c.k_scale == nullptr || (overlap::nested(k_scale) && !overlap::share(k_scale, v_scale) &&
+                                    !meet_index(k_scale) && !meet_index(v_scale));
+  }
+};
 
 }  // namespace
 }  // namespace persona
@@ -123,20 +136,12 @@ int persona_paged_rope_cache(const persona_paged_cache* cache, const persona_row
   a.rows = static_cast<int>(rows);
   a.Hq = static_cast<int>(Hq);
   const int D = a.c.D;
-  // (the scales may lie inside the pool of the pages, so those two are not compared)
-  const View pk = pages_view(a.c, a.c.k), pv = pages_view(a.c, a.c.v);
-  if (!overlap::nested(pk) || overlap::share(pk, pv) || meets_index(pk, a.c) || meets_index(pv, a.c))
-    return PERSONA_ERR_OVERLAP;
-  if (a.c.k_scale != nullptr) {
-    const View sk = scales_view(a.c, a.c.k_scale), sv = scales_view(a.c, a.c.v_scale);
-    if (!overlap::nested(sk) || overlap::share(sk, sv) || meets_index(sk, a.c) || meets_index(sv, a.c))
-      return PERSONA_ERR_OVERLAP;
-  }
+  const CacheViews m(a.c);
   const View vq = rows_view(a.q, rows, Hq, D), vo = rows_view(a.q_out, rows, Hq, D), vk = rows_view(a.k, rows, a.c.Hkv, D),
              vv = rows_view(a.v, rows, a.c.Hkv, D);
   const bool in_place = a.q.p == a.q_out.p && a.q.row_stride == a.q_out.row_stride && a.q.head_stride == a.q_out.head_stride;
-  if (!rows_apart(vo, a.c) || (!in_place && overlap::share(vq, vo)) || overlap::share(vk, vo) || overlap::share(vv, vo) ||
-      meets_pages(vq, a.c) || meets_pages(vk, a.c) || meets_pages(vv, a.c))
+  if (!m.writable() || !m.apart(vo) || (!in_place && overlap::share(vq, vo)) || overlap::share(vk, vo) ||
+      overlap::share(vv, vo) || m.meet_pages(vq) || m.meet_pages(vk) || m.meet_pages(vv))
     return PERSONA_ERR_OVERLAP;
   // theta^(-2j / D) / (2 pi) by multiplication: 63 roundings of 2^-53
   const double ratio = std::pow(static_cast<double>(theta), -2.0 / D);
@@ -154,7 +159,8 @@ int persona_paged_cache_read(const persona_paged_cache* cache, const persona_row
   PERSONA_TRY(check_rows(k, a.k));
   PERSONA_TRY(check_rows(v, a.v));
   const View vk = rows_view(a.k, rows, a.c.Hkv, a.c.D), vv = rows_view(a.v, rows, a.c.Hkv, a.c.D);
-  if (!rows_apart(vk, a.c) || !rows_apart(vv, a.c) || overlap::share(vk, vv)) return PERSONA_ERR_OVERLAP;
+  const CacheViews m(a.c);
+  if (!m.apart(vk) || !m.apart(vv) || overlap::share(vk, vv)) return PERSONA_ERR_OVERLAP;
   a.rows = static_cast<int>(rows);
   return status(launch_paged_read(a, dtype, dev_err, stream));
 }
@@ -184,8 +190,9 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
   // a row's q is read again by the CTAs that share its positions
   const View vq = rows_view(a.q, rows, Hq, a.c.D), vo = rows_view(a.out, rows, Hq, a.c.D);
   const View ws = array_view(static_cast<const char*>(workspace), static_cast<int64_t>(persona_paged_attention_workspace_size(a.c.D)));
-  if (!rows_apart(vo, a.c) || overlap::share(vq, vo) || overlap::ranges_meet(ws, vo) || overlap::ranges_meet(ws, vq) ||
-      meets_pages(ws, a.c) || meets_index(ws, a.c))
+  const CacheViews m(a.c);
+  if (!m.apart(vo) || overlap::share(vq, vo) || overlap::ranges_meet(ws, vo) || overlap::ranges_meet(ws, vq) ||
+      m.meet_pages(ws) || m.meet_index(ws))
     return PERSONA_ERR_OVERLAP;
   a.rows = static_cast<int>(rows);
   a.G = static_cast<int>(Hq / cache->Hkv);
