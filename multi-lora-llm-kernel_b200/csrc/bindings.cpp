@@ -14,7 +14,9 @@
 // op first reads that word (no sync) and raises RuntimeError if an earlier
 // call flagged it, and PERSONA_STRICT_SLOTS=1 makes each op synchronise and
 // raise on its own call instead.
+#include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 #include <torch/library.h>
@@ -1063,14 +1065,32 @@ void sgmv_fused_tp_op(const at::Tensor& x, const at::Tensor& a_pool, const at::T
 }
 }  // namespace
 
+namespace {
+// Whether a dispatch or function mode, or the subclass of a tensor, has to see
+// a call (a fake tensor among them, which has no memory to hand to a kernel).
+bool watched(const at::Tensor& t) { return t.key_set().has(c10::DispatchKey::Python); }
+bool watched(const c10::optional<at::Tensor>& t) { return t.has_value() && watched(*t); }
+template <typename T> bool watched(const T&) { return false; }
+template <typename... A> void def_direct(pybind11::module& m, const char* name, void (*op)(A...)) {
+  m.def(name, [name, op](A... a) {
+    if (C10_UNLIKELY(c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled() ||
+                     (watched(a) || ...))) {
+      pybind11::module_::import("torch").attr("ops").attr("persona").attr(name)(a...);
+      return;
+    }
+    op(a...);
+  });
+}
+}  // namespace
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // The paged-cache ops for persona.ops, past the dispatcher: half of a small
   // call's time on the host is spent there.  The same functions are registered
   // as torch.ops.persona.*.
-  m.def("paged_rope_cache", &paged_rope_cache_op);
-  m.def("paged_cache_read", &paged_cache_read_op);
-  m.def("paged_attention", &paged_attention_op);
-  m.def("verify_draft", &verify_draft_op);
+  def_direct(m, "paged_rope_cache", &paged_rope_cache_op);
+  def_direct(m, "paged_cache_read", &paged_cache_read_op);
+  def_direct(m, "paged_attention", &paged_attention_op);
+  def_direct(m, "verify_draft", &verify_draft_op);
   m.def("sgmv_fused_tp", &sgmv_fused_tp_op,
         "Tensor-parallel segmented fused LoRA: columns [n0, n1) of y, every finished tile also stored into the "
         "peers' y (pointers from ipc_import).");

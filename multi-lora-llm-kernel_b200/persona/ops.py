@@ -242,12 +242,14 @@ def bgmv_lora_delta_multi(xs, a_pools, b_pools, slots: torch.Tensor, deltas):
 
 # ---- paged KV cache and drafted tokens ---------------------------------------
 # These calls are short enough for the host's time to count: they go straight
-# to the extension's functions (the same as torch.ops.persona.*), which check
-# every tensor themselves.
+# to the extension's functions, which check every tensor themselves (and pass
+# the call on to torch.ops.persona.* where a mode or a tensor subclass has to
+# see it).  A compiler traces the operators.
 def _paged(op: str, first: torch.Tensor):
     if not first.is_cuda:
         _require_cuda(op, first)
-    return _load()
+    ext = _load()
+    return torch.ops.persona if torch.compiler.is_dynamo_compiling() else ext
 
 
 def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
