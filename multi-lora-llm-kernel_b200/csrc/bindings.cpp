@@ -1071,6 +1071,11 @@ namespace {
 bool watched(const at::Tensor& t) { return t.key_set().has(c10::DispatchKey::Python); }
 bool watched(const c10::optional<at::Tensor>& t) { return t.has_value() && watched(*t); }
 template <typename T> bool watched(const T&) { return false; }
+// Gives Python's lock up for its lifetime.
+struct Unlocked {
+  PyThreadState* const thread = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(thread); }
+};
 template <typename... A> void def_direct(pybind11::module& m, const char* name, void (*op)(A...)) {
   m.def(name, [name, op](A... a) {
     if (C10_UNLIKELY(c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled() ||
@@ -1078,6 +1083,7 @@ template <typename... A> void def_direct(pybind11::module& m, const char* name, 
       pybind11::module_::import("torch").attr("ops").attr("persona").attr(name)(a...);
       return;
     }
+    const Unlocked others;  // as torch.ops does: the call may wait for its stream, or for room in it
     op(a...);
   });
 }
