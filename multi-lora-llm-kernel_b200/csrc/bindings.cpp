@@ -847,16 +847,18 @@ void paged_rope_cache_op(const at::Tensor& q, const at::Tensor& k, const at::Ten
   TORCH_CHECK(k.size(1) == c.Hkv && v.size(1) == c.Hkv && q_out.size(1) == q.size(1), op, ": head count mismatch");
   TORCH_CHECK((c.num_pages <= 1 || c.page_stride >= c.D) && (c.Hkv <= 1 || c.head_stride >= c.D), op,
               ": caches are written and must not overlap themselves");
-  TORCH_CHECK(same_rows(q, q_out) || !rows_meet(q, q_out), op, ": q_out must be q or not overlap it");
-  TORCH_CHECK(!rows_meet(k, q_out) && !rows_meet(v, q_out), op, ": q_out must not overlap k or v");
   const at::cuda::OptionalCUDAGuard guard(q.device());
   const int dev = q.get_device();
   raise_pending(dev, op);
   if (q.size(0) == 0) return;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  check_status(persona_paged_rope_cache(&c, &qr, &qo, &kr, &vr, q.size(0), q.size(1), static_cast<float>(theta), dt,
-                                        error_word_device(dev), stream),
-               op);
+  const int st = persona_paged_rope_cache(&c, &qr, &qo, &kr, &vr, q.size(0), q.size(1), static_cast<float>(theta), dt,
+                                          error_word_device(dev), stream);
+  if (st == PERSONA_ERR_OVERLAP) {  // which
+    TORCH_CHECK(same_rows(q, q_out) || !rows_meet(q, q_out), op, ": q_out must be q or not overlap it");
+    TORCH_CHECK(!rows_meet(k, q_out) && !rows_meet(v, q_out), op, ": q_out must not overlap k or v");
+  }
+  check_status(st, op);
   after_launch(dev, op, stream);
 }
 
@@ -868,13 +870,14 @@ void paged_cache_read_op(const at::Tensor& k_cache, const at::Tensor& v_cache, c
   const int dt = dtype_code(k_out, op);
   const persona_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale, page_table, indptr, lengths, k_out, op);
   TORCH_CHECK(k_out.size(1) == c.Hkv && v_out.size(1) == c.Hkv, op, ": head count mismatch");
-  TORCH_CHECK(!rows_meet(k_out, v_out), op, ": k_out and v_out must not overlap");
   const at::cuda::OptionalCUDAGuard guard(k_out.device());
   const int dev = k_out.get_device();
   raise_pending(dev, op);
   if (k_out.size(0) == 0) return;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  check_status(persona_paged_cache_read(&c, &kr, &vr, k_out.size(0), dt, error_word_device(dev), stream), op);
+  const int st = persona_paged_cache_read(&c, &kr, &vr, k_out.size(0), dt, error_word_device(dev), stream);
+  TORCH_CHECK(st != PERSONA_ERR_OVERLAP || !rows_meet(k_out, v_out), op, ": k_out and v_out must not overlap");
+  check_status(st, op);
   after_launch(dev, op, stream);
 }
 
@@ -888,8 +891,6 @@ void paged_attention_op(const at::Tensor& q, const at::Tensor& k_cache, const at
   const persona_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale, page_table, indptr, lengths, q, op);
   TORCH_CHECK(out.size(1) == q.size(1) && c.Hkv > 0 && q.size(1) % c.Hkv == 0, op,
               ": the heads of q and out must be a multiple of the kv heads");
-  // a row's q is read again by the CTAs that share its positions
-  TORCH_CHECK(!rows_meet(q, out), op, ": out must not overlap q");
   TORCH_CHECK(window >= 0, op, ": window must not be negative (0: none)");
   TORCH_CHECK(max_new >= 1, op, ": max_new must be positive");
   const at::cuda::OptionalCUDAGuard guard(q.device());
@@ -900,9 +901,10 @@ void paged_attention_op(const at::Tensor& q, const at::Tensor& k_cache, const at
   // a buffer of this call's own (from the graph's pool under capture)
   at::Tensor ws = at::empty({static_cast<int64_t>(persona_paged_attention_workspace_size(c.D))},
                             q.options().dtype(at::kByte));
-  check_status(persona_paged_attention(&c, &qr, &orow, q.size(0), q.size(1), static_cast<float>(scale), window, max_new,
-                                       dt, ws.data_ptr(), ws.numel(), error_word_device(dev), stream),
-               op);
+  const int st = persona_paged_attention(&c, &qr, &orow, q.size(0), q.size(1), static_cast<float>(scale), window, max_new,
+                                         dt, ws.data_ptr(), ws.numel(), error_word_device(dev), stream);
+  TORCH_CHECK(st != PERSONA_ERR_OVERLAP || !rows_meet(q, out), op, ": out must not overlap q");
+  check_status(st, op);
   after_launch(dev, op, stream);
 }
 

@@ -36,6 +36,8 @@ from typing import Optional
 import torch
 
 _EXT = None
+_MODULE = type(torch)
+_compiling = torch.compiler.is_dynamo_compiling
 
 
 def _load():
@@ -248,8 +250,8 @@ def bgmv_lora_delta_multi(xs, a_pools, b_pools, slots: torch.Tensor, deltas):
 def _paged(op: str, first: torch.Tensor):
     if not first.is_cuda:
         _require_cuda(op, first)
-    ext = _load()
-    return torch.ops.persona if torch.compiler.is_dynamo_compiling() else ext
+    ext = _load() if type(_EXT) is not _MODULE else _EXT
+    return torch.ops.persona if _compiling() else ext
 
 
 def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
