@@ -64,7 +64,6 @@ __device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t saddr, uint32_t lbo
   d &= ~(static_cast<uint64_t>(0x3FFFu) << 16);
   return d | static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFFu) << 16;
 }
-constexpr uint32_t kIdescAMnMajor = 1u << 15;  // A transposed: M is the fast dimension
 constexpr uint32_t kIdescBMnMajor = 1u << 16;  // B transposed: N is the fast dimension
 
 // kind::f16 instruction descriptor: fp32 accumulate, A/B both f16 (fmt 0) or
@@ -97,15 +96,6 @@ __device__ __forceinline__ void mma_f16_lo(uint32_t d_tmem, uint32_t a_lo, uint3
       "add.u32 y, %2, %4;\n\tmov.b64 a, {x, %3};\n\tmov.b64 b, {y, %3};\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d_tmem),
       "r"(a_lo), "r"(b_lo), "r"(hi), "r"(off), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// The same for operands whose descriptors differ in the high half.
-__device__ __forceinline__ void mma_f16_lo2(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
-                                           uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // D[tmem] (+)= A[tmem] * B[smem]; A: 16-bit pairs, lane = row, 8 columns per 16
