@@ -361,7 +361,9 @@ int persona_rope_decode_attention(void* q, void* k, const void* v, void* k_cache
  * size, unit inner stride, the same other strides for both (in elements,
  * multiples of 16 bytes).  PERSONA_PAGES_16BIT: the activations' own type.
  * PERSONA_PAGES_E4M3: 8-bit codes and one fp32 scale per page, head and
- * position (unit position stride): value = code * scale.                    */
+ * position (unit position stride): value = code * scale.  Scales are finite and
+ * not negative; attention takes a v scale below 2^-60 as 2^-60 (the write's
+ * smallest is 2^-40).                                                       */
 #define PERSONA_PAGES_16BIT 0
 #define PERSONA_PAGES_E4M3 1
 typedef struct persona_paged_cache {
@@ -391,7 +393,9 @@ typedef struct persona_rows {
  * (exact at far positions), the rotation in fp32, one rounding.  E4M3: scale =
  * max(max |x| / 448, 2^-40) over a head of D values, codes rounded from the
  * fp32 value / scale.  Values have to be finite for 8-bit pages: an infinity
- * or NaN makes that token's head NaN.                                       */
+ * makes that token's head NaN; a NaN is left out of the maximum and stays one
+ * (for k, with the value it is rotated with).  theta is an fp32 number, the
+ * angles those of that number.                                              */
 int persona_paged_rope_cache(const persona_paged_cache* cache, const persona_rows* q, const persona_rows* q_out,
                              const persona_rows* k, const persona_rows* v, int64_t rows, int64_t Hq, float theta,
                              int dtype, int32_t* dev_err, cudaStream_t stream);
@@ -409,7 +413,8 @@ int persona_paged_cache_read(const persona_paged_cache* cache, const persona_row
  * entries for the latter are not either; a NaN or infinity at a position of the sequence itself may reach
  * every new row of that sequence.  out does not overlap q.
  * max_new: an upper bound of the new tokens of one sequence, for the choice of
- * the kernel; a larger number of them is still computed correctly.
+ * the kernel; a larger number of them is still computed correctly.  scale *
+ * log2(e) has to be an fp32 number.
  * workspace: persona_paged_attention_workspace_size(D) bytes for the current
  * device, 16-byte aligned, any contents; calls that can overlap need one each. */
 size_t persona_paged_attention_workspace_size(int64_t D);

@@ -16,10 +16,14 @@
 // per tile instead, whose CTAs hold equal parts of its units and join them
 // through distributed shared memory, in one launch.
 //
-// Measured (32 heads over 8, D = 128): 64 sequences of 500 to 8192 positions,
-// bf16, 118 us, 0.91 of the measured HBM rate; 32 x 5 drafted tokens over 300 to
-// 6000 positions of 8-bit pages 70 us, 0.32 of it: there the eight warps that an
-// SM's registers hold are short of issue slots for conversions and products.
+// Measured (32 heads over 8, D = 128, a call among others): 64 sequences of 500
+// to 8192 positions, bf16, 119 us, 0.90 of the measured HBM rate; over 8-bit
+// pages 100 us, 0.55 of it.  32 x 5 drafted tokens over 300 to 6000 positions of
+// 16-bit pages 67 us, 0.64; of 8-bit ones 70 us, 0.32: no unit is full there
+// (issue slots 37 %, tensor 25 %, exponentials 10 %).  An SM's registers hold
+// eight warps, two per scheduler, too few to cover the latency of each one's
+// chain of loads, conversions, products and exponentials; and of the products'
+// 32 rows 12 are not there (20 rows; with one token 12 of 16).
 //
 // A CTA.  Four warps; warp w takes positions [16 w, 16 w + 16) of every unit
 // through a ring of its own shared memory filled with cp.async, so no warp
@@ -33,11 +37,12 @@
 // run in fp16 for either type of q (a bf16 row is first scaled by a power of
 // two into fp16's range).  The k scale multiplies the fp32 score.  The v scale
 // goes into the exponent: the running maximum is taken over x + log2(vs), so
-// that p vs is at most 1 whatever the scales' range, and the sum of p is
-// accumulated as (p vs) / vs.
+// that p vs is at most 2^kGrow whatever the scales' range, and the sum of p is
+// accumulated as (p vs) / vs.  Scales are not negative; a v scale below
+// kLeastScale counts as that.
 //
-// mma.sync, not tcgen05: a tile has 16 or 32 rows, an eighth or a quarter of
-// tcgen05's smallest M, and the tensor work per byte of pages is far below
+// mma.sync, not tcgen05: a tile has 16 or 32 rows, a quarter or half of
+// tcgen05's smallest M (64), and the tensor work per byte of pages is far below
 // what the warp-level product delivers.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -774,8 +779,8 @@ cudaError_t attention_launch(const PagedAttention& a, int max_new, cudaStream_t 
   const int sms = sm_count();
   // Where the page table cannot hold long sequences: a cluster per tile, in one
   // launch, as many CTAs as keep every cluster resident.  8 sequences of up to
-  // 255 positions take 7.1 us so, and 10.2 by ranges of the line and the join
-  // that goes with them; 4 of up to 8000 15.8 and 19.0.  A CTA takes at most 16
+  // 255 positions take 7.1 us so in a graph (8.2 as calls), and 10.2 by ranges of
+  // the line and the join that goes with them; 4 of up to 8000 15.8 and 19.0.  A CTA takes at most 16
   // units so: from 32 on longer sequences are balanced better by the line (one
   // of 16000: 32.3 and 27.5).
   const int64_t units = (static_cast<int64_t>(a.c.max_pages) * a.c.page_size + kUnit - 1) / kUnit;

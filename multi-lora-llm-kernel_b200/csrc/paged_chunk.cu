@@ -26,13 +26,16 @@
 // What bounds it: per block and both halves 2048 cycles of tensor work against
 // 3400 of the chain scores - softmax - products of each half; the exponentials
 // (128 x 128 a half, 16 per cycle and SM) are not it: an eighth of them by a
-// polynomial on the FMA units took 4 % longer.  Measured (f16, 32 heads over 8): 4096 new
-// tokens over 16384 positions 797 us in bursts, 1.21 PFLOP/s, 0.73 of the
-// measured bf16 rate; 32 prompts of 512 171 us.
+// polynomial on the FMA units took 4 % longer.  Measured (f16, 32 heads over 8,
+// D = 128, calls in a row): 4096 new tokens over 16384 positions 919 us, 1.05
+// PFLOP/s, 0.75 of the measured sustained bf16 rate (792 us in bursts, 0.73 of
+// the burst rate).  At D = 64 655 us: half the products, the same chain.  32
+// prompts of 512 with nothing cached 174 us: 35 blocks per SM are 62 us of it,
+// most of the rest is starting and ending fourteen tiles.
 //
 // 8-bit pages: codes become fp16 in shared memory, exactly; the k scale
 // multiplies the fp32 score and log2 of the v scale joins its exponent (see
-// paged_attention.cu).  The same chunk then takes 1.39 ms: the codes are
+// paged_attention.cu).  The same chunk then takes 1.41 ms: the codes are
 // converted once per tile of 256 rows, and each row reads every column's
 // scales.
 #include <cuda_bf16.h>

@@ -7,8 +7,9 @@
 // What it must read is one row of each distribution per sequence, so it is
 // bound by its chain of dependent steps (rows, tokens, their probabilities, the
 // row, the sums, the tile): 8 sequences of 4 drafts over 32000 tokens take 5.6
-// us, 256 of up to 7 over 50257 16 us in fp16 (0.49 of the measured HBM
-// rate; 17 in a graph, and 21 in bf16, whose sums take more conversions to 64 bits).
+// us, 256 of up to 7 over 50257 16 us in fp16 (0.48 of the measured HBM
+// rate; 17 in a graph), 21 us in bf16 and 23 in fp32 (0.69 of it), whose sums
+// take more conversions to 64 bits.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -268,7 +268,9 @@ def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache:
     ``lengths[b] - 1``.  Caches [pages, Hkv, page size, D]; position p of
     sequence b is in page ``page_table[b, p // page_size]``.  Caches of
     ``float8_e4m3fn`` take fp32 scales [pages, Hkv, page size]: one per token
-    and head, ``max|x| / 448``.  Rows of no sequence are left alone."""
+    and head, ``max|x| / 448``.  Rows of no sequence are left alone.  ``theta``
+    is taken as an fp32 number.  What is written must not overlap itself or
+    another argument, but for ``q_out``, which may be ``q``."""
     q_out = q if q_out is None else q_out
     _paged("paged_rope_cache", q).paged_rope_cache(q, k, v, q_out, k_cache, v_cache, page_table, indptr, lengths, theta,
                                                    k_scale, v_scale)
@@ -318,8 +320,10 @@ def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_p
     token).  Drafts are kept while ``u_accept[row] * q < p``.  Then one token
     is drawn with ``u_sample[b]``: from ``max(p - q, 0)`` where a draft was
     rejected, else from the last row.  ``tokens`` [rows] int64: the kept
-    drafts, the drawn token, then -1 (a buffer apart from ``draft_tokens``);
-    ``accepted`` [B] int32: how many."""
+    drafts, the drawn token, then -1; ``accepted`` [B] int32: how many (buffers
+    apart from each other and from the inputs).  ``u_sample`` lies in [0, 1): a
+    smaller number or NaN counts as 0, a larger one draws the last token with
+    weight."""
     _paged("verify_draft", target_probs).verify_draft(target_probs, draft_tokens, draft_probs, indptr, u_accept,
                                                       u_sample, tokens, accepted)
     return tokens, accepted

@@ -66,3 +66,19 @@ def test_codes_of_random_values(dtype, size):
     _write(bt, k, v)
     _check(bt, "k", k)
     _check(bt, "v", v)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_values_that_are_not_finite(dtype):
+    """A NaN stays one and spoils no other value but, in k, the one it is rotated
+    with; an infinity makes its head NaN; the other heads and tokens are as ever."""
+    bt = R.Batch([3], [5], 16, 2, 128, dtype, True)
+    k, v = bt.randn(3, 2, 128), bt.randn(3, 2, 128)
+    k[0, 0, 10], v[0, 0, 10], k[1, 1, 70], v[1, 1, 70] = [float("nan")] * 2 + [float("inf")] * 2
+    _write(bt, k, v)
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    ops.paged_cache_read(*bt.args(), ko, vo, **bt.scales())
+    want_k, want_v = torch.zeros_like(k, dtype=torch.bool), torch.zeros_like(v, dtype=torch.bool)
+    want_k[0, 0, [10, 74]] = want_v[0, 0, 10] = True
+    want_k[1, 1] = want_v[1, 1] = True
+    assert torch.equal(ko.isnan(), want_k) and torch.equal(vo.isnan(), want_v)
