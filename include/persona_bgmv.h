@@ -37,7 +37,7 @@ extern "C" {
 /* 16-bit storage types of x / pools / y. */
 #define PERSONA_DTYPE_F16 0
 #define PERSONA_DTYPE_BF16 1
-#define PERSONA_DTYPE_F32 2 /* probabilities of persona_verify_draft only */
+#define PERSONA_DTYPE_F32 2 /* probabilities and logits (persona_verify_draft, persona_sample_tokens) only */
 
 /* Host-side status codes. */
 #define PERSONA_OK 0
@@ -60,6 +60,7 @@ extern "C" {
                                      plan entry was out of range (that item skipped) */
 #define PERSONA_DEV_ERR_PAGE 16  /* a position behind the page table, or a page outside the cache */
 #define PERSONA_DEV_ERR_TOKEN 32 /* a drafted token outside the vocabulary (taken as rejected)    */
+#define PERSONA_DEV_ERR_FULL 64  /* a planned step outgrows the free pages or the page table (nothing was done) */
 
 /* Flags of the BGMV ops. */
 #define PERSONA_REUSE_PLAN 1 /* workspace already holds the plan of these slots */
@@ -363,13 +364,17 @@ int persona_rope_decode_attention(void* q, void* k, const void* v, void* k_cache
  * PERSONA_PAGES_E4M3: 8-bit codes and one fp32 scale per page, head and
  * position (unit position stride): value = code * scale.  Scales are finite and
  * not negative; attention takes a v scale below 2^-60 as 2^-60 (the write's
- * smallest is 2^-40).                                                       */
+ * smallest is 2^-40).
+ * PERSONA_PAGES_E4M3_BLOCK(n): the same with one scale for every 2^n positions
+ * of a page and head (n 1 to 7, 2^n divides the page): [num_pages, Hkv,
+ * page_size >> n].                                                          */
 #define PERSONA_PAGES_16BIT 0
 #define PERSONA_PAGES_E4M3 1
+#define PERSONA_PAGES_E4M3_BLOCK(n) (PERSONA_PAGES_E4M3 | (n) << 8)
 typedef struct persona_paged_cache {
   void* k;
   void* v;
-  float* k_scale; /* NULL for 16-bit pages */
+  float* k_scale; /* NULL for 16-bit pages; [num_pages, Hkv, scales of a page] */
   float* v_scale;
   int64_t page_stride, head_stride, pos_stride;
   int64_t scale_page_stride, scale_head_stride;
@@ -395,7 +400,16 @@ typedef struct persona_rows {
  * fp32 value / scale.  Values have to be finite for 8-bit pages: an infinity
  * makes that token's head NaN; a NaN is left out of the maximum and stays one
  * (for k, with the value it is rotated with).  theta is an fp32 number, the
- * angles those of that number.                                              */
+ * angles those of that number.
+ * A scale per block: the block's scale becomes the smallest power of two s >=
+ * 2^-40 with max |x| <= 448 s over its new tokens, or stays what it was if
+ * earlier tokens of the sequence are in the block and it was larger.  Where it
+ * grows their codes become those of code * old / s, which is exact but for
+ * codes that fall below the smallest normal one (2^-6).  Contents of the block
+ * behind the last token are left alone, and mean something else then.  Whole
+ * blocks belong to one sequence: two sequences that share a block must not both
+ * write it.  Of values that are not finite, infinities become NaN themselves
+ * and NaN stay; the others of the block are written with the largest scale then. */
 int persona_paged_rope_cache(const persona_paged_cache* cache, const persona_rows* q, const persona_rows* q_out,
                              const persona_rows* k, const persona_rows* v, int64_t rows, int64_t Hq, float theta,
                              int dtype, int32_t* dev_err, cudaStream_t stream);
@@ -421,6 +435,49 @@ size_t persona_paged_attention_workspace_size(int64_t D);
 int persona_paged_attention(const persona_paged_cache* cache, const persona_rows* q, const persona_rows* out,
                             int64_t rows, int64_t Hq, float scale, int64_t window, int64_t max_new, int dtype,
                             void* workspace, size_t workspace_bytes, int32_t* dev_err, cudaStream_t stream);
+
+/* ---- the plan of a step over a paged cache -------------------------------------
+ * What the paged operators need for the next step, made on the device from the
+ * sequences' lengths, so that a captured step follows them.  Sequence b keeps
+ * its first keep[b] tokens (keep NULL: all lengths[b]) and gets add[b] new
+ * ones.  Pages of what it does not keep go back to free_pages (a stack of
+ * *num_free pages in a buffer of `pool`), pages for the new tokens come from its
+ * top: back the last sequence's last page first, out the first sequence's first
+ * page first, so a step that is taken back and made again gets its old pages.
+ * Written: page_table (entries of pages taken; others are left), free_pages,
+ * num_free, lengths[b] = keep[b] + add[b], indptr [B + 1] (running sums of add),
+ * places [rows]: page * page_size + place in the page of every new row, -1
+ * behind the last; row_slots [rows] (may be NULL): seq_slots of the row's
+ * sequence (an adapter slot, say), -1 behind the last.
+ * A step that cannot be made changes nothing but indptr (all 0), places and
+ * row_slots (all -1), and raises PERSONA_DEV_ERR_FULL (free pages or a page
+ * table's columns do not suffice), _SEGMENT (keep outside [0, lengths], add
+ * negative, more new tokens than rows) or _PAGE (lengths or the list's count do
+ * not fit the table or the pool).  At most PERSONA_PLAN_MAX_SEQS sequences.
+ * Nothing that is written overlaps another argument (PERSONA_ERR_OVERLAP).   */
+#define PERSONA_PLAN_MAX_SEQS 8192
+int persona_paged_plan(const int32_t* add, const int32_t* keep, int32_t* lengths, int64_t B, int32_t* page_table,
+                       int64_t table_stride, int64_t max_pages, int32_t* free_pages, int64_t pool, int32_t* num_free,
+                       int64_t page_size, int32_t* indptr, int64_t* places, const int32_t* seq_slots, int32_t* row_slots,
+                       int64_t rows, int32_t* dev_err, cudaStream_t stream);
+
+/* ---- sampling from given random numbers -----------------------------------------
+ * tokens[b] from logits row b (fp16, bf16 or fp32, rows ld elements apart):
+ * w_i = exp((x_i - max x) / temperature[b]); in the order of larger x first and
+ * equal ones by their index, top_k[b] > 0 keeps the first top_k[b] tokens, top_p[b]
+ * < 1 of those the ones before which the weights sum to at most top_p[b] of the
+ * weights that top-k keeps (the first one always), min_p[b] > 0 those with w_i >= min(min_p[b], 1);
+ * the token is the first i, by index, whose running sum of kept weights exceeds
+ * u[b] times their sum.  temperature NULL: 1; a temperature that is not positive
+ * (or NaN): the largest logit of lowest index.  top_k, top_p, min_p NULL or
+ * outside of what is said above (NaN too): that condition is off.
+ * u in [0, 1): a smaller number or NaN counts as 0, a larger one draws the last
+ * kept token with weight.  A logit of -infinity or NaN is never drawn; -1 where there is
+ * nothing else; where a logit is +infinity, those that are share the weight.
+ * Weights, sums and comparisons in 64 bits.  tokens overlaps no input.       */
+int persona_sample_tokens(const void* logits, int64_t ld, int logits_type, const float* u, const float* temperature,
+                          const int32_t* top_k, const float* top_p, const float* min_p, int64_t* tokens, int64_t B, int64_t V,
+                          cudaStream_t stream);
 
 /* ---- verification of drafted tokens -------------------------------------------
  * Speculative sampling from given random numbers.  Row indptr[b] + i of target

@@ -35,7 +35,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 CU_SOURCES = ["capi.cu", "bgmv_plan.cu", "bgmv_split.cu", "sgmv_tcgen05.cu", "simple_kernels.cu",
               "noalloc.cu", "nf4.cu", "decode_ops.cu", "bgmv_small.cu", "paged_capi.cu",
-              "paged_cache.cu", "paged_attention.cu", "paged_chunk.cu", "verify_draft.cu"]
+              "paged_cache.cu", "paged_attention.cu", "paged_chunk.cu", "verify_draft.cu",
+              "paged_plan.cu", "sample_tokens.cu"]
 LIB = OUT / "libpersona_bgmv.so"
 EXT = OUT / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 

@@ -76,6 +76,7 @@ std::string describe_error(int bits) {
   if (bits & PERSONA_DEV_ERR_PLAN) os << " reused plan does not match the call;";
   if (bits & PERSONA_DEV_ERR_PAGE) os << " page or position outside the paged cache;";
   if (bits & PERSONA_DEV_ERR_TOKEN) os << " drafted token outside the vocabulary;";
+  if (bits & PERSONA_DEV_ERR_FULL) os << " no room for a planned step in the free pages or the page table;";
   return os.str();
 }
 
@@ -810,12 +811,19 @@ persona_paged_cache cache_of(const at::Tensor& k_cache, const at::Tensor& v_cach
   c.pos_stride = c.page_size <= 1 ? c.D : k_cache.stride(2);
   c.kind = e4m3 ? PERSONA_PAGES_E4M3 : PERSONA_PAGES_16BIT;
   if (e4m3) {
+    const int64_t n = k_scale->dim() == 3 ? k_scale->size(2) : 0;  // scales of a page
     for (const at::Tensor* t : {&*k_scale, &*v_scale}) {
       TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat && t->dim() == 3 && t->size(0) == c.num_pages &&
-                      t->size(1) == c.Hkv && t->size(2) == c.page_size && (c.page_size <= 1 || t->stride(2) == 1) &&
+                      t->size(1) == c.Hkv && t->size(2) == n && (n <= 1 || t->stride(2) == 1) &&
                       t->strides() == k_scale->strides() && t->get_device() == like.get_device(),
-                  op, ": scales must be float32 [pages, kv heads, page size] with unit inner stride, strides alike");
+                  op, ": scales must be float32 [pages, kv heads, page size or blocks of a page] with unit inner stride, "
+                      "strides alike");
     }
+    int shift = 0;
+    while (shift < 7 && (n << shift) < c.page_size) ++shift;
+    TORCH_CHECK(n << shift == c.page_size, op,
+                ": a page has a scale per position, or per block of 2, 4, ... 128 of them");
+    c.kind = PERSONA_PAGES_E4M3_BLOCK(shift);
     c.k_scale = k_scale->data_ptr<float>();
     c.v_scale = v_scale->data_ptr<float>();
     c.scale_page_stride = c.num_pages <= 1 ? 0 : k_scale->stride(0);
@@ -908,6 +916,86 @@ void paged_attention_op(const at::Tensor& q, const at::Tensor& k_cache, const at
   after_launch(dev, op, stream);
 }
 
+void paged_plan_op(const at::Tensor& add, at::Tensor& lengths, at::Tensor& page_table, at::Tensor& free_pages,
+                   at::Tensor& num_free, int64_t page_size, at::Tensor& indptr, at::Tensor& places,
+                   const c10::optional<at::Tensor>& keep, const c10::optional<at::Tensor>& seq_slots,
+                   const c10::optional<at::Tensor>& row_slots) {
+  const char* op = "paged_plan";
+  const int64_t B = lengths.dim() == 1 ? lengths.size(0) : -1;
+  auto vec = [&](const at::Tensor& t, at::ScalarType ty, int64_t n, const char* name, const char* want) {
+    TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.dim() == 1 && t.scalar_type() == ty && (n < 0 || t.size(0) == n) &&
+                    t.get_device() == add.get_device(),
+                op, ": ", name, " must be a contiguous CUDA ", want);
+  };
+  TORCH_CHECK(B >= 0, op, ": lengths must be a contiguous CUDA int32 [B] tensor");
+  TORCH_CHECK(B <= PERSONA_PLAN_MAX_SEQS, op, ": at most ", PERSONA_PLAN_MAX_SEQS, " sequences");
+  vec(add, at::kInt, B, "new", "int32 [B] tensor");
+  vec(lengths, at::kInt, B, "lengths", "int32 [B] tensor");
+  vec(free_pages, at::kInt, -1, "free_pages", "int32 vector");
+  vec(num_free, at::kInt, 1, "num_free", "int32 tensor of one element");
+  vec(indptr, at::kInt, B + 1, "indptr", "int32 [B + 1] tensor");
+  vec(places, at::kLong, -1, "places", "int64 [rows] tensor");
+  if (keep.has_value()) vec(*keep, at::kInt, B, "keep", "int32 [B] tensor");
+  TORCH_CHECK(seq_slots.has_value() == row_slots.has_value(), op, ": seq_slots and row_slots go together");
+  if (row_slots.has_value()) {
+    vec(*seq_slots, at::kInt, B, "seq_slots", "int32 [B] tensor");
+    vec(*row_slots, at::kInt, places.size(0), "row_slots", "int32 [rows] tensor");
+  }
+  check_index(page_table, 2, add, op, "page_table");
+  TORCH_CHECK(page_table.size(0) == B && (B <= 1 || page_table.stride(0) >= page_table.size(1)), op,
+              ": page_table must be [B, max pages] and not overlap itself");
+  TORCH_CHECK(page_size >= 1, op, ": page_size must be positive");
+  const at::cuda::OptionalCUDAGuard guard(add.device());
+  const int dev = add.get_device();
+  raise_pending(dev, op);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  auto ptr = [](const c10::optional<at::Tensor>& t) { return t.has_value() ? t->data_ptr<int32_t>() : nullptr; };
+  check_status(persona_paged_plan(add.data_ptr<int32_t>(), ptr(keep), lengths.data_ptr<int32_t>(), B,
+                                  page_table.data_ptr<int32_t>(), B <= 1 ? page_table.size(1) : page_table.stride(0),
+                                  page_table.size(1), free_pages.data_ptr<int32_t>(), free_pages.size(0),
+                                  num_free.data_ptr<int32_t>(), page_size, indptr.data_ptr<int32_t>(),
+                                  places.data_ptr<int64_t>(), ptr(seq_slots), ptr(row_slots), places.size(0),
+                                  error_word_device(dev), stream),
+               op);
+  after_launch(dev, op, stream);
+}
+
+void sample_tokens_op(const at::Tensor& logits, const at::Tensor& u, at::Tensor& tokens,
+                      const c10::optional<at::Tensor>& temperature, const c10::optional<at::Tensor>& top_k,
+                      const c10::optional<at::Tensor>& top_p, const c10::optional<at::Tensor>& min_p) {
+  const char* op = "sample_tokens";
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1), op,
+              ": logits must be a CUDA [B, V] matrix with unit inner stride");
+  const int64_t B = logits.size(0), V = logits.size(1);
+  const int type = logits.scalar_type() == at::kFloat ? PERSONA_DTYPE_F32 : logits.scalar_type() == at::kHalf
+                       ? PERSONA_DTYPE_F16 : PERSONA_DTYPE_BF16;
+  TORCH_CHECK(type != PERSONA_DTYPE_BF16 || logits.scalar_type() == at::kBFloat16, op,
+              ": logits must be float32, float16 or bfloat16");
+  TORCH_CHECK(V >= 1 && V <= PERSONA_VERIFY_MAX_VOCAB, op, ": vocabulary of 1 to ", PERSONA_VERIFY_MAX_VOCAB, " tokens");
+  auto vec = [&](const at::Tensor& t, at::ScalarType ty, const char* name, const char* want) {
+    TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.dim() == 1 && t.scalar_type() == ty && t.size(0) == B &&
+                    t.get_device() == logits.get_device(),
+                op, ": ", name, " must be a contiguous CUDA ", want);
+  };
+  vec(u, at::kFloat, "u", "float32 [B] tensor");
+  vec(tokens, at::kLong, "tokens", "int64 [B] tensor");
+  if (temperature.has_value()) vec(*temperature, at::kFloat, "temperature", "float32 [B] tensor");
+  if (top_k.has_value()) vec(*top_k, at::kInt, "top_k", "int32 [B] tensor");
+  if (top_p.has_value()) vec(*top_p, at::kFloat, "top_p", "float32 [B] tensor");
+  if (min_p.has_value()) vec(*min_p, at::kFloat, "min_p", "float32 [B] tensor");
+  const at::cuda::OptionalCUDAGuard guard(logits.device());
+  const int dev = logits.get_device();
+  raise_pending(dev, op);
+  if (B == 0) return;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  auto f32 = [](const c10::optional<at::Tensor>& t) { return t.has_value() ? t->data_ptr<float>() : nullptr; };
+  check_status(persona_sample_tokens(logits.data_ptr(), B <= 1 ? V : logits.stride(0), type, u.data_ptr<float>(),
+                                     f32(temperature), top_k.has_value() ? top_k->data_ptr<int32_t>() : nullptr, f32(top_p),
+                                     f32(min_p), tokens.data_ptr<int64_t>(), B, V, stream),
+               op);
+  after_launch(dev, op, stream);
+}
+
 void verify_draft_op(const at::Tensor& target, const at::Tensor& draft_tokens, const c10::optional<at::Tensor>& draft,
                      const at::Tensor& indptr, const at::Tensor& u_accept, const at::Tensor& u_sample,
                      at::Tensor& tokens, at::Tensor& accepted) {
@@ -997,6 +1085,11 @@ TORCH_LIBRARY(persona, m) {
         "Tensor(a!) out, float scale, int window, int max_new, Tensor? k_scale=None, Tensor? v_scale=None) -> ()");
   m.def("verify_draft(Tensor target_probs, Tensor draft_tokens, Tensor? draft_probs, Tensor indptr, Tensor u_accept, "
         "Tensor u_sample, Tensor(a!) tokens, Tensor(b!) accepted) -> ()");
+  m.def("paged_plan(Tensor new, Tensor(a!) lengths, Tensor(b!) page_table, Tensor(c!) free_pages, Tensor(d!) num_free, "
+        "int page_size, Tensor(e!) indptr, Tensor(f!) places, Tensor? keep=None, Tensor? seq_slots=None, "
+        "Tensor(g!)? row_slots=None) -> ()");
+  m.def("sample_tokens(Tensor logits, Tensor u, Tensor(a!) tokens, Tensor? temperature=None, Tensor? top_k=None, "
+        "Tensor? top_p=None, Tensor? min_p=None) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(persona, CUDA, m) {
@@ -1014,6 +1107,8 @@ TORCH_LIBRARY_IMPL(persona, CUDA, m) {
   m.impl("paged_cache_read", &paged_cache_read_op);
   m.impl("paged_attention", &paged_attention_op);
   m.impl("verify_draft", &verify_draft_op);
+  m.impl("paged_plan", &paged_plan_op);
+  m.impl("sample_tokens", &sample_tokens_op);
   m.impl("bgmv_shrink", &bgmv_shrink_cuda);
   m.impl("bgmv_expand", &bgmv_expand_cuda);
   m.impl("gemv_fp16", &persona::gemv_fp16_cuda);
@@ -1099,6 +1194,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   def_direct(m, "paged_cache_read", &paged_cache_read_op);
   def_direct(m, "paged_attention", &paged_attention_op);
   def_direct(m, "verify_draft", &verify_draft_op);
+  def_direct(m, "paged_plan", &paged_plan_op);
+  def_direct(m, "sample_tokens", &sample_tokens_op);
   m.def("sgmv_fused_tp", &sgmv_fused_tp_op,
         "Tensor-parallel segmented fused LoRA: columns [n0, n1) of y, every finished tile also stored into the "
         "peers' y (pointers from ipc_import).");

@@ -10,7 +10,7 @@ namespace persona {
 
 // A paged cache and the ragged batch that uses it, as the kernels read it.
 // k and v share their shape and strides (in elements); the scales (e4m3
-// only) have unit position stride.  Sequence b's new tokens are rows
+// only), one for 2^scale_shift positions, have unit position stride.  Sequence b's new tokens are rows
 // [indptr[b], indptr[b + 1]) and sit at its last positions, the last one at
 // lengths[b] - 1.
 struct PagedCache {
@@ -26,6 +26,7 @@ struct PagedCache {
   const int32_t* lengths;
   int num_pages, page_size, max_pages, Hkv, D, B;
   int page_shift;  // log2(page_size), -1 if it is no power of two
+  int scale_shift;  // 0: a scale per position, else per block of 2^scale_shift, which divides the page
 };
 
 // One [rows, heads, D] activation: unit inner stride, others in elements.
@@ -60,6 +61,8 @@ struct PagedAttention {
 };
 
 cudaError_t launch_paged_write(const PagedWrite& a, int dtype, int32_t* err, cudaStream_t st);
+// The same into e4m3 pages with a scale per block (c.scale_shift > 0).
+cudaError_t launch_paged_block_write(const PagedWrite& a, int dtype, int32_t* err, cudaStream_t st);
 cudaError_t launch_paged_read(const PagedRead& a, int dtype, int32_t* err, cudaStream_t st);
 // Bytes of part and desc for any call with this head size on the current device.
 size_t paged_attention_ws_bytes(int D);
@@ -67,6 +70,38 @@ cudaError_t launch_paged_attention(PagedAttention a, int dtype, int max_new, voi
 // The same for many rows per kv head (paged_chunk.cu).
 size_t paged_chunk_ws_bytes(int D);
 cudaError_t launch_paged_chunk(PagedAttention a, int dtype, void* workspace, cudaStream_t st);
+
+// The next step's plan (paged_plan.cu): tokens kept and added per sequence.
+struct PagedPlan {
+  const int32_t* add;
+  const int32_t* keep;  // nullptr: all
+  int32_t* lengths;
+  int32_t* table;
+  int64_t table_stride;
+  int32_t* free_pages;  // [pool], the first *num_free of them free
+  int32_t* num_free;
+  int32_t* indptr;
+  int64_t* places;
+  const int32_t* seq_slots;
+  int32_t* row_slots;  // nullptr: none
+  int B, max_pages, page_size, pool, rows;
+  int32_t* err;
+};
+cudaError_t launch_paged_plan(const PagedPlan& a, cudaStream_t st);
+
+struct SampleTokens {
+  const void* logits;  // [B, V], row stride ld
+  int64_t ld;
+  const float* u;
+  const float* temperature;  // nullptr: 1; the others nullptr: off
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t* tokens;
+  int B, V;
+};
+// type: 0 fp16, 1 bf16, 2 fp32
+cudaError_t launch_sample_tokens(const SampleTokens& a, int type, cudaStream_t st);
 
 struct VerifyDraft {
   const void* target;  // [rows, V], row stride ld_target

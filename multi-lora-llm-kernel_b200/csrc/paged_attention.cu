@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         if (kE4m3) {
           const int r = lane & 15;
           const bool live = static_cast<uint32_t>(r - skip) < static_cast<uint32_t>(rem);
-          cp_async4(dst + 2 * kHalf + lane * 4, live ? sl + (pg * a.c.scale_page_stride + at + r) : sl, live);
+          cp_async4(dst + 2 * kHalf + lane * 4, live ? sl + (pg * a.c.scale_page_stride + ((at + r) >> a.c.scale_shift)) : sl, live);
         }
       } else {
 #pragma unroll
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           const int p = p0 + (lane & 15);
           int at = 0;
           const int pg = p >= pbegin && p < pend ? page_of(p, at) : -1;
-          cp_async4(dst + 2 * kHalf + lane * 4, pg >= 0 ? sl + (pg * a.c.scale_page_stride + at) : sl, pg >= 0);
+          cp_async4(dst + 2 * kHalf + lane * 4, pg >= 0 ? sl + (pg * a.c.scale_page_stride + (at >> a.c.scale_shift)) : sl, pg >= 0);
         }
       }
     };

@@ -139,6 +139,157 @@ __global__ void __launch_bounds__(kWriteThreads, 12) paged_write_kernel(const __
   }
 }
 
+// ---- 8-bit pages with a scale per block ----
+constexpr int kBlockThreads = 128;
+
+// The smallest power of two s with amax <= 448 s (448 = 1.75 2^8), from
+// kMinScale up to 2^120.
+__device__ __forceinline__ float two_power(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = static_cast<int>(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return __uint_as_float(static_cast<uint32_t>(min(max(e, 127 - 40), 247)) << 23);
+}
+
+// The new rows that fall into one block of one sequence are a run.  Sequence
+// b has the runs [(indptr[b] >> shift) + 2 b, the same of b + 1): at least as
+// many as blocks that it touches, so no scan is needed to number them, and
+// those behind the last one have nothing to do.  This finds the sequence of a
+// run, like find_seq.
+__device__ __forceinline__ int find_run_seq(const int32_t* indptr, int B, int shift, int64_t run) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = B;
+  while (true) {
+    const int step = (n + 31) / 32;
+    const int i = lane * step;
+    const bool le = i < n && (indptr[lo + i] >> shift) + 2 * static_cast<int64_t>(lo + i) <= run;
+    const int cnt = __popc(__ballot_sync(0xffffffffu, le));
+    if (cnt == 0) return -1;
+    lo += (cnt - 1) * step;
+    n = min(step, n - (cnt - 1) * step);
+    if (step == 1) return lo;
+  }
+}
+
+// One CTA per run and slice of the heads (gridDim.y of them).  D / 16 lanes
+// take one head as in paged_write_kernel; for k and v they go over the run's
+// rows twice: once for the block's maximum, once to write the codes (the second
+// read comes out of the caches).  The scale is a power of two, so codes lose
+// nothing by it (8-bit floats), it can grow with the block, and the codes of
+// the block's earlier tokens move to the larger one exactly unless they fall
+// below the smallest normal code.  The angles of every row are made once per
+// CTA.
+template <typename T, int D>
+__global__ void __launch_bounds__(kBlockThreads) paged_block_write_kernel(const __grid_constant__ PagedWrite a, int32_t* err) {
+  constexpr int kLanes = D / 16, kGroups = kBlockThreads / kLanes;
+  extern __shared__ float2 s_turn[];  // [rows of the run][D / 2]: cosine and sine
+  pdl_wait();
+  pdl_launch();
+  const PagedCache& c = a.c;
+  const int b = find_run_seq(c.indptr, c.B, c.scale_shift, blockIdx.x);
+  if (b < 0) return;
+  const int start = c.indptr[b], end = c.indptr[b + 1];
+  const int64_t ctx = static_cast<int64_t>(c.lengths[b]) - (static_cast<int64_t>(end) - start);
+  const int64_t run = blockIdx.x - ((start >> c.scale_shift) + 2 * static_cast<int64_t>(b));
+  const int64_t p_new = ctx > 0 ? ctx : 0;  // the first new position
+  const int64_t blk0 = ((p_new >> c.scale_shift) + run) << c.scale_shift;
+  // new positions [p0, p1) of the block, rows from r0 on; rows outside of the activations are left out
+  int64_t p0 = blk0 > p_new ? blk0 : p_new, p1 = blk0 + (int64_t{1} << c.scale_shift);
+  if (p1 > c.lengths[b]) p1 = c.lengths[b];
+  const int64_t row_of = static_cast<int64_t>(start) - ctx;  // row of position p: p + row_of
+  if (p0 + row_of < 0) p0 = -row_of;
+  if (p1 + row_of > a.rows) p1 = a.rows - row_of;
+  if (p0 >= p1) return;
+  const int64_t pi = p0 / c.page_size;
+  const int pg = pi < c.max_pages ? c.table[b * c.table_stride + pi] : -1;
+  if (pg < 0 || pg >= c.num_pages) {
+    if (threadIdx.x == 0) raise_error(err, PERSONA_DEV_ERR_PAGE);
+    return;
+  }
+  const int cnt = static_cast<int>(p1 - p0), at = static_cast<int>(p0 - pi * c.page_size);
+  const int older = static_cast<int>(p0 - blk0);  // tokens of the block from before the call
+  const int64_t r0 = p0 + row_of;
+  for (int x = threadIdx.x; x < cnt * (D / 2); x += kBlockThreads) {
+    const double t = static_cast<double>(p0 + x / (D / 2)) * a.turns[x % (D / 2)];
+    float sn, cs;
+    sincospif(2.f * static_cast<float>(t - rint(t)), &sn, &cs);
+    s_turn[x] = make_float2(cs, sn);
+  }
+  __syncthreads();
+  const int i = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  auto load = [&](const PagedRows& src, int j, int h, bool turn, float (&lo)[8], float (&hi)[8]) {
+    const T* x = static_cast<const T*>(src.p) + (r0 + j) * src.row_stride + static_cast<int64_t>(h) * src.head_stride;
+    unpack8<T>(*reinterpret_cast<const uint4*>(x + 8 * i), lo);
+    unpack8<T>(*reinterpret_cast<const uint4*>(x + D / 2 + 8 * i), hi);
+    if (turn) {
+#pragma unroll
+      for (int z = 0; z < 8; ++z) {
+        const float2 w = s_turn[j * (D / 2) + 8 * i + z];
+        const float x1 = lo[z], x2 = hi[z];
+        lo[z] = fmaf(x1, w.x, -x2 * w.y);
+        hi[z] = fmaf(x2, w.x, x1 * w.y);
+      }
+    }
+  };
+  float lo[8], hi[8];
+  const int64_t page_at = static_cast<int64_t>(pg) * c.page_stride;
+  const int units = 2 * c.Hkv, slices = static_cast<int>(gridDim.y);
+  for (int u0 = blockIdx.y; u0 < units; u0 += kGroups * slices) {  // uniform trips: the lanes of a warp shuffle together
+    const int u = u0 + group * slices;
+    const bool live = u < units, is_v = u >= c.Hkv;
+    const int h = is_v ? u - c.Hkv : u;
+    const PagedRows& src = is_v ? a.v : a.k;
+    float amax = 0.f;
+    for (int j = 0; live && j < cnt; ++j) {
+      load(src, j, h, !is_v, lo, hi);
+#pragma unroll
+      for (int z = 0; z < 8; ++z) amax = fmaxf(amax, fmaxf(fabsf(lo[z]), fabsf(hi[z])));
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    float* const sc = (is_v ? c.v_scale : c.k_scale) + pg * c.scale_page_stride + (at >> c.scale_shift) +
+                      static_cast<int64_t>(live ? h : 0) * c.scale_head_stride;
+    const float old = live && older > 0 ? *sc : 0.f;
+    __syncwarp();  // every lane has the old scale
+    if (!live) continue;
+    const float scale = fmaxf(old, two_power(amax)), inv = 1.f / scale;
+    uint8_t* o = static_cast<uint8_t*>(is_v ? c.v : c.k) + page_at + at * c.pos_stride + static_cast<int64_t>(h) * c.head_stride + 8 * i;
+    if (older > 0 && scale > old) {
+      const float ratio = old / scale;
+      for (int j = -older; j < 0; ++j)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint2* w = reinterpret_cast<uint2*>(o + j * c.pos_stride + half * (D / 2));
+          const uint2 v = *w;
+          uint32_t x[4];
+          e4m3x4_to_half(v.x, x[0], x[1]);
+          e4m3x4_to_half(v.y, x[2], x[3]);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            const float2 f = Cvt<__half>::to2(x[z]);
+            lo[2 * z] = f.x * ratio;
+            lo[2 * z + 1] = f.y * ratio;
+          }
+          *w = make_uint2(to_e4m3x2(lo[0], lo[1]) | static_cast<uint32_t>(to_e4m3x2(lo[2], lo[3])) << 16,
+                          to_e4m3x2(lo[4], lo[5]) | static_cast<uint32_t>(to_e4m3x2(lo[6], lo[7])) << 16);
+        }
+    }
+    for (int j = 0; j < cnt; ++j, o += c.pos_stride) {
+      load(src, j, h, !is_v, lo, hi);
+      *reinterpret_cast<uint2*>(o) = pack8_e4m3(lo, scale, inv);
+      *reinterpret_cast<uint2*>(o + D / 2) = pack8_e4m3(hi, scale, inv);
+    }
+    if (i == 0) *sc = scale;
+  }
+  for (int x = group; x < cnt * a.Hq; x += kGroups) {
+    const int j = x / a.Hq, h = x % a.Hq;
+    if (h % slices != static_cast<int>(blockIdx.y)) continue;
+    load(a.q, j, h, true, lo, hi);
+    T* o = static_cast<T*>(a.q_out.p) + (r0 + j) * a.q_out.row_stride + static_cast<int64_t>(h) * a.q_out.head_stride;
+    *reinterpret_cast<uint4*>(o + 8 * i) = pack8<T>(lo);
+    *reinterpret_cast<uint4*>(o + D / 2 + 8 * i) = pack8<T>(hi);
+  }
+}
+
 // One warp per row: the position's k and v of every head, 16 bytes of the cache
 // a lane and step.  Codes times scale are rounded once, to the rows' 16-bit
 // type.  (Two to eight rows a warp, to share the search for the sequence, took
@@ -153,7 +304,7 @@ __global__ void __launch_bounds__(128) paged_read_kernel(const __grid_constant__
   int64_t page;
   if (!locate_row(a.c, r, err, pos, page, at)) return;
   const int64_t from = page * a.c.page_stride + at * a.c.pos_stride;
-  const int64_t sfrom = page * a.c.scale_page_stride + at;
+  const int64_t sfrom = page * a.c.scale_page_stride + (at >> a.c.scale_shift);
   constexpr int kEach = kE4m3 ? 16 : 8;  // elements of 16 bytes in the cache
   constexpr int kChunks = D / kEach;
   const int n = 2 * a.c.Hkv * kChunks;
@@ -197,6 +348,17 @@ cudaError_t write_for(const PagedWrite& a, int32_t* err, cudaStream_t st) {
   return launch_paged(k, dim3(a.rows), dim3(kWriteThreads), 0, 1, true, st, a, err);
 }
 template <typename T>
+cudaError_t block_write_for(const PagedWrite& a, int32_t* err, cudaStream_t st) {
+  auto k = a.c.D == 128 ? paged_block_write_kernel<T, 128> : paged_block_write_kernel<T, 64>;
+  const int smem = (a.c.D / 2 << a.c.scale_shift) * static_cast<int>(sizeof(float2));
+  static std::atomic<bool> done[2][64];
+  const cudaError_t e = prepare_kernel(done[a.c.D == 128], k, (64 << 7) * static_cast<int>(sizeof(float2)), 0);
+  if (e != cudaSuccess) return e;
+  const int slices = a.c.scale_shift > 4 ? 1 << (a.c.scale_shift - 4) : 1;
+  const int64_t runs = (a.rows >> a.c.scale_shift) + 2 * static_cast<int64_t>(a.c.B);
+  return launch_paged(k, dim3(static_cast<unsigned>(runs), slices), dim3(kBlockThreads), smem, 1, true, st, a, err);
+}
+template <typename T>
 cudaError_t read_for(const PagedRead& a, int32_t* err, cudaStream_t st) {
   const bool e = a.c.k_scale != nullptr;
   auto k = a.c.D == 128 ? (e ? paged_read_kernel<T, 128, true> : paged_read_kernel<T, 128, false>)
@@ -208,6 +370,9 @@ cudaError_t read_for(const PagedRead& a, int32_t* err, cudaStream_t st) {
 
 cudaError_t launch_paged_write(const PagedWrite& a, int dtype, int32_t* err, cudaStream_t st) {
   return dtype == PERSONA_DTYPE_BF16 ? write_for<__nv_bfloat16>(a, err, st) : write_for<__half>(a, err, st);
+}
+cudaError_t launch_paged_block_write(const PagedWrite& a, int dtype, int32_t* err, cudaStream_t st) {
+  return dtype == PERSONA_DTYPE_BF16 ? block_write_for<__nv_bfloat16>(a, err, st) : block_write_for<__half>(a, err, st);
 }
 cudaError_t launch_paged_read(const PagedRead& a, int dtype, int32_t* err, cudaStream_t st) {
   return dtype == PERSONA_DTYPE_BF16 ? read_for<__nv_bfloat16>(a, err, st) : read_for<__half>(a, err, st);

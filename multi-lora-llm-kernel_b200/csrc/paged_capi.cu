@@ -20,6 +20,7 @@ constexpr float kLog2E = 1.4426950408889634f;
 // the tcgen05 kernel 77 (20 rows: 66 and 77); over 8-bit pages, whose codes the
 // tcgen05 kernel has to convert for each of its tiles, 64 rows take 129 and 149.
 constexpr int64_t kFewRows16 = 32, kFewRows8 = 64;
+constexpr int kMaxScaleShift = 7;  // blocks of at most 128 positions
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 int status(cudaError_t e) { return e == cudaSuccess ? PERSONA_OK : PERSONA_ERR_CUDA; }
@@ -27,7 +28,8 @@ int status(cudaError_t e) { return e == cudaSuccess ? PERSONA_OK : PERSONA_ERR_C
 int check_cache(const persona_paged_cache* c, int dtype, PagedCache& out) {
   if (c == nullptr) return PERSONA_ERR_INVALID_ARG;
   if (dtype != PERSONA_DTYPE_F16 && dtype != PERSONA_DTYPE_BF16) return PERSONA_ERR_DTYPE;
-  const bool e4m3 = c->kind == PERSONA_PAGES_E4M3;
+  const int shift = c->kind >> 8;  // log2 of the positions that share a scale
+  const bool e4m3 = (c->kind & 255) == PERSONA_PAGES_E4M3 && shift >= 0 && shift <= kMaxScaleShift;
   if (!e4m3 && c->kind != PERSONA_PAGES_16BIT) return PERSONA_ERR_DTYPE;
   // (arrays without an element may be null: no sequences, or a table without columns)
   if (c->k == nullptr || c->v == nullptr || (c->B != 0 && (c->indptr == nullptr || c->lengths == nullptr)) ||
@@ -38,6 +40,7 @@ int check_cache(const persona_paged_cache* c, int dtype, PagedCache& out) {
       c->page_size <= 0 || c->page_size > kI32Max || c->max_pages < 0 || c->max_pages > kI32Max || c->B < 0 ||
       c->B > kI32Max / 2 || c->table_stride < c->max_pages)
     return PERSONA_ERR_SHAPE;
+  if (e4m3 && (c->page_size & ((int64_t{1} << shift) - 1)) != 0) return PERSONA_ERR_SHAPE;
   const int64_t unit = e4m3 ? 16 : 8;  // elements of 16 bytes
   if (c->page_stride < 0 || c->head_stride < 0 || c->pos_stride < c->D) return PERSONA_ERR_SHAPE;
   if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->page_stride % unit || c->head_stride % unit || c->pos_stride % unit)
@@ -49,7 +52,7 @@ int check_cache(const persona_paged_cache* c, int dtype, PagedCache& out) {
   out = PagedCache{c->k, c->v, c->k_scale, c->v_scale, c->page_stride, c->head_stride, c->pos_stride,
                    c->scale_page_stride, c->scale_head_stride, c->page_table, c->table_stride, c->indptr, c->lengths,
                    static_cast<int>(c->num_pages), static_cast<int>(c->page_size), static_cast<int>(c->max_pages),
-                   static_cast<int>(c->Hkv), static_cast<int>(c->D), static_cast<int>(c->B), -1};
+                   static_cast<int>(c->Hkv), static_cast<int>(c->D), static_cast<int>(c->B), -1, e4m3 ? shift : 0};
   if ((c->page_size & (c->page_size - 1)) == 0)
     for (out.page_shift = 0; (int64_t{1} << out.page_shift) < c->page_size;) ++out.page_shift;
   return PERSONA_OK;
@@ -85,7 +88,7 @@ struct CacheViews {
     return View{p, c.D * e, {c.num_pages, c.Hkv, c.page_size}, {c.page_stride * e, c.head_stride * e, c.pos_stride * e}};
   }
   View scales(const void* p) const {
-    return View{p, p != nullptr ? int64_t{4} * c.page_size : 0, {c.num_pages, c.Hkv, 1},
+    return View{p, p != nullptr ? int64_t{4} * (c.page_size >> c.scale_shift) : 0, {c.num_pages, c.Hkv, 1},
                 {c.scale_page_stride * 4, c.scale_head_stride * 4, 0}};
   }
   // Whether the address range of x meets that of the page table, indptr or lengths,
@@ -143,11 +146,14 @@ int persona_paged_rope_cache(const persona_paged_cache* cache, const persona_row
   if (!m.writable() || !m.apart(vo) || (!in_place && overlap::share(vq, vo)) || overlap::share(vk, vo) ||
       overlap::share(vv, vo) || m.meet_pages(vq) || m.meet_pages(vk) || m.meet_pages(vv))
     return PERSONA_ERR_OVERLAP;
+  // (a run of rows per block and two more per sequence number the grid)
+  if (a.c.scale_shift > 0 && (rows >> a.c.scale_shift) + 2 * cache->B > kI32Max) return PERSONA_ERR_SHAPE;
   // theta^(-2j / D) / (2 pi) by multiplication: 63 roundings of 2^-53
   const double ratio = std::pow(static_cast<double>(theta), -2.0 / D);
   double f = 1.0 / 6.283185307179586476925;
   for (int j = 0; j < 64; ++j, f *= ratio) a.turns[j] = j < D / 2 ? f : 0.0;
-  return status(launch_paged_write(a, dtype, dev_err, stream));
+  return status(a.c.scale_shift > 0 ? launch_paged_block_write(a, dtype, dev_err, stream)
+                                    : launch_paged_write(a, dtype, dev_err, stream));
 }
 
 int persona_paged_cache_read(const persona_paged_cache* cache, const persona_rows* k, const persona_rows* v,
@@ -204,6 +210,59 @@ int persona_paged_attention(const persona_paged_cache* cache, const persona_rows
   if (static_cast<int64_t>(most) * a.G > (a.c.k_scale != nullptr ? kFewRows8 : kFewRows16))
     return status(launch_paged_chunk(a, dtype, workspace, stream));
   return status(launch_paged_attention(a, dtype, most, workspace, stream));
+}
+
+int persona_paged_plan(const int32_t* add, const int32_t* keep, int32_t* lengths, int64_t B, int32_t* page_table,
+                       int64_t table_stride, int64_t max_pages, int32_t* free_pages, int64_t pool, int32_t* num_free,
+                       int64_t page_size, int32_t* indptr, int64_t* places, const int32_t* seq_slots, int32_t* row_slots,
+                       int64_t rows, int32_t* dev_err, cudaStream_t stream) {
+  if (B < 0 || B > PERSONA_PLAN_MAX_SEQS || rows < 0 || rows > kI32Max - 8192 || max_pages < 0 || max_pages > kI32Max ||
+      table_stride < max_pages || pool < 0 || pool > kI32Max - 8192 || page_size <= 0 || page_size > kI32Max)
+    return PERSONA_ERR_SHAPE;
+  if (num_free == nullptr || indptr == nullptr || (B != 0 && (add == nullptr || lengths == nullptr)) ||
+      (B != 0 && max_pages != 0 && page_table == nullptr) || (pool != 0 && free_pages == nullptr) ||
+      (rows != 0 && places == nullptr) || (row_slots != nullptr && B != 0 && seq_slots == nullptr))
+    return PERSONA_ERR_INVALID_ARG;
+  if (!aligned(add, 4) || !aligned(keep, 4) || !aligned(lengths, 4) || !aligned(page_table, 4) || !aligned(free_pages, 4) ||
+      !aligned(num_free, 4) || !aligned(indptr, 4) || !aligned(places, 8) || !aligned(seq_slots, 4) || !aligned(row_slots, 4))
+    return PERSONA_ERR_ALIGNMENT;
+  const View written[] = {array_view(lengths, B), View{page_table, int64_t{4} * max_pages, {B, 1, 1}, {table_stride * 4, 0, 0}},
+                          array_view(free_pages, pool), array_view(num_free, 1), array_view(indptr, B + 1),
+                          array_view(places, rows), array_view(row_slots, row_slots != nullptr ? rows : 0)};
+  const View read[] = {array_view(add, B), array_view(keep, keep != nullptr ? B : 0),
+                       array_view(seq_slots, row_slots != nullptr ? B : 0)};
+  for (int i = 0; i < 7; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (overlap::ranges_meet(written[i], written[j])) return PERSONA_ERR_OVERLAP;
+    for (const View& v : read)
+      if (overlap::ranges_meet(written[i], v)) return PERSONA_ERR_OVERLAP;
+  }
+  const PagedPlan a{add, keep, lengths, page_table, table_stride, free_pages, num_free, indptr, places, seq_slots, row_slots,
+                    static_cast<int>(B), static_cast<int>(max_pages), static_cast<int>(page_size), static_cast<int>(pool),
+                    static_cast<int>(rows), dev_err};
+  return status(launch_paged_plan(a, stream));
+}
+
+int persona_sample_tokens(const void* logits, int64_t ld, int logits_type, const float* u, const float* temperature,
+                          const int32_t* top_k, const float* top_p, const float* min_p, int64_t* tokens, int64_t B, int64_t V,
+                          cudaStream_t stream) {
+  if (logits_type < PERSONA_DTYPE_F16 || logits_type > PERSONA_DTYPE_F32) return PERSONA_ERR_DTYPE;
+  if (B < 0 || B > kI32Max / 8 || V <= 0 || V > PERSONA_VERIFY_MAX_VOCAB || ld < 0) return PERSONA_ERR_SHAPE;
+  if (B == 0) return PERSONA_OK;
+  if (logits == nullptr || u == nullptr || tokens == nullptr) return PERSONA_ERR_INVALID_ARG;
+  const int64_t e = logits_type == PERSONA_DTYPE_F32 ? 4 : 2;
+  if (!aligned(logits, e) || !aligned(u, 4) || !aligned(temperature, 4) || !aligned(top_k, 4) || !aligned(top_p, 4) ||
+      !aligned(min_p, 4) || !aligned(tokens, 8))
+    return PERSONA_ERR_ALIGNMENT;
+  // rows of other sequences are read at any time
+  const View out = array_view(tokens, B);
+  const View in[] = {View{logits, V * e, {B, 1, 1}, {ld * e, 0, 0}}, array_view(u, B), array_view(temperature, temperature != nullptr ? B : 0),
+                     array_view(top_k, top_k != nullptr ? B : 0), array_view(top_p, top_p != nullptr ? B : 0),
+                     array_view(min_p, min_p != nullptr ? B : 0)};
+  for (const View& v : in)
+    if (overlap::ranges_meet(out, v)) return PERSONA_ERR_OVERLAP;
+  const SampleTokens a{logits, ld, u, temperature, top_k, top_p, min_p, tokens, static_cast<int>(B), static_cast<int>(V)};
+  return status(launch_sample_tokens(a, logits_type, stream));
 }
 
 int persona_verify_draft(const void* target, int64_t ld_target, const void* draft, int64_t ld_draft, int prob_type,

@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           if (kE4m3) {
             k_sc = v_sc = 0.f;
             if (there) {
-              const int64_t so = pg * a.c.scale_page_stride + at + static_cast<int64_t>(w.h) * a.c.scale_head_stride;
+              const int64_t so = pg * a.c.scale_page_stride + (at >> a.c.scale_shift) + static_cast<int64_t>(w.h) * a.c.scale_head_stride;
               k_sc = a.c.k_scale[so];
               v_sc = a.c.v_scale[so];
             }

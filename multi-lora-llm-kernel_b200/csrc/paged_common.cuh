@@ -90,6 +90,27 @@ inline int sm_count() {
   return n;
 }
 
+// A kernel's attributes, set once per device: allows `smem` bytes of dynamic
+// shared memory and, where regs > 0, checks that the kernel is launched with
+// that many registers a thread.  `done`: one flag per device, static at the
+// caller.
+template <typename K> cudaError_t prepare_kernel(std::atomic<bool> (&done)[64], K kernel, int smem, int regs) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  if (regs > 0) {
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, kernel);
+    if (e != cudaSuccess) return e;
+    if (attr.numRegs != regs) return cudaErrorInvalidConfiguration;
+  }
+  if (dev < 64) done[dev].store(true, std::memory_order_release);
+  return cudaSuccess;
+}
+
 // Launches `kern`, as a programmatic dependent of the kernel before it if
 // `early`.  A kernel that takes most of an SM's shared memory is not launched
 // early: the SM keeps the division of its memory for as long as the kernel

@@ -24,7 +24,8 @@ New in this build:
 * ``paged_rope_cache`` / ``paged_cache_read`` / ``paged_attention`` -- a
   ragged batch of new tokens (single ones, drafted ones, prompt chunks) over a
   paged KV cache with 16-bit or e4m3 pages; ``verify_draft`` -- acceptance of
-  drafted tokens.
+  drafted tokens; ``paged_plan`` -- pages, row offsets and slots of the next
+  step on the device; ``sample_tokens`` -- next tokens from given numbers.
 * ``check_errors`` -- out-of-range slots are detected on the device (no
   per-row host sync); the next op on that device, or this function, raises.
 """
@@ -190,6 +191,8 @@ def check_errors(device: Optional[torch.device] = None, synchronize: bool = True
             what.append("page or position outside the paged cache")
         if bits & 32:
             what.append("drafted token outside the vocabulary")
+        if bits & 64:
+            what.append("no room for a planned step in the free pages or the page table")
         raise RuntimeError(f"persona: device error 0x{bits:x}: {', '.join(what)}")
 
 
@@ -268,8 +271,11 @@ def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache:
     ``lengths[b] - 1``.  Caches [pages, Hkv, page size, D]; position p of
     sequence b is in page ``page_table[b, p // page_size]``.  Caches of
     ``float8_e4m3fn`` take fp32 scales [pages, Hkv, page size]: one per token
-    and head, ``max|x| / 448``.  Rows of no sequence are left alone.  ``theta``
-    is taken as an fp32 number.  What is written must not overlap itself or
+    and head, ``max|x| / 448``; scales [pages, Hkv, n] with n a fraction of the
+    page size: one per block of 2, 4, ... 128 tokens and head, a power of two
+    that grows with the block (its earlier codes move to the new scale; a block
+    is written by one sequence only).  Rows of no sequence are left alone.
+    ``theta`` is taken as an fp32 number.  What is written must not overlap itself or
     another argument, but for ``q_out``, which may be ``q``."""
     q_out = q if q_out is None else q_out
     _paged("paged_rope_cache", q).paged_rope_cache(q, k, v, q_out, k_cache, v_cache, page_table, indptr, lengths, theta,
@@ -305,6 +311,49 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         max_new = max(1, q.shape[0] - lengths.shape[0] + 1)
     ext.paged_attention(q, k_cache, v_cache, page_table, indptr, lengths, out, scale, window, max_new, k_scale, v_scale)
     return out
+
+
+def paged_plan(new: torch.Tensor, lengths: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
+               num_free: torch.Tensor, page_size: int, indptr: torch.Tensor, places: torch.Tensor,
+               keep: Optional[torch.Tensor] = None, seq_slots: Optional[torch.Tensor] = None,
+               row_slots: Optional[torch.Tensor] = None) -> None:
+    """The next step over a paged cache, planned on the device from its
+    sequences' lengths: ``indptr``, ``lengths`` and ``page_table`` as the other
+    paged operators take them.
+
+    Sequence b keeps its first ``keep[b]`` tokens (None: all) and gets
+    ``new[b]`` more.  ``free_pages`` [pool] int32 is a stack whose first
+    ``num_free`` [1] int32 pages are free: pages of what is not kept go back,
+    those of the new tokens come out, and the same step made again gets the
+    same pages.  Written beside them: ``lengths`` [B] int32, ``page_table`` [B,
+    max pages] int32 (entries of the pages taken), ``indptr`` [B + 1] int32,
+    ``places`` [rows] int64 (page * page_size + place in the page of every new
+    row, -1 behind the last) and ``row_slots`` [rows] int32 (``seq_slots[b]``
+    of the row's sequence, -1 behind the last).  A step that cannot be made
+    changes nothing but ``indptr`` (zeros), ``places`` and ``row_slots`` (-1),
+    so that the operators behind it do nothing, and is reported by the next
+    call or ``check_errors``.  What is written overlaps no other argument."""
+    _paged("paged_plan", new).paged_plan(new, lengths, page_table, free_pages, num_free, page_size, indptr, places, keep,
+                                         seq_slots, row_slots)
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, tokens: torch.Tensor,
+                  temperature: Optional[torch.Tensor] = None, top_k: Optional[torch.Tensor] = None,
+                  top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Next tokens [B] int64 from ``logits`` [B, V] (fp16, bf16 or fp32) and
+    uniform numbers ``u`` [B]; returns ``tokens``.
+
+    Every row has its own parameters, fp32 [B] tensors (``top_k`` int32), each of
+    which may be None.  With weights ``exp((x - max) / temperature)``: ``top_k``
+    > 0 keeps that many of the largest (equal ones by their index), ``top_p`` <
+    1 of those the ones before which the weights sum to at most ``top_p`` of
+    them all, ``min_p`` > 0 those of at least ``min_p`` times the largest
+    weight.  The token is the first, by index, whose running sum of kept weights
+    exceeds ``u`` times their sum.  Temperature 0 (or below): the largest logit
+    of lowest index.  Logits of -infinity or NaN are never drawn; a row of
+    nothing else gives -1.  ``tokens`` overlaps no input."""
+    _paged("sample_tokens", logits).sample_tokens(logits, u, tokens, temperature, top_k, top_p, min_p)
+    return tokens
 
 
 def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_probs: Optional[torch.Tensor],
