@@ -78,24 +78,37 @@ __device__ __forceinline__ void seq_units(const Seq& s, int window, int TR, int 
 }
 
 // Shared memory of the ring, which also holds the warps' results at a piece's end.
-template <int D, int MT, bool kE4m3, int kStages> struct RingBytes {
-  static constexpr int kSlot = 2 * kPos * D * (kE4m3 ? 1 : 2) + (kE4m3 ? 2 * kPos * 4 : 0);
-  static constexpr int kRing = kWarps * kStages * kSlot, kWarpOut = kWarps * 16 * MT * D * 4;
-  static constexpr int kJoin = kWarpOut + 16 * MT * D * 4;  // the warps' results, and a cluster's share of them
+template <int D, int TR, bool kE4m3, int kStages, bool kBlocks> struct RingBytes {
+  static constexpr int kSlot = 2 * kPos * D * (kE4m3 ? 1 : 2) + (kBlocks ? 16 : kE4m3 ? 2 * kPos * 4 : 0);
+  static constexpr int kRing = kWarps * kStages * kSlot, kWarpOut = kWarps * TR * D * 4;
+  static constexpr int kJoin = kWarpOut + TR * D * 4;  // the warps' results, and a cluster's share of them
   static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
 };
 
-template <typename T, int D, int MT, bool kE4m3, int kStages, bool kCluster>
-__global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_constant__ PagedAttention a) {
+// The matrix that this lane has two elements of a row of, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// CTAs of an SM that have to be resident, by row tiles of eight (0: none; the
+// other form takes what its registers allow).
+constexpr int block_ctas(int NT) { return NT == 1 ? 4 : NT == 2 ? 3 : NT > 2 ? 2 : 1; }
+
+// NT > 0: the form with the rows as columns, for a scale per block (above).
+template <typename T, int D, int MT, bool kE4m3, int kStages, bool kCluster, int NT>
+__global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   using MT16 = typename std::conditional<kE4m3, __half, T>::type;  // type of the products
-  constexpr int TR = 16 * MT;
+  constexpr bool kBlocks = NT > 0;
+  constexpr int TR = kBlocks ? 8 * NT : 16 * MT;
   constexpr int kElt = kE4m3 ? 1 : 2;
   constexpr int kRowBytes = D * kElt;                  // one position in a ring slot
   constexpr int kChunks = kRowBytes / 16;
   constexpr int kHalf = kPos * kRowBytes;              // k (or v) of one warp step
-  constexpr int kSlot = 2 * kHalf + (kE4m3 ? 2 * kPos * 4 : 0);
+  using Ring = RingBytes<D, TR, kE4m3, kStages, kBlocks>;
+  constexpr int kSlot = Ring::kSlot;
   constexpr int kSteps = D / 16;
-  constexpr int kQAt = RingBytes<D, MT, kE4m3, kStages>::kBytes;  // q fragments behind the ring (MT = 2)
+  constexpr int kQAt = Ring::kBytes;  // q fragments behind the ring (two row tiles, or more than two of eight)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_scan[kWarps], s_items[kWarps], s_begin;
   __shared__ int s_b;
@@ -257,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
     const uint8_t* const kl = kb + lr * a.c.pos_stride * kElt + ch * 16;
     const uint8_t* const vl = vb + lr * a.c.pos_stride * kElt + ch * 16;
     const int64_t row_step = kRowsPer * a.c.pos_stride * kElt;
-    const float* const sl = kE4m3 ? (lane < 16 ? a.c.k_scale : a.c.v_scale) + static_cast<int64_t>(h) * a.c.scale_head_stride : nullptr;
+    const float* const sl = kE4m3 ? (lane < (kBlocks ? 1 : 16) ? a.c.k_scale : a.c.v_scale) + static_cast<int64_t>(h) * a.c.scale_head_stride : nullptr;
     // 16-byte chunks are XORed by the row so that the fragment reads below touch
     // every bank once (8-bit: k reads two rows of four chunks, v reads even rows
     // of two chunks, per quarter warp).  A lane's row is lr plus a multiple of
@@ -298,7 +311,11 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           cp_async16(to + (ck & kMask) * 16, live ? kp : kl, live);
           cp_async16(to + kHalf + (cv & kMask) * 16, live ? vp : vl, live);
         }
-        if (kE4m3) {
+        if (kBlocks) {  // the step's two scales: all of its positions are in one block
+          const bool live = rem > 0;
+          if (lane < 2)
+            cp_async4(dst + 2 * kHalf + lane * 4, live ? sl + (pg * a.c.scale_page_stride + (at >> a.c.scale_shift)) : sl, live);
+        } else if (kE4m3) {
           const int r = lane & 15;
           const bool live = static_cast<uint32_t>(r - skip) < static_cast<uint32_t>(rem);
           cp_async4(dst + 2 * kHalf + lane * 4, live ? sl + (pg * a.c.scale_page_stride + ((at + r) >> a.c.scale_shift)) : sl, live);
@@ -316,7 +333,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           cp_async16(to + (ck & kMask) * 16, kb + src + ch * 16, live);
           cp_async16(to + kHalf + (cv & kMask) * 16, vb + src + ch * 16, live);
         }
-        if (kE4m3) {
+        if (kE4m3 && !kBlocks) {
           const int p = p0 + (lane & 15);
           int at = 0;
           const int pg = p >= pbegin && p < pend ? page_of(p, at) : -1;
@@ -338,61 +355,63 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
     uint32_t qf[MT][kSteps][4];
     float qmul[MT][2];
     int hi_pos[MT][2];
+    if constexpr (!kBlocks) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int m = mt * 16 + half * 8 + g;
-        const bool live = m < mrows;
-        const int mm = m0 + (live ? m : 0);
-        const int tok = mm / G, hg = mm - tok * G;
-        const T* qp = static_cast<const T*>(a.q.p) + static_cast<int64_t>(seq.row0 + tok) * a.q.row_stride +
-                      static_cast<int64_t>(h * G + hg) * a.q.head_stride;
-        hi_pos[mt][half] = live ? ctx + tok : -1;
-        qmul[mt][half] = a.scale_log2;
+        for (int half = 0; half < 2; ++half) {
+          const int m = mt * 16 + half * 8 + g;
+          const bool live = m < mrows;
+          const int mm = m0 + (live ? m : 0);
+          const int tok = mm / G, hg = mm - tok * G;
+          const T* qp = static_cast<const T*>(a.q.p) + static_cast<int64_t>(seq.row0 + tok) * a.q.row_stride +
+                        static_cast<int64_t>(h * G + hg) * a.q.head_stride;
+          hi_pos[mt][half] = live ? ctx + tok : -1;
+          qmul[mt][half] = a.scale_log2;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          if (!kE4m3) {
-            qf[mt][s][half] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * s + 2 * t) : 0u;
-            qf[mt][s][half + 2] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * s + 8 + 2 * t) : 0u;
-          } else {
-            const int d = 64 * (s / 4) + 16 * t + 4 * (s % 4);
-            const uint2 w = live ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0u, 0u);
-            qf[mt][s][half] = w.x;
-            qf[mt][s][half + 2] = w.y;
+          for (int s = 0; s < kSteps; ++s) {
+            if (!kE4m3) {
+              qf[mt][s][half] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * s + 2 * t) : 0u;
+              qf[mt][s][half + 2] = live ? *reinterpret_cast<const uint32_t*>(qp + 16 * s + 8 + 2 * t) : 0u;
+            } else {
+              const int d = 64 * (s / 4) + 16 * t + 4 * (s % 4);
+              const uint2 w = live ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0u, 0u);
+              qf[mt][s][half] = w.x;
+              qf[mt][s][half + 2] = w.y;
+            }
+          }
+          if (kE4m3 && !std::is_same<T, __half>::value) {
+            // bf16 row -> fp16: scaled by the power of two that brings its
+            // largest element into [1, 2); elements 2^-24 below that vanish
+            float mx = 0.f;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float2 f = Cvt<T>::to2(qf[mt][s][half + 2 * x]);
+                mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+              }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // exponent field of mx, kept where both powers are normal numbers
+            const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23), 2), 252);
+            const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+            qmul[mt][half] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float2 f = Cvt<T>::to2(qf[mt][s][half + 2 * x]);
+                qf[mt][s][half + 2 * x] = Mma<__half>::pack(f.x * down, f.y * down);
+              }
           }
         }
-        if (kE4m3 && !std::is_same<T, __half>::value) {
-          // bf16 row -> fp16: scaled by the power of two that brings its
-          // largest element into [1, 2); elements 2^-24 below that vanish
-          float mx = 0.f;
-#pragma unroll
-          for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const float2 f = Cvt<T>::to2(qf[mt][s][half + 2 * x]);
-              mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          // exponent field of mx, kept where both powers are normal numbers
-          const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23), 2), 252);
-          const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-          qmul[mt][half] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e) << 23);
-#pragma unroll
-          for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const float2 f = Cvt<T>::to2(qf[mt][s][half + 2 * x]);
-              qf[mt][s][half + 2 * x] = Mma<__half>::pack(f.x * down, f.y * down);
-            }
-        }
-      }
+    }
 
     // With two row tiles the fragments would take 64 registers beside 128 of
     // outputs: they go to shared memory, one 16-byte read a lane, row tile and step.
     const uint32_t s_qf = smem_u32(smem) + kQAt + lane * 16;
-    if constexpr (MT == 2) {
+    if constexpr (MT == 2 && !kBlocks) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -416,11 +435,92 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
       }
     };
 
-    // ---- one pass over the piece's positions ----
-    float acc[MT][D / 8][4];
-    float m_run[MT][2], l_run[MT][2];
+    // Rows as columns: the lane's column g of a tile of eight, the same d; what
+    // it needs to know of the rows is that of its scores, 2 t and 2 t + 1.
+    uint32_t qb[kBlocks ? NT : 1][kSteps][2];
+    float qrow[kBlocks ? NT : 1][2];
+    int hi_row[kBlocks ? NT : 1][2];
+    const uint32_t s_qb = smem_u32(smem) + kQAt + lane * 8;
+    if constexpr (kBlocks) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+      for (int nt = 0; nt < NT; ++nt) {
+        const int m = nt * 8 + g;
+        const bool live = m < mrows;
+        const int mm = m0 + (live ? m : 0);
+        const int tok = mm / G, hg = mm - tok * G;
+        const T* qp = static_cast<const T*>(a.q.p) + static_cast<int64_t>(seq.row0 + tok) * a.q.row_stride +
+                      static_cast<int64_t>(h * G + hg) * a.q.head_stride;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const uint2 w = live ? *reinterpret_cast<const uint2*>(qp + 64 * (s / 4) + 16 * t + 4 * (s % 4)) : make_uint2(0u, 0u);
+          qb[nt][s][0] = w.x;
+          qb[nt][s][1] = w.y;
+        }
+        float mul = a.scale_log2;
+        if (!std::is_same<T, __half>::value) {
+          // bf16 -> fp16 by a power of two, as below
+          float mx = 0.f;
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float2 f = Cvt<T>::to2(qb[nt][s][x]);
+              mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23), 2), 252);
+          const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+          mul = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float2 f = Cvt<T>::to2(qb[nt][s][x]);
+              qb[nt][s][x] = Mma<__half>::pack(f.x * down, f.y * down);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int mr = nt * 8 + 2 * t + e;
+          qrow[nt][e] = __shfl_sync(0xffffffffu, mul, (2 * t + e) * 4);
+          hi_row[nt][e] = mr < mrows ? ctx + (m0 + mr) / G : -1;
+        }
+        if (NT > 2) {  // 16 registers a tile: to shared memory, one 8-byte read a lane, tile and step
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s)
+            if (s / (kSteps / kWarps) == warp)
+              asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(s_qb + (nt * kSteps + s) * 256), "r"(qb[nt][s][0]),
+                           "r"(qb[nt][s][1])
+                           : "memory");
+        }
+      }
+      if (NT > 2) __syncthreads();
+    }
+
+    // ---- one pass over the piece's positions ----
+    // (as many accumulators in either form: rows as columns have D / 16 tiles of
+    // sixteen dims for each tile of eight rows)
+    constexpr int kAccs = kBlocks ? 1 : MT;
+    float ot[kBlocks ? NT : 1][D / 16][4], m_row[kBlocks ? NT : 1][2], l_row[kBlocks ? NT : 1][2];
+    if constexpr (kBlocks) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) ot[nt][i][x] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          m_row[nt][e] = kNegInf;
+          l_row[nt][e] = 0.f;
+        }
+      }
+    }
+    float acc[kAccs][D / 8][4];
+    float m_run[kAccs][2], l_run[kAccs][2];
+#pragma unroll
+    for (int mt = 0; mt < kAccs; ++mt) {
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
 #pragma unroll
@@ -441,6 +541,131 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
       const int p0 = p_lo + s * kUnit + warp * kPos;
       if (p0 >= pend) continue;
       const uint32_t slot = ring + (s % kStages) * kSlot;
+      if constexpr (kBlocks) {
+        // ---- S^T = K Q^T: positions as rows ----
+        float st[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) st[nt][x] = 0.f;
+#pragma unroll
+        for (int blk = 0; blk < D / 64; ++blk) {
+          uint32_t u[2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int r = n * 8 + g;
+            const uint4 w = lds128(slot + r * kRowBytes + (((4 * blk + t) ^ ((r & 1) << 2)) & (kChunks - 1)) * 16);
+            u[n][0] = w.x;
+            u[n][1] = w.y;
+            u[n][2] = w.z;
+            u[n][3] = w.w;
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t ka[4];
+            e4m3x4_to_half(u[0][x], ka[0], ka[2]);
+            e4m3x4_to_half(u[1][x], ka[1], ka[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t b[2];
+              if constexpr (NT > 2) {
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(b[0]), "=r"(b[1]) : "r"(s_qb + (nt * kSteps + 4 * blk + x) * 256));
+              } else {
+                b[0] = qb[nt][4 * blk + x][0];
+                b[1] = qb[nt][4 * blk + x][1];
+              }
+              Mma<__half>::k16(st[nt], ka, b);
+            }
+          }
+        }
+        // ---- scores in the log2 domain, masked ----
+        const float ks = __uint_as_float(lds32(slot + 2 * kHalf));
+        const float vs = fmaxf(__uint_as_float(lds32(slot + 2 * kHalf + 4)), kLeastScale);
+        const float lv = log2_approx(vs), rv = rcp_approx(vs);
+        const bool need_mask = p0 + kPos - 1 > full_hi || p0 < full_lo;
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float& v = st[nt][x];
+            v = fmaf(v, ks * qrow[nt][x & 1], lv);
+            if (need_mask) {
+              const int p = p0 + g + 8 * (x >> 1), top = hi_row[nt][x & 1];
+              v = p <= top && (a.window == 0 || p > top - a.window) ? v : kNegInf;
+            }
+            grow |= v > m_row[nt][x & 1] + kGrow;  // (-inf: with the first key)
+          }
+        if (__any_sync(0xffffffffu, grow)) {  // a row's maximum is outgrown by 2^8: it moves
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(st[nt][e], st[nt][2 + e]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              const float old = m_row[nt][e];
+              const bool up = mx > old + kGrow;
+              const float f = up && old != kNegInf ? exp2_approx(old - mx) : 1.f;
+              if (up) m_row[nt][e] = mx;
+              l_row[nt][e] *= f;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                ot[nt][i][e] *= f;
+                ot[nt][i][2 + e] *= f;
+              }
+            }
+        }
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float ma = m_row[nt][0] == kNegInf ? 0.f : m_row[nt][0], mb = m_row[nt][1] == kNegInf ? 0.f : m_row[nt][1];
+          const float e0 = exp2_approx(st[nt][0] - ma), e1 = exp2_approx(st[nt][1] - mb);
+          const float e2 = exp2_approx(st[nt][2] - ma), e3 = exp2_approx(st[nt][3] - mb);
+          l_row[nt][0] = fmaf(e0 + e2, rv, l_row[nt][0]);
+          l_row[nt][1] = fmaf(e1 + e3, rv, l_row[nt][1]);
+          // 16 bits for the product, as below
+          pb[nt][0] = transposed(Mma<__half>::pack(e0, e1));
+          pb[nt][1] = transposed(Mma<__half>::pack(e2, e3));
+        }
+        // ---- O^T += V^T P^T: lane g holds dims [g D / 8, ...) of its four positions ----
+        const uint32_t vslot = slot + kHalf;
+        constexpr int kW = D / 32;
+        uint32_t w[4][kW];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int r = 2 * t + (x & 1) + 8 * (x >> 1);
+          if (D == 128) {
+            const uint4 v = lds128(vslot + r * kRowBytes + ((g ^ (((r >> 1) & 3) << 1)) & (kChunks - 1)) * 16);
+            w[x][0] = v.x;
+            w[x][1] = v.y;
+            w[x][kW - 2] = v.z;
+            w[x][kW - 1] = v.w;
+          } else {
+            const uint32_t ad = vslot + r * kRowBytes + (((g >> 1) ^ (((r >> 1) & 3) << 1)) & (kChunks - 1)) * 16 + (g & 1) * 8;
+            w[x][0] = lds32(ad);
+            w[x][1] = lds32(ad + 4);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kW; ++j) {
+          uint32_t va[2][4];  // dims 4 j, 4 j + 1 and 4 j + 2, 4 j + 3
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t ab = __byte_perm(w[2 * x][j], w[2 * x + 1][j], 0x5140);
+            const uint32_t cd = __byte_perm(w[2 * x][j], w[2 * x + 1][j], 0x7362);
+            e4m3x4_to_half(ab, va[0][2 * x], va[0][2 * x + 1]);
+            e4m3x4_to_half(cd, va[1][2 * x], va[1][2 * x + 1]);
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) Mma<__half>::k16(ot[nt][2 * j + y], va[y], pb[nt]);
+        }
+        __syncwarp();
+        continue;
+      }
 
       float sc[MT][2][4];
 #pragma unroll
@@ -642,40 +867,65 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
     // Where dim d of row m is: 8-dim chunks XORed by the row, or (8-bit pages,
     // whose lanes hold D / 8 dims in a row) those dims turned by row and lane.
     auto join_at = [&](int m, int d) {
+      if (kBlocks) return d ^ (((m >> 1) & 3) << 2);
       if (!kE4m3) return d ^ ((m & 7) << 3);
       constexpr int kW = D / 8;
       const int blk = d / kW;
       return blk * kW + ((d + 2 * (m & 7) + (blk >> 2)) & (kW - 1));
     };
+    if constexpr (kBlocks) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int m = mt * 16 + half * 8 + g;
-        float l = l_run[mt][half];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) {
-          s_m[warp][m] = m_run[mt][half];
-          s_l[warp][m] = l;
+        for (int e = 0; e < 2; ++e) {
+          const int m = nt * 8 + 2 * t + e;
+          float l = l_row[nt][e];
+          l += __shfl_xor_sync(0xffffffffu, l, 4);
+          l += __shfl_xor_sync(0xffffffffu, l, 8);
+          l += __shfl_xor_sync(0xffffffffu, l, 16);
+          if (g == 0) {
+            s_m[warp][m] = m_row[nt][e];
+            s_l[warp][m] = l;
+          }
+          if (m >= mrows) continue;
+          float* dst = accs + (warp * TR + m) * D;
+#pragma unroll
+          for (int i = 0; i < D / 16; i += 2)
+            *reinterpret_cast<float4*>(dst + join_at(m, g * (D / 8) + 2 * i)) =
+                make_float4(ot[nt][i][e], ot[nt][i][2 + e], ot[nt][i + 1][e], ot[nt][i + 1][2 + e]);
         }
-        if (mt * 16 + half * 8 >= mrows) continue;  // no such rows
-        float* dst = accs + (warp * TR + m) * D;
+    }
+    if constexpr (!kBlocks) {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const float x0 = acc[mt][i][2 * half], x1 = acc[mt][i][2 * half + 1];
-          if (!kE4m3) {
-            *reinterpret_cast<float2*>(dst + join_at(m, 8 * i + 2 * t)) = make_float2(x0, x1);
-          } else {  // the odd lanes the other way round: 32 lanes, 32 banks
-            const int a0 = join_at(m, 2 * t * (D / 8) + i), a1 = join_at(m, (2 * t + 1) * (D / 8) + i);
-            dst[(t & 1) == 0 ? a0 : a1] = (t & 1) == 0 ? x0 : x1;
-            dst[(t & 1) == 0 ? a1 : a0] = (t & 1) == 0 ? x1 : x0;
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int m = mt * 16 + half * 8 + g;
+          float l = l_run[mt][half];
+          l += __shfl_xor_sync(0xffffffffu, l, 1);
+          l += __shfl_xor_sync(0xffffffffu, l, 2);
+          if (t == 0) {
+            s_m[warp][m] = m_run[mt][half];
+            s_l[warp][m] = l;
+          }
+          if (mt * 16 + half * 8 >= mrows) continue;  // no such rows
+          float* dst = accs + (warp * TR + m) * D;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const float x0 = acc[mt][i][2 * half], x1 = acc[mt][i][2 * half + 1];
+            if (!kE4m3) {
+              *reinterpret_cast<float2*>(dst + join_at(m, 8 * i + 2 * t)) = make_float2(x0, x1);
+            } else {  // the odd lanes the other way round: 32 lanes, 32 banks
+              const int a0 = join_at(m, 2 * t * (D / 8) + i), a1 = join_at(m, (2 * t + 1) * (D / 8) + i);
+              dst[(t & 1) == 0 ? a0 : a1] = (t & 1) == 0 ? x0 : x1;
+              dst[(t & 1) == 0 ? a1 : a0] = (t & 1) == 0 ? x1 : x0;
+            }
           }
         }
-      }
+    }
     __syncthreads();
     const bool complete = !kCluster && k0 == 0 && k1 == per;
-    float* const mine = reinterpret_cast<float*>(smem + RingBytes<D, MT, kE4m3, kStages>::kWarpOut);  // [TR][D], cluster
+    float* const mine = reinterpret_cast<float*>(smem + Ring::kWarpOut);  // [TR][D], cluster
     float* part = a.part + static_cast<int64_t>(2 * cta + (first_piece ? 0 : 1)) * Part<TR, D>::kFloats;
     for (int i = tid; i < mrows * (D / 8); i += kThreads) {
       const int m = i / (D / 8), d = (i % (D / 8)) * 8;
@@ -692,7 +942,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           l = fmaf(f, s_l[w][m], l);
           const float* src = accs + (w * TR + m) * D;
 #pragma unroll
-          for (int x = 0; x < 8; ++x) o[x] = fmaf(f, src[kE4m3 ? join_at(m, d + x) : join_at(m, d) + x], o[x]);
+          for (int x = 0; x < 8; ++x) o[x] = fmaf(f, src[kBlocks ? join_at(m, d + (x & 4)) + (x & 3) : kE4m3 ? join_at(m, d + x) : join_at(m, d) + x], o[x]);
         }
       }
       if (complete) {
@@ -769,13 +1019,17 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
 
 constexpr int kCtasPerSm = 2;
 
-template <typename T, int D, int MT, bool kE4m3>
-cudaError_t attention_launch(const PagedAttention& a, int max_new, cudaStream_t st) {
+template <typename T, int D, int MT, bool kE4m3, int NT>
+cudaError_t attention_launch(PagedAttention a, int max_new, cudaStream_t st) {
   // Ring slots of 8 KB (16-bit) or 4.1 KB (8-bit) per warp at D = 128, two CTAs
   // per SM: 3 and 6 (96 KB a CTA); with two row tiles over 8-bit pages 4 (77.7
-  // against 81.3 us for 32 x 5 rows).
-  constexpr int kStages = (kE4m3 ? (MT == 2 ? 4 : 6) : 3) * (128 / D);
-  constexpr int kSmem = RingBytes<D, MT, kE4m3, kStages>::kBytes + (MT == 2 ? MT * (D / 16) * 512 : 0);
+  // against 81.3 us for 32 x 5 rows).  Rows as columns: as many as the CTAs of
+  // block_ctas have room for.
+  constexpr int kStages = (NT == 1 ? 3 : NT == 2 ? 4 : NT > 2 ? 5 : kE4m3 ? (MT == 2 ? 4 : 6) : 3) * (128 / D);
+  constexpr int TR = NT > 0 ? 8 * NT : 16 * MT;
+  constexpr int kSmem = RingBytes<D, TR, kE4m3, kStages, (NT > 0)>::kBytes +
+                        (NT > 2 ? NT * (D / 16) * 256 : NT == 0 && MT == 2 ? MT * (D / 16) * 512 : 0);
+  constexpr int kCtas = NT > 0 ? block_ctas(NT) : kCtasPerSm;
   const int sms = sm_count();
   // Where the page table cannot hold long sequences: a cluster per tile, in one
   // launch, as many CTAs as keep every cluster resident.  8 sequences of up to
@@ -784,38 +1038,48 @@ cudaError_t attention_launch(const PagedAttention& a, int max_new, cudaStream_t 
   // units so: from 32 on longer sequences are balanced better by the line (one
   // of 16000: 32.3 and 27.5).
   const int64_t units = (static_cast<int64_t>(a.c.max_pages) * a.c.page_size + kUnit - 1) / kUnit;
-  const int64_t most = (static_cast<int64_t>(max_new) * a.G + 16 * MT - 1) / (16 * MT);  // tiles of a sequence
+  const int64_t most = (static_cast<int64_t>(max_new) * a.G + TR - 1) / TR;  // tiles of a sequence
   const int64_t items = most * a.c.Hkv * a.c.B;
   int split = 8;
-  while (split > 1 && (items * split > kCtasPerSm * sms || split / 2 >= units)) split /= 2;
-  if (items * split <= kCtasPerSm * sms && units <= 16 * split) {
+  while (split > 1 && (items * split > kCtas * sms || split / 2 >= units)) split /= 2;
+  if (items * split <= kCtas * sms && units <= 16 * split) {
     PagedAttention c = a;
     c.split = split;
     c.tile_step = static_cast<int>(most);
-    auto k = paged_attention_kernel<T, D, MT, kE4m3, kStages, true>;
+    auto k = paged_attention_kernel<T, D, MT, kE4m3, kStages, true, NT>;
     static std::atomic<bool> done[64];
     const cudaError_t e = prepare_kernel(done, k, kSmem, 0);
     if (e != cudaSuccess) return e;
     return launch_paged(k, dim3(static_cast<unsigned>(items * split)), dim3(kThreads), kSmem, split, false, st, c);
   }
-  auto k = paged_attention_kernel<T, D, MT, kE4m3, kStages, false>;
+  auto k = paged_attention_kernel<T, D, MT, kE4m3, kStages, false, NT>;
   static std::atomic<bool> done[64];
   cudaError_t e = prepare_kernel(done, k, kSmem, 0);
   if (e != cudaSuccess) return e;
-  const int ctas = kCtasPerSm * sms;
+  const int ctas = kCtas * sms;
+  static_assert(kCtas * (2 * sizeof(int4) + 2 * sizeof(float) * Part<TR, D>::kFloats) <=
+                    kCtasPerSm * (2 * sizeof(int4) + 2 * sizeof(float) * Part<32, D>::kFloats),
+                "workspace");
+  a.part = reinterpret_cast<float*>(a.desc + 2 * ctas);
   e = launch_paged(k, dim3(ctas), dim3(kThreads), kSmem, 1, false, st, a);
   if (e != cudaSuccess) return e;
-  return launch_paged(paged_combine_kernel<T, D, 16 * MT>, dim3(ctas, 2 * MT), dim3(256), 0, 1, true, st, a);
+  return launch_paged(paged_combine_kernel<T, D, TR>, dim3(ctas, TR / 8), dim3(256), 0, 1, true, st, a);
 }
 template <typename T, int D, int MT>
 cudaError_t attention_pages(const PagedAttention& a, int max_new, cudaStream_t st) {
-  return a.c.k_scale != nullptr ? attention_launch<T, D, MT, true>(a, max_new, st)
-                                : attention_launch<T, D, MT, false>(a, max_new, st);
+  return a.c.k_scale != nullptr ? attention_launch<T, D, MT, true, 0>(a, max_new, st)
+                                : attention_launch<T, D, MT, false, 0>(a, max_new, st);
 }
 template <typename T, int D>
 cudaError_t attention_rows(const PagedAttention& a, int max_new, cudaStream_t st) {
-  return static_cast<int64_t>(max_new) * a.G <= 16 ? attention_pages<T, D, 1>(a, max_new, st)
-                                                  : attention_pages<T, D, 2>(a, max_new, st);
+  const int64_t rows = static_cast<int64_t>(max_new) * a.G;
+  // A step's sixteen positions share a block: rows as columns.
+  if (a.c.scale_shift >= 4)
+    return rows <= 8    ? attention_launch<T, D, 1, true, 1>(a, max_new, st)
+           : rows <= 16 ? attention_launch<T, D, 1, true, 2>(a, max_new, st)
+           : rows <= 24 ? attention_launch<T, D, 1, true, 3>(a, max_new, st)
+                        : attention_launch<T, D, 1, true, 4>(a, max_new, st);
+  return rows <= 16 ? attention_pages<T, D, 1>(a, max_new, st) : attention_pages<T, D, 2>(a, max_new, st);
 }
 template <typename T>
 cudaError_t attention_dim(const PagedAttention& a, int max_new, cudaStream_t st) {
@@ -830,9 +1094,7 @@ size_t paged_attention_ws_bytes(int D) {
 }
 
 cudaError_t launch_paged_attention(PagedAttention a, int dtype, int max_new, void* workspace, cudaStream_t st) {
-  const size_t ctas = static_cast<size_t>(kCtasPerSm) * sm_count();
-  a.desc = static_cast<int4*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + ctas * 2 * sizeof(int4));
+  a.desc = static_cast<int4*>(workspace);  // the parts behind it, by the form's number of CTAs
   return dtype == PERSONA_DTYPE_BF16 ? attention_dim<__nv_bfloat16>(a, max_new, st) : attention_dim<__half>(a, max_new, st);
 }
 
