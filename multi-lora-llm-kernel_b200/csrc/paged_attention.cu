@@ -60,7 +60,9 @@ constexpr int kPos = 16;              // positions of one warp step
 constexpr int kUnit = kPos * kWarps;  // positions of one unit
 // What starting and ending a tile costs, in units: so many stand before its
 // first one in the line.  None where every unit has a CTA of its own.
+// (Rows as columns: 4 and 10 us of a CTA by the clock, against 1.3 and 1.6 a unit.)
 constexpr int kPieceUnits = 3;
+template <int NT> constexpr int kLead = NT < 2 ? kPieceUnits : 6;
 
 __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -93,7 +95,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 // CTAs of an SM that have to be resident, by row tiles of eight (0: none; the
 // other form takes what its registers allow).
-constexpr int block_ctas(int NT) { return NT == 1 ? 4 : NT == 2 ? 3 : NT > 2 ? 2 : 1; }
+constexpr int block_ctas(int NT) { return NT == 1 ? 4 : NT == 2 || NT == 3 ? 3 : NT > 3 ? 2 : 1; }
 
 // NT > 0: the form with the rows as columns, for a scale per block (above).
 template <typename T, int D, int MT, bool kE4m3, int kStages, bool kCluster, int NT>
@@ -163,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
       }
       __syncthreads();
     }
-    lead = total <= gridDim.x ? 0 : kPieceUnits;
+    lead = total <= gridDim.x ? 0 : kLead<NT>;
     total += lead * items;
     if (tid == 0) a.desc[2 * cta] = make_int4(0, 0, 0, 0);
     // no more CTAs than units, so that every range (before the move below) has one
@@ -280,6 +282,11 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
     // Where a step's positions share a page, the pages of 32 steps are read at
     // once, one a lane.
     int pages32 = -1;
+    // Steps of sixteen positions that are all there, in pages without gaps between
+    // positions (block scales): every copy at a fixed distance from the first.
+    const bool dense = kBlocks && a.c.pos_stride == D;
+    const uint32_t to_k = lr * kRowBytes + (ck0 & kMask) * 16, to_v = kHalf + lr * kRowBytes + (cv0 & kMask) * 16,
+                   to_v2 = kHalf + lr * kRowBytes + ((cv0 ^ (((kRowsPer / 2) & 3) << 1)) & kMask) * 16;
     auto load = [&](int s) {
       const int p0 = p_lo + s * kUnit + warp * kPos;
       const uint32_t dst = ring + (s % kStages) * kSlot;
@@ -300,6 +307,17 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
         rem = max(rem, 0);
         const int lrs = lr - skip;
         const int at = p0 - page_index(a.c, p0) * a.c.page_size;
+        if (dense && rem == kPos) {
+          const int64_t base = pg * a.c.page_stride + static_cast<int64_t>(at) * D;
+          const uint8_t *kp = kl + base, *vp = vl + base;
+#pragma unroll
+          for (int i = 0; i < kPos / kRowsPer; ++i) {
+            cp_async16(dst + to_k + i * kRowsPer * kRowBytes, kp + i * kRowsPer * D);
+            cp_async16(dst + ((i & 1) == 0 ? to_v : to_v2) + i * kRowsPer * kRowBytes, vp + i * kRowsPer * D);
+          }
+          if (lane < 2) cp_async4(dst + 2 * kHalf + lane * 4, sl + (pg * a.c.scale_page_stride + (at >> a.c.scale_shift)), true);
+          return;
+        }
         const int64_t base = rem > 0 ? (pg * a.c.page_stride + at * a.c.pos_stride) * kElt : 0;
         const uint8_t *kp = kl + base, *vp = vl + base;
 #pragma unroll
@@ -341,11 +359,37 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
         }
       }
     };
+    // Rows as columns: the lane's column g of a tile of eight, the same d; what
+    // it needs to know of the rows is that of its scores, 2 t and 2 t + 1.  Where
+    // there is much of it, read ahead of the pages, behind which it would wait (24
+    // rows: 170 us instead of 173; 8 rows: 109 instead of 107).
+    uint32_t qb[kBlocks ? NT : 1][kSteps][2];
+    float qrow[kBlocks ? NT : 1][2];
+    int hi_row[kBlocks ? NT : 1][2];
+    auto read_q = [&] {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int m = nt * 8 + g;
+        const bool live = m < mrows;
+        const int mm = m0 + (live ? m : 0);
+        const int tok = mm / G, hg = mm - tok * G;
+        const T* qp = static_cast<const T*>(a.q.p) + static_cast<int64_t>(seq.row0 + tok) * a.q.row_stride +
+                      static_cast<int64_t>(h * G + hg) * a.q.head_stride;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const uint2 w = live ? *reinterpret_cast<const uint2*>(qp + 64 * (s / 4) + 16 * t + 4 * (s % 4)) : make_uint2(0u, 0u);
+          qb[nt][s][0] = w.x;
+          qb[nt][s][1] = w.y;
+        }
+      }
+    };
+    if constexpr (NT > 1) read_q();
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) {
       if (s < steps) load(s);
       cp_commit();
     }
+    if constexpr (NT == 1) read_q();
 
     // ---- q fragments ----
     // 16-bit pages: the operand's own order of d.  8-bit pages: a lane reads
@@ -435,27 +479,10 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
       }
     };
 
-    // Rows as columns: the lane's column g of a tile of eight, the same d; what
-    // it needs to know of the rows is that of its scores, 2 t and 2 t + 1.
-    uint32_t qb[kBlocks ? NT : 1][kSteps][2];
-    float qrow[kBlocks ? NT : 1][2];
-    int hi_row[kBlocks ? NT : 1][2];
     const uint32_t s_qb = smem_u32(smem) + kQAt + lane * 8;
     if constexpr (kBlocks) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int m = nt * 8 + g;
-        const bool live = m < mrows;
-        const int mm = m0 + (live ? m : 0);
-        const int tok = mm / G, hg = mm - tok * G;
-        const T* qp = static_cast<const T*>(a.q.p) + static_cast<int64_t>(seq.row0 + tok) * a.q.row_stride +
-                      static_cast<int64_t>(h * G + hg) * a.q.head_stride;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const uint2 w = live ? *reinterpret_cast<const uint2*>(qp + 64 * (s / 4) + 16 * t + 4 * (s % 4)) : make_uint2(0u, 0u);
-          qb[nt][s][0] = w.x;
-          qb[nt][s][1] = w.y;
-        }
         float mul = a.scale_log2;
         if (!std::is_same<T, __half>::value) {
           // bf16 -> fp16 by a power of two, as below
@@ -543,11 +570,15 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
       const uint32_t slot = ring + (s % kStages) * kSlot;
       if constexpr (kBlocks) {
         // ---- S^T = K Q^T: positions as rows ----
-        float st[NT][4];
+        // (few tiles: two sums each, so that a product does not wait for the one before)
+        constexpr int kSums = NT < 3 ? 2 : 1;
+        float st[NT][4], half_st[kSums][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int y = 0; y < kSums; ++y)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) st[nt][x] = 0.f;
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) half_st[y][nt][x] = 0.f;
 #pragma unroll
         for (int blk = 0; blk < D / 64; ++blk) {
           uint32_t u[2][4];
@@ -574,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
                 b[0] = qb[nt][4 * blk + x][0];
                 b[1] = qb[nt][4 * blk + x][1];
               }
-              Mma<__half>::k16(st[nt], ka, b);
+              Mma<__half>::k16(half_st[x % kSums][nt], ka, b);
             }
           }
         }
@@ -589,6 +620,7 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             float& v = st[nt][x];
+            v = kSums == 2 ? half_st[0][nt][x] + half_st[kSums - 1][nt][x] : half_st[0][nt][x];
             v = fmaf(v, ks * qrow[nt][x & 1], lv);
             if (need_mask) {
               const int p = p0 + g + 8 * (x >> 1), top = hi_row[nt][x & 1];
@@ -1019,13 +1051,17 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
 
 constexpr int kCtasPerSm = 2;
 
+// Notes and pieces that the CTAs of an SM leave: four notes at most, and rows
+// for three CTAs of 24.
+constexpr size_t sm_ws_bytes(int D) { return 4 * 2 * sizeof(int4) + 2 * 3 * 24 * (static_cast<size_t>(D) + 2) * sizeof(float); }
+
 template <typename T, int D, int MT, bool kE4m3, int NT>
 cudaError_t attention_launch(PagedAttention a, int max_new, cudaStream_t st) {
   // Ring slots of 8 KB (16-bit) or 4.1 KB (8-bit) per warp at D = 128, two CTAs
   // per SM: 3 and 6 (96 KB a CTA); with two row tiles over 8-bit pages 4 (77.7
   // against 81.3 us for 32 x 5 rows).  Rows as columns: as many as the CTAs of
   // block_ctas have room for.
-  constexpr int kStages = (NT == 1 ? 3 : NT == 2 ? 4 : NT > 2 ? 5 : kE4m3 ? (MT == 2 ? 4 : 6) : 3) * (128 / D);
+  constexpr int kStages = (NT == 1 ? 3 : NT == 2 || NT == 3 ? 4 : NT > 3 ? 5 : kE4m3 ? (MT == 2 ? 4 : 6) : 3) * (128 / D);
   constexpr int TR = NT > 0 ? 8 * NT : 16 * MT;
   constexpr int kSmem = RingBytes<D, TR, kE4m3, kStages, (NT > 0)>::kBytes +
                         (NT > 2 ? NT * (D / 16) * 256 : NT == 0 && MT == 2 ? MT * (D / 16) * 512 : 0);
@@ -1057,9 +1093,7 @@ cudaError_t attention_launch(PagedAttention a, int max_new, cudaStream_t st) {
   cudaError_t e = prepare_kernel(done, k, kSmem, 0);
   if (e != cudaSuccess) return e;
   const int ctas = kCtas * sms;
-  static_assert(kCtas * (2 * sizeof(int4) + 2 * sizeof(float) * Part<TR, D>::kFloats) <=
-                    kCtasPerSm * (2 * sizeof(int4) + 2 * sizeof(float) * Part<32, D>::kFloats),
-                "workspace");
+  static_assert(kCtas * (2 * sizeof(int4) + 2 * sizeof(float) * Part<TR, D>::kFloats) <= sm_ws_bytes(D), "workspace");
   a.part = reinterpret_cast<float*>(a.desc + 2 * ctas);
   e = launch_paged(k, dim3(ctas), dim3(kThreads), kSmem, 1, false, st, a);
   if (e != cudaSuccess) return e;
@@ -1088,10 +1122,7 @@ cudaError_t attention_dim(const PagedAttention& a, int max_new, cudaStream_t st)
 
 }  // namespace
 
-size_t paged_attention_ws_bytes(int D) {
-  const size_t ctas = static_cast<size_t>(kCtasPerSm) * sm_count();
-  return ctas * 2 * sizeof(int4) + ctas * 2 * (32 * static_cast<size_t>(D) + 64) * sizeof(float);
-}
+size_t paged_attention_ws_bytes(int D) { return static_cast<size_t>(sm_count()) * sm_ws_bytes(D); }
 
 cudaError_t launch_paged_attention(PagedAttention a, int dtype, int max_new, void* workspace, cudaStream_t st) {
   a.desc = static_cast<int4*>(workspace);  // the parts behind it, by the form's number of CTAs
