@@ -140,7 +140,6 @@ __global__ void __launch_bounds__(kWriteThreads, 12) paged_write_kernel(const __
 }
 
 // ---- 8-bit pages with a scale per block ----
-constexpr int kBlockThreads = 128;
 
 // The smallest power of two s with amax <= 448 s (448 = 1.75 2^8), from
 // kMinScale up to 2^120.
@@ -171,17 +170,22 @@ __device__ __forceinline__ int find_run_seq(const int32_t* indptr, int B, int sh
 }
 
 // One CTA per run and slice of the heads (gridDim.y of them).  D / 16 lanes
-// take one head as in paged_write_kernel; for k and v they go over the run's
-// rows twice: once for the block's maximum, once to write the codes (the second
-// read comes out of the caches).  The scale is a power of two, so codes lose
-// nothing by it (8-bit floats), it can grow with the block, and the codes of
-// the block's earlier tokens move to the larger one exactly unless they fall
-// below the smallest normal code.  The angles of every row are made once per
-// CTA.
-template <typename T, int D>
-__global__ void __launch_bounds__(kBlockThreads) paged_block_write_kernel(const __grid_constant__ PagedWrite a, int32_t* err) {
-  constexpr int kLanes = D / 16, kGroups = kBlockThreads / kLanes;
-  extern __shared__ float2 s_turn[];  // [rows of the run][D / 2]: cosine and sine
+// take one row of one head as in paged_write_kernel.  k and v are gone over
+// twice: for the block's maxima, and to write the codes (the second read comes
+// out of the caches).  The scale is a power of two, so codes lose nothing by it
+// (8-bit floats), it can grow with the block, and the codes of the block's
+// earlier tokens move to the larger one exactly unless they fall below the
+// smallest normal code.  The angles of every row are made once per CTA.
+// Measured: 8000 rows of 32 + 2 x 8 heads 52 us in blocks of 8 to 64, 57 in
+// blocks of 128 (0.53 of the measured HBM rate; 16000 rows 0.61): every CTA
+// is resident at once, so all of them wait for the same chain of reads, then
+// for the angles.  With 40 registers a thread 72 us, with 100 64.
+template <typename T, int D, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) paged_block_write_kernel(const __grid_constant__ PagedWrite a, int32_t* err) {
+  constexpr int kLanes = D / 16, kGroups = kThreads / kLanes;
+  extern __shared__ float2 s_turn[];  // [rows of the run][D / 2]: cosine and sine; then by k and v head of the slice:
+  int* const s_amax = reinterpret_cast<int*>(s_turn + (D / 2 << a.c.scale_shift));  // maximum, as bits
+  float2* const s_scale = s_turn + (D / 2 << a.c.scale_shift) + a.c.Hkv;            // new scale, and old over new
   pdl_wait();
   pdl_launch();
   const PagedCache& c = a.c;
@@ -208,12 +212,15 @@ __global__ void __launch_bounds__(kBlockThreads) paged_block_write_kernel(const 
   const int cnt = static_cast<int>(p1 - p0), at = static_cast<int>(p0 - pi * c.page_size);
   const int older = static_cast<int>(p0 - blk0);  // tokens of the block from before the call
   const int64_t r0 = p0 + row_of;
-  for (int x = threadIdx.x; x < cnt * (D / 2); x += kBlockThreads) {
+  const int slices = static_cast<int>(gridDim.y), slice = blockIdx.y;
+  const int units = 2 * c.Hkv, mine = (units - slice + slices - 1) / slices;  // k and v heads: slice, slice + slices, ...
+  for (int x = threadIdx.x; x < cnt * (D / 2); x += kThreads) {
     const double t = static_cast<double>(p0 + x / (D / 2)) * a.turns[x % (D / 2)];
     float sn, cs;
     sincospif(2.f * static_cast<float>(t - rint(t)), &sn, &cs);
     s_turn[x] = make_float2(cs, sn);
   }
+  for (int x = threadIdx.x; x < mine; x += kThreads) s_amax[x] = 0;
   __syncthreads();
   const int i = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   auto load = [&](const PagedRows& src, int j, int h, bool turn, float (&lo)[8], float (&hi)[8]) {
@@ -222,67 +229,88 @@ __global__ void __launch_bounds__(kBlockThreads) paged_block_write_kernel(const 
     unpack8<T>(*reinterpret_cast<const uint4*>(x + D / 2 + 8 * i), hi);
     if (turn) {
 #pragma unroll
-      for (int z = 0; z < 8; ++z) {
-        const float2 w = s_turn[j * (D / 2) + 8 * i + z];
-        const float x1 = lo[z], x2 = hi[z];
+      for (int z = 0; z < 8; z += 2) {
+        const float4 w = *reinterpret_cast<const float4*>(&s_turn[j * (D / 2) + 8 * i + z]);
+        const float x1 = lo[z], x2 = hi[z], y1 = lo[z + 1], y2 = hi[z + 1];
         lo[z] = fmaf(x1, w.x, -x2 * w.y);
         hi[z] = fmaf(x2, w.x, x1 * w.y);
+        lo[z + 1] = fmaf(y1, w.z, -y2 * w.w);
+        hi[z + 1] = fmaf(y2, w.z, y1 * w.w);
       }
     }
   };
   float lo[8], hi[8];
-  const int64_t page_at = static_cast<int64_t>(pg) * c.page_stride;
-  const int units = 2 * c.Hkv, slices = static_cast<int>(gridDim.y);
-  for (int u0 = blockIdx.y; u0 < units; u0 += kGroups * slices) {  // uniform trips: the lanes of a warp shuffle together
-    const int u = u0 + group * slices;
-    const bool live = u < units, is_v = u >= c.Hkv;
-    const int h = is_v ? u - c.Hkv : u;
-    const PagedRows& src = is_v ? a.v : a.k;
+  // ---- the maxima of the block's new rows ----
+#pragma unroll 2
+  for (int x0 = 0; x0 < mine * cnt; x0 += kGroups) {  // uniform trips: the lanes of a warp shuffle together
+    const int x = x0 + group, u = x / cnt, j = x - u * cnt, uu = slice + u * slices;
+    const bool live = x < mine * cnt, is_v = uu >= c.Hkv;
     float amax = 0.f;
-    for (int j = 0; live && j < cnt; ++j) {
-      load(src, j, h, !is_v, lo, hi);
+    if (live) {
+      load(is_v ? a.v : a.k, j, is_v ? uu - c.Hkv : uu, !is_v, lo, hi);
 #pragma unroll
       for (int z = 0; z < 8; ++z) amax = fmaxf(amax, fmaxf(fabsf(lo[z]), fabsf(hi[z])));
     }
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    float* const sc = (is_v ? c.v_scale : c.k_scale) + pg * c.scale_page_stride + (at >> c.scale_shift) +
-                      static_cast<int64_t>(live ? h : 0) * c.scale_head_stride;
-    const float old = live && older > 0 ? *sc : 0.f;
-    __syncwarp();  // every lane has the old scale
-    if (!live) continue;
-    const float scale = fmaxf(old, two_power(amax)), inv = 1.f / scale;
-    uint8_t* o = static_cast<uint8_t*>(is_v ? c.v : c.k) + page_at + at * c.pos_stride + static_cast<int64_t>(h) * c.head_stride + 8 * i;
-    if (older > 0 && scale > old) {
-      const float ratio = old / scale;
-      for (int j = -older; j < 0; ++j)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint2* w = reinterpret_cast<uint2*>(o + j * c.pos_stride + half * (D / 2));
-          const uint2 v = *w;
-          uint32_t x[4];
-          e4m3x4_to_half(v.x, x[0], x[1]);
-          e4m3x4_to_half(v.y, x[2], x[3]);
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const float2 f = Cvt<__half>::to2(x[z]);
-            lo[2 * z] = f.x * ratio;
-            lo[2 * z + 1] = f.y * ratio;
-          }
-          *w = make_uint2(to_e4m3x2(lo[0], lo[1]) | static_cast<uint32_t>(to_e4m3x2(lo[2], lo[3])) << 16,
-                          to_e4m3x2(lo[4], lo[5]) | static_cast<uint32_t>(to_e4m3x2(lo[6], lo[7])) << 16);
-        }
-    }
-    for (int j = 0; j < cnt; ++j, o += c.pos_stride) {
-      load(src, j, h, !is_v, lo, hi);
-      *reinterpret_cast<uint2*>(o) = pack8_e4m3(lo, scale, inv);
-      *reinterpret_cast<uint2*>(o + D / 2) = pack8_e4m3(hi, scale, inv);
-    }
-    if (i == 0) *sc = scale;
+    if (live && i == 0) atomicMax(&s_amax[u], __float_as_int(amax));
   }
-  for (int x = group; x < cnt * a.Hq; x += kGroups) {
-    const int j = x / a.Hq, h = x % a.Hq;
-    if (h % slices != static_cast<int>(blockIdx.y)) continue;
+  __syncthreads();
+  const int64_t scale_at = pg * c.scale_page_stride + (at >> c.scale_shift);
+  bool grown = false;
+  for (int u = threadIdx.x; u < mine; u += kThreads) {
+    const int uu = slice + u * slices;
+    const bool is_v = uu >= c.Hkv;
+    float* const sc = (is_v ? c.v_scale : c.k_scale) + scale_at + static_cast<int64_t>(is_v ? uu - c.Hkv : uu) * c.scale_head_stride;
+    const float old = older > 0 ? *sc : 0.f, scale = fmaxf(old, two_power(__int_as_float(s_amax[u])));
+    *sc = scale;
+    s_scale[u] = make_float2(scale, older > 0 && scale > old ? old / scale : 1.f);
+    grown |= older > 0 && scale > old;
+  }
+  const bool again = __syncthreads_or(grown);
+  uint8_t *const k_at = static_cast<uint8_t*>(c.k) + static_cast<int64_t>(pg) * c.page_stride + at * c.pos_stride + 8 * i,
+          *const v_at = static_cast<uint8_t*>(c.v) + static_cast<int64_t>(pg) * c.page_stride + at * c.pos_stride + 8 * i;
+  // ---- the codes of the new rows ----
+#pragma unroll 2
+  for (int x = group; x < mine * cnt; x += kGroups) {
+    const int u = x / cnt, j = x - u * cnt, uu = slice + u * slices;
+    const bool is_v = uu >= c.Hkv;
+    const int h = is_v ? uu - c.Hkv : uu;
+    load(is_v ? a.v : a.k, j, h, !is_v, lo, hi);
+    const float scale = s_scale[u].x, inv = 1.f / scale;
+    uint8_t* o = (is_v ? v_at : k_at) + static_cast<int64_t>(h) * c.head_stride + j * c.pos_stride;
+    *reinterpret_cast<uint2*>(o) = pack8_e4m3(lo, scale, inv);
+    *reinterpret_cast<uint2*>(o + D / 2) = pack8_e4m3(hi, scale, inv);
+  }
+  // ---- those of the block's earlier tokens, where its scale has grown ----
+  for (int x = group; again && x < mine * older; x += kGroups) {
+    const int u = x / older, j = x - u * older - older, uu = slice + u * slices;
+    const float ratio = s_scale[u].y;
+    if (ratio == 1.f) continue;
+    const bool is_v = uu >= c.Hkv;
+    uint8_t* o = (is_v ? v_at : k_at) + static_cast<int64_t>(is_v ? uu - c.Hkv : uu) * c.head_stride + j * c.pos_stride;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint2* w = reinterpret_cast<uint2*>(o + half * (D / 2));
+      const uint2 v = *w;
+      uint32_t y[4];
+      e4m3x4_to_half(v.x, y[0], y[1]);
+      e4m3x4_to_half(v.y, y[2], y[3]);
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const float2 f = Cvt<__half>::to2(y[z]);
+        lo[2 * z] = f.x * ratio;
+        lo[2 * z + 1] = f.y * ratio;
+      }
+      *w = make_uint2(to_e4m3x2(lo[0], lo[1]) | static_cast<uint32_t>(to_e4m3x2(lo[2], lo[3])) << 16,
+                      to_e4m3x2(lo[4], lo[5]) | static_cast<uint32_t>(to_e4m3x2(lo[6], lo[7])) << 16);
+    }
+  }
+  // ---- q ----
+  const int heads = (a.Hq - slice + slices - 1) / slices;
+#pragma unroll 2
+  for (int x = group; x < heads * cnt; x += kGroups) {
+    const int j = x / heads, h = slice + (x - j * heads) * slices;
     load(a.q, j, h, true, lo, hi);
     T* o = static_cast<T*>(a.q_out.p) + (r0 + j) * a.q_out.row_stride + static_cast<int64_t>(h) * a.q_out.head_stride;
     *reinterpret_cast<uint4*>(o + 8 * i) = pack8<T>(lo);
@@ -347,16 +375,28 @@ cudaError_t write_for(const PagedWrite& a, int32_t* err, cudaStream_t st) {
                         : (e ? paged_write_kernel<T, 64, true> : paged_write_kernel<T, 64, false>);
   return launch_paged(k, dim3(a.rows), dim3(kWriteThreads), 0, 1, true, st, a, err);
 }
+template <typename T, int D, int kThreads>
+cudaError_t block_write_launch(const PagedWrite& a, int slices, int32_t* err, cudaStream_t st) {
+  auto k = paged_block_write_kernel<T, D, kThreads>;
+  // angles; maxima, scales and ratios by head
+  const int smem = ((D / 2 << a.c.scale_shift) + 3 * a.c.Hkv) * static_cast<int>(sizeof(float2));
+  static std::atomic<bool> done[64];
+  const cudaError_t e = prepare_kernel(done, k, ((64 << 7) + 3 * 1024) * static_cast<int>(sizeof(float2)), 0);
+  if (e != cudaSuccess) return e;
+  const int64_t runs = (a.rows >> a.c.scale_shift) + 2 * static_cast<int64_t>(a.c.B);
+  return launch_paged(k, dim3(static_cast<unsigned>(runs), slices), dim3(kThreads), smem, 1, true, st, a, err);
+}
+template <typename T, int D>
+cudaError_t block_write_dim(const PagedWrite& a, int32_t* err, cudaStream_t st) {
+  // Threads by the block's size, and few slices, since each makes the angles anew.
+  const int block = 1 << a.c.scale_shift;
+  return block < 32   ? block_write_launch<T, D, 128>(a, block < 16 ? 1 : 2, err, st)
+         : block < 64 ? block_write_launch<T, D, 128>(a, 4, err, st)
+                      : block_write_launch<T, D, 512>(a, block < 128 ? 2 : 4, err, st);
+}
 template <typename T>
 cudaError_t block_write_for(const PagedWrite& a, int32_t* err, cudaStream_t st) {
-  auto k = a.c.D == 128 ? paged_block_write_kernel<T, 128> : paged_block_write_kernel<T, 64>;
-  const int smem = (a.c.D / 2 << a.c.scale_shift) * static_cast<int>(sizeof(float2));
-  static std::atomic<bool> done[2][64];
-  const cudaError_t e = prepare_kernel(done[a.c.D == 128], k, (64 << 7) * static_cast<int>(sizeof(float2)), 0);
-  if (e != cudaSuccess) return e;
-  const int slices = a.c.scale_shift > 4 ? 1 << (a.c.scale_shift - 4) : 1;
-  const int64_t runs = (a.rows >> a.c.scale_shift) + 2 * static_cast<int64_t>(a.c.B);
-  return launch_paged(k, dim3(static_cast<unsigned>(runs), slices), dim3(kBlockThreads), smem, 1, true, st, a, err);
+  return a.c.D == 128 ? block_write_dim<T, 128>(a, err, st) : block_write_dim<T, 64>(a, err, st);
 }
 template <typename T>
 cudaError_t read_for(const PagedRead& a, int32_t* err, cudaStream_t st) {
