@@ -9,6 +9,10 @@ replay per new token, greedy inside the graph (the reference's
 ``decode_step_greedy`` / ``sample_next_token`` semantics; rows that sample
 at a temperature overwrite the greedy token from the step's logits).
 Prompts are token ids: this build ships no tokenizer.
+
+``run_ragged_generate`` takes prompts of any lengths, each request with its own
+parameters and budget, over a paged cache, and decodes in a captured step that
+plans its pages and draws its tokens on the device.
 """
 
 from __future__ import annotations
@@ -20,7 +24,7 @@ import torch
 
 from persona.adapter_pool import AdapterCache, AdapterPool
 from persona.mistral import MistralLoRAModel
-from persona.sampling import SamplingParams, sample_next_token
+from persona.sampling import BatchSampling, SamplingParams, sample_batch, sample_next_token
 
 
 @dataclass
@@ -101,6 +105,48 @@ class StaticBatchEngine:
         new = len(requests) * max_new_tokens
         return {"tokens": out.cpu(), "prefill_ms": prefill_ms, "decode_ms": decode_ms, "new_tokens": new,
                 "tok_per_s": new / ((prefill_ms + decode_ms) * 1e-3)}
+
+    @torch.inference_mode()
+    def run_ragged_generate(self, requests: Sequence[Request], max_new_tokens: int = 128, use_cuda_graph: bool = True,
+                            kv_dtype: torch.dtype = torch.float16, kv_block: int = 1, page_size: int = 16,
+                            num_pages: Optional[int] = None, generator: Optional[torch.Generator] = None) -> dict:
+        """Generate up to ``max_new_tokens`` (and the request's own
+        ``max_tokens``) per request, prompts of any lengths; returns the new
+        token ids as a list per request, and device times as
+        ``run_static_generate``.  ``num_pages``: of the cache (default: what all
+        requests need at their longest)."""
+        slots = self.plan_batch(requests)
+        budget = [min(max_new_tokens, r.sampling.max_tokens) for r in requests]
+        if not requests or min(budget) < 1 or any(len(r.prompt) == 0 for r in requests):
+            raise ValueError("every request has a prompt and a budget")
+        longest = max(len(r.prompt) + n for r, n in zip(requests, budget))
+        if longest > self.max_seq_len:
+            raise ValueError("prompt + new tokens exceed max_seq_len")
+        if num_pages is None:
+            num_pages = sum(-(-(len(r.prompt) + n) // page_size) for r, n in zip(requests, budget))
+        st = self.model.new_paged_state(slots, num_pages, page_size, longest, kv_dtype, kv_block)
+        sampling = BatchSampling([r.sampling for r in requests], self.device)
+        B, steps = len(requests), max(budget)
+        out = torch.zeros(B, steps, dtype=torch.int64, device=self.device)
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
+        ev[0].record()
+        logits, indptr = self.model.extend(st, [list(r.prompt) for r in requests])
+        first = sample_batch(logits.index_select(0, indptr[1:] - 1), sampling, generator=generator)
+        dec = self.model.start_decode(st, first, sampling)
+        out[:, 0] = first
+        ev[1].record()
+        for i in range(1, steps):
+            ended = [b for b in range(B) if budget[b] == i]
+            if ended:
+                dec.alive[ended] = 0
+            out[:, i] = self.model.paged_step(dec, use_graph=use_cuda_graph, generator=generator)
+        ev[2].record()
+        self.model.finish_decode(dec)
+        prefill_ms = ev[0].elapsed_time(ev[1])
+        decode_ms = ev[1].elapsed_time(ev[2])
+        tokens = [row[:n] for row, n in zip(out.tolist(), budget)]
+        return {"tokens": tokens, "prefill_ms": prefill_ms, "decode_ms": decode_ms, "new_tokens": sum(budget),
+                "tok_per_s": sum(budget) / ((prefill_ms + decode_ms) * 1e-3)}
 
     @staticmethod
     def _next(logits: torch.Tensor, requests: Sequence[Request], sampled: List[int]) -> torch.Tensor:

@@ -16,7 +16,9 @@ package's kernels:
 * LoRA: ``ops.bgmv_fused_multi`` on a plan computed once per batch at decode;
   ``ops.sgmv_fused`` over the request segments at prefill;
 * ragged chunks over a paged cache (``extend``): ``ops.paged_rope_cache`` and
-  ``ops.paged_attention``, LoRA over the sequences as segments;
+  ``ops.paged_attention``, LoRA over the sequences as segments; single tokens
+  over it (``start_decode``, ``paged_step``) in a captured step that finds its
+  pages by ``ops.paged_plan`` and its tokens by ``ops.sample_tokens``;
 * the rest: ``ops.add_rmsnorm`` (residual add fused into the
   next norm), ``rope_cache`` (rotary embedding + KV-cache write) at prefill,
   ``rope_decode_attention`` (the same and the attention, one launch) at
@@ -38,6 +40,7 @@ import torch.nn.functional as F
 
 from persona import nf4, ops
 from persona.adapter_pool import AdapterPool
+from persona.sampling import BatchSampling
 
 @dataclass
 class MistralConfig:
@@ -100,15 +103,21 @@ class PagedState:
     page_table: torch.Tensor      # [B, max_pages] int32
     k_cache: List[torch.Tensor]   # per layer [pages, Hkv, page_size, 128], fp16 or e4m3
     v_cache: List[torch.Tensor]
-    k_scale: List[Optional[torch.Tensor]]  # per layer [pages, Hkv, page_size], e4m3 only
+    k_scale: List[Optional[torch.Tensor]]  # per layer [pages, Hkv, page_size or blocks of a page], e4m3 only
     v_scale: List[Optional[torch.Tensor]]
     lengths: List[int]            # cached tokens per sequence
     pages: List[List[int]]        # pages held by each sequence
     free: List[int]
+    decode: Optional["PagedDecode"] = field(default=None, repr=False, compare=False)  # while the device keeps the lengths and the pages
+
+    def _host(self) -> None:
+        if self.decode is not None:
+            raise ValueError("the sequences are being decoded (finish_decode first)")
 
     def set_length(self, b: int, length: int) -> None:
         """Sequence b keeps its first ``length`` tokens (rejected drafts, or 0
         to start over); pages behind them are free again."""
+        self._host()
         if not 0 <= length <= self.lengths[b]:
             raise ValueError("a sequence can only be cut back")
         keep = -(-length // self.page_size)
@@ -141,6 +150,28 @@ class PagedState:
             for b, p in enumerate(self.pages):
                 host[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
             self.page_table.copy_(host)
+
+
+@dataclass
+class PagedDecode:
+    """A ``PagedState`` whose next tokens are made one a step without the host:
+    lengths, pages and free list are device arrays that the step itself moves on."""
+
+    st: PagedState
+    sampling: BatchSampling
+    tok: torch.Tensor       # [B + 1] int64: the token that each sequence feeds next (and a place for padded rows)
+    alive: torch.Tensor     # [B] int32: 1 gets a token a step; 0 has ended, its pages go back with the next step
+    u: torch.Tensor         # [B] fp32: the numbers that the next step draws with
+    lengths: torch.Tensor   # [B] int32
+    keep: torch.Tensor      # [B] int32
+    free: torch.Tensor      # [pages] int32, the first num_free of them free
+    num_free: torch.Tensor  # [1] int32
+    indptr: torch.Tensor    # [B + 1] int32
+    places: torch.Tensor    # [B] int64
+    seqs: torch.Tensor      # [B] int32: 0 .. B - 1
+    row_seq: torch.Tensor   # [B] int32: the sequence of each row, -1 behind the last
+    bufs: dict = field(default_factory=dict)
+    graph: Optional[torch.cuda.CUDAGraph] = None
 
 
 class MistralLoRAModel:
@@ -262,16 +293,19 @@ class MistralLoRAModel:
 
     # ---- ragged chunks over a paged cache --------------------------------------
     def new_paged_state(self, slots: torch.Tensor, num_pages: int, page_size: int = 16, max_seq: int = 4096,
-                        kv_dtype: torch.dtype = torch.float16) -> PagedState:
+                        kv_dtype: torch.dtype = torch.float16, kv_block: int = 1) -> PagedState:
         """Empty sequences, one per adapter slot of ``slots``, over ``num_pages``
         pages per layer; ``kv_dtype`` fp16, or float8_e4m3fn with one scale per
-        token and head."""
+        ``kv_block`` tokens (1, 2, 4, ... 128, a divisor of the page) and head."""
         cfg, d = self.cfg, self.device
         e4m3 = kv_dtype == torch.float8_e4m3fn
         if not e4m3 and kv_dtype != torch.float16:
             raise ValueError("paged caches are float16 or float8_e4m3fn")
+        if kv_block not in (1, 2, 4, 8, 16, 32, 64, 128) or page_size % kv_block or (kv_block > 1 and not e4m3):
+            raise ValueError("kv_block is a power of two up to 128 that divides the page, for float8_e4m3fn caches")
         B = int(slots.numel())
         shape = (num_pages, cfg.n_kv_heads, page_size, 128)
+        scales = (*shape[:2], page_size // kv_block)
 
         def per_layer(*size, dtype):
             return [torch.zeros(*size, dtype=dtype, device=d) for _ in range(cfg.num_layers)]
@@ -280,8 +314,8 @@ class MistralLoRAModel:
         return PagedState(slots=slots.to(d, torch.int32).contiguous(), page_size=page_size,
                           page_table=torch.zeros(B, -(-max_seq // page_size), dtype=torch.int32, device=d),
                           k_cache=per_layer(*shape, dtype=kv_dtype), v_cache=per_layer(*shape, dtype=kv_dtype),
-                          k_scale=per_layer(*shape[:3], dtype=torch.float32) if e4m3 else none,
-                          v_scale=per_layer(*shape[:3], dtype=torch.float32) if e4m3 else none,
+                          k_scale=per_layer(*scales, dtype=torch.float32) if e4m3 else none,
+                          v_scale=per_layer(*scales, dtype=torch.float32) if e4m3 else none,
                           lengths=[0] * B, pages=[[] for _ in range(B)], free=list(range(num_pages)))
 
     @torch.inference_mode()
@@ -291,6 +325,7 @@ class MistralLoRAModel:
         [B + 1] int32: sequence b's rows are indptr[b] .. indptr[b + 1] (what
         ``sampling.verify_drafts`` takes for chunks of a last token and drafts).
         A call that raises leaves the sequences as they were."""
+        st._host()
         new = [len(c) for c in chunks]
         if len(new) != len(st.lengths):
             raise ValueError("one chunk per sequence")
@@ -350,6 +385,122 @@ class MistralLoRAModel:
             delta = dn
         ops.add_rmsnorm(h, delta, self.final_norm, xn, cfg.rms_eps)
         return torch.matmul(xn, self.lm_head.t()), indptr
+
+    # ---- single tokens over a paged cache, without the host ----------------------
+    def start_decode(self, st: PagedState, tokens: torch.Tensor, sampling: BatchSampling) -> PagedDecode:
+        """Hands the sequences of ``st`` over to the device: ``tokens`` [B] are
+        what each feeds first, ``sampling`` how the next ones are drawn.  Until
+        ``finish_decode`` only ``paged_step`` moves them."""
+        st._host()
+        cfg, d = self.cfg, self.device
+        B, pages = len(st.lengths), st.k_cache[0].shape[0]
+        if tokens.shape != (B,) or sampling.temperature.shape != (B,):
+            raise ValueError("one token and one set of parameters per sequence")
+        i32 = dict(dtype=torch.int32, device=d)
+        free = torch.zeros(pages, **i32)
+        free[:len(st.free)] = torch.tensor(st.free, **i32)
+        dec = PagedDecode(st=st, sampling=sampling, tok=torch.zeros(B + 1, dtype=torch.int64, device=d),
+                          alive=torch.ones(B, **i32), u=torch.zeros(B, device=d),
+                          lengths=torch.tensor(st.lengths, **i32), keep=torch.zeros(B, **i32), free=free,
+                          num_free=torch.tensor([len(st.free)], **i32), indptr=torch.zeros(B + 1, **i32),
+                          places=torch.zeros(B, dtype=torch.int64, device=d), seqs=torch.arange(B, **i32),
+                          row_seq=torch.zeros(B, **i32))
+        dec.tok[:B].copy_(tokens)
+        f16 = dict(dtype=torch.float16, device=d)
+        dec.bufs = {n: torch.zeros(B, w, **f16) for n, w in
+                    dict(h=cfg.hidden, xn=cfg.hidden, q=cfg.q_dim, k=cfg.kv_dim, v=cfg.kv_dim, attn=cfg.q_dim,
+                         o=cfg.hidden, g=cfg.intermediate, u=cfg.intermediate, act=cfg.intermediate, d=cfg.hidden,
+                         logits=cfg.vocab).items()}
+        st.decode = dec
+        return dec
+
+    def finish_decode(self, dec: PagedDecode) -> None:
+        """The host has the sequences again (their lengths and pages are read
+        back).  A step that found no free page raises here, or in the next
+        operator's call; it and the steps behind it have changed nothing."""
+        st = dec.st
+        if st.decode is not dec:
+            raise ValueError("this decode is not the sequences' own")
+        torch.cuda.synchronize(self.device)
+        lengths, table, free = dec.lengths.tolist(), st.page_table.tolist(), dec.free[:int(dec.num_free)].tolist()
+        st.lengths[:] = lengths
+        st.pages[:] = [table[b][:-(-n // st.page_size)] for b, n in enumerate(lengths)]
+        st.free[:] = free
+        st.decode = None
+        ops.check_errors(self.device)
+
+    def _paged_body(self, dec: PagedDecode) -> None:
+        cfg, st, b = self.cfg, dec.st, dec.bufs
+        B = len(dec.seqs)
+        # ended sequences give their pages back, the others get a row and, where they need one, a page
+        torch.mul(dec.lengths, dec.alive, out=dec.keep)
+        ops.paged_plan(dec.alive, dec.lengths, st.page_table, dec.free, dec.num_free, st.page_size, dec.indptr, dec.places,
+                       keep=dec.keep, seq_slots=dec.seqs, row_slots=dec.row_seq)
+        seq = dec.row_seq.clamp_min(0)
+        slots = torch.where(dec.row_seq < 0, dec.row_seq, st.slots.index_select(0, seq))
+        plan = ops.bgmv_plan(slots, self.pool.max_slots)
+        torch.index_select(self.embed, 0, dec.tok.index_select(0, seq), out=b["h"])
+        scale = 1.0 / math.sqrt(128)
+        delta = None
+        for li, lw in enumerate(self.layers):
+            lora = self._lora[li]
+            kv = (st.k_cache[li], st.v_cache[li], st.page_table, dec.indptr, dec.lengths)
+            scales = dict(k_scale=st.k_scale[li], v_scale=st.v_scale[li])
+            ops.add_rmsnorm(b["h"], delta, lw.in_norm, b["xn"], cfg.rms_eps)
+            nf4.linear(b["xn"], [lw.q, lw.k, lw.v], outs=[b["q"], b["k"], b["v"]])
+            ops.bgmv_fused_multi([b["xn"]] * 3, [lora[m][0] for m in ("q_proj", "k_proj", "v_proj")],
+                                 [lora[m][1] for m in ("q_proj", "k_proj", "v_proj")], slots,
+                                 [b["q"], b["k"], b["v"]], plan=plan)
+            q, k, v, attn = (b[n].view(B, -1, 128) for n in ("q", "k", "v", "attn"))
+            ops.paged_rope_cache(q, k, v, *kv, cfg.rope_theta, **scales)
+            ops.paged_attention(q, *kv, attn, scale, max_new=1, **scales)
+            nf4.linear(b["attn"], [lw.o], outs=[b["o"]])
+            ops.bgmv_fused(b["attn"], *lora["o_proj"], slots, b["o"], plan=plan)
+            ops.add_rmsnorm(b["h"], b["o"], lw.post_norm, b["xn"], cfg.rms_eps)
+            nf4.linear(b["xn"], [lw.gate, lw.up], outs=[b["g"], b["u"]])
+            ops.bgmv_fused_multi([b["xn"]] * 2, [lora[m][0] for m in ("gate_proj", "up_proj")],
+                                 [lora[m][1] for m in ("gate_proj", "up_proj")], slots, [b["g"], b["u"]], plan=plan)
+            ops.silu_mul(b["g"], b["u"], b["act"])
+            nf4.linear(b["act"], [lw.down], outs=[b["d"]])
+            ops.bgmv_fused(b["act"], *lora["down_proj"], slots, b["d"], plan=plan)
+            delta = b["d"]
+        ops.add_rmsnorm(b["h"], delta, self.final_norm, b["xn"], cfg.rms_eps)
+        torch.matmul(b["xn"], self.lm_head.t(), out=b["logits"])
+        drawn = torch.empty(B, dtype=torch.int64, device=self.device)
+        ops.sample_tokens(b["logits"], dec.u.index_select(0, seq), drawn, **dec.sampling.rows(seq))
+        dec.tok.index_copy_(0, torch.where(dec.row_seq < 0, B, dec.row_seq).long(), drawn)
+
+    @torch.inference_mode()
+    def paged_step(self, dec: PagedDecode, use_graph: bool = True,
+                   generator: Optional[torch.Generator] = None) -> torch.Tensor:
+        """Every sequence that is alive feeds its token and draws the next one,
+        with numbers from ``generator`` (by sequence, whoever else is alive).
+        Returns ``dec.tok[:B]``, on the device (an ended sequence's stays what it was)."""
+        dec.u.uniform_(generator=generator)
+        B = len(dec.seqs)
+        if not use_graph:
+            self._paged_body(dec)
+            return dec.tok[:B]
+        if dec.graph is None:
+            # Warmed up on a side stream by a step in which nobody is alive, whose
+            # pages stay (nothing is written but the padded rows' own buffers).
+            alive, lengths, table = dec.alive.clone(), dec.lengths.clone(), dec.st.page_table.clone()
+            free, num_free = dec.free.clone(), dec.num_free.clone()
+            s = torch.cuda.Stream(self.device)
+            dec.alive.zero_()
+            s.wait_stream(torch.cuda.current_stream(self.device))
+            with torch.cuda.stream(s):
+                self._paged_body(dec)
+            torch.cuda.current_stream(self.device).wait_stream(s)
+            for to, was in ((dec.alive, alive), (dec.lengths, lengths), (dec.st.page_table, table), (dec.free, free),
+                            (dec.num_free, num_free)):
+                to.copy_(was)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                self._paged_body(dec)
+            dec.graph = g
+        dec.graph.replay()
+        return dec.tok[:B]
 
     # ---- decode --------------------------------------------------------------
     def _decode_body(self, st: DecodeState) -> None:

@@ -1,19 +1,22 @@
 """Per-request sampling parameters and next-token choice.
 
 The parameter set is the reference's (``persona/sampling.py:8-13``:
-temperature, top-p, a token budget).  The choice itself is written around
+temperature, top-p, a token budget) with top-k and min-p beside it.  The choice
+of ``sample_next_token`` is written around
 the Gumbel-max identity instead of an explicit draw from a renormalised
 distribution: ``argmax(z + G)`` with ``G`` i.i.d. standard Gumbel noise picks
 index ``i`` with probability ``softmax(z)_i``.  That needs no renormalisation,
 no ``multinomial`` and no host round trip, and a top-p cut becomes a mask on
 ``z`` (a per-row log-probability threshold), so every row of a batch is
-handled in one set of tensor ops on the device.
+handled in one set of tensor ops on the device.  Rows with parameters of their
+own, top-k or min-p go to ``ops.sample_tokens``, which draws from given uniform
+numbers (``sample_batch``).
 """
 
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -23,6 +26,45 @@ class SamplingParams:
     temperature: float = 0.0
     top_p: float = 1.0
     max_tokens: int = 128
+    top_k: int = 0      # 0: all
+    min_p: float = 0.0  # 0: off
+
+
+class BatchSampling:
+    """The parameters of a batch's rows as tensors on ``device``, what
+    ``ops.sample_tokens`` takes (None where no row uses one)."""
+
+    def __init__(self, params: Sequence[SamplingParams], device):
+        def column(name, dtype, used):
+            values = [getattr(p, name) for p in params]
+            return torch.tensor(values, dtype=dtype, device=device) if any(used(v) for v in values) else None
+
+        self.temperature = torch.tensor([p.temperature for p in params], dtype=torch.float32, device=device)
+        self.top_k = column("top_k", torch.int32, lambda k: k > 0)
+        self.top_p = column("top_p", torch.float32, lambda p: p < 1.0)
+        self.min_p = column("min_p", torch.float32, lambda m: m > 0)
+
+    def rows(self, index: Optional[torch.Tensor] = None) -> dict:
+        """Keyword arguments of ``ops.sample_tokens``, for the rows ``index`` of the batch."""
+        columns = dict(temperature=self.temperature, top_k=self.top_k, top_p=self.top_p, min_p=self.min_p)
+        return {n: c if c is None or index is None else c.index_select(0, index) for n, c in columns.items()}
+
+
+def sample_batch(logits: torch.Tensor, params, generator: Optional[torch.Generator] = None,
+                 u: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """logits [batch, vocab] on the GPU -> next token ids [batch] (int64), each
+    row by its own parameters (a ``BatchSampling`` or one ``SamplingParams`` per
+    row).  ``u`` [batch] fp32 are the uniform numbers the tokens are drawn with;
+    drawn from ``generator`` if not given."""
+    from persona import ops
+
+    if not isinstance(params, BatchSampling):
+        params = BatchSampling(params, logits.device)
+    B = logits.shape[0]
+    if u is None:
+        u = torch.rand(B, device=logits.device, generator=generator)
+    tokens = torch.empty(B, dtype=torch.int64, device=logits.device)
+    return ops.sample_tokens(logits, u, tokens, **params.rows())
 
 
 def _nucleus_mask(z: torch.Tensor, top_p: float) -> torch.Tensor:
@@ -49,10 +91,12 @@ def sample_next_token(logits: torch.Tensor, params: SamplingParams,
 
     Temperature 0 (or below) is greedy.  Otherwise the logits are divided by
     the temperature, cut to the top-p nucleus when ``top_p < 1``, and one
-    token per row is drawn by Gumbel-max.
+    token per row is drawn by Gumbel-max.  With top-k or min-p: ``sample_batch``.
     """
     if params.temperature <= 0:
         return logits.argmax(dim=-1)
+    if params.top_k > 0 or params.min_p > 0:
+        return sample_batch(logits, [params] * logits.shape[0], generator=generator)
     z = logits.float() / params.temperature
     if params.top_p < 1.0:
         z = _nucleus_mask(z, params.top_p)
@@ -75,6 +119,8 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, draft
     most probable token."""
     from persona import ops
 
+    if params.temperature > 0 and (params.top_k > 0 or params.min_p > 0):
+        raise ValueError("drafts are verified by temperature and top_p")
     rows, dev = target_logits.shape[0], target_logits.device
     B = indptr.numel() - 1
     if params.temperature <= 0:
