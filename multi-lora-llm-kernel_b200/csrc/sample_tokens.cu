@@ -14,7 +14,7 @@
 // Every condition but the draw keeps a beginning of the order, so a row is cut
 // at one (value, index) pair: a 64-bit number `pair` whose high half orders the
 // floats and whose low half is the index, counted down.  The pair is found by
-// counts of tokens in 2048 classes, first by distance from the maximum (1/128
+// counts of tokens in 2048 classes, first by distance from the maximum (1/64
 // of a power of two of weight each), then by pair: for top-k the class of the
 // k-th token; for top-p the classes in which the sum can pass its mark, by the
 // least and the largest weight that a class can have.  The tokens of those
@@ -42,7 +42,7 @@ constexpr int kList = 1024;     // pairs that are sorted at most
 constexpr int kWhole = 512;     // and of which the list is to hold all that are kept
 static_assert(static_cast<int64_t>(kMaxTiles - 2) * kTile * kMaxSplit >= PERSONA_VERIFY_MAX_VOCAB, "tiles");
 constexpr int kStepBits = 9, kSteps = 1 << kStepBits;  // of the table of powers, per power of two
-constexpr int kPerClass = 4;   // steps of a class: 1/128 of a power of two
+constexpr int kPerClass = 8;   // steps of a class: 1/64 of a power of two
 constexpr int kCopies = 320;     // tokens that a warp can copy
 static_assert(kSteps == kThreads && kWarps >= 2 * (kMaxSplit - 1), "a thread makes one power, two warps fetch a list");
 static_assert(kBinsEach == 4, "a thread reads its classes at once");
@@ -91,7 +91,7 @@ struct Row {
   int V, x0, w0, w1;  // w0, w1: the warp's tiles
   bool inf;    // a logit is +infinity: those that are count as 0, all others as none
   float top, least;  // the largest; the last one whose weight is a normal number
-  double rate;       // log2(e) / T
+  double rate, unit;  // log2(e) / T, and one over it
 };
 
 struct Shared {
@@ -106,7 +106,7 @@ struct Shared {
   double wt[kList];
   double dsum[kWarps], part;
   u64 best, cut;
-  u64 copy[kWarps][kCopies];     // pairs, tile by tile
+  u64 copy[kWarps][kCopies];     // values and indexes, tile by tile
   uint16_t copied[kMaxTiles];    // and how many of the warp's up to and with a tile
   Row row[kWarps];
   float fmax[kWarps], top;
@@ -158,12 +158,15 @@ __device__ __forceinline__ void weights4(const Row& r, const double* power, cons
     w[i] = __hiloint2double(__double2hiint(v) - ((n[i] >> kStepBits) << 20), __double2loint(v));
   }
 }
+// One weight by itself.
 __device__ __forceinline__ double weight(const Row& r, const double* power, float x) {
-  const float f[4] = {x, x, x, x};
-  double w[4];
-  int n[4];
-  weights4(r, power, f, w, n);
-  return x >= r.least ? w[0] : 0.0;
+  constexpr double kShift = 6755399441055744.0, kLn2 = 0.69314718055994530942;
+  const double t = (static_cast<double>(x) - static_cast<double>(r.top)) * r.rate;
+  const double m = fma(t, -static_cast<double>(kSteps), kShift);
+  const int n = __double2loint(m);
+  const double p = power[n & (kSteps - 1)], f = fma(m - kShift, 1.0 / kSteps, t);
+  const double v = fma(p, fma(f, fma(f, kLn2 * kLn2 * kLn2 / 6, kLn2 * kLn2 / 2), kLn2) * f, p);
+  return x >= r.least ? __hiloint2double(__double2hiint(v) - ((n >> kStepBits) << 20), __double2loint(v)) : 0.0;
 }
 
 // fn(tile, index of the first, values) for the eight tokens a lane has of each
@@ -209,6 +212,14 @@ template <typename T> __device__ __forceinline__ float largest(const Raw<T>& raw
   }
 }
 
+template <typename T> __device__ __forceinline__ float value_at(const Row& r, int i) {
+  if constexpr (sizeof(T) == 4) {
+    return __ldg(static_cast<const float*>(r.logits) + r.at + i);
+  } else {
+    return Cvt<T>::to1(__ldg(static_cast<const uint16_t*>(r.logits) + r.at + i));
+  }
+}
+
 // A comparison with a pair, most of it with its value.
 struct Border {
   float x;
@@ -235,7 +246,7 @@ __device__ __noinline__ void count_pass(u64 lo_pair, double& sum_out, int& tail_
   const Border lo(lo_pair);
   const bool ties = lo.at < static_cast<unsigned>(r.V);
   // (a class is known from 1 / 256 of a power of two of weight before its end)
-  const float least = fmaxf(r.least, __double2float_ru(static_cast<double>(r.top) - (kBins - 1.5) * kPerClass / kSteps / r.rate));
+  const float least = fmaxf(r.least, __double2float_ru(static_cast<double>(r.top) - (kBins - 1.5) * kPerClass / kSteps * r.unit));
   const uint32_t bins = smem_u32(sh.bins);
   double sum = 0.0;
   int tail = 0;
@@ -258,13 +269,13 @@ __device__ __noinline__ void count_pass(u64 lo_pair, double& sum_out, int& tail_
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const bool near = in[j] && f[h + j] >= least;
-        if (kWeighed && in[j] && f[h + j] >= r.least) sum += w[j];
+        const float v = in[j] ? f[h + j] : -INFINITY;
+        if (kWeighed && v >= r.least) sum += w[j];
         // (a predicated instruction: a branch for each costs more than the count)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %0, 0;\n\t@p red.shared.add.u32 [%1], 1;\n\t}" ::"r"(near ? 1u : 0u),
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ge.f32 p, %0, %1;\n\t@p red.shared.add.u32 [%2], 1;\n\t}" ::"f"(v), "f"(least),
                      "r"(bins + 4u * (static_cast<unsigned>(n[j]) / kPerClass))
                      : "memory");
-        tail += in[j] != near ? 1 : 0;
+        tail += in[j] && v < least ? 1 : 0;
       }
     }
   });
@@ -333,12 +344,10 @@ template <typename T> __device__ __noinline__ int copy_pass(u64 lo_pair) {
       if (lane >= o) inc += up;
     }
     int at = n + inc - own;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (mine >> i & 1) {
-        if (at < kCopies) to[at] = pair_of(f[i], x + i);
-        ++at;
-      }
+    for (; mine != 0; mine &= mine - 1, ++at) {  // two or three rounds; the values once more, out of the caches
+      const int i = x + __ffs(mine) - 1;
+      if (at < kCopies) to[at] = static_cast<u64>(__float_as_uint(r.inf ? 0.f : value_at<T>(r, i))) << 32 | static_cast<uint32_t>(i);
+    }
     n += __shfl_sync(0xffffffffu, inc, 31);
     if (lane == 0) sh.copied[t] = static_cast<uint16_t>(min(n, kCopies));
   });
@@ -353,10 +362,11 @@ __device__ __noinline__ void split_copies(u64 hi, bool weighed, int n, double& s
   double sum = 0.0;
   int over = 0;
   for (int i = threadIdx.x & 31; i < n; i += 32) {
-    const u64 p = from[i];
+    const float x = __uint_as_float(static_cast<uint32_t>(from[i] >> 32));
+    const u64 p = pair_of(x, static_cast<int>(from[i]));
     if (p > hi) {
       ++over;
-      if (weighed) sum += weight(r, sh.power, value_of(static_cast<uint32_t>(p >> 32)));
+      if (weighed) sum += weight(r, sh.power, x);
     } else {
       const int at = atomicAdd(&sh.count, 1);
       if (at < kList) sh.list[at] = p;
@@ -369,6 +379,7 @@ __device__ __noinline__ void split_copies(u64 hi, bool weighed, int n, double& s
 __device__ __noinline__ void draw_copies(u64 heavy, float least, double& sum_out) {
   Shared& sh = shared();
   const Row r = sh.row[threadIdx.x >> 5];
+  const Border lo(heavy);
   const int lane = threadIdx.x & 31;
   const u64* const from = sh.copy[threadIdx.x >> 5];
   double sum = 0.0;
@@ -376,9 +387,8 @@ __device__ __noinline__ void draw_copies(u64 heavy, float least, double& sum_out
     const int i1 = sh.copied[t];
     double s = 0.0;
     for (int i = i0 + lane; i < i1; i += 32) {
-      const u64 p = from[i];
-      const float x = value_of(static_cast<uint32_t>(p >> 32));
-      if (p >= heavy && x >= least) s += weight(r, sh.power, x);
+      const float x = __uint_as_float(static_cast<uint32_t>(from[i] >> 32));
+      if (x >= least && lo.upto(x, static_cast<int>(from[i]))) s += weight(r, sh.power, x);
     }
     i0 = i1;
     s = warp_sum(s);
@@ -423,18 +433,29 @@ __device__ __noinline__ void sort_list(int n) {
   u64 *const list = sh.list, *const sorted = sh.sorted;
   const int tid = threadIdx.x;
   if (n <= kThreads) {
+    // as many threads an element as there are, each for a part of the others
+    int* const rank = reinterpret_cast<int*>(sh.wt);
+    const int share = n <= 64 ? 8 : n <= 128 ? 4 : n <= 256 ? 2 : 1, own = kThreads / share;
+    if (tid < n) rank[tid] = 0;
     if (tid == 0 && (n & 1)) list[n] = 0;  // (n < kList)
     __syncthreads();
-    if (tid < n) {
-      const u64 p = list[tid];
-      int rank = 0;
+    const int e = tid % own, part = tid / own, pairs = (n + 1) / 2;
+    const u64 p = e < n ? list[e] : 0;
+    if (e < n) {
+      int larger = 0;
 #pragma unroll 4
-      for (int j = 0; j < n; j += 2) {
-        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(list + j);
-        rank += (q.x > p ? 1 : 0) + (q.y > p ? 1 : 0);
+      for (int j = pairs * part / share; j < pairs * (part + 1) / share; ++j) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(list + 2 * j);
+        larger += (q.x > p ? 1 : 0) + (q.y > p ? 1 : 0);
       }
-      sorted[rank] = p;
+      if (share == 1) {
+        rank[e] = larger;
+      } else {
+        atomicAdd(&rank[e], larger);
+      }
     }
+    __syncthreads();
+    if (tid < n) sorted[rank[tid]] = p;
     __syncthreads();
     return;
   }
@@ -460,6 +481,16 @@ __device__ __noinline__ void sort_list(int n) {
       }
     }
 }
+// Sum over the lanes up to and with this one.
+template <typename F> __device__ __forceinline__ F scan_lanes(F v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const F up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
 // Running sums of wt[0 .. n) in place (every entry the sum up to and with it).
 __device__ __noinline__ void running_sums(int n) {
   Shared& sh = shared();
@@ -471,9 +502,8 @@ __device__ __noinline__ void running_sums(int n) {
   const double inc = warp_scan(s);
   if ((tid & 31) == 31) warps[warp] = inc;
   __syncthreads();
-  double run = inc - s;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) run += w < warp ? warps[w] : 0.0;
+  const double to = warp_scan((tid & 31) < kWarps ? warps[tid & 31] : 0.0);
+  double run = inc - s + (warp > 0 ? __shfl_sync(0xffffffffu, to, max(warp - 1, 0)) : 0.0);
   for (int i = i0; i < i1; ++i) {
     run += wt[i];
     wt[i] = run;
@@ -512,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
       static_cast<int>(((reinterpret_cast<uintptr_t>(a.logits) + static_cast<uint64_t>(row) * kSize) & 15) / kSize);
   const int all = (a.V + lead + kTile - 1) / kTile, per = (all + split - 1) / split;
   const int t0 = min(all, rank * per), tiles = min(all, t0 + per) - t0;
-  Row r{a.logits, row, a.V, t0 * kTile - lead, tiles * warp / kWarps, tiles * (warp + 1) / kWarps, false, 0.f, 0.f, 0.0};
+  Row r{a.logits, row, a.V, t0 * kTile - lead, tiles * warp / kWarps, tiles * (warp + 1) / kWarps, false, 0.f, 0.f, 0.0, 0.0};
   auto barrier = [&] {
     if (split > 1) {
       cluster.sync();
@@ -586,7 +616,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
   const double top64 = top, rate = 1.4426950408889634074 / static_cast<double>(temp);  // log2(e) / T
   r.top = top;
   r.rate = rate;
-  r.least = fmaxf(__double2float_ru(top64 - 1000.0 / rate), -3.4028234663852886e38f);
+  const double unit = static_cast<double>(temp) * 0.69314718055994530942;  // logits to half the weight: 1 / rate
+  r.least = fmaxf(__double2float_ru(top64 - 1000.0 * unit), -3.4028234663852886e38f);
+  r.unit = unit;
   if (lane == 0) {
     Row& to = sh.row[warp];
     to.logits = r.logits;
@@ -599,6 +631,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
     to.top = top;
     to.least = r.least;
     to.rate = rate;
+    to.unit = unit;
   }
   __syncwarp();
   const u64 best = static_cast<u64>(key_of(top)) << 32 | 0xffffffffu;  // no pair is larger
@@ -609,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
     const double min_w = fmin(static_cast<double>(want_m), 1.0);
     u64 lo = 0, hi = key_of(top);  // in keys: too light, heavy enough
     {
-      const double about = top64 + log2(min_w) / rate, off = (fabs(about) + fabs(top64)) * 1e-6 + 1e-6 / rate;
+      const double about = top64 + log2(min_w) * unit, off = (fabs(about) + fabs(top64)) * 1e-6 + 1e-6 * unit;
       const float x0 = __double2float_rd(about - off), x1 = __double2float_ru(about + off);
       if (x0 > -3.4e38f && x0 < top) lo = key_of(x0 + 0.f);
       if (x1 < top) hi = key_of(x1 + 0.f);
@@ -669,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
     const bool by_k = need_k;
     u64 lo = cut != 0 ? cut : 1, hi = best;  // where the cut can lie (0 is no token)
     bool linear = true;
-    const double width = kPerClass / (kSteps * rate);  // of a linear class, in logits
+    const double width = static_cast<double>(kPerClass) / kSteps * unit;  // of a linear class, in logits
     while (true) {
       const int bits = max(0, 64 - __clzll(static_cast<long long>(hi - lo)) - 11);  // (hi - lo) >> bits < 2^11
 
@@ -721,6 +754,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
       for (int i = tid; i < kBins / 2; i += kThreads) sh.slice[i] = 0;
       // Pairs of a class, largest and least.  The linear ones end half a step off
       // their distances; a little more allows for roundings.
+      const int end_class = linear ? kBins - 1 : static_cast<int>((hi - lo) >> bits);
       auto upper = [&](int c) -> u64 {
         if (!linear) return hi - (static_cast<u64>(c) << bits);
         if (c == 0) return hi;
@@ -728,10 +762,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
         return p < hi ? p : hi;
       };
       auto lower = [&](int c) -> u64 {
-        if (!linear) {
-          const u64 span = (static_cast<u64>(c) + 1) << bits;
-          return span > hi - lo ? lo : hi - span + 1;
-        }
+        if (!linear) return c >= end_class ? lo : hi - ((static_cast<u64>(c) + 1) << bits) + 1;
         if (c == kBins - 1) return lo;
         const double v = top64 - (c + 1.0) * width;
         const u64 p = static_cast<u64>(key_of((v > -3.4e38 ? __double2float_rd(v) : -3.4028234663852886e38f) + 0.f)) << 32;
@@ -739,36 +770,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
       };
       // ---- the classes that hold the cut ----
       const double mark = p_of * whole;
-      double up = 0.0, dn = 0.0, w_up[kBinsEach], w_dn[kBinsEach];
-      if (!by_k) {
-        // sums of the largest and of the least weights that the classes can have
-        // (linear: powers of two by distance, which end half a step above it)
-#pragma unroll
-        for (int i = 0; i < kBinsEach; ++i) {
-          const int c = tid * kBinsEach + i;
-          w_up[i] = w_dn[i] = 0.0;
-          if (cnt[i] != 0 && linear) {
-            w_up[i] = exp2f(static_cast<float>(c) * (-1.f * kPerClass / kSteps) + 1.f / kSteps) * static_cast<float>(cnt[i]);
-            w_dn[i] = c == kBins - 1 ? 0.f : exp2f(static_cast<float>(c + 1) * (-1.f * kPerClass / kSteps)) * static_cast<float>(cnt[i]);
-          } else if (cnt[i] != 0) {
-            w_up[i] = weight(r, sh.power, value_of(static_cast<uint32_t>(upper(c) >> 32))) * cnt[i];
-            w_dn[i] = weight(r, sh.power, value_of(static_cast<uint32_t>(lower(c) >> 32))) * cnt[i];
-          }
-          up += w_up[i];
-          dn += w_dn[i];
-        }
-        const double su = warp_scan(up), sd = warp_scan(dn);
-        if (lane == 31) {
-          sh.wt[warp] = su;
-          sh.wt[kWarps + warp] = sd;
-        }
-        up = su - up;
-        dn = sd - dn;
-      }
       __syncthreads();
-      uint32_t before = inc - mine;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) before += w < warp ? sh.isum[w] : 0;
+      const int to_warp = scan_lanes(lane < kWarps ? sh.isum[lane] : 0);
+      const uint32_t before = inc - mine + (warp > 0 ? __shfl_sync(0xffffffffu, to_warp, max(warp - 1, 0)) : 0);
       int c_lo = kBins, c_hi = kBins;
       if (by_k) {
         const uint32_t k = static_cast<uint32_t>(want_k - above);
@@ -779,20 +783,55 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
           run += cnt[i];
         }
       } else {
-        constexpr double kSlack = 1e-12;
-        double run_up = mass + up, run_dn = mass + dn;
+        // sums of the largest and of the least weights that the classes can have
+        const auto by_mass = [&](auto zero, auto slack, auto bounds) {
+          using F = decltype(zero);
+          F up = 0, dn = 0, w_up[kBinsEach], w_dn[kBinsEach];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          run_up += w < warp ? sh.wt[w] : 0.0;
-          run_dn += w < warp ? sh.wt[kWarps + w] : 0.0;
-        }
+          for (int i = 0; i < kBinsEach; ++i) {
+            w_up[i] = w_dn[i] = 0;
+            if (cnt[i] != 0) bounds(tid * kBinsEach + i, static_cast<F>(cnt[i]), w_up[i], w_dn[i]);
+            up += w_up[i];
+            dn += w_dn[i];
+          }
+          const F su = scan_lanes(up), sd = scan_lanes(dn);
+          F* const sums = reinterpret_cast<F*>(sh.wt);
+          if (lane == 31) {
+            sums[warp] = su;
+            sums[kWarps + warp] = sd;
+          }
+          __syncthreads();
+          const F wu = scan_lanes(lane < kWarps ? sums[lane] : F(0)), wd = scan_lanes(lane < kWarps ? sums[kWarps + lane] : F(0));
+          F run_up = static_cast<F>(mass) + (su - up), run_dn = static_cast<F>(mass) + (sd - dn);
+          if (warp > 0) {
+            run_up += __shfl_sync(0xffffffffu, wu, max(warp - 1, 0));
+            run_dn += __shfl_sync(0xffffffffu, wd, max(warp - 1, 0));
+          }
+          // What the classes behind hold bounds it too, where those are all there
+          // is (a mark near the whole: the error is that of the rest)
+          const F all_up = __shfl_sync(0xffffffffu, wu, 31), all_dn = __shfl_sync(0xffffffffu, wd, 31), sum = static_cast<F>(whole);
+          const F low = static_cast<F>(mark) * (1 - slack), high = static_cast<F>(mark) * (1 + slack);
 #pragma unroll
-        for (int i = 0; i < kBinsEach; ++i) {
-          run_up += w_up[i];
-          run_dn += w_dn[i];
-          if (cnt[i] == 0) continue;
-          if (c_lo == kBins && run_up > mark * (1.0 - kSlack)) c_lo = tid * kBinsEach + i;
-          if (c_hi == kBins && run_dn > mark * (1.0 + kSlack)) c_hi = tid * kBinsEach + i;
+          for (int i = 0; i < kBinsEach; ++i) {
+            run_up += w_up[i];
+            run_dn += w_dn[i];
+            if (cnt[i] == 0) continue;
+            if (c_lo == kBins && run_up > low && (!linear || sum - (all_dn - run_dn) > low)) c_lo = tid * kBinsEach + i;
+            if (c_hi == kBins && (run_dn > high || (linear && sum - (all_up - run_up) > high))) c_hi = tid * kBinsEach + i;
+          }
+        };
+        if (linear) {
+          // powers of two by distance, which end half a step above it; fp32 does
+          // (sums of 2048 terms, to 2^-16: a class is 2^-6 of its weight wide)
+          by_mass(0.f, 1.f / 65536, [&](int c, float n, float& u, float& d) {
+            u = exp2f(static_cast<float>(c) * (-1.f * kPerClass / kSteps) + 1.f / kSteps) * n;
+            d = c == kBins - 1 ? 0.f : exp2f(static_cast<float>(c + 1) * (-1.f * kPerClass / kSteps)) * n;
+          });
+        } else {
+          by_mass(0.0, 1e-12, [&](int c, double n, double& u, double& d) {
+            u = weight(r, sh.power, value_of(static_cast<uint32_t>(upper(c) >> 32))) * n;
+            d = weight(r, sh.power, value_of(static_cast<uint32_t>(lower(c) >> 32))) * n;
+          });
         }
       }
       if (c_lo < kBins) atomicMin(&sh.lo, c_lo);
@@ -802,8 +841,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
       c_hi = sh.hi;
       if (by_k && c_lo == kBins) break;  // fewer tokens than k: all are kept
       // (no class where the sum stays below its mark: the cut lies behind all of them)
-      if (c_lo == kBins) c_lo = kBins - 1;
-      if (c_hi == kBins) c_hi = kBins - 1;
+      if (c_lo == kBins) c_lo = end_class;
+      if (c_hi == kBins) c_hi = end_class;
       // tokens down to the last of these classes, and before the first
       if (tid == c_hi / kBinsEach) {
         uint32_t run = before;
@@ -840,7 +879,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
             split_copies(ghi, !by_k, copies, sum, over);
           } else {
             copied = false;
-            pair_pass<T>(nlo, ghi, !by_k && !from_top, true, 0, sum, over);
+            double above_mass = 0.0;
+            if (!by_k && !from_top) draw_pass<T>(ghi + 1, -3.4028234663852886e38f, above_mass);
+            pair_pass<T>(nlo, ghi, false, true, 0, sum, over);
+            sum = above_mass;
           }
           publish(sum, over, 0);
         }
@@ -907,6 +949,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
         }
         barrier();  // the counts have been read
         if (tid == 0) sh.count = 0;
+        for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;  // (tiles lie over them)
       }
       if (!by_k && !linear && nhi - nlo > (hi - lo) / 2) {
         // Classes so wide that their bounds say little (a tiny temperature): one

@@ -108,6 +108,19 @@ def test_flat_rows(dtype):
         _both(x, u, top_k=_i(*[k] * 6), top_p=_f(*[0.7] * 6), min_p=_f(0, 0.1, 0.3, 0.5, 0.9, 1.5))
 
 
+@pytest.mark.parametrize("V", [300, 3000, 9000, 20000])
+@pytest.mark.parametrize("t", [0.3, 1.0, 100.0, 1000.0])
+def test_nuclei_that_end_anywhere(V, t):
+    """fp32 logits, all different: a class of the first search holds thousands,
+    or the end lies in its last one."""
+    x, u = _logits(24, V, torch.float32, 5)
+    T = torch.full((24,), t, device="cuda")
+    for p in (0.5, 0.9, 0.99, 0.999, 0.9999999):
+        _both(x, u, temperature=T, top_p=torch.full((24,), p, device="cuda"))
+    for k in (V // 2, V - 1):
+        _both(x, u, temperature=T, top_k=torch.full((24,), k, dtype=torch.int32, device="cuda"))
+
+
 def test_equal_logits_are_cut_by_index():
     V = 40000
     x = torch.zeros(8, V, device="cuda")
