@@ -214,11 +214,25 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) paged_block_write_k
   const int64_t r0 = p0 + row_of;
   const int slices = static_cast<int>(gridDim.y), slice = blockIdx.y;
   const int units = 2 * c.Hkv, mine = (units - slice + slices - 1) / slices;  // k and v heads: slice, slice + slices, ...
-  for (int x = threadIdx.x; x < cnt * (D / 2); x += kThreads) {
-    const double t = static_cast<double>(p0 + x / (D / 2)) * a.turns[x % (D / 2)];
-    float sn, cs;
-    sincospif(2.f * static_cast<float>(t - rint(t)), &sn, &cs);
-    s_turn[x] = make_float2(cs, sn);
+  {
+    // Sines and cosines in 64 bits, rounded once: a code flips where k is nearer to
+    // a tie than its error.  A thread has one frequency and a few rows: the first
+    // one's angle by the function, the next ones' by a turn of one position each.
+    constexpr int kParts = kThreads / (D / 2);
+    const int f = threadIdx.x % (D / 2), each = (cnt + kParts - 1) / kParts;
+    const int j0 = threadIdx.x / (D / 2) * each, j1 = min(cnt, j0 + each);
+    if (j0 < j1) {
+      const double t = static_cast<double>(p0 + j0) * a.turns[f];
+      double sn, cs, s1 = 0.0, c1 = 1.0;
+      sincospi(2.0 * (t - rint(t)), &sn, &cs);
+      if (j0 + 1 < j1) sincospi(2.0 * a.turns[f], &s1, &c1);
+      for (int j = j0; j < j1; ++j) {
+        s_turn[j * (D / 2) + f] = make_float2(static_cast<float>(cs), static_cast<float>(sn));
+        const double c = cs * c1 - sn * s1;
+        sn = sn * c1 + cs * s1;
+        cs = c;
+      }
+    }
   }
   for (int x = threadIdx.x; x < mine; x += kThreads) s_amax[x] = 0;
   __syncthreads();
