@@ -41,6 +41,20 @@
 // accumulated as (p vs) / vs.  Scales are not negative; a v scale below
 // kLeastScale counts as that.
 //
+// A scale per block of at least 16 positions (NT > 0 below): a warp's step has
+// one k scale and one v scale, two numbers instead of 32, and the products are
+// turned around.  S^T = K Q^T has the positions as rows and O^T = V^T P^T the
+// dims, so that a tile's query rows are columns, which come in eights: 4 rows
+// take 8 instead of 16 (half the products, half the accumulators, four CTAs an
+// SM instead of two), 20 take 24 instead of 32.  The codes' words are the
+// operand's own, as they are in the other form; P^T comes out of the scores'
+// layout by transposing 8 x 8 matrices in registers, and a row's maximum is
+// looked for across the lanes only when some score has outgrown it.  64
+// sequences of 500 to 8192 positions take 78 us so, 0.74 of the measured HBM
+// rate (105 in the other form with the same scales), 32 x 5 drafts 59.6 us, 0.35
+// (66): there the instructions of 24 columns (620 a step, 370 with 8), and
+// starting and ending tiles (10 us of a CTA each), are what counts.
+//
 // mma.sync, not tcgen05: a tile has 16 or 32 rows, a quarter or half of
 // tcgen05's smallest M (64), and the tensor work per byte of pages is far below
 // what the warp-level product delivers.

@@ -23,6 +23,13 @@
 // are summed tile by tile, over copies of the tokens down to the cut where
 // those fit into shared memory (a twentieth of a language model's row, say:
 // weights of all tokens would cost as much again), else over the row.
+// What it must read is the logits, once.  What bounds it is instructions: 25 to
+// 30 a token and pass with a weight (ten of them in 64 bits), and for few rows
+// the chain of passes, exchanges between the CTAs of a cluster, and the list.
+// Measured: 8 rows of 32000 tokens, fp16: 4.4 us greedy, 8 us by temperature or
+// min-p, 25 us by top-p or top-k; 256 of 50257: 11 (0.36 of the measured HBM
+// rate), 32, 114 and 53 us, 106 with every row a rule of its own; 64 fp32 rows
+// of 130001 by temperature 30 us (0.17).
 #include <cooperative_groups.h>
 
 #include <type_traits>
