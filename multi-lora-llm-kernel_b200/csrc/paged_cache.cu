@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kWriteThreads, 12) paged_write_kernel(const __
 }
 
 // ---- 8-bit pages with a scale per block ----
+constexpr int kMostHeads = 1024;  // kv heads that the entry point lets through
 
 // The smallest power of two s with amax <= 448 s (448 = 1.75 2^8), from
 // kMinScale up to 2^120.
@@ -395,7 +396,7 @@ cudaError_t block_write_launch(const PagedWrite& a, int slices, int32_t* err, cu
   // angles; maxima, scales and ratios by head
   const int smem = ((D / 2 << a.c.scale_shift) + 3 * a.c.Hkv) * static_cast<int>(sizeof(float2));
   static std::atomic<bool> done[64];
-  const cudaError_t e = prepare_kernel(done, k, ((64 << 7) + 3 * 1024) * static_cast<int>(sizeof(float2)), 0);
+  const cudaError_t e = prepare_kernel(done, k, ((64 << 7) + 3 * kMostHeads) * static_cast<int>(sizeof(float2)), 0);
   if (e != cudaSuccess) return e;
   const int64_t runs = (a.rows >> a.c.scale_shift) + 2 * static_cast<int64_t>(a.c.B);
   return launch_paged(k, dim3(static_cast<unsigned>(runs), slices), dim3(kThreads), smem, 1, true, st, a, err);

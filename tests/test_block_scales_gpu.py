@@ -242,6 +242,63 @@ def test_interleaved_pages_and_other_stream():
     _check(out, want, tol)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_pages_with_gaps(D):
+    """Positions further apart than a head is wide, heads and pages with gaps, scales in one pool."""
+    bt = K.BlockBatch([1, 3, 40], [100, 20, 9], 32, 2, D, H, 16, seed=12)
+    pools = [torch.full((bt.num_pages, 2, 34, D + 16), float("nan"), device="cuda").to(R.E4M3) for _ in range(2)]
+    bt.k_cache, bt.v_cache = (p[:, :, 1:33, :D] for p in pools)
+    scales = torch.full((bt.num_pages, 2, 2, 3), float("nan"), device="cuda")
+    bt.blocks = {"k": scales[:, 0, :, :2], "v": scales[:, 1, :, :2]}
+    bt.fill(upto=[100, 20, 9])
+    before = K.state(bt)
+    q, k, v, q_out = _write(bt, 8)
+    K.check_write(bt, before, q, k, v, q_out, THETA)
+    for max_new in (1, 40):
+        out = torch.zeros_like(q)
+        ops.paged_attention(q_out, *bt.args(), out, 0.09, max_new=max_new, **bt.scales())
+        want, tol = R.attention(bt, q_out, 0.09)
+        _check(out, want, tol)
+    ko, vo = torch.zeros_like(k), torch.zeros_like(v)
+    ops.paged_cache_read(*bt.args(), ko, vo, **bt.scales())
+    assert torch.equal(ko[4:], bt.get("k", 2, 9, 49).to(H)) and torch.equal(vo[:1], bt.get("v", 0, 100, 101).to(H))
+    ops.check_errors(q.device)
+
+
+def test_captured_into_two_graphs():
+    """Write, attention and read back of two batches, replayed on two streams with changed lengths."""
+    graphs, parts = [], []
+    for i in range(2):
+        bt = K.BlockBatch([1, 1, 2], [40, 200, 13], 32, 2, 128, H, 16, seed=20 + i, width=9)
+        bt.fill(upto=[40, 200, 13])
+        q, k, v = bt.randn(4, 8, 128), bt.randn(4, 2, 128), bt.randn(4, 2, 128)
+        q_out, out = torch.zeros_like(q), torch.zeros_like(q)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.paged_rope_cache(q, k, v, *bt.args(), THETA, q_out=q_out, **bt.scales())
+            ops.paged_attention(q_out, *bt.args(), out, 0.09, max_new=2, **bt.scales())
+        graphs.append(g)
+        parts.append((bt, q, k, v, q_out, out))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for step in range(3):
+        states = [K.state(p[0]) for p in parts]
+        for s, g in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for (bt, q, k, v, q_out, out), before in zip(parts, states):
+            K.check_write(bt, before, q, k, v, q_out, THETA)
+            want, tol = R.attention(bt, q_out, 0.09)
+            _check(out, want, tol)
+            for b in range(3):  # the next tokens, other rows
+                bt.len[b] += bt.new[b]
+            bt.lengths.copy_(torch.tensor(bt.len, dtype=torch.int32))
+            for t in (q, k, v):
+                t.copy_(bt.randn(*t.shape))
+    ops.check_errors(torch.device("cuda", 0))
+
+
 def test_refusals():
     bt = K.BlockBatch([1, 1], [20, 70], 48, 2, 128, H, 16)
     bt.fill()

@@ -109,3 +109,25 @@ def test_cpu_tensors_are_refused(built):  # noqa: F811
         ops.paged_plan(i32(2), i32(2), i32(2, 2), i32(4), i32(1), 16, i32(3), torch.zeros(4, dtype=torch.int64))
     with pytest.raises(RuntimeError, match="must be CUDA"):
         ops.sample_tokens(torch.zeros(2, 9), torch.zeros(2), torch.zeros(2, dtype=torch.int64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["paged_plan", "sample_tokens"])
+def test_compiled_calls(name):
+    """Captured whole, and with the results of the plain calls."""
+    from persona import ops
+
+    a, b = _arguments()[name], _arguments()[name]
+    for args in (a, b):
+        if name == "paged_plan":
+            args[0].fill_(1)
+            args[3].copy_(torch.arange(12))
+            args[4].fill_(12)
+        else:
+            args[0].uniform_(generator=torch.Generator(device="cuda").manual_seed(1))
+            args[1].fill_(0.5)
+    getattr(ops, name)(*a)
+    torch.compile(lambda *t: getattr(ops, name)(*t), fullgraph=True, backend="eager")(*b)
+    ops.check_errors(torch.device("cuda", 0))
+    assert all(torch.equal(x, y) for x, y in zip(a, b) if torch.is_tensor(x))
+    assert int(a[-1].sum()) != 0  # it did something
