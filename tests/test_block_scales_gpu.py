@@ -137,7 +137,7 @@ def test_attention_few_rows(dtype, Hq, Hkv, D, page, block, window):
     out = torch.full_like(q, 9.0)
     want, tol = R.attention(bt, q, D ** -0.5, window)
     n = sum(bt.new)
-    for max_new in (1, 4):  # a bound that is too small is still computed right
+    for max_new in (1, 3, 4, 5, 8):  # a bound that is too small is still computed right
         ops.paged_attention(q, *bt.args(), out, D ** -0.5, window=window, max_new=max_new, **bt.scales())
         ops.check_errors(q.device)
         _check(out[:n], want[:n], tol[:n])
@@ -175,6 +175,24 @@ def test_attention_batches(B, L):
         again = torch.zeros_like(q)
         ops.paged_attention(q, *bt.args(), again, 128 ** -0.5, **bt.scales())
         assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("dtype", [H, BF])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (7, 1, 64), (5, 5, 128)])
+@pytest.mark.parametrize("new,ctx", [([5, 3, 5], [40, 0, 200]), ([6] * 40, [31 * i % 700 for i in range(40)]),
+                                     ([2, 9, 1, 4], [9000, 30, 4000, 0]), ([3] * 100, [17 * i for i in range(100)])])
+def test_attention_of_drafts(dtype, Hq, Hkv, D, new, ctx):
+    """17 to 64 rows per kv head: clusters, ranges that end inside tiles, more than one tile."""
+    bt = K.BlockBatch(new, ctx, 64, Hkv, D, dtype, 32, pad=1, seed=15)
+    bt.fill(spread=1.0)
+    q = bt.randn(bt.rows, Hq, D, scale=1.5)
+    for window in (0, 130):
+        out = torch.full_like(q, 9.0)
+        ops.paged_attention(q, *bt.args(), out, D ** -0.5, window=window, max_new=max(new), **bt.scales())
+        ops.check_errors(q.device)
+        want, tol = R.attention(bt, q, D ** -0.5, window)
+        _check(out[:-1], want[:-1], tol[:-1])
+        assert torch.all(out[-1] == 9.0)
 
 
 def test_attention_leaves_other_contents_out():
