@@ -18,7 +18,8 @@ constexpr float kLog2E = 1.4426950408889634f;
 // warp-level kernel, which reads the pages once per 32 rows.  Measured with 32
 // sequences of up to 6000 tokens: over 16-bit pages 36 rows take it 118 us and
 // the tcgen05 kernel 77 (20 rows: 66 and 77); over 8-bit pages, whose codes the
-// tcgen05 kernel has to convert for each of its tiles, 64 rows take 129 and 149.
+// tcgen05 kernel has to convert for each of its tiles, 64 rows take 129 and 149
+// (109 and 144 with a scale per block: two tiles of 32; a third would be too many).
 constexpr int64_t kFewRows16 = 32, kFewRows8 = 64;
 constexpr int kMaxScaleShift = 7;  // blocks of at most 128 positions
 
