@@ -626,6 +626,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(const __grid
   const double unit = static_cast<double>(temp) * 0.69314718055994530942;  // logits to half the weight: 1 / rate
   r.least = fmaxf(__double2float_ru(top64 - 1000.0 * unit), -3.4028234663852886e38f);
   r.unit = unit;
+  // (field by field: nvcc 12.9 leaves a copy of the whole unset, since the functions
+  // above capture r)
   if (lane == 0) {
     Row& to = sh.row[warp];
     to.logits = r.logits;
