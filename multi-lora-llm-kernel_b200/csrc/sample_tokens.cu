@@ -252,8 +252,10 @@ __device__ __noinline__ void count_pass(u64 lo_pair, double& sum_out, int& tail_
   const Row r = sh.row[threadIdx.x >> 5];
   const Border lo(lo_pair);
   const bool ties = lo.at < static_cast<unsigned>(r.V);
-  // (a class is known from 1 / 256 of a power of two of weight before its end)
-  const float least = fmaxf(r.least, __double2float_ru(static_cast<double>(r.top) - (kBins - 1.5) * kPerClass / kSteps * r.unit));
+  // What is further than 2046.9 classes from the maximum is in the last one.  Steps are
+  // rounded, so class 2046 by them ends at 2046.94; the last class has its upper border
+  // at 2046.85 (upper) and its largest weight at 2046.875 (by_mass), both above these tokens.
+  const float least = fmaxf(r.least, __double2float_ru(static_cast<double>(r.top) - (kBins - 1.1) * kPerClass / kSteps * r.unit));
   const uint32_t bins = smem_u32(sh.bins);
   double sum = 0.0;
   int tail = 0;

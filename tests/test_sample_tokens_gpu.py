@@ -121,6 +121,34 @@ def test_nuclei_that_end_anywhere(V, t):
         _both(x, u, temperature=T, top_k=torch.full((24,), k, dtype=torch.int32, device="cuda"))
 
 
+@pytest.mark.parametrize("B", [1, 304])  # eight CTAs a row, and one
+@pytest.mark.parametrize("t", [0.01, 1.0, 50.0])
+@pytest.mark.parametrize("at", [2046.45, 2046.55, 2046.8, 2046.87, 2046.93, 2046.97, 2047.5])
+def test_cuts_where_the_last_class_begins(B, t, at):
+    """Tokens around 32 powers of two below the largest, where the classes of the
+    first search end: the k-th one, and the end of a nucleus, among them.  The
+    last kept token of a number of 1 shows the cut."""
+    far = -at / 64 * math.log(2.0) * t
+    one, zeros = _f(*[1.0] * B), 600
+    T = torch.full((B,), t, device="cuda")
+
+    def both(row, **kw):
+        x = torch.tensor(row, dtype=torch.float32, device="cuda").expand(B, -1)
+        got = _run(x, one, temperature=T, **kw)
+        assert got == plain(x[:1], one[:1], T[:1], *(kw[n][:1] if n in kw else None for n in ("top_k", "top_p"))) * B
+        return got[0]
+
+    # one token there, more than a list of all would hold above it
+    k = torch.full((B,), zeros + 1, dtype=torch.int32, device="cuda")
+    assert both([0.0] * zeros + [far, far * 30 / 22.166], top_k=k) == zeros
+    # more of them than are sorted at once, cut by their index
+    k = torch.full((B,), zeros + 700, dtype=torch.int32, device="cuda")
+    assert both([0.0] * zeros + [far] * 1500 + [1.4 * far] * 500, top_k=k) == zeros + 699
+    # a nucleus that ends among them
+    p = torch.full((B,), 1 - 2.0 ** -24, device="cuda")
+    assert 0 < both([0.0] + [far] * 2000 + [1.4 * far] * 500, top_p=p) < 2501
+
+
 def test_equal_logits_are_cut_by_index():
     V = 40000
     x = torch.zeros(8, V, device="cuda")
