@@ -114,7 +114,8 @@ class StaticBatchEngine:
         ``max_tokens``) per request, prompts of any lengths; returns the new
         token ids as a list per request, and device times as
         ``run_static_generate``.  ``num_pages``: of the cache (default: what all
-        requests need at their longest)."""
+        requests need at their longest).  A request whose logits leave nothing to
+        draw (all NaN or -infinity) ends there, with the tokens that it has."""
         slots = self.plan_batch(requests)
         budget = [min(max_new_tokens, r.sampling.max_tokens) for r in requests]
         if not requests or min(budget) < 1 or any(len(r.prompt) == 0 for r in requests):
@@ -145,8 +146,10 @@ class StaticBatchEngine:
         prefill_ms = ev[0].elapsed_time(ev[1])
         decode_ms = ev[1].elapsed_time(ev[2])
         tokens = [row[:n] for row, n in zip(out.tolist(), budget)]
-        return {"tokens": tokens, "prefill_ms": prefill_ms, "decode_ms": decode_ms, "new_tokens": sum(budget),
-                "tok_per_s": sum(budget) / ((prefill_ms + decode_ms) * 1e-3)}
+        tokens = [row[:row.index(-1)] if -1 in row else row for row in tokens]
+        new = sum(len(row) for row in tokens)
+        return {"tokens": tokens, "prefill_ms": prefill_ms, "decode_ms": decode_ms, "new_tokens": new,
+                "tok_per_s": new / ((prefill_ms + decode_ms) * 1e-3)}
 
     @staticmethod
     def _next(logits: torch.Tensor, requests: Sequence[Request], sampled: List[int]) -> torch.Tensor:

@@ -161,6 +161,7 @@ class PagedDecode:
     sampling: BatchSampling
     tok: torch.Tensor       # [B + 1] int64: the token that each sequence feeds next (and a place for padded rows)
     alive: torch.Tensor     # [B] int32: 1 gets a token a step; 0 has ended, its pages go back with the next step
+                            # (so has one whose token is none of the vocabulary, -1 say: nothing could be drawn)
     u: torch.Tensor         # [B] fp32: the numbers that the next step draws with
     lengths: torch.Tensor   # [B] int32
     keep: torch.Tensor      # [B] int32
@@ -390,12 +391,16 @@ class MistralLoRAModel:
     def start_decode(self, st: PagedState, tokens: torch.Tensor, sampling: BatchSampling) -> PagedDecode:
         """Hands the sequences of ``st`` over to the device: ``tokens`` [B] are
         what each feeds first, ``sampling`` how the next ones are drawn.  Until
-        ``finish_decode`` only ``paged_step`` moves them."""
+        ``finish_decode`` only ``paged_step`` moves them.  A sequence whose token
+        is -1, what ``sample_batch`` gives for a row without any, ends with the
+        first step."""
         st._host()
         cfg, d = self.cfg, self.device
         B, pages = len(st.lengths), st.k_cache[0].shape[0]
         if tokens.shape != (B,) or sampling.temperature.shape != (B,):
             raise ValueError("one token and one set of parameters per sequence")
+        if B and not -1 <= int(tokens.min()) <= int(tokens.max()) < cfg.vocab:
+            raise ValueError("token id outside the vocabulary")
         i32 = dict(dtype=torch.int32, device=d)
         free = torch.zeros(pages, **i32)
         free[:len(st.free)] = torch.tensor(st.free, **i32)
@@ -432,6 +437,8 @@ class MistralLoRAModel:
     def _paged_body(self, dec: PagedDecode) -> None:
         cfg, st, b = self.cfg, dec.st, dec.bufs
         B = len(dec.seqs)
+        # A token outside of the vocabulary is not one to feed: its sequence has ended.
+        dec.alive.mul_((dec.tok[:B] >= 0) & (dec.tok[:B] < cfg.vocab))
         # ended sequences give their pages back, the others get a row and, where they need one, a page
         torch.mul(dec.lengths, dec.alive, out=dec.keep)
         ops.paged_plan(dec.alive, dec.lengths, st.page_table, dec.free, dec.num_free, st.page_size, dec.indptr, dec.places,
@@ -439,7 +446,8 @@ class MistralLoRAModel:
         seq = dec.row_seq.clamp_min(0)
         slots = torch.where(dec.row_seq < 0, dec.row_seq, st.slots.index_select(0, seq))
         plan = ops.bgmv_plan(slots, self.pool.max_slots)
-        torch.index_select(self.embed, 0, dec.tok.index_select(0, seq), out=b["h"])
+        # (rows of no sequence look a token up too, be it one that ended its sequence)
+        torch.index_select(self.embed, 0, dec.tok.index_select(0, seq).clamp_(0, cfg.vocab - 1), out=b["h"])
         scale = 1.0 / math.sqrt(128)
         delta = None
         for li, lw in enumerate(self.layers):
@@ -475,7 +483,9 @@ class MistralLoRAModel:
                    generator: Optional[torch.Generator] = None) -> torch.Tensor:
         """Every sequence that is alive feeds its token and draws the next one,
         with numbers from ``generator`` (by sequence, whoever else is alive).
-        Returns ``dec.tok[:B]``, on the device (an ended sequence's stays what it was)."""
+        Returns ``dec.tok[:B]``, on the device (an ended sequence's stays what it
+        was).  A row whose logits leave nothing to draw (all NaN or -infinity)
+        gives -1, and its sequence ends with the next step."""
         dec.u.uniform_(generator=generator)
         B = len(dec.seqs)
         if not use_graph:

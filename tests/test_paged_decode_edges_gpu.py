@@ -1,0 +1,100 @@
+"""Decoding over a paged cache where something goes wrong: rows without a token,
+calls that raise, steps without a page."""
+
+import pytest
+import torch
+
+from persona import ops
+from persona.engine import Request, StaticBatchEngine
+from persona.sampling import BatchSampling, SamplingParams, sample_batch
+from test_decode_gpu import CFG, _dev, _small_model
+from test_paged_decode_gpu import E4M3, _generator, _prompts
+
+pytestmark = pytest.mark.gpu
+SAMPLED = [SamplingParams(temperature=0.8, top_p=0.9), SamplingParams(temperature=1.2, top_k=30), SamplingParams()]
+
+
+def _start(model, pool, prompts, params=SAMPLED, pages=40, seed=3, **kv):
+    slots = torch.tensor([pool.name_to_slot["a0"], -1, pool.name_to_slot["a2"]], dtype=torch.int32)
+    st = model.new_paged_state(slots, pages, 16, 160, **kv)
+    sampling = BatchSampling(params, _dev())
+    g = _generator(seed)
+    logits, ip = model.extend(st, prompts)
+    first = sample_batch(logits[ip[1:].long() - 1], sampling, generator=g)
+    return model.start_decode(st, first, sampling), first.tolist(), g
+
+
+def _unused(seen):
+    return next(t for t in range(CFG.vocab) if t not in seen)
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+@pytest.mark.parametrize("kv", [dict(), dict(kv_dtype=E4M3, kv_block=16)])
+def test_a_row_without_a_token_ends_its_sequence(use_graph, kv):
+    """A token whose embedding is NaN leaves its row no logit to draw from.  The
+    other sequences, which take the pages over that it filled with NaN, go on as
+    they do alone."""
+    pool, model = _small_model()
+    prompts = _prompts([20, 33, 16], 21)
+
+    def run(end, poison=None):
+        dec, first, g = _start(model, pool, prompts, **kv)
+        rows = [first]
+        for i in range(40):
+            if i == 6 and poison is not None:
+                dec.tok[1] = poison
+            if i == end:
+                dec.alive[1] = 0
+            rows.append(model.paged_step(dec, use_graph=use_graph, generator=g).tolist())
+        model.finish_decode(dec)
+        return dec.st, [list(c) for c in zip(*rows)]
+
+    st, clean = run(7)
+    nan = _unused(sum(clean, sum(prompts, [])))
+    model.embed[nan] = float("nan")
+    ended, got = run(None, nan)
+    assert got[0] == clean[0] and got[2] == clean[2]
+    assert got[1][:7] == clean[1][:7] and got[1][7:] == [-1] * 34
+    assert (ended.lengths, ended.pages, ended.free) == (st.lengths, st.pages, st.free)
+    assert ended.lengths == [60, 0, 56]
+
+
+def test_a_prompt_without_a_token_ends_at_once():
+    """-1 is what ``sample_batch`` hands to ``start_decode`` then."""
+    pool, model = _small_model()
+    prompts = _prompts([20, 33, 16], 22)
+    nan = _unused(sum(prompts, []))
+    model.embed[nan] = float("nan")
+    prompts[0][-1] = nan
+    dec, first, g = _start(model, pool, prompts)
+    assert first[0] == -1 and min(first[1:]) >= 0
+    for _ in range(3):
+        got = model.paged_step(dec, generator=g).tolist()
+        assert got[0] == -1 and min(got[1:]) >= 0
+    model.finish_decode(dec)
+    assert dec.st.lengths == [0, 36, 19] and dec.st.pages[0] == []
+    for bad in (CFG.vocab, -2):
+        with pytest.raises(ValueError, match="outside the vocabulary"):
+            model.start_decode(dec.st, torch.tensor([1, bad, 2], device=_dev()), dec.sampling)
+    # a token that was put there from outside ends its sequence too, whatever it is
+    dec = model.start_decode(dec.st, torch.tensor([1, 2, 3], device=_dev()), dec.sampling)
+    dec.tok[1] = 1 << 40
+    got = model.paged_step(dec, generator=g).tolist()
+    assert got[1] == 1 << 40 and min(got[0], got[2]) >= 0
+    model.finish_decode(dec)
+    assert dec.st.lengths == [1, 0, 20]
+
+
+def test_ragged_generation_of_a_request_without_a_token():
+    pool, model = _small_model()
+    eng = StaticBatchEngine(model, pool, max_batch=4, max_seq_len=256)
+    prompts = _prompts([5, 40, 12], 23)
+    nan = _unused(sum(prompts, []))
+    reqs = [Request(f"r{i}", "a", p, slot=i, sampling=SamplingParams()) for i, p in enumerate(prompts)]
+    clean = eng.run_ragged_generate(reqs, 12)
+    assert nan not in sum(clean["tokens"], [])
+    model.embed[nan] = float("nan")
+    reqs[1].prompt = prompts[1][:-1] + [nan]
+    got = eng.run_ragged_generate(reqs, 12)
+    assert got["tokens"] == [clean["tokens"][0], [], clean["tokens"][2]] and got["new_tokens"] == 24
+    ops.check_errors(_dev())
