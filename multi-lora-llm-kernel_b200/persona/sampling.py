@@ -91,12 +91,14 @@ def sample_next_token(logits: torch.Tensor, params: SamplingParams,
 
     Temperature 0 (or below) is greedy.  Otherwise the logits are divided by
     the temperature, cut to the top-p nucleus when ``top_p < 1``, and one
-    token per row is drawn by Gumbel-max.  With top-k or min-p: ``sample_batch``.
+    token per row is drawn by Gumbel-max.  With top-k or min-p: ``sample_batch``,
+    but a row of NaN or -infinity alone gives its ``argmax``, as without them.
     """
     if params.temperature <= 0:
         return logits.argmax(dim=-1)
     if params.top_k > 0 or params.min_p > 0:
-        return sample_batch(logits, [params] * logits.shape[0], generator=generator)
+        token = sample_batch(logits, [params] * logits.shape[0], generator=generator)
+        return torch.where(token < 0, logits.argmax(dim=-1), token)  # (callers feed it: always a token of the vocabulary)
     z = logits.float() / params.temperature
     if params.top_p < 1.0:
         z = _nucleus_mask(z, params.top_p)

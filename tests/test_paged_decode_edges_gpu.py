@@ -6,7 +6,7 @@ import torch
 
 from persona import ops
 from persona.engine import Request, StaticBatchEngine
-from persona.sampling import BatchSampling, SamplingParams, sample_batch
+from persona.sampling import BatchSampling, SamplingParams, sample_batch, sample_next_token
 from test_decode_gpu import CFG, _dev, _small_model
 from test_paged_decode_gpu import E4M3, _generator, _prompts
 
@@ -98,3 +98,29 @@ def test_ragged_generation_of_a_request_without_a_token():
     got = eng.run_ragged_generate(reqs, 12)
     assert got["tokens"] == [clean["tokens"][0], [], clean["tokens"][2]] and got["new_tokens"] == 24
     ops.check_errors(_dev())
+
+
+@pytest.mark.parametrize("params", [SamplingParams(), SamplingParams(temperature=1.0), SamplingParams(temperature=1.0, top_p=0.9),
+                                    SamplingParams(temperature=1.0, top_k=5), SamplingParams(temperature=1.0, min_p=0.1),
+                                    SamplingParams(temperature=0.7, top_k=5, top_p=0.9, min_p=0.1)])
+def test_next_tokens_are_always_of_the_vocabulary(params):
+    """``sample_next_token`` feeds the static engine's embedding."""
+    logits = torch.randn(4, 300, device=_dev(), generator=_generator(2)).half()
+    logits[1] = float("nan")
+    logits[2] = -float("inf")
+    got = sample_next_token(logits, params, generator=_generator(3)).tolist()
+    assert all(0 <= t < 300 for t in got)
+    assert got[1] == int(logits[1].argmax())
+
+
+def test_static_generation_of_a_request_without_a_token():
+    pool, model = _small_model()
+    eng = StaticBatchEngine(model, pool, max_batch=4, max_seq_len=64)
+    prompts = _prompts([12, 12, 12], 24)
+    nan = _unused(sum(prompts, []))
+    prompts[1][-1] = nan
+    model.embed[nan] = float("nan")
+    reqs = [Request(f"r{i}", "a", p, slot=i, sampling=SamplingParams(temperature=1.0, top_k=4)) for i, p in enumerate(prompts)]
+    out = eng.run_static_generate(reqs, 6)["tokens"]
+    ops.check_errors(_dev())
+    assert 0 <= int(out.min()) and int(out.max()) < CFG.vocab
