@@ -174,6 +174,10 @@ class PagedDecode:
     bufs: dict = field(default_factory=dict)
     graph: Optional[torch.cuda.CUDAGraph] = None
 
+    def _moved(self) -> list:
+        """What a step moves on, beside the pages' contents behind the lengths."""
+        return [self.tok, self.alive, self.lengths, self.st.page_table, self.free, self.num_free]
+
 
 class MistralLoRAModel:
     """Random-init Mistral-architecture decoder with NF4 base weights."""
@@ -485,26 +489,33 @@ class MistralLoRAModel:
         with numbers from ``generator`` (by sequence, whoever else is alive).
         Returns ``dec.tok[:B]``, on the device (an ended sequence's stays what it
         was).  A row whose logits leave nothing to draw (all NaN or -infinity)
-        gives -1, and its sequence ends with the next step."""
+        gives -1, and its sequence ends with the next step.  A call that raises
+        leaves the sequences as they were."""
         dec.u.uniform_(generator=generator)
         B = len(dec.seqs)
         if not use_graph:
-            self._paged_body(dec)
+            was = [t.clone() for t in dec._moved()]
+            try:
+                self._paged_body(dec)
+            except BaseException:
+                for to, t in zip(dec._moved(), was):
+                    to.copy_(t)
+                raise
             return dec.tok[:B]
         if dec.graph is None:
-            # Warmed up on a side stream by a step in which nobody is alive, whose
-            # pages stay (nothing is written but the padded rows' own buffers).
-            alive, lengths, table = dec.alive.clone(), dec.lengths.clone(), dec.st.page_table.clone()
-            free, num_free = dec.free.clone(), dec.num_free.clone()
+            # Warmed up on a side stream by a step in which nobody is alive; what it
+            # moves is put back (nothing else is written but the padded rows' own buffers).
+            was = [t.clone() for t in dec._moved()]
             s = torch.cuda.Stream(self.device)
-            dec.alive.zero_()
-            s.wait_stream(torch.cuda.current_stream(self.device))
-            with torch.cuda.stream(s):
-                self._paged_body(dec)
-            torch.cuda.current_stream(self.device).wait_stream(s)
-            for to, was in ((dec.alive, alive), (dec.lengths, lengths), (dec.st.page_table, table), (dec.free, free),
-                            (dec.num_free, num_free)):
-                to.copy_(was)
+            try:
+                dec.alive.zero_()
+                s.wait_stream(torch.cuda.current_stream(self.device))
+                with torch.cuda.stream(s):
+                    self._paged_body(dec)
+            finally:
+                torch.cuda.current_stream(self.device).wait_stream(s)
+                for to, t in zip(dec._moved(), was):
+                    to.copy_(t)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
                 self._paged_body(dec)

@@ -124,3 +124,71 @@ def test_static_generation_of_a_request_without_a_token():
     out = eng.run_static_generate(reqs, 6)["tokens"]
     ops.check_errors(_dev())
     assert 0 <= int(out.min()) and int(out.max()) < CFG.vocab
+
+
+def _state(dec):
+    return [t.tolist() for t in (dec.tok[:3], dec.alive, dec.lengths, dec.st.page_table, dec.num_free, dec.free[:int(dec.num_free)])]
+
+
+@pytest.mark.parametrize("use_graph,calls", [(False, 1), (True, 1), (True, 2)])
+@pytest.mark.parametrize("behind", [True, False])
+def test_a_step_that_raises_leaves_the_sequences(monkeypatch, use_graph, calls, behind):
+    """The step raises on the host, before or behind its operators: the eager
+    one, the warm-up before a capture, or the capture.  Made again, it gives the
+    tokens of a step that never failed."""
+    pool, model = _small_model()
+    prompts = _prompts([20, 32, 16], 25)
+    greedy = [SamplingParams()] * 3
+    kv = dict(kv_dtype=E4M3, kv_block=16)
+    clean, _, _ = _start(model, pool, prompts, greedy, **kv)
+    want = [model.paged_step(clean, use_graph=use_graph).tolist() for _ in range(4)]
+    dec, _, _ = _start(model, pool, prompts, greedy, **kv)
+    if not use_graph:
+        assert model.paged_step(dec, use_graph=False).tolist() == want[0]
+    before, body, left = _state(dec), model._paged_body, [calls]
+
+    def failing(d):
+        left[0] -= 1
+        if left[0] == 0 and not behind:
+            raise RuntimeError("on the host")
+        body(d)
+        if left[0] == 0:
+            raise RuntimeError("on the host")
+
+    monkeypatch.setattr(model, "_paged_body", failing)
+    with pytest.raises(RuntimeError, match="on the host"):
+        model.paged_step(dec, use_graph=use_graph)
+    monkeypatch.undo()
+    assert _state(dec) == before and dec.graph is None
+    for w in want[0 if use_graph else 1:]:
+        assert model.paged_step(dec, use_graph=use_graph).tolist() == w
+    model.finish_decode(dec)
+    assert dec.st.lengths == [24, 36, 20]
+    ops.check_errors(_dev())
+
+
+def _leave_an_error():
+    """A step that finds no page, over buffers of its own."""
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=_dev())  # noqa: E731
+    ops.paged_plan(i32(1), i32(0), i32(0).view(1, 1), i32(0), i32(0), 16, i32(0, 0),
+                   torch.zeros(1, dtype=torch.int64, device=_dev()))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_an_error_from_before_costs_no_sequence(use_graph):
+    """What an earlier operator left pending is raised by the first step."""
+    pool, model = _small_model()
+    prompts = _prompts([20, 32, 16], 26)
+    greedy = [SamplingParams()] * 3
+    clean, _, _ = _start(model, pool, prompts, greedy)
+    want = [model.paged_step(clean, use_graph=use_graph).tolist() for _ in range(3)]
+    dec, _, _ = _start(model, pool, prompts, greedy)
+    before = _state(dec)
+    _leave_an_error()
+    with pytest.raises(RuntimeError, match="no room for a planned step"):
+        model.paged_step(dec, use_graph=use_graph)
+    assert _state(dec) == before
+    assert [model.paged_step(dec, use_graph=use_graph).tolist() for _ in range(3)] == want
+    model.finish_decode(dec)
+    assert dec.st.lengths == [23, 35, 19]
