@@ -491,6 +491,8 @@ class MistralLoRAModel:
         was).  A row whose logits leave nothing to draw (all NaN or -infinity)
         gives -1, and its sequence ends with the next step.  A call that raises
         leaves the sequences as they were."""
+        if dec.st.decode is not dec:  # its lengths and pages are others' now
+            raise ValueError("this decode is not the sequences' own")
         dec.u.uniform_(generator=generator)
         B = len(dec.seqs)
         if not use_graph:

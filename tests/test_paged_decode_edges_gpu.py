@@ -130,6 +130,7 @@ def _state(dec):
     return [t.tolist() for t in (dec.tok[:3], dec.alive, dec.lengths, dec.st.page_table, dec.num_free, dec.free[:int(dec.num_free)])]
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")  # (what a capture that raises leaves)
 @pytest.mark.parametrize("use_graph,calls", [(False, 1), (True, 1), (True, 2)])
 @pytest.mark.parametrize("behind", [True, False])
 def test_a_step_that_raises_leaves_the_sequences(monkeypatch, use_graph, calls, behind):
@@ -192,3 +193,25 @@ def test_an_error_from_before_costs_no_sequence(use_graph):
     assert [model.paged_step(dec, use_graph=use_graph).tolist() for _ in range(3)] == want
     model.finish_decode(dec)
     assert dec.st.lengths == [23, 35, 19]
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_a_decode_that_ended_moves_nothing(use_graph):
+    """Its sequences' pages are the host's, or another decode's."""
+    pool, model = _small_model()
+    dec, _, _ = _start(model, pool, _prompts([20, 32, 16], 27))
+    model.paged_step(dec, use_graph=use_graph)
+    model.finish_decode(dec)
+    st = dec.st
+    st.set_length(1, 0)
+    model.extend(st, [[5] * 30, [], []])
+    table, k = st.page_table.clone(), [c.clone() for c in st.k_cache]
+    for again in (False, True):
+        other = model.start_decode(st, torch.tensor([1, 2, 3], device=_dev()), dec.sampling) if again else None
+        with pytest.raises(ValueError, match="not the sequences' own"):
+            model.paged_step(dec, use_graph=use_graph)
+        assert st.decode is other and torch.equal(st.page_table, table)
+        assert all(torch.equal(a, b) for a, b in zip(st.k_cache, k))
+    model.paged_step(st.decode, use_graph=use_graph)
+    model.finish_decode(st.decode)
+    assert st.lengths == [52, 1, 18]
