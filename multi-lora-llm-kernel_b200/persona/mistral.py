@@ -171,6 +171,7 @@ class PagedDecode:
     places: torch.Tensor    # [B] int64
     seqs: torch.Tensor      # [B] int32: 0 .. B - 1
     row_seq: torch.Tensor   # [B] int32: the sequence of each row, -1 behind the last
+    out: torch.Tensor       # [B + 1] int64: what the last step drew by sequence (and a place for padded rows)
     bufs: dict = field(default_factory=dict)
     graph: Optional[torch.cuda.CUDAGraph] = None
 
@@ -413,7 +414,7 @@ class MistralLoRAModel:
                           lengths=torch.tensor(st.lengths, **i32), keep=torch.zeros(B, **i32), free=free,
                           num_free=torch.tensor([len(st.free)], **i32), indptr=torch.zeros(B + 1, **i32),
                           places=torch.zeros(B, dtype=torch.int64, device=d), seqs=torch.arange(B, **i32),
-                          row_seq=torch.zeros(B, **i32))
+                          row_seq=torch.zeros(B, **i32), out=torch.zeros(B + 1, dtype=torch.int64, device=d))
         dec.tok[:B].copy_(tokens)
         f16 = dict(dtype=torch.float16, device=d)
         dec.bufs = {n: torch.zeros(B, w, **f16) for n, w in
@@ -425,8 +426,8 @@ class MistralLoRAModel:
 
     def finish_decode(self, dec: PagedDecode) -> None:
         """The host has the sequences again (their lengths and pages are read
-        back).  A step that found no free page raises here, or in the next
-        operator's call; it and the steps behind it have changed nothing."""
+        back).  A step that found no free page raises here, if no ``paged_step``
+        has; it has changed nothing."""
         st = dec.st
         if st.decode is not dec:
             raise ValueError("this decode is not the sequences' own")
@@ -480,19 +481,39 @@ class MistralLoRAModel:
         torch.matmul(b["xn"], self.lm_head.t(), out=b["logits"])
         drawn = torch.empty(B, dtype=torch.int64, device=self.device)
         ops.sample_tokens(b["logits"], dec.u.index_select(0, seq), drawn, **dec.sampling.rows(seq))
-        dec.tok.index_copy_(0, torch.where(dec.row_seq < 0, B, dec.row_seq).long(), drawn)
+        place = torch.where(dec.row_seq < 0, B, dec.row_seq).long()
+        dec.tok.index_copy_(0, place, drawn)
+        # nothing for those alive whose step could not be made
+        dec.out[:B].copy_(torch.where(dec.alive > 0, -1, dec.tok[:B]))
+        dec.out.index_copy_(0, place, drawn)
 
     @torch.inference_mode()
     def paged_step(self, dec: PagedDecode, use_graph: bool = True,
                    generator: Optional[torch.Generator] = None) -> torch.Tensor:
         """Every sequence that is alive feeds its token and draws the next one,
         with numbers from ``generator`` (by sequence, whoever else is alive).
-        Returns ``dec.tok[:B]``, on the device (an ended sequence's stays what it
-        was).  A row whose logits leave nothing to draw (all NaN or -infinity)
-        gives -1, and its sequence ends with the next step.  A call that raises
-        leaves the sequences as they were."""
+        Returns the tokens [B] on the device (``dec.out``; an ended sequence's
+        stays what it was).  A row whose logits leave nothing to draw (all NaN or
+        -infinity) gives -1, and its sequence ends with the next step.  A step
+        that finds no page for some sequence is made for none and gives -1 for
+        all that are alive; the next call that sees it raises (an eager step may
+        see it itself), and the one behind that tries again (with some sequences
+        ended, say).  A call that raises leaves the sequences as they were."""
         if dec.st.decode is not dec:  # its lengths and pages are others' now
             raise ValueError("this decode is not the sequences' own")
+        try:
+            ops.check_errors(self.device, synchronize=False)
+            return self._paged_step(dec, use_graph, generator)
+        except RuntimeError as error:
+            # Steps that were on their way behind the one at fault have failed like it:
+            # nothing of them stays pending for other calls.
+            try:
+                ops.check_errors(self.device)
+            except RuntimeError as more:
+                raise error from more
+            raise
+
+    def _paged_step(self, dec: PagedDecode, use_graph: bool, generator: Optional[torch.Generator]) -> torch.Tensor:
         dec.u.uniform_(generator=generator)
         B = len(dec.seqs)
         if not use_graph:
@@ -503,7 +524,7 @@ class MistralLoRAModel:
                 for to, t in zip(dec._moved(), was):
                     to.copy_(t)
                 raise
-            return dec.tok[:B]
+            return dec.out[:B]
         if dec.graph is None:
             # Warmed up on a side stream by a step in which nobody is alive; what it
             # moves is put back (nothing else is written but the padded rows' own buffers).
@@ -523,7 +544,7 @@ class MistralLoRAModel:
                 self._paged_body(dec)
             dec.graph = g
         dec.graph.replay()
-        return dec.tok[:B]
+        return dec.out[:B]
 
     # ---- decode --------------------------------------------------------------
     def _decode_body(self, st: DecodeState) -> None:

@@ -215,3 +215,41 @@ def test_a_decode_that_ended_moves_nothing(use_graph):
     model.paged_step(st.decode, use_graph=use_graph)
     model.finish_decode(st.decode)
     assert st.lengths == [52, 1, 18]
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_a_step_without_pages_gives_no_tokens(use_graph):
+    """Two sequences need a page and one is free: no token for anybody, an error
+    with the next step, and the old tokens once there is room."""
+    pool, model = _small_model()
+    prompts, greedy = _prompts([31, 31, 14], 28), [SamplingParams()] * 3
+    clean, first, _ = _start(model, pool, prompts, greedy)
+    want = [first] + [model.paged_step(clean, use_graph=use_graph).tolist() for _ in range(6)]
+    dec, _, _ = _start(model, pool, prompts, greedy, pages=6)
+    assert model.paged_step(dec, use_graph=use_graph).tolist() == want[1]
+    before = _state(dec)
+    assert before[2] == [32, 32, 15] and before[0] == want[1]
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="no room for a planned step"):
+            for _ in range(2):  # (operators of an eager step may see it before the step is through)
+                assert model.paged_step(dec, use_graph=use_graph).tolist() == [-1] * 3
+        assert _state(dec) == before
+    dec.alive[0] = 0
+    for w in want[2:]:
+        assert model.paged_step(dec, use_graph=use_graph).tolist() == [want[1][0]] + w[1:]
+    model.finish_decode(dec)
+    assert dec.st.lengths == [0, 37, 20]
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_ragged_generation_with_too_few_pages_raises(use_graph):
+    """The loop does not wait for its steps: nothing of those behind the one
+    without a page is left for later calls."""
+    pool, model = _small_model()
+    eng = StaticBatchEngine(model, pool, max_batch=4, max_seq_len=256)
+    reqs = [Request(f"r{i}", "a", p, slot=i, sampling=SamplingParams()) for i, p in enumerate(_prompts([15, 15], 29))]
+    with pytest.raises(RuntimeError, match="no room for a planned step"):
+        eng.run_ragged_generate(reqs, 100, use_graph, num_pages=3)
+    ops.check_errors(_dev())
+    got = eng.run_ragged_generate(reqs, 10, use_graph, num_pages=4)["tokens"]
+    assert [len(t) for t in got] == [10, 10]
