@@ -697,7 +697,9 @@ struct Nf4Plan {
 // chunks (tile-major, problem after problem).  A tile that one CTA covers
 // whole is written straight to y; a tile split between CTAs is summed from
 // their pieces, so the partial buffer holds two pieces (a CTA's first and
-// last tile) per CTA.
+// last tile) per CTA.  The buffer comes first and is as large for every set of
+// problems, so that the counters behind it, which have to be zero between
+// launches, are where no other set's launch writes pieces.
 int nf4_plan(const persona_nf4_problem* probs, int n, Nf4Plan* out) {
   using namespace persona;
   if (n < 1 || n > kNf4MaxProblems || probs == nullptr) return PERSONA_ERR_INVALID_ARG;
@@ -724,7 +726,7 @@ int nf4_plan(const persona_nf4_problem* probs, int n, Nf4Plan* out) {
   a.chunks = chunks;
   a.max_ctas = static_cast<int>(chunks < cap ? chunks : cap);
   out->counter_bytes = (static_cast<size_t>(tiles) * 4 + 255) & ~size_t(255);
-  out->partial_bytes = static_cast<size_t>(a.max_ctas) * 2 * kNf4Tile * kNf4MaxRows * 4;
+  out->partial_bytes = static_cast<size_t>(cap) * 2 * kNf4Tile * kNf4MaxRows * 4;
   return PERSONA_OK;
 }
 }  // namespace
@@ -823,8 +825,8 @@ int nf4_linear_impl(const persona_nf4_problem* problems, int num_problems, const
     return PERSONA_ERR_WORKSPACE;
   if (!aligned16(workspace)) return PERSONA_ERR_ALIGNMENT;
   Nf4GemmArgs& a = plan.args;
-  a.counters = static_cast<int*>(workspace);
-  a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.counter_bytes);
+  a.partials = static_cast<float*>(workspace);
+  a.counters = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + plan.partial_bytes);
   a.err = dev_err;
   for (int64_t m0 = 0; m0 < M; m0 += kNf4MaxRows) {
     const int mc = static_cast<int>(M - m0 < kNf4MaxRows ? M - m0 : kNf4MaxRows);

@@ -31,7 +31,7 @@ struct Nf4GemmArgs {
   Nf4Problem prob[kNf4MaxProblems];
   int64_t chunks;    // all problems' chunks
   int num_problems;
-  int max_ctas;      // grid bound that the partial buffer is sized for
+  int max_ctas;      // grid bound: chunks, and what the partial buffer is sized for
   int M;
   float* partials;   // [CTA][2][128][M_pad] fp32: a CTA's first and last tile pieces
   int* counters;     // per tile, zero between launches (the finishing piece resets it)
