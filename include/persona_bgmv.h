@@ -291,6 +291,9 @@ typedef struct persona_nf4_problem {
  * per CTA, 19 MB on a B200, and a counter per 128 rows of the weights); a call
  * that finds it too small returns PERSONA_ERR_WORKSPACE.                     */
 size_t persona_nf4_linear_workspace_size(const persona_nf4_problem* problems, int num_problems);
+/* Bytes in front of the workspace's counters: only what is behind them has to be
+ * zero at first (current device).                                           */
+size_t persona_nf4_linear_counter_offset(void);
 /* Up to PERSONA_NF4_MAX_PROBLEMS linears in one launch (e.g. q / k / v on the
  * same x); any M (launches of at most 64 rows each).                        */
 int persona_nf4_linear(const persona_nf4_problem* problems, int num_problems, int64_t M, void* workspace,

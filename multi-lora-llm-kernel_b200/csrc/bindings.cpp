@@ -21,9 +21,11 @@
 #include <torch/extension.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <mutex>
 #include <sstream>
+#include <vector>
 
 #include "overlap.h"
 #include "persona_bgmv.h"
@@ -509,18 +511,41 @@ at::Tensor nf4_dequantize_op(const at::Tensor& packed, const at::Tensor& offset,
   return w;
 }
 
-// Per-device workspace of the NF4 linear: zero-filled when made or grown
-// (its counters must start at zero; the kernel leaves them at zero).
-at::Tensor nf4_workspace(size_t bytes, const at::Tensor& like) {
+// Workspace of the NF4 linear on a stream, whose counters are zeroed when it is
+// made (the kernel leaves them at zero).  Calls on two streams never share one,
+// nor do two captured graphs: each capture makes its own, in the graph's memory,
+// zeroed once per replay (64 KB and more of counters, so that it is made once).
+at::Tensor nf4_workspace(const persona_nf4_problem* probs, int n, const at::Tensor& like, cudaStream_t stream) {
+  struct Entry {
+    cudaStream_t stream;
+    unsigned long long capture;  // 0: none
+    at::Tensor t;
+  };
   static std::mutex mu;
-  static std::vector<at::Tensor> cache(64);
+  static auto* const made = new std::vector<Entry>[kMaxDevices];  // (lives on: no tensor is freed behind the context)
   const int dev = like.get_device();
-  TORCH_CHECK(dev >= 0 && dev < 64, "nf4_linear: device index out of range");
+  TORCH_CHECK(dev >= 0 && dev < kMaxDevices, "nf4_linear: device index out of range");
+  const int64_t bytes = static_cast<int64_t>(persona_nf4_linear_workspace_size(probs, n));
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &capture));
+  if (status == cudaStreamCaptureStatusNone) capture = 0;
   std::lock_guard<std::mutex> lock(mu);
-  at::Tensor& t = cache[dev];
-  if (!t.defined() || static_cast<size_t>(t.numel()) < bytes)
-    t = at::zeros({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
-  return t;
+  std::vector<Entry>& list = made[dev];
+  if (capture != 0)  // those of a graph that has been captured belong to it alone
+    list.erase(std::remove_if(list.begin(), list.end(),
+                              [&](const Entry& e) { return e.capture != 0 && e.capture != capture; }),
+               list.end());
+  auto e = std::find_if(list.begin(), list.end(),
+                        [&](const Entry& x) { return x.stream == stream && x.capture == capture; });
+  if (e == list.end()) e = list.insert(list.end(), Entry{stream, capture, at::Tensor()});
+  if (!e->t.defined() || e->t.numel() < bytes) {
+    const int64_t from = static_cast<int64_t>(persona_nf4_linear_counter_offset());
+    e->t = at::Tensor();
+    e->t = at::empty({std::max(bytes, from + 65536)}, like.options().dtype(at::kByte));
+    e->t.narrow(0, from, e->t.numel() - from).zero_();
+  }
+  return e->t;
 }
 
 void nf4_linear_op(const at::Tensor& x, at::TensorList packed, at::TensorList offsets, at::TensorList ys) {
@@ -548,8 +573,8 @@ void nf4_linear_op(const at::Tensor& x, at::TensorList packed, at::TensorList of
   const int dev = x.get_device();
   raise_pending(dev, op);
   if (M == 0) return;
-  at::Tensor ws = nf4_workspace(persona_nf4_linear_workspace_size(probs, n), x);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  at::Tensor ws = nf4_workspace(probs, n, x, stream);
   check_status(persona_nf4_linear(probs, n, M, ws.data_ptr(), ws.numel(), error_word_device(dev), stream), op);
   after_launch(dev, op, stream);
 }
@@ -738,8 +763,8 @@ void nf4_linear_add_op(const at::Tensor& x, at::TensorList packed, at::TensorLis
   const int dev = x.get_device();
   raise_pending(dev, op);
   if (M == 0) return;
-  at::Tensor ws = nf4_workspace(persona_nf4_linear_workspace_size(probs, n), x);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  at::Tensor ws = nf4_workspace(probs, n, x, stream);
   check_status(persona_nf4_linear_add(probs, n, add, ldadd, M, ws.data_ptr(), ws.numel(), error_word_device(dev),
                                       stream),
                op);

@@ -693,6 +693,15 @@ struct Nf4Plan {
   size_t partial_bytes;
 };
 
+// The most CTAs of a launch on the current device, and the bytes of their pieces.
+int64_t nf4_most_ctas() {
+  const int sms = persona::nf4_sm_count();
+  return static_cast<int64_t>(persona::kNf4MaxCtasPerSm) * (sms > 0 ? sms : 148);
+}
+size_t nf4_partial_bytes() {
+  return static_cast<size_t>(nf4_most_ctas()) * 2 * persona::kNf4Tile * persona::kNf4MaxRows * 4;
+}
+
 // Every CTA of the launch gets an equal contiguous range of the problems'
 // chunks (tile-major, problem after problem).  A tile that one CTA covers
 // whole is written straight to y; a tile split between CTAs is summed from
@@ -720,13 +729,11 @@ int nf4_plan(const persona_nf4_problem* probs, int n, Nf4Plan* out) {
     chunks += (p.N / kNf4Tile) * (p.K / kNf4Tile);
     tiles += p.N / kNf4Tile;
   }
-  int sms = nf4_sm_count();
-  if (sms <= 0) sms = 148;
-  const int64_t cap = static_cast<int64_t>(kNf4MaxCtasPerSm) * sms;
+  const int64_t cap = nf4_most_ctas();
   a.chunks = chunks;
   a.max_ctas = static_cast<int>(chunks < cap ? chunks : cap);
+  out->partial_bytes = nf4_partial_bytes();
   out->counter_bytes = (static_cast<size_t>(tiles) * 4 + 255) & ~size_t(255);
-  out->partial_bytes = static_cast<size_t>(cap) * 2 * kNf4Tile * kNf4MaxRows * 4;
   return PERSONA_OK;
 }
 }  // namespace
@@ -783,6 +790,8 @@ size_t persona_nf4_linear_workspace_size(const persona_nf4_problem* problems, in
   if (nf4_plan(problems, num_problems, &plan) != PERSONA_OK) return 0;
   return plan.counter_bytes + plan.partial_bytes;
 }
+
+size_t persona_nf4_linear_counter_offset(void) { return nf4_partial_bytes(); }
 
 int persona_nf4_linear(const persona_nf4_problem* problems, int num_problems, int64_t M, void* workspace,
                        size_t workspace_bytes, int32_t* dev_err, cudaStream_t stream) {

@@ -111,3 +111,68 @@ def test_steps_of_full_width_layers_agree_with_their_prompt(graph):
             got.append(model.extend(st, tokens[:, i:i + 1].tolist())[0].float())
     ops.check_errors(DEV)
     torch.testing.assert_close(torch.stack(got, 1), want, rtol=0, atol=0.03 * want.abs().max().item())
+
+
+def _graph(x, qs, ys):
+    nf4.linear(x, qs, outs=ys)  # (kernel attributes are set outside of a capture)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        nf4.linear(x, qs, outs=ys)
+    return g
+
+
+def _prepare(shapes, M, seed):
+    (sets, g) = _weights(shapes, seed)
+    out = []
+    for qs, ws in sets:
+        x = torch.randn(M, qs[0].K, generator=g, device=DEV).half()
+        ys = [torch.full((M, q.N), float("nan"), dtype=torch.float16, device=DEV) for q in qs]
+        out.append((x, qs, ws, ys))
+    return out
+
+
+def test_graphs_keep_their_workspace():
+    """Captured, then calls with far more tiles, then memory of all sizes taken:
+    a replay writes its outputs and nothing else."""
+    few, many = _prepare([[(1024, 1024)], [(1 << 21, 128)]], 8, 4)
+    x, qs, ws, ys = few
+    g = _graph(x, qs, ys)
+    nf4.linear(many[0], many[1], outs=many[3])
+    _check(many[0], many[2], many[3])
+    taken = [torch.full((n << 20,), 17, dtype=torch.uint8, device=DEV) for n in (1, 2, 4, 18, 19, 20, 21, 24, 32) for _ in range(3)]
+    for _ in range(3):
+        ys[0].fill_(float("nan"))
+        g.replay()
+        _check(x, ws, ys)
+    assert all(bool((t == 17).all()) for t in taken)
+    # another capture in between leaves the first graph's alone
+    h = _graph(*[many[i] for i in (0, 1, 3)])
+    for graph, (a, _, w, b) in ((g, few), (h, many), (g, few)):
+        b[0].fill_(float("nan"))
+        graph.replay()
+        _check(a, w, b)
+
+
+@pytest.mark.parametrize("captured", [True, False])
+def test_linears_on_two_streams(captured):
+    """Launches that run at the same time have a workspace each."""
+    calls = _prepare([[(1024, 4096)], [(4096, 1024)]], 8, 6)
+    graphs = [_graph(x, qs, ys) for x, qs, _, ys in calls] if captured else None
+    want = []
+    for x, qs, ws, ys in calls:
+        nf4.linear(x, qs, outs=ys)
+        _check(x, ws, ys)
+        want.append(ys[0].clone())
+    streams = [torch.cuda.Stream(DEV) for _ in calls]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream(DEV))
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            x, qs, _, ys = calls[i]
+            with torch.cuda.stream(s):
+                ys[0].fill_(float("nan"))
+                graphs[i].replay() if captured else nf4.linear(x, qs, outs=ys)
+        torch.cuda.synchronize()
+        for (_, _, _, ys), w in zip(calls, want):
+            assert torch.equal(ys[0], w)
+    ops.check_errors(DEV)
