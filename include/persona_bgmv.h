@@ -410,7 +410,12 @@ typedef struct persona_rows {
  * 2^-40 with max |x| <= 448 s over its new tokens, or stays what it was if
  * earlier tokens of the sequence are in the block and it was larger.  Where it
  * grows their codes become those of code * old / s, which is exact but for
- * codes that fall below the smallest normal one (2^-6).  Contents of the block
+ * codes that fall below the smallest normal one (2^-6); those are rounded to
+ * steps of 2^-9 of the new scale.  A scale does not shrink again while earlier
+ * tokens stay in the block: drafted tokens that are larger than those before them
+ * and are taken back leave the kept ones with the larger scale, and so do the
+ * tokens that follow (pages with a scale per position know no such trace; nor do
+ * blocks of which nothing is kept).  Contents of the block
  * behind the last token are left alone, and mean something else then.  Whole
  * blocks belong to one sequence: two sequences that share a block must not both
  * write it.  Of values that are not finite, infinities become NaN themselves
@@ -479,7 +484,8 @@ int persona_paged_plan(const int32_t* add, const int32_t* keep, int32_t* lengths
  * u in [0, 1): a smaller number or NaN counts as 0, a larger one draws the last
  * kept token with weight.  A logit of -infinity or NaN is never drawn; -1 where there is
  * nothing else; where a logit is +infinity, those that are share the weight.
- * Weights, sums and comparisons in 64 bits.  tokens overlaps no input.       */
+ * Weights, sums and comparisons in 64 bits; weights below 2^-1000 count as 0.
+ * tokens overlaps no input.                                                 */
 int persona_sample_tokens(const void* logits, int64_t ld, int logits_type, const float* u, const float* temperature,
                           const int32_t* top_k, const float* top_p, const float* min_p, int64_t* tokens, int64_t B, int64_t V,
                           cudaStream_t stream);

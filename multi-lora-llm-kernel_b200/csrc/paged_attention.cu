@@ -55,6 +55,14 @@
 // (66): there the instructions of 24 columns (620 a step, 370 with 8), and
 // starting and ending tiles (10 us of a CTA each), are what counts.
 //
+// Roundings to fewer bits than fp32, in either form and in the chunk kernel: the
+// weights of the second product to 16 bits (fp16: 2^-11 of each, what the tensor
+// cores take; outputs of 32 x 5 drafts are off by 2.8e-4 of their size, 2.1e-4 with
+// fp32 weights, most of it the 16-bit output's own); elements of a bf16 q row below
+// 2^-14 of its largest, over 8-bit pages, to steps of 2^-24 of that; exponentials,
+// and the logarithm and the reciprocal of a v scale, to about 2^-22, the accuracy of
+// the instructions.
+//
 // mma.sync, not tcgen05: a tile has 16 or 32 rows, a quarter or half of
 // tcgen05's smallest M (64), and the tensor work per byte of pages is far below
 // what the warp-level product delivers.
@@ -440,7 +448,8 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
           }
           if (kE4m3 && !std::is_same<T, __half>::value) {
             // bf16 row -> fp16: scaled by the power of two that brings its
-            // largest element into [1, 2); elements 2^-24 below that vanish
+            // largest element into [1, 2); elements below 2^-14 lose bits, those
+            // below 2^-25 vanish
             float mx = 0.f;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
@@ -671,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, block_ctas(NT)) paged_attention_kern
           const float e2 = exp2_approx(st[nt][2] - ma), e3 = exp2_approx(st[nt][3] - mb);
           l_row[nt][0] = fmaf(e0 + e2, rv, l_row[nt][0]);
           l_row[nt][1] = fmaf(e1 + e3, rv, l_row[nt][1]);
-          // 16 bits for the product, as below
+          // 16 bits for the product: half a step of fp16, 2^-11 of a weight
           pb[nt][0] = transposed(Mma<__half>::pack(e0, e1));
           pb[nt][1] = transposed(Mma<__half>::pack(e2, e3));
         }
@@ -1073,8 +1082,11 @@ template <typename T, int D, int MT, bool kE4m3, int NT>
 cudaError_t attention_launch(PagedAttention a, int max_new, cudaStream_t st) {
   // Ring slots of 8 KB (16-bit) or 4.1 KB (8-bit) per warp at D = 128, two CTAs
   // per SM: 3 and 6 (96 KB a CTA); with two row tiles over 8-bit pages 4 (77.7
-  // against 81.3 us for 32 x 5 rows).  Rows as columns: as many as the CTAs of
-  // block_ctas have room for.
+  // against 81.3 us for 32 x 5 rows).  Rows as columns: about as many as the CTAs of
+  // block_ctas have room for.  One more would cost a CTA of the SM, and with it far
+  // more than depth gives: 64 long sequences of 4 rows 80 us with 3 slots, 103 with 4
+  // (74 with 2), 12 rows 93 with 4, 146 with 5 (91 with 3), 20 rows 130 with 4, 202 with 5
+  // (129 with 3); 32 rows 140, 141 and 142 with 4, 5 and 6.
   constexpr int kStages = (NT == 1 ? 3 : NT == 2 || NT == 3 ? 4 : NT > 3 ? 5 : kE4m3 ? (MT == 2 ? 4 : 6) : 3) * (128 / D);
   constexpr int TR = NT > 0 ? 8 * NT : 16 * MT;
   constexpr int kSmem = RingBytes<D, TR, kE4m3, kStages, (NT > 0)>::kBytes +

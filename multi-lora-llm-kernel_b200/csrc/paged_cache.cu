@@ -177,7 +177,7 @@ __device__ __forceinline__ int find_run_seq(const int32_t* indptr, int B, int sh
 // (8-bit floats), it can grow with the block, and the codes of the block's
 // earlier tokens move to the larger one exactly unless they fall below the
 // smallest normal code.  The angles of every row are made once per CTA.
-// Measured: 8000 rows of 32 + 2 x 8 heads 52 us in blocks of 8 to 64, 57 in
+// Measured: 7982 rows of 32 + 2 x 8 heads 49 to 52 us in blocks of 2 to 64, 54 in
 // blocks of 128 (0.53 of the measured HBM rate; 16000 rows 0.61): every CTA
 // is resident at once, so all of them wait for the same chain of reads, then
 // for the angles.  With 40 registers a thread 72 us, with 100 64.
@@ -404,6 +404,11 @@ cudaError_t block_write_launch(const PagedWrite& a, int slices, int32_t* err, cu
 template <typename T, int D>
 cudaError_t block_write_dim(const PagedWrite& a, int32_t* err, cudaStream_t st) {
   // Threads by the block's size, and few slices, since each makes the angles anew.
+  // 7982 prompt rows of 32 + 2 x 8 heads, threads x slices as chosen and beside it, us:
+  // blocks of 2 128 x 1 49 (x 2 54, 256 x 1 55), of 8 128 x 1 51 (x 2 50, 256 x 1 52), of 16
+  // 128 x 2 52 (x 1 66, x 4 50), of 32 128 x 4 52 (x 2 67, 256 x 2 52), of 64 512 x 2 52 (x 1
+  // 93, x 4 56, 128 x 4 75), of 128 512 x 4 54 (x 2 93, 256 x 8 72).  64 single tokens take
+  // 5.6 to 5.8 in any of these, but 7.8 with 512 x 4.
   const int block = 1 << a.c.scale_shift;
   return block < 32   ? block_write_launch<T, D, 128>(a, block < 16 ? 1 : 2, err, st)
          : block < 64 ? block_write_launch<T, D, 128>(a, 4, err, st)

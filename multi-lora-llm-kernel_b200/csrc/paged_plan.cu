@@ -44,13 +44,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_plan_kernel(const __grid_co
   __shared__ long long s_sum[3][kWarps];
   __shared__ int s_bad[kWarps];
   const int B = a.B, ps = a.page_size;
-  // of every sequence: first row, pages taken and given back before it, tokens kept, pages kept and held
+  // of every sequence: first row, pages taken and given back before it, tokens kept, pages kept
   int* const s_row = s_seq;
   int* const s_take = s_row + B;
   int* const s_back = s_take + B;
   int* const s_keep = s_back + B;
   int* const s_kept = s_keep + B;
-  int* const s_held = s_kept + B;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   pdl_wait();
@@ -77,7 +76,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_plan_kernel(const __grid_co
     s_back[b] = held - kept;
     s_keep[b] = keep;
     s_kept[b] = kept;
-    s_held[b] = held;
     sum[0] += add;
     sum[1] += need - kept;
     sum[2] += held - kept;
@@ -176,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_plan_kernel(const __grid_co
   }
 }
 
-constexpr int kSeqBytes = 6 * sizeof(int);
+constexpr int kSeqBytes = 5 * sizeof(int);
 static_assert(PERSONA_PLAN_MAX_SEQS * kSeqBytes <= 200 * 1024, "shared memory");
 
 }  // namespace
@@ -185,6 +183,10 @@ cudaError_t launch_paged_plan(const PagedPlan& a, cudaStream_t st) {
   static std::atomic<bool> done[64];
   const cudaError_t e = prepare_kernel(done, paged_plan_kernel, PERSONA_PLAN_MAX_SEQS * kSeqBytes, 0);
   if (e != cudaSuccess) return e;
+  // One CTA for few rows, which has no cluster barriers: 512 rows 4.9 us (eight CTAs
+  // 5.5), 1024 5.1 (5.9), 2048 5.8 (5.8), 4096 7.4 (6.0), 14700 16.7 (7.5).  Pages given
+  // back, which the host does not know, are not in the rule: 3000 of them cost one CTA
+  // 4.4 us (4.7), 32000, sequences of half a million tokens that end together, 17.7 (4.7).
   const int ctas = a.rows <= 2048 ? 1 : 8;
   return launch_paged(paged_plan_kernel, dim3(ctas), dim3(kThreads), static_cast<size_t>(a.B) * kSeqBytes, ctas, true, st, a);
 }

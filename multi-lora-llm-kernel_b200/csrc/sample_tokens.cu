@@ -9,7 +9,8 @@
 //
 // Weights, sums and comparisons are in 64 bits: the draw, and the end of the
 // nucleus, compare a sum over up to 2^21 tokens with a number that falls
-// between two of them.
+// between two of them.  A weight below 2^-1000 counts as none: it changes no sum
+// that holds the largest weight, 1, and would be drawn by a number of 0 alone.
 //
 // Every condition but the draw keeps a beginning of the order, so a row is cut
 // at one (value, index) pair: a 64-bit number `pair` whose high half orders the
@@ -26,10 +27,10 @@
 // What it must read is the logits, once.  What bounds it is instructions: 25 to
 // 30 a token and pass with a weight (ten of them in 64 bits), and for few rows
 // the chain of passes, exchanges between the CTAs of a cluster, and the list.
-// Measured: 8 rows of 32000 tokens, fp16: 4.4 us greedy, 8 us by temperature or
-// min-p, 25 us by top-p or top-k; 256 of 50257: 11 (0.36 of the measured HBM
-// rate), 32, 114 and 53 us, 106 with every row a rule of its own; 64 fp32 rows
-// of 130001 by temperature 30 us (0.17).
+// Measured, with inputs that change from call to call: 8 rows of 32000 tokens,
+// fp16: 4.9 us greedy, 8.7 by temperature, 8.9 by min-p, 24 by top-k, 29 by top-p;
+// 256 of 50257: 14 (0.28 of the measured HBM rate), 35, 36, 56 and 122 us, 104 with
+// every row a rule of its own; 64 fp32 rows of 130001: 14 (0.36), 31, 32, 50, 105, 86.
 #include <cooperative_groups.h>
 
 #include <type_traits>

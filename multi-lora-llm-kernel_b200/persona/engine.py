@@ -113,7 +113,8 @@ class StaticBatchEngine:
         """Generate up to ``max_new_tokens`` (and the request's own
         ``max_tokens``) per request, prompts of any lengths; returns the new
         token ids as a list per request, and device times as
-        ``run_static_generate``.  ``num_pages``: of the cache (default: what all
+        ``run_static_generate``; every call captures its step anew, which is part
+        of ``decode_ms``.  ``num_pages``: of the cache (default: what all
         requests need at their longest).  A request whose logits leave nothing to
         draw (all NaN or -infinity) ends there, with the tokens that it has."""
         slots = self.plan_batch(requests)

@@ -273,8 +273,9 @@ def paged_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache:
     ``float8_e4m3fn`` take fp32 scales [pages, Hkv, page size]: one per token
     and head, ``max|x| / 448``; scales [pages, Hkv, n] with n a fraction of the
     page size: one per block of 2, 4, ... 128 tokens and head, a power of two
-    that grows with the block (its earlier codes move to the new scale; a block
-    is written by one sequence only).  Rows of no sequence are left alone.
+    that grows with the block (its earlier codes move to the new scale, and stay
+    there if the tokens that made it grow are taken back; a block is written by
+    one sequence only).  Rows of no sequence are left alone.
     ``theta`` is taken as an fp32 number.  What is written must not overlap itself or
     another argument, but for ``q_out``, which may be ``q``."""
     q_out = q if q_out is None else q_out
