@@ -176,3 +176,24 @@ def test_linears_on_two_streams(captured):
         for (_, _, _, ys), w in zip(calls, want):
             assert torch.equal(ys[0], w)
     ops.check_errors(DEV)
+
+
+def test_only_the_counters_have_to_be_zero():
+    lib = capi_lib.load()
+    lib.persona_nf4_linear_counter_offset.restype = ctypes.c_size_t
+    (qs, ws), = _weights([[(2048, 4096), (128, 4096)]], 9)[0]
+    x = torch.randn(5, 4096, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).half()
+    ys = [torch.full((5, q.N), float("nan"), dtype=torch.float16, device=DEV) for q in qs]
+    arr = (capi_lib.Nf4Problem * 2)(*[
+        capi_lib.Nf4Problem(q.packed.data_ptr(), q.offset.data_ptr(), x.data_ptr(), q.K, y.data_ptr(), q.N, q.N, q.K)
+        for q, y in zip(qs, ys)])
+    size, at = lib.persona_nf4_linear_workspace_size(arr, 2), lib.persona_nf4_linear_counter_offset()
+    assert 0 < at < size and size - at >= 4 * 17
+    space = torch.full((size,), 255, dtype=torch.uint8, device=DEV)
+    space[at:] = 0
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for _ in range(2):
+        capi_lib.check(lib.persona_nf4_linear(arr, 2, 5, space.data_ptr(), size, err.data_ptr(), st))
+        _check(x, ws, ys)
+    assert int(err.item()) == 0 and not space[at:].any()  # left at zero again
