@@ -54,7 +54,7 @@ def sample_batch(logits: torch.Tensor, params, generator: Optional[torch.Generat
                  u: Optional[torch.Tensor] = None) -> torch.Tensor:
     """logits [batch, vocab] on the GPU -> next token ids [batch] (int64), each
     row by its own parameters (a ``BatchSampling`` or one ``SamplingParams`` per
-    row).  ``u`` [batch] fp32 are the uniform numbers the tokens are drawn with;
+    row); -1 for a row of NaN or -infinity alone.  ``u`` [batch] fp32 are the uniform numbers the tokens are drawn with;
     drawn from ``generator`` if not given."""
     from persona import ops
 
