@@ -23,7 +23,7 @@ from typing import List, Optional, Sequence
 import torch
 
 from persona.adapter_pool import AdapterCache, AdapterPool
-from persona.mistral import MistralLoRAModel
+from persona.mistral import MistralLoRAModel, on_its_device
 from persona.sampling import BatchSampling, SamplingParams, sample_batch, sample_next_token
 
 
@@ -67,6 +67,7 @@ class StaticBatchEngine:
                     r.slot = next(slots)
         return torch.tensor([r.slot for r in requests], dtype=torch.int32, device=self.device)
 
+    @on_its_device
     @torch.inference_mode()
     def run_static_generate(self, requests: Sequence[Request], max_new_tokens: int = 128,
                             use_cuda_graph: bool = True) -> dict:
@@ -106,6 +107,7 @@ class StaticBatchEngine:
         return {"tokens": out.cpu(), "prefill_ms": prefill_ms, "decode_ms": decode_ms, "new_tokens": new,
                 "tok_per_s": new / ((prefill_ms + decode_ms) * 1e-3)}
 
+    @on_its_device
     @torch.inference_mode()
     def run_ragged_generate(self, requests: Sequence[Request], max_new_tokens: int = 128, use_cuda_graph: bool = True,
                             kv_dtype: torch.dtype = torch.float16, kv_block: int = 1, page_size: int = 16,

@@ -31,6 +31,7 @@ so it is captured once as a CUDA graph and replayed for every token.
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence
@@ -41,6 +42,18 @@ import torch.nn.functional as F
 from persona import nf4, ops
 from persona.adapter_pool import AdapterPool
 from persona.sampling import BatchSampling
+
+def on_its_device(method):
+    """The method runs with ``self.device`` as the current device: graphs are
+    captured and replayed, and events recorded, on the current device's streams."""
+
+    @functools.wraps(method)
+    def call(self, *args, **kwargs):
+        with torch.cuda.device(self.device):
+            return method(self, *args, **kwargs)
+
+    return call
+
 
 @dataclass
 class MistralConfig:
@@ -487,6 +500,7 @@ class MistralLoRAModel:
         dec.out[:B].copy_(torch.where(dec.alive > 0, -1, dec.tok[:B]))
         dec.out.index_copy_(0, place, drawn)
 
+    @on_its_device
     @torch.inference_mode()
     def paged_step(self, dec: PagedDecode, use_graph: bool = True,
                    generator: Optional[torch.Generator] = None) -> torch.Tensor:
@@ -540,7 +554,7 @@ class MistralLoRAModel:
                 for to, t in zip(dec._moved(), was):
                     to.copy_(t)
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
+            with torch.cuda.graph(g, stream=s):  # (the default one is of the device that captured first)
                 self._paged_body(dec)
             dec.graph = g
         dec.graph.replay()
@@ -581,6 +595,7 @@ class MistralLoRAModel:
         st.pos.add_(1)
         st.length.add_(1)
 
+    @on_its_device
     @torch.inference_mode()
     def decode_step(self, st: DecodeState, use_graph: bool = True) -> torch.Tensor:
         """Feed ``st.tok`` at ``st.pos``; greedy next tokens land in
@@ -601,7 +616,7 @@ class MistralLoRAModel:
             st.length.copy_(pos0 + 1)
             st.tok.copy_(tok0)
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
+            with torch.cuda.graph(g, stream=s):  # (the default one is of the device that captured first)
                 self._decode_body(st)
             st.graph = g
             # capture does not run the body: run it now
