@@ -515,6 +515,8 @@ at::Tensor nf4_dequantize_op(const at::Tensor& packed, const at::Tensor& offset,
 // made (the kernel leaves them at zero).  Calls on two streams never share one,
 // nor do two captured graphs: each capture makes its own, in the graph's memory,
 // zeroed once per replay (64 KB and more of counters, so that it is made once).
+// Kept for the streams used last; what is freed stays its stream's until the
+// launches there have run, so a stream that comes back just makes another.
 at::Tensor nf4_workspace(const persona_nf4_problem* probs, int n, const at::Tensor& like, cudaStream_t stream) {
   struct Entry {
     cudaStream_t stream;
@@ -538,7 +540,14 @@ at::Tensor nf4_workspace(const persona_nf4_problem* probs, int n, const at::Tens
                list.end());
   auto e = std::find_if(list.begin(), list.end(),
                         [&](const Entry& x) { return x.stream == stream && x.capture == capture; });
-  if (e == list.end()) e = list.insert(list.end(), Entry{stream, capture, at::Tensor()});
+  if (e == list.end()) {
+    constexpr size_t kStreams = 8;  // 19 MB each
+    if (list.size() >= kStreams) list.erase(list.begin());
+    list.push_back(Entry{stream, capture, at::Tensor()});
+  } else {
+    std::rotate(e, e + 1, list.end());  // (the one used last is the last)
+  }
+  e = list.end() - 1;
   if (!e->t.defined() || e->t.numel() < bytes) {
     const int64_t from = static_cast<int64_t>(persona_nf4_linear_counter_offset());
     e->t = at::Tensor();

@@ -197,3 +197,22 @@ def test_only_the_counters_have_to_be_zero():
         capi_lib.check(lib.persona_nf4_linear(arr, 2, 5, space.data_ptr(), size, err.data_ptr(), st))
         _check(x, ws, ys)
     assert int(err.item()) == 0 and not space[at:].any()  # left at zero again
+
+
+def test_many_streams_keep_few_workspaces():
+    """One launch on each of 60 streams: right everywhere, and the memory that
+    stays is that of a few."""
+    (x, qs, ws, ys), = _prepare([[(1024, 4096)]], 8, 12)
+    outs = [torch.full_like(ys[0], float("nan")) for _ in range(60)]
+    streams = [torch.cuda.Stream(DEV) for _ in outs]
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(DEV)
+    for _ in range(2):
+        for s, y in zip(streams, outs):
+            with torch.cuda.stream(s):
+                nf4.linear(x, qs, outs=[y])
+    torch.cuda.synchronize()
+    for y in outs:
+        _check(x, ws, [y])
+    assert torch.cuda.memory_allocated(DEV) - before <= 8 * (21 << 20)
+    ops.check_errors(DEV)
